@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define SA_ABI_VERSION 18
+#define SA_ABI_VERSION 19
 
 enum sa_status {
     SA_OK = 0,
@@ -491,6 +491,104 @@ int sa_sparse_attention_decode_mask(const void *q, const int64_t q_strides[4], c
                                     const uint8_t *mask, const int64_t mask_strides[4], int B, int H, int Sq, int Sk, int D,
                                     int BK, int dtype, float sm_scale_log2, int num_splits, void *workspace, size_t workspace_bytes,
                                     float *lse, const int64_t lse_strides[3], void *stream);
+
+/*
+ * 8-bit paged K/V cache.  No counterpart in the reference, which keeps no cache; the attention over it
+ * (sa_sparse_attention_decode_paged) is the function of its forward (sparseattention/sparse_attn_kernel.py:149-185).
+ *
+ * A pool of pages of page_size tokens (32, 64, 128 or 256) of all H K/V heads; a sequence's tokens lie in the pages that its row of a
+ * page table names.  Blocks of 32 consecutive tokens of one head are held as e4m3 codes (float8_e4m3fn) with a scale 2^e: e is the least
+ * integer with max|x| <= 448 * 2^e over the block's finite values, from -96 to 119; x is held as round(x / 2^e) * 2^e, NaN and infinities
+ * as NaN.  D is 64, 128 or 256.
+ *   k, v               uint8 [num_pages, H, page_size / 32, 32 * D], contiguous, 16-byte aligned; the order inside a block is the kernels' own
+ *                      (csrc/paged.h): sa_paged_cache_gather gives the values
+ *   k_scales, v_scales float32 [num_pages, H, page_size / 32], contiguous
+ * The structure is read before a call returns.  In all calls
+ *   page_table         device int32 [B, pages_per_sequence], strides in elements; token t of sequence b lies in page page_table[b][t / page_size].
+ *                      An entry that is no page (outside [0, num_pages)) is as if nothing were there: nothing is stored, read as zeros,
+ *                      attended to.
+ *   lens               device int32 [B]: tokens that each sequence holds; below 0 counts as 0.
+ * Pages may be shared by sequences that read them.  Two sequences of one call that store into the same block leave it undefined.
+ */
+typedef struct sa_paged_cache {
+    uint8_t *k, *v;
+    float *k_scales, *v_scales;
+    int num_pages; /* 1 .. 2^20 */
+    int H, page_size, D;
+} sa_paged_cache;
+
+/*
+ * Stores new tokens: the first counts[b] (NULL: all S) rows of k, v [B,H,S,D] (bf16 or fp16, strides multiples of 8 elements, last dimension
+ * contiguous, 16-byte aligned) become tokens lens[b] .. lens[b] + counts[b] - 1 of sequence b.  lens is not changed.  Tokens past the
+ * table are not stored.  A block that holds tokens keeps its scale or takes a larger one, with which what it holds is rounded again.
+ */
+int sa_paged_cache_append(const sa_paged_cache *cache, const void *k, const int64_t k_strides[4], const void *v,
+                          const int64_t v_strides[4], const int32_t *page_table, const int64_t page_table_strides[2],
+                          const int32_t *lens, const int32_t *counts, int B, int S, int pages_per_sequence, int dtype,
+                          void *stream);
+
+/* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,D] (bf16 or fp16, as above); rows from lens[b] on are zero. */
+int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_strides[4], void *v, const int64_t v_strides[4],
+                          const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, int B, int length,
+                          int pages_per_sequence, int dtype, void *stream);
+
+/*
+ * Copies page src[i] to page dst[i], i < n (device int32).  A pair with a number that is no page is left out; a destination named more than
+ * once takes the last one's page.  A page that is a source and a destination of one call is undefined where it is read.
+ */
+int sa_paged_cache_copy(const sa_paged_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/*
+ * n new sequences that continue old ones: new_table[i] (int32 [n, pages_per_sequence], contiguous) is the row of parents[i] with -1
+ * behind its last page, new_lens[i] its length.  Full pages are shared.  A last page that is not full is copied to page new_pages[i],
+ * which takes its place in the row; where new_pages[i] is no page the child keeps the parent's.  A parent outside [0, B) gives an
+ * empty sequence.  The new pages must be free; one named twice holds the last one's copy.
+ */
+int sa_paged_cache_fork(const sa_paged_cache *cache, const int32_t *page_table, const int64_t page_table_strides[2],
+                        const int32_t *lens, int B, int pages_per_sequence, const int32_t *parents, const int32_t *new_pages, int n,
+                        int32_t *new_table, int32_t *new_lens, void *stream);
+
+/*
+ * Moves the pages in use to the front of the pool.  In use are the pages that hold the first lens[b] tokens of a sequence, *used of them
+ * (device int32); those from *used on move to the free ones below, the lowest to the lowest.  new_table (int32
+ * [B, pages_per_sequence], contiguous, not page_table's memory) names the pages where they are then, -1 behind a sequence's last.
+ * workspace: sa_paged_cache_compact_workspace_bytes(num_pages) bytes of device memory (0: invalid argument).
+ */
+size_t sa_paged_cache_compact_workspace_bytes(int num_pages);
+int sa_paged_cache_compact(const sa_paged_cache *cache, const int32_t *page_table, const int64_t page_table_strides[2],
+                           const int32_t *lens, int B, int pages_per_sequence, int32_t *new_table, int32_t *used, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/*
+ * The pages that no sequence uses (as above): free_pages (int32 [num_pages]) in rising order, -1 behind the last, *free_count (int32) of
+ * them.  A sequence is freed by a length of 0.
+ */
+int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, int B,
+                              int pages_per_sequence, int num_pages, int page_size, int32_t *free_pages, int32_t *free_count,
+                              void *stream);
+
+/*
+ * sa_sparse_attention_decode over the cache: q, o [B,Hq,Sq,D], Sq <= 32, Hq a multiple of H (query heads h * Hq/H .. of K/V head h).
+ *   lens      the keys of every sequence, the call's own tokens among them (append, then attend)
+ *   counts    device int32 [B], valid query rows of every sequence, or NULL for Sq; the rows behind give 0 and -inf
+ *   without lists (all NULL) row i of sequence b attends to keys 0 .. lens[b] - counts[b] + i, with window > 0 to the last `window` of these
+ *   lists     of a mask [B,H,Sq,tiles * page_size] by sa_mask_classify_packed with BQ = Sq, BK = page_size: ids [B,H,1,tiles], lens
+ *             [B,H,1], packed tiles with strides in bytes along B and H.  The mask alone says who attends, among the keys below
+ *             lens[b]; window must be 0.  Tile indices out of range are skipped.
+ * workspace, lse, dtype, sm_scale_log2: as for sa_sparse_attention_decode; sa_decode_paged_workspace_bytes(...) bytes, 16-byte aligned (of
+ * the current device).  K and V are read as they are held, exactly; a value beyond fp16's range is infinite there.  A masked NaN or
+ * infinity has no effect.
+ */
+size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size);
+int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache,
+                                     const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens,
+                                     const int32_t *counts, int pages_per_sequence, void *o, const int64_t o_strides[4],
+                                     const int32_t *full_ids, const int64_t full_ids_strides[4], const int32_t *full_lens,
+                                     const int64_t full_lens_strides[3], const int32_t *part_ids, const int64_t part_ids_strides[4],
+                                     const int32_t *part_lens, const int64_t part_lens_strides[3], const uint8_t *packed,
+                                     const int64_t packed_strides[2], int tiles, int B, int Hq, int Sq, int window, int dtype,
+                                     float sm_scale_log2, void *workspace, size_t workspace_bytes, float *lse,
+                                     const int64_t lse_strides[3], void *stream);
 
 /*
  * Merge of n attention results over disjoint key ranges of the same queries (what sharding the key axis over

@@ -10,7 +10,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsparseattn_hip.so")
 
-SA_ABI_VERSION = 18
+SA_ABI_VERSION = 19
 SA_OK = 0
 SA_ERR_INVALID_ARGUMENT = -1
 SA_ERR_UNSUPPORTED = -2
@@ -66,6 +66,15 @@ EXPORTS = (
     "sa_mask_terms_workspace_bytes",
     "sa_mask_classify_terms",
     "sa_mask_classify_terms_pair",
+    "sa_paged_cache_append",
+    "sa_paged_cache_gather",
+    "sa_paged_cache_copy",
+    "sa_paged_cache_fork",
+    "sa_paged_cache_compact_workspace_bytes",
+    "sa_paged_cache_compact",
+    "sa_paged_cache_free_pages",
+    "sa_decode_paged_workspace_bytes",
+    "sa_sparse_attention_decode_paged",
 )
 
 _lib = None
@@ -73,6 +82,13 @@ _host = None
 
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _vp = ctypes.c_void_p
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """sa_paged_cache of the C ABI."""
+
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scales", "v_scales")]
+                + [(n, ctypes.c_int) for n in ("num_pages", "H", "page_size", "D")])
 
 
 class SparseAttnError(RuntimeError):
@@ -194,6 +210,29 @@ def load() -> ctypes.CDLL:
     lib.sa_mask_classify_terms.argtypes = (
         [ctypes.POINTER(ctypes.c_int32), ctypes.c_int] + [_vp, _i64p] * 2 + [ctypes.c_int] * 6 + [_vp, _i64p] * 4
         + [_vp, _i64p] + [_vp, ctypes.c_size_t, _vp]
+    )
+    cache = ctypes.POINTER(PagedCacheStruct)
+    table = [_vp, _i64p, _vp]  # page table, its strides, lengths
+    lib.sa_paged_cache_append.restype = ctypes.c_int
+    lib.sa_paged_cache_append.argtypes = [cache] + [_vp, _i64p] * 2 + table + [_vp] + [ctypes.c_int] * 4 + [_vp]
+    lib.sa_paged_cache_gather.restype = ctypes.c_int
+    lib.sa_paged_cache_gather.argtypes = [cache] + [_vp, _i64p] * 2 + table + [ctypes.c_int] * 4 + [_vp]
+    lib.sa_paged_cache_copy.restype = ctypes.c_int
+    lib.sa_paged_cache_copy.argtypes = [cache, _vp, _vp, ctypes.c_int, _vp]
+    lib.sa_paged_cache_fork.restype = ctypes.c_int
+    lib.sa_paged_cache_fork.argtypes = [cache] + table + [ctypes.c_int] * 2 + [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]
+    lib.sa_paged_cache_compact_workspace_bytes.restype = ctypes.c_size_t
+    lib.sa_paged_cache_compact_workspace_bytes.argtypes = [ctypes.c_int]
+    lib.sa_paged_cache_compact.restype = ctypes.c_int
+    lib.sa_paged_cache_compact.argtypes = [cache] + table + [ctypes.c_int] * 2 + [_vp, _vp] + [_vp, ctypes.c_size_t] + [_vp]
+    lib.sa_paged_cache_free_pages.restype = ctypes.c_int
+    lib.sa_paged_cache_free_pages.argtypes = table + [ctypes.c_int] * 4 + [_vp, _vp, _vp]
+    lib.sa_decode_paged_workspace_bytes.restype = ctypes.c_size_t
+    lib.sa_decode_paged_workspace_bytes.argtypes = [ctypes.c_int] * 7
+    lib.sa_sparse_attention_decode_paged.restype = ctypes.c_int
+    lib.sa_sparse_attention_decode_paged.argtypes = (
+        [_vp, _i64p, cache] + table + [_vp, ctypes.c_int] + [_vp, _i64p] + [_vp, _i64p] * 4 + [_vp, _i64p]
+        + [ctypes.c_int] * 6 + [ctypes.c_float] + [_vp, ctypes.c_size_t] + [_vp, _i64p] + [_vp]
     )
     if lib.sa_abi_version() != SA_ABI_VERSION:
         raise RuntimeError(f"libsparseattn_hip ABI {lib.sa_abi_version()} != expected {SA_ABI_VERSION}")

@@ -368,6 +368,249 @@ py::object decode(const Tensor &q, const Tensor &k, const Tensor &v, const OptTe
     return as_object(decode_impl(q, k, v, mask, BK, md, num_splits, return_lse));
 }
 
+// ---- the 8-bit paged K/V cache ------------------------------------------------------------------------------------
+const Name kCacheK{"k"}, kCacheV{"v"}, kCacheKScales{"k_scales"}, kCacheVScales{"v_scales"}, kHeadDim{"head_dim"};
+struct Cache {
+    Tensor k, v, k_scales, v_scales;
+    int64_t D;  // the caller's head dim; the pool's is the kernels' (kernel_head_dim)
+    sa_paged_cache c;
+    int64_t H() const { return c.H; }
+    int64_t page() const { return c.page_size; }
+    int64_t Dk() const { return c.D; }
+};
+// (read under the interpreter's lock)
+Cache cache_of(py::handle o) {
+    Cache x;
+    const Name *names[4] = {&kCacheK, &kCacheV, &kCacheKScales, &kCacheVScales};
+    Tensor *to[4] = {&x.k, &x.v, &x.k_scales, &x.v_scales};
+    for (int i = 0; i < 4; i++) {
+        const py::object t = attr(o, *names[i]);
+        if (!t || !THPVariable_Check(t.ptr())) type_error(std::string("cache.") + names[i]->text + " is not a tensor");
+        *to[i] = THPVariable_Unpack(t.ptr());
+    }
+    const py::object d = attr(o, kHeadDim);
+    if (!d) type_error("cache.head_dim is missing");
+    x.D = d.cast<int64_t>();
+    if (x.k.dim() != 4 || x.k.scalar_type() != at::kByte || x.k.size(3) % 32 || !x.k.is_contiguous())
+        value_error("cache.k must be contiguous uint8 [pages, H, page_size / 32, 32 * D], got " + str(x.k));
+    if (!x.k.is_cuda()) throw std::runtime_error("the paged cache's operators need it on a ROCm GPU; there is no CPU path");
+    const int64_t N = x.k.size(0), H = x.k.size(1), per = x.k.size(2), Dk = x.k.size(3) / 32;
+    if (x.v.sizes() != x.k.sizes() || x.v.scalar_type() != at::kByte || !x.v.is_contiguous() || x.v.device() != x.k.device())
+        value_error("cache.v must be like cache.k, got " + str(x.v));
+    const int64_t want[3] = {N, H, per};
+    for (const Tensor *t : {&x.k_scales, &x.v_scales})
+        if (t->sizes() != at::IntArrayRef(want, 3) || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != x.k.device())
+            value_error("cache scales must be contiguous float32 [pages, H, page_size / 32] on the cache's device, got " + str(*t));
+    if (N > (1 << 20) || per > 8 || H > 0x7fffffff) value_error("cache of " + std::to_string(N) + " pages of " + std::to_string(32 * per) + " tokens");
+    if (x.D < 1 || kernel_head_dim(x.D, true) != Dk) value_error("cache.head_dim " + std::to_string(x.D) + " does not belong to a pool of " + std::to_string(Dk));
+    x.c = {ptr<uint8_t>(x.k), ptr<uint8_t>(x.v), ptr<float>(x.k_scales), ptr<float>(x.v_scales), (int)N, (int)H, (int)(32 * per), (int)Dk};
+    return x;
+}
+
+Tensor cache_ints(const Cache &c, const char *name, const Tensor &t, int64_t n) {
+    if (t.dim() != 1 || t.size(0) != n || t.scalar_type() != at::kInt || t.device() != c.k.device())
+        value_error(std::string(name) + ": expected int32 (" + std::to_string(n) + ",) on " + c.k.device().str() + ", got " + str(t));
+    return t.is_contiguous() ? t : t.contiguous();
+}
+// B of a page table and its sequences' lengths
+int64_t check_table(const Cache &c, const Tensor &table) {
+    if (table.dim() != 2 || table.scalar_type() != at::kInt || table.device() != c.k.device() || table.size(1) < 1)
+        value_error("page_table: expected int32 [B, pages] on " + c.k.device().str() + ", got " + str(table));
+    return table.size(0);
+}
+int cache_dtype(at::ScalarType t, const char *what) {
+    const int dt = dtype_code(t);
+    if (dt != SA_DTYPE_BF16 && dt != SA_DTYPE_FP16) type_error(std::string(what) + " must be bfloat16 or float16 (got " + c10::toString(t) + ")");
+    return dt;
+}
+int as_int(int64_t x, const char *name) {
+    if (x < 0 || x > 0x7fffffff) value_error(std::string(name) + " out of range: " + std::to_string(x));
+    return (int)x;
+}
+
+void paged_append(py::object cache, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens_in, const OptTensor &counts_in) {
+    const Cache c = cache_of(cache);
+    const py::gil_scoped_release unlocked;
+    const int64_t B = check_table(c, table);
+    const c10::DeviceGuard guard(c.k.device());
+    const Tensor lens = cache_ints(c, "lens", lens_in, B);
+    OptTensor counts;
+    if (counts_in) counts = cache_ints(c, "counts", *counts_in, B);
+    if (k.dim() != 4 || k.size(0) != B || k.size(1) != c.H() || k.size(3) != c.D || v.sizes() != k.sizes())
+        value_error("k, v must be [" + std::to_string(B) + ", " + std::to_string(c.H()) + ", S, " + std::to_string(c.D) + "] (got " + str(k.sizes()) + ", " +
+                    str(v.sizes()) + ")");
+    const int dt = cache_dtype(k.scalar_type(), "k, v");
+    if (v.scalar_type() != k.scalar_type()) type_error("k and v must share a dtype");
+    for (const Tensor *t : {&k, &v})
+        if (t->device() != c.k.device()) value_error("k, v must be on the cache's device " + c.k.device().str() + ", got " + t->device().str());
+    const int64_t S = k.size(2);
+    if (B == 0 || S == 0) return;
+    const Tensor kc = kernel_ready(pad_head_dim(k, c.Dk())), vc = kernel_ready(pad_head_dim(v, c.Dk()));
+    check_rc(sa_paged_cache_append(&c.c, kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), ptr<int32_t>(table), st(table), ptr<int32_t>(lens),
+                                   ptr<int32_t>(counts), as_int(B, "B"), as_int(S, "S"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
+}
+
+py::tuple paged_gather(py::object cache, const Tensor &table, const Tensor &lens_in, std::optional<int64_t> length, at::ScalarType dtype) {
+    const Cache c = cache_of(cache);
+    Tensor out[2];
+    {
+        const py::gil_scoped_release unlocked;
+        const int64_t B = check_table(c, table);
+        const c10::DeviceGuard guard(c.k.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        const int dt = cache_dtype(dtype, "dtype");
+        const int64_t n = length.value_or(table.size(1) * c.page());
+        if (n < 0) value_error("length must not be negative (got " + std::to_string(n) + ")");
+        for (Tensor &t : out) t = at::empty({B, c.H(), n, c.Dk()}, at::TensorOptions().dtype(dtype).device(c.k.device()));
+        if (B > 0 && n > 0)
+            check_rc(sa_paged_cache_gather(&c.c, out[0].data_ptr(), st(out[0]), out[1].data_ptr(), st(out[1]), ptr<int32_t>(table), st(table),
+                                           ptr<int32_t>(lens), as_int(B, "B"), as_int(n, "length"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
+        for (Tensor &t : out) t = cut_head_dim(t, c.D);
+    }
+    return py::make_tuple(out[0], out[1]);
+}
+
+void paged_copy(py::object cache, const Tensor &src_in, const Tensor &dst_in) {
+    const Cache c = cache_of(cache);
+    const py::gil_scoped_release unlocked;
+    const c10::DeviceGuard guard(c.k.device());
+    if (src_in.dim() != 1) value_error("src: expected int32 [n], got " + str(src_in));
+    const int64_t n = src_in.size(0);
+    const Tensor src = cache_ints(c, "src", src_in, n), dst = cache_ints(c, "dst", dst_in, n);
+    if (n == 0) return;
+    check_rc(sa_paged_cache_copy(&c.c, ptr<int32_t>(src), ptr<int32_t>(dst), as_int(n, "n"), stream_of(c.k)));
+}
+
+py::tuple paged_fork(py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &parents_in, const Tensor &new_pages_in) {
+    const Cache c = cache_of(cache);
+    Tensor new_table, new_lens;
+    {
+        const py::gil_scoped_release unlocked;
+        const int64_t B = check_table(c, table);
+        const c10::DeviceGuard guard(c.k.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        if (parents_in.dim() != 1) value_error("parents: expected int32 [n], got " + str(parents_in));
+        const int64_t n = parents_in.size(0);
+        const Tensor parents = cache_ints(c, "parents", parents_in, n), new_pages = cache_ints(c, "new_pages", new_pages_in, n);
+        if (B == 0 && n > 0) value_error("no sequences to fork");
+        new_table = at::empty({n, table.size(1)}, lens.options());
+        new_lens = at::empty({n}, lens.options());
+        if (n > 0)
+            check_rc(sa_paged_cache_fork(&c.c, ptr<int32_t>(table), st(table), ptr<int32_t>(lens), as_int(B, "B"), as_int(table.size(1), "pages"),
+                                         ptr<int32_t>(parents), ptr<int32_t>(new_pages), as_int(n, "n"), ptr<int32_t>(new_table), ptr<int32_t>(new_lens),
+                                         stream_of(c.k)));
+    }
+    return py::make_tuple(new_table, new_lens);
+}
+
+py::tuple paged_compact(py::object cache, const Tensor &table, const Tensor &lens_in) {
+    const Cache c = cache_of(cache);
+    Tensor new_table, used;
+    {
+        const py::gil_scoped_release unlocked;
+        const int64_t B = check_table(c, table);
+        const c10::DeviceGuard guard(c.k.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        new_table = at::empty({B, table.size(1)}, lens.options());
+        if (B == 0) {
+            used = at::zeros({1}, lens.options());
+        } else {
+            used = at::empty({1}, lens.options());
+            const size_t bytes = sa_paged_cache_compact_workspace_bytes(c.c.num_pages);
+            const Tensor ws = at::empty({(int64_t)(bytes / 4)}, lens.options());
+            check_rc(sa_paged_cache_compact(&c.c, ptr<int32_t>(table), st(table), ptr<int32_t>(lens), as_int(B, "B"), as_int(table.size(1), "pages"),
+                                            ptr<int32_t>(new_table), ptr<int32_t>(used), ws.data_ptr(), bytes, stream_of(c.k)));
+        }
+    }
+    return py::make_tuple(new_table, used);
+}
+
+py::tuple paged_free_pages(py::object cache, const Tensor &table, const Tensor &lens_in) {
+    const Cache c = cache_of(cache);
+    Tensor free_pages, count;
+    {
+        const py::gil_scoped_release unlocked;
+        const int64_t B = check_table(c, table);
+        const c10::DeviceGuard guard(c.k.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        if (B == 0) {
+            free_pages = at::arange(c.c.num_pages, lens.options());
+            count = at::full({1}, c.c.num_pages, lens.options());
+        } else {
+            free_pages = at::empty({c.c.num_pages}, lens.options());
+            count = at::empty({1}, lens.options());
+            check_rc(sa_paged_cache_free_pages(ptr<int32_t>(table), st(table), ptr<int32_t>(lens), as_int(B, "B"), as_int(table.size(1), "pages"),
+                                               c.c.num_pages, c.c.page_size, ptr<int32_t>(free_pages), ptr<int32_t>(count), stream_of(c.k)));
+        }
+    }
+    return py::make_tuple(free_pages, count);
+}
+
+py::object decode_paged(const Tensor &q, py::object cache, const Tensor &table, const Tensor &lens_in, const OptTensor &mask, py::object md,
+                        const OptTensor &counts_in, std::optional<int64_t> window, bool return_lse) {
+    const Cache c = cache_of(cache);
+    const int64_t B = check_table(c, table), P = c.page(), H = c.H();
+    if (q.dim() != 4 || q.size(0) != B || q.size(3) != c.D || q.size(1) % H || q.size(1) == 0)
+        value_error("q must be [" + std::to_string(B) + ", a multiple of " + std::to_string(H) + ", Sq, " + std::to_string(c.D) + "] (got " + str(q.sizes()) + ")");
+    if (q.device() != c.k.device()) value_error("q is on " + q.device().str() + ", expected " + c.k.device().str() + " (the cache's device)");
+    const int dt = cache_dtype(q.scalar_type(), "q");
+    const int64_t Hq = q.size(1), Sq = q.size(2);
+    const bool has_md = !md.is_none();
+    if (window && *window < 1) value_error("window must be positive (got " + std::to_string(*window) + ")");
+    if (window && (has_md || mask)) value_error("a window goes with no mask (make it part of the mask)");
+    Lists l;
+    int64_t tiles = 0;
+    if (has_md) {
+        l = lists_of(md);
+        if (l.fid.dim() != 4) value_error("mask_metadata.unmasked_kv_ids: expected int32 [B, H, 1, tiles], got " + str(l.fid));
+        tiles = l.fid.size(3);
+        check_lists(l, q, B, H, 1, tiles, "mask_metadata");
+        if (tiles < 1 || tiles > table.size(1))
+            value_error("mask_metadata has " + std::to_string(tiles) + " tiles (one per page of the cache), page_table " + std::to_string(table.size(1)) + " pages");
+        checked_metadata(md, l, tiles * P, P);
+        if (!l.packed) value_error("sparse_attention_decode_paged needs mask_metadata with packed_masks");
+        check_packed(*l.packed, q, B, H, 1, tiles, Sq * P / 8, "mask_metadata");
+    }
+    Out r;
+    {
+        const py::gil_scoped_release unlocked;
+        const c10::DeviceGuard guard(q.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        OptTensor counts;
+        if (counts_in) counts = cache_ints(c, "counts", *counts_in, B);
+        if (!has_md && mask && B > 0 && Sq > 0) {
+            if (mask->dim() != 4) value_error("mask must be [B,H,Sq,Sk] (got " + str(mask->sizes()) + ")");
+            same_device(q, "mask", mask);
+            const int64_t Sk = mask->size(3);
+            if (Sk < 1 || Sk % P || Sk / P > table.size(1))
+                value_error("mask of " + std::to_string(Sk) + " keys: expected whole pages of " + std::to_string(P) + " and at most " + std::to_string(table.size(1)) +
+                            " of them");
+            tiles = Sk / P;
+            l = classify_lists(mask->expand({B, H, Sq, Sk}), Sq, P, true);
+        }
+        const Tensor qc = kernel_ready(pad_head_dim(q, c.Dk()));
+        const Tensor o = at::empty_like(qc);
+        const auto f32 = at::TensorOptions().dtype(at::kFloat).device(q.device());
+        if (return_lse) r.lse = at::empty({B, Hq, Sq}, f32);
+        if (B > 0 && Sq > 0) {
+            const int Bi = as_int(B, "B"), pages = as_int(table.size(1), "pages"), w = window ? (int)std::min<int64_t>(*window, 1 << 30) : 0;
+            const size_t bytes = sa_decode_paged_workspace_bytes(Bi, as_int(Hq, "Hq"), (int)H, (int)Sq, (int)c.Dk(), pages, (int)P);
+            Tensor ws;
+            if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+            const bool lists = l.fid.defined();
+            auto ip = [&](const Tensor &t) { return lists ? ptr<int32_t>(t) : nullptr; };
+            auto is = [&](const Tensor &t) { return lists ? st(t) : nullptr; };
+            check_rc(sa_sparse_attention_decode_paged(qc.data_ptr(), st(qc), &c.c, ptr<int32_t>(table), st(table), ptr<int32_t>(lens), ptr<int32_t>(counts),
+                                                      pages, o.data_ptr(), st(o), ip(l.fid), is(l.fid), ip(l.fl), is(l.fl), ip(l.pid), is(l.pid), ip(l.pl),
+                                                      is(l.pl), ptr<uint8_t>(l.packed), st(l.packed), (int)tiles, Bi, (int)Hq, as_int(Sq, "Sq"), w, dt,
+                                                      (float)scale_log2(c.D), bytes ? ws.data_ptr() : nullptr, bytes, ptr<float>(r.lse), st(r.lse),
+                                                      stream_of(q)));
+        }
+        r.o = cut_head_dim(o, c.D);
+    }
+    return as_object(r);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------
 // Whether the kernels tile by the caller's own sizes (kernel_tiles of sparse_attn_kernel.py returns them unchanged).
 bool tiles_as_asked(int64_t Sq, int64_t Sk, int64_t D, int64_t BQ, int64_t BK, bool f32) {
@@ -866,6 +1109,13 @@ PYBIND11_MODULE(_host, m) {
     m.def("forward_kernel", &forward_kernel);
     m.def("forward_tiled", &forward_tiled);
     m.def("decode", &decode);
+    m.def("decode_paged", &decode_paged);
+    m.def("paged_append", &paged_append);
+    m.def("paged_gather", &paged_gather);
+    m.def("paged_copy", &paged_copy);
+    m.def("paged_fork", &paged_fork);
+    m.def("paged_compact", &paged_compact);
+    m.def("paged_free_pages", &paged_free_pages);
     m.def("classify", &classify);
     m.def("classify_terms", &classify_terms);
     m.def("classify_terms_backward", &classify_terms_backward);

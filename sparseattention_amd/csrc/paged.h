@@ -1,0 +1,107 @@
+// The 8-bit paged K/V cache: its layout and the parameters of its kernels (paged_cache.hip, paged_decode.hip).
+//
+// A page holds page_size tokens of every head, as blocks of 32 consecutive tokens of one head; a block is 32 * D bytes,
+// e4m3 codes, and has one scale 2^e.  The power of two costs no accuracy, as the codes are floating-point numbers, and makes
+// scaling exact: what a block holds does not change when its scale grows, but for codes that become subnormal.
+// Inside a block the codes lie in the order in which the attention's matrix instructions take them, so that a wave reads a
+// block with D / 32 loads of 1 KiB each, straight into their operands:
+//   K  16 bytes of lane (key = lane % 32, hh = lane / 32) of piece c: d = 32 c + 16 hh ..+15 of that key
+//   V  16 bytes of lane (d % 32 = lane % 32, hh) of piece d / 32: keys 16 (j / 8) + 8 (j % 8 / 4) + 4 hh + j % 4, j = 0..15
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace sa {
+
+constexpr int kPagedBlock = 32;                  // tokens that share a scale
+constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^119 is the largest that bf16 and float32 hold
+constexpr int kPagedMostPages = 1 << 20;         // (compaction keeps a bit per page in LDS)
+
+struct PagedPool {
+    uint8_t *k, *v;            // [pages, H, per, 32 * D]
+    float *k_scales, *v_scales;  // [pages, H, per]
+    int pages, H, lper, D;     // per = page_size / 32 = 2^lper
+};
+struct PageTable {
+    const int32_t *ids;
+    int64_t s0, s1;  // strides in elements
+    const int32_t *lens;
+    int B, width;
+};
+
+struct PagedAppendParams {
+    PagedPool c;
+    PageTable t;
+    const uint16_t *k, *v;
+    int64_t ks[3], vs[3];   // b, h, token strides in elements (d stride 1)
+    const int32_t *counts;  // or null: S of every sequence
+    int S, blocks;          // blocks: the most that S tokens touch
+};
+hipError_t launch_paged_append(const PagedAppendParams &p, int dtype, hipStream_t stream);
+
+struct PagedGatherParams {
+    PagedPool c;
+    PageTable t;
+    uint16_t *k, *v;
+    int64_t ks[3], vs[3];
+    int length;
+};
+hipError_t launch_paged_gather(const PagedGatherParams &p, int dtype, hipStream_t stream);
+
+struct PagedCopyParams {
+    PagedPool c;
+    const int32_t *src, *dst;
+    int n;
+};
+hipError_t launch_paged_copy(const PagedCopyParams &p, hipStream_t stream);
+
+struct PagedForkParams {
+    PagedPool c;
+    PageTable t;
+    const int32_t *parents, *new_pages;
+    int n;
+    int32_t *new_ids, *new_lens;  // [n, width], [n]
+};
+hipError_t launch_paged_fork(const PagedForkParams &p, hipStream_t stream);
+
+// Which pages are in use, by a bit per page in LDS, and what follows from it.
+struct PagedPlanParams {
+    PageTable t;
+    int pages, lP;
+    int32_t *count;  // pages in use (compaction) or free (free list)
+    // compaction: the j-th lowest free page below `count` and the j-th lowest page in use from `count` on, how many such pairs
+    // there are, and where a page in use from `count` on goes
+    int32_t *holes, *movers, *moves, *to;
+    int32_t *free_list;  // or the free pages in rising order, -1 behind the last
+};
+hipError_t launch_paged_plan(const PagedPlanParams &p, hipStream_t stream);
+
+struct PagedCompactParams {
+    PagedPool c;
+    PageTable t;
+    const int32_t *count, *holes, *movers, *moves, *to;
+    int32_t *new_ids;  // [B, width]
+};
+hipError_t launch_paged_compact(const PagedCompactParams &p, hipStream_t stream);
+
+struct PagedDecodeParams {
+    PagedPool c;
+    PageTable t;
+    const uint16_t *q;
+    uint16_t *o;
+    float *lse;  // or null
+    int64_t qs[3], os[3], lses[3];  // b, h, row strides in elements
+    const int32_t *counts;  // valid query rows of each sequence, or null: Sq
+    int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT tiles of 32
+    int window;             // or 0
+    // tile lists, tile = page, all null: every key that causality and window leave
+    const int32_t *full_ids, *full_lens, *part_ids, *part_lens;
+    int64_t fis[3], fls[2], pis[3], pls[2];  // b, h (and entry) strides
+    const uint8_t *packed;  // PARTIAL tiles, Sq rows of page_size bits (PackParams layout)
+    int64_t pks[2];
+    int nK;
+    float scale;  // softmax scale / ln 2
+};
+hipError_t launch_paged_decode(const PagedDecodeParams &p, int dtype, hipStream_t stream);
+
+}  // namespace sa

@@ -1,0 +1,478 @@
+// The 8-bit paged K/V cache on gfx950 (MI355X): storing tokens, reading them back, copying, forking, compacting and
+// listing pages.  No counterpart in the reference, which keeps no cache; the attention over it is paged_decode.hip, the
+// layout of a block paged.h.
+//
+// A block of 32 tokens of one head holds codes c and a scale 2^e:  x = c * 2^e, c of e4m3, e the least integer with
+// max|x| <= 448 * 2^e over the finite values.  Tokens that come to a block that holds some take
+//     e' = max(e, e of the new ones),   c = round(x / 2^e'),   and the old ones   c' = round(c * 2^(e - e')),
+// which changes nothing but codes that fall below 2^-6.  NaN and infinities are held as NaN.
+// All of it moves memory: per element 2 bytes read and 1 written (append) or the reverse (gather).
+#include "fwd_common.h"
+#include "paged.h"
+
+namespace sa {
+
+namespace {
+
+template <int DT>
+struct Half16;  // what a pair of input values is, as bits
+template <>
+struct Half16<0> {
+    static constexpr uint32_t kInf = 0x7f80u;
+    static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t cvt_lo(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+    }
+    static __device__ __forceinline__ uint32_t cvt_hi(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true));
+    }
+};
+template <>
+struct Half16<1> {
+    static constexpr uint32_t kInf = 0x7c00u;
+    static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w).x; }
+    static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w).y; }
+    static __device__ __forceinline__ uint32_t cvt_lo(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
+    }
+    static __device__ __forceinline__ uint32_t cvt_hi(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true));
+    }
+};
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+
+// The least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), within the scales' range.
+__device__ __forceinline__ int scale_exp(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, kScaleExpMin), kScaleExpMax);
+}
+__device__ __forceinline__ int exp_of_scale(float s) {
+    return min(max((int)((__float_as_uint(s) >> 23) & 0xffu) - 127, kScaleExpMin), kScaleExpMax);
+}
+
+// Larger of m and the magnitudes of the finite values of the pair w, as bits (which order like the values).
+template <int DT>
+__device__ __forceinline__ uint32_t amax2(uint32_t m, uint32_t w) {
+    const uint32_t a = w & 0x7fffu, b = (w >> 16) & 0x7fffu;
+    m = max(m, a < Half16<DT>::kInf ? a : 0u);
+    return max(m, b < Half16<DT>::kInf ? b : 0u);
+}
+// What a value becomes before it is rounded to a code: in range (beyond it only at the largest scale), infinities NaN.
+__device__ __forceinline__ float scaled(float x, float inv) {
+    const float y = __builtin_amdgcn_fmed3f(x * inv, -448.f, 448.f);
+    return __builtin_fabsf(x) < __builtin_inff() ? y : __builtin_nanf("");
+}
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+}
+// Four codes times f <= 1, rounded again.
+__device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return codes4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+}
+// The bytes of four codes whose tokens are base .. base + 3 that lie in [a, z), as a mask.
+__device__ __forceinline__ uint32_t bytes_in(int base, int a, int z) {
+    const int lo = min(max(a - base, 0), 4), hi = min(max(z - base, 0), 4);
+    const uint32_t upto = hi >= 4 ? ~0u : (1u << (8 * hi)) - 1u, below = lo >= 4 ? ~0u : (1u << (8 * lo)) - 1u;
+    return upto & ~below;
+}
+
+// The page of block `blk` of sequence b, or -1.
+__device__ __forceinline__ int page_at(const PageTable &t, int b, int slot, int pages) {
+    if (slot < 0 || slot >= t.width) return -1;
+    const int page = t.ids[b * t.s0 + slot * t.s1];
+    return page >= 0 && page < pages ? page : -1;
+}
+__device__ __forceinline__ int64_t block_at(const PagedPool &c, int page, int h, int sub) {
+    return (((int64_t)page * c.H + h) << c.lper) + sub;
+}
+
+// One wave stores the new tokens of one block of one head, K or V.
+template <int DT, int ND>
+__global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParams p) {
+    using X = Half16<DT>;
+    constexpr int NG = ND / 2;  // groups of 64 d
+    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5;
+    unsigned item = blockIdx.x;
+    const bool values = item & 1u;
+    item >>= 1;
+    const int h = (int)(item % (unsigned)p.c.H);
+    item /= (unsigned)p.c.H;
+    const int nb = (int)(item % (unsigned)p.blocks), b = (int)(item / (unsigned)p.blocks);
+    const int room = p.t.width << (p.c.lper + 5);  // tokens that the table has place for
+    const int len = max(p.t.lens[b], 0);
+    if (len >= room) return;
+    const int n = p.counts != nullptr ? min(max(p.counts[b], 0), p.S) : p.S;
+    const int blk = (len >> 5) + nb;
+    // tokens [a, z) of the block are new, [0, held) are there
+    const int first = 32 * blk;
+    if (first >= room) return;
+    const int held = max(len - first, 0), a = held, z = min(len + n - first, 32);
+    if (a >= z) return;
+    const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
+    if (page < 0) return;
+    const int64_t at = block_at(p.c, page, h, blk & ((1 << p.c.lper) - 1));
+    uint8_t *const out = (values ? p.c.v : p.c.k) + at * (ND * 1024);
+    float *const scale = (values ? p.c.v_scales : p.c.k_scales) + at;
+    const int64_t *const xs = values ? p.vs : p.ks;
+    // row t of the block is token first + t of the sequence, first + t - len of the new ones
+    const uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)(first - len) * xs[2];
+    const int64_t row = xs[2];
+    const int e_old = held > 0 ? exp_of_scale(*scale) : kScaleExpMin;
+
+    // the new values: K as 16 of one token per piece, V as two neighbouring d of 16 tokens per group
+    uint32_t w[16 * NG];
+    uint32_t m = 0u;
+    if (!values) {
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            u32x4 u[2] = {};
+            if (l32 >= a && l32 < z) {
+                const uint16_t *src = x + l32 * row + 32 * c + 16 * hh;
+                u[0] = *(const u32x4 *)src;
+                u[1] = *(const u32x4 *)(src + 8);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[8 * c + i] = u[i >> 2][i & 3];
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int t = 16 * (j >> 3) + 8 * ((j >> 2) & 1) + 4 * hh + (j & 3);
+                w[16 * g + j] = t >= a && t < z ? *(const uint32_t *)(x + t * row + 64 * g + 2 * l32) : 0u;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 * NG; i++) m = amax2<DT>(m, w[i]);
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, s));
+    const int e = max(e_old, scale_exp(DT == 0 ? __uint_as_float(m << 16) : X::lo(m)));
+    const float inv = exp2i(-e);
+    const bool grows = held > 0 && e > e_old;
+    const float f = exp2i(max(e_old - e, -126));
+    if (lane == 0 && (grows || held == 0)) *scale = exp2i(e);
+
+    if (!values) {
+        const bool fresh = l32 >= a && l32 < z, old = grows && l32 < held;
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            u32x4 *const to = (u32x4 *)(out + 1024 * c + 16 * lane);
+            if (fresh) {
+                u32x4 u;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t lo = w[8 * c + 2 * i], hi = w[8 * c + 2 * i + 1];
+                    u[i] = codes4(scaled(X::lo(lo), inv), scaled(X::hi(lo), inv), scaled(X::lo(hi), inv), scaled(X::hi(hi), inv));
+                }
+                *to = u;
+            } else if (old) {
+                u32x4 u = *to;
+#pragma unroll
+                for (int i = 0; i < 4; i++) u[i] = again4(u[i], f);
+                *to = u;
+            }
+        }
+    } else {
+        uint32_t isnew[4], isold[4], any = 0u, all = ~0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int base = 16 * (i >> 1) + 8 * (i & 1) + 4 * hh;
+            isnew[i] = bytes_in(base, a, z);
+            isold[i] = grows ? bytes_in(base, 0, held) : 0u;
+            any |= isnew[i] | isold[i];
+            all &= isnew[i];
+        }
+        if (any == 0u) return;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            // d = 64 g + 2 l32 and the next one
+            u32x4 *const to = (u32x4 *)(out + 1024 * (2 * g + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15)));
+            u32x4 u[2] = {};
+            if (all != ~0u) {
+                u[0] = to[0];
+                u[1] = to[1];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t *const q = &w[16 * g + 4 * i];
+                const uint32_t lo = codes4(scaled(X::lo(q[0]), inv), scaled(X::lo(q[1]), inv), scaled(X::lo(q[2]), inv), scaled(X::lo(q[3]), inv));
+                const uint32_t hi = codes4(scaled(X::hi(q[0]), inv), scaled(X::hi(q[1]), inv), scaled(X::hi(q[2]), inv), scaled(X::hi(q[3]), inv));
+                if (grows) {
+                    u[0][i] = (u[0][i] & ~isold[i]) | (again4(u[0][i], f) & isold[i]);
+                    u[1][i] = (u[1][i] & ~isold[i]) | (again4(u[1][i], f) & isold[i]);
+                }
+                u[0][i] = (u[0][i] & ~isnew[i]) | (lo & isnew[i]);
+                u[1][i] = (u[1][i] & ~isnew[i]) | (hi & isnew[i]);
+            }
+            to[0] = u[0];
+            to[1] = u[1];
+        }
+    }
+}
+
+// One wave reads one block of one head, K or V, into rows; rows that hold nothing become zero.
+template <int DT, int ND>
+__global__ __launch_bounds__(64) void paged_gather_kernel(const PagedGatherParams p) {
+    using X = Half16<DT>;
+    constexpr int NG = ND / 2;
+    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5;
+    const unsigned blocks = ((unsigned)p.length + 31) / 32;
+    unsigned item = blockIdx.x;
+    const bool values = item & 1u;
+    item >>= 1;
+    const int blk = (int)(item % blocks);
+    item /= blocks;
+    const int h = (int)(item % (unsigned)p.c.H), b = (int)(item / (unsigned)p.c.H);
+    const int first = 32 * blk;
+    const int rows = min(p.length - first, 32);
+    int n = min(max(p.t.lens[b] - first, 0), rows);  // rows that hold something
+    const int page = n > 0 ? page_at(p.t, b, blk >> p.c.lper, p.c.pages) : -1;
+    if (page < 0) n = 0;
+    const int64_t at = block_at(p.c, max(page, 0), h, blk & ((1 << p.c.lper) - 1));
+    const uint8_t *const in = (values ? p.c.v : p.c.k) + at * (ND * 1024);
+    const float scale = n > 0 ? exp2i(exp_of_scale((values ? p.c.v_scales : p.c.k_scales)[at])) : 0.f;
+    const int64_t *const xs = values ? p.vs : p.ks;
+    uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)first * xs[2];
+    const int64_t row = xs[2];
+    if (!values) {
+        if (l32 >= rows) return;
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            u32x4 u = {};
+            if (l32 < n) u = *(const u32x4 *)(in + 1024 * c + 16 * lane);
+            uint16_t *const to = x + l32 * row + 32 * c + 16 * hh;
+            *(u32x4 *)to = u32x4{X::cvt_lo(u.x, scale), X::cvt_hi(u.x, scale), X::cvt_lo(u.y, scale), X::cvt_hi(u.y, scale)};
+            *(u32x4 *)(to + 8) = u32x4{X::cvt_lo(u.z, scale), X::cvt_hi(u.z, scale), X::cvt_lo(u.w, scale), X::cvt_hi(u.w, scale)};
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            u32x4 u[2] = {};
+            if (n > 0) {
+                const u32x4 *const from = (const u32x4 *)(in + 1024 * (2 * g + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15)));
+                u[0] = from[0];
+                u[1] = from[1];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int base = 16 * (i >> 1) + 8 * (i & 1) + 4 * hh;
+                const uint32_t a0 = X::cvt_lo(u[0][i], scale), a1 = X::cvt_hi(u[0][i], scale);
+                const uint32_t b0 = X::cvt_lo(u[1][i], scale), b1 = X::cvt_hi(u[1][i], scale);
+                const uint32_t v[4] = {(a0 & 0xffffu) | (b0 << 16), (a0 >> 16) | (b0 & 0xffff0000u), (a1 & 0xffffu) | (b1 << 16),
+                                       (a1 >> 16) | (b1 & 0xffff0000u)};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (base + j < rows) *(uint32_t *)(x + (base + j) * row + 64 * g + 2 * l32) = base + j < n ? v[j] : 0u;
+            }
+        }
+    }
+}
+
+// The first `blocks` blocks of head h of page `src` to page `dst`, by a workgroup of 256.
+__device__ __forceinline__ void copy_head(const PagedPool &c, int src, int dst, int h, int blocks) {
+    const int64_t from = block_at(c, src, h, 0), to = block_at(c, dst, h, 0);
+    const int pieces = blocks * c.D * 2;  // of 16 bytes
+    const u32x4 *const k0 = (const u32x4 *)(c.k + from * (32 * c.D)), *const v0 = (const u32x4 *)(c.v + from * (32 * c.D));
+    u32x4 *const k1 = (u32x4 *)(c.k + to * (32 * c.D)), *const v1 = (u32x4 *)(c.v + to * (32 * c.D));
+    for (int i = threadIdx.x; i < pieces; i += 256) {
+        const u32x4 a = k0[i], b = v0[i];
+        k1[i] = a;
+        v1[i] = b;
+    }
+    if ((int)threadIdx.x < blocks) {
+        c.k_scales[to + threadIdx.x] = c.k_scales[from + threadIdx.x];
+        c.v_scales[to + threadIdx.x] = c.v_scales[from + threadIdx.x];
+    }
+}
+// Whether one of n copies behind copy i, of those that take place, has the same destination (the last one's page stays).
+template <class F>
+__device__ __forceinline__ bool named_again(const int32_t *dst, int i, int n, F &&takes_place) {
+    const int mine = dst[i];
+    int found = 0;
+    for (int j = i + 1 + (int)threadIdx.x; j < n; j += 256)
+        if (dst[j] == mine) found |= takes_place(j) ? 1 : 0;
+    return __syncthreads_or(found) != 0;
+}
+
+__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyParams p) {
+    const int i = (int)(blockIdx.x / (unsigned)p.c.H), h = (int)(blockIdx.x - (unsigned)i * (unsigned)p.c.H);
+    const int dst = p.dst[i];
+    if (dst < 0 || dst >= p.c.pages) return;
+    auto takes_place = [&](int j) { return p.src[j] >= 0 && p.src[j] < p.c.pages && p.src[j] != dst; };
+    if (!takes_place(i) || named_again(p.dst, i, p.n, takes_place)) return;
+    copy_head(p.c, p.src[i], dst, h, 1 << p.c.lper);
+}
+
+__global__ __launch_bounds__(256) void paged_fork_kernel(const PagedForkParams p) {
+    const int i = (int)(blockIdx.x / (unsigned)p.c.H), h = (int)(blockIdx.x - (unsigned)i * (unsigned)p.c.H);
+    const int lP = p.c.lper + 5, fresh = p.new_pages[i];
+    struct Child {
+        int b, len, full, tail, src;  // src: the page that is copied, or -1
+    };
+    auto child = [&](int j) {
+        Child x{p.parents[j], 0, 0, 0, -1};
+        if (x.b >= 0 && x.b < p.t.B) x.len = min(max(p.t.lens[x.b], 0), p.t.width << lP);
+        x.full = x.len >> lP;
+        x.tail = x.len & ((1 << lP) - 1);
+        if (x.tail != 0 && fresh >= 0 && fresh < p.c.pages) x.src = page_at(p.t, x.b, x.full, p.c.pages);
+        if (x.src == fresh) x.src = -1;
+        return x;
+    };
+    const Child x = child(i);
+    if (h == 0) {
+        const int used = x.full + (x.tail != 0 ? 1 : 0);
+        for (int j = threadIdx.x; j < p.t.width; j += 256)
+            p.new_ids[(int64_t)i * p.t.width + j] = j >= used ? -1 : x.src >= 0 && j == x.full ? fresh : p.t.ids[x.b * p.t.s0 + j * p.t.s1];
+        if (threadIdx.x == 0) p.new_lens[i] = x.len;
+    }
+    if (x.src < 0 || named_again(p.new_pages, i, p.n, [&](int j) { return child(j).src >= 0; })) return;
+    copy_head(p.c, x.src, fresh, h, (x.tail + 31) >> 5);
+}
+
+constexpr int kPlanThreads = 1024;
+// Sum over the threads in front of this one, and of all.
+__device__ __forceinline__ int before_me(int x, int *waves, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = x;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int up = __shfl_up(sum, s);
+        if (lane >= s) sum += up;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
+    int base = 0;
+    total = 0;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+        if (w < wave) base += waves[w];
+        total += waves[w];
+    }
+    return base + sum - x;
+}
+
+// One workgroup: a bit per page that a sequence uses, then the pairs of the compaction or the free list.  The table is read
+// once and the bits stay in LDS (2^20 pages: 128 KiB), which beats launches over them in memory by what a launch costs.
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPlanParams p) {
+    extern __shared__ uint32_t bits[];
+    __shared__ int waves[kPlanThreads / 64];
+    const int tid = threadIdx.x, words = (p.pages + 31) >> 5;
+    for (int i = tid; i < words; i += kPlanThreads) bits[i] = 0u;
+    __syncthreads();
+    const int64_t entries = (int64_t)p.t.B * p.t.width;
+    for (int64_t i = tid; i < entries; i += kPlanThreads) {
+        const int b = (int)(i / p.t.width), j = (int)(i - (int64_t)b * p.t.width);
+        if (((int64_t)j << p.lP) >= p.t.lens[b]) continue;
+        const int page = p.t.ids[b * p.t.s0 + j * p.t.s1];
+        if (page >= 0 && page < p.pages) atomicOr(&bits[page >> 5], 1u << (page & 31));
+    }
+    __syncthreads();
+    // this thread's words
+    const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    auto valid = [&](int w) { return 32 * w + 32 <= p.pages ? ~0u : (1u << (p.pages & 31)) - 1u; };
+    int used = 0, total;
+    for (int w = w0; w < w1; w++) used += __popc(bits[w]);
+    const int used_before = before_me(used, waves, total);
+    if (p.free_list != nullptr) {
+        const int free_total = p.pages - total;
+        int at = min(32 * w0, p.pages) - used_before;
+        for (int w = w0; w < w1; w++)
+            for (uint32_t left = ~bits[w] & valid(w); left != 0u; left &= left - 1u) p.free_list[at++] = 32 * w + __ffs(left) - 1;
+        for (int i = free_total + tid; i < p.pages; i += kPlanThreads) p.free_list[i] = -1;
+        if (tid == 0) *p.count = free_total;
+        return;
+    }
+    const int L = total;
+    auto below = [&](int w) { return 32 * w + 32 <= L ? ~0u : 32 * w >= L ? 0u : (1u << (L & 31)) - 1u; };  // pages < L
+    int holes = 0, movers = 0, hole_total, mover_total;
+    for (int w = w0; w < w1; w++) {
+        holes += __popc(~bits[w] & below(w));
+        movers += __popc(bits[w] & ~below(w));
+    }
+    int hole_at = before_me(holes, waves, hole_total), mover_at = before_me(movers, waves, mover_total);
+    const int mover_first = mover_at;
+    for (int w = w0; w < w1; w++) {
+        for (uint32_t left = ~bits[w] & below(w); left != 0u; left &= left - 1u) p.holes[hole_at++] = 32 * w + __ffs(left) - 1;
+        for (uint32_t left = bits[w] & ~below(w); left != 0u; left &= left - 1u) p.movers[mover_at++] = 32 * w + __ffs(left) - 1;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int i = mover_first; i < mover_at; i++) p.to[p.movers[i]] = p.holes[i];
+    if (tid == 0) {
+        *p.count = L;
+        *p.moves = mover_total;
+    }
+}
+
+// Moves the pages of the plan and writes the table that goes with them.
+__global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactParams p) {
+    const int64_t entries = (int64_t)p.t.B * p.t.width;
+    const int L = *p.count, lP = p.c.lper + 5;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
+        const int b = (int)(i / p.t.width), j = (int)(i - (int64_t)b * p.t.width);
+        int page = -1;
+        if (((int64_t)j << lP) < p.t.lens[b]) page = page_at(p.t, b, j, p.c.pages);
+        p.new_ids[i] = page >= L ? p.to[page] : page;
+    }
+    const int64_t items = (int64_t)*p.moves * p.c.H;
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const int m = (int)(i / p.c.H);
+        copy_head(p.c, p.movers[m], p.holes[m], (int)(i - (int64_t)m * p.c.H), 1 << p.c.lper);
+    }
+}
+
+template <class F>
+hipError_t with_sizes(int dtype, int D, F &&f) {
+    auto by_dim = [&](auto dt) {
+        if (D == 64) return f(dt, std::integral_constant<int, 2>{});
+        if (D == 128) return f(dt, std::integral_constant<int, 4>{});
+        if (D == 256) return f(dt, std::integral_constant<int, 8>{});
+        return hipErrorInvalidValue;
+    };
+    if (dtype == 0) return by_dim(std::integral_constant<int, 0>{});
+    if (dtype == 1) return by_dim(std::integral_constant<int, 1>{});
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedAppendParams &p, int dtype, hipStream_t stream) {
+    return with_sizes(dtype, p.c.D, [&](auto dt, auto nd) {
+        hipLaunchKernelGGL((paged_append_kernel<decltype(dt)::value, decltype(nd)::value>), dim3(2u * p.c.H * p.blocks * p.t.B), dim3(64), 0, stream, p);
+        return hipGetLastError();
+    });
+}
+hipError_t launch_paged_gather(const PagedGatherParams &p, int dtype, hipStream_t stream) {
+    const unsigned blocks = ((unsigned)p.length + 31) / 32;
+    return with_sizes(dtype, p.c.D, [&](auto dt, auto nd) {
+        hipLaunchKernelGGL((paged_gather_kernel<decltype(dt)::value, decltype(nd)::value>), dim3(2u * p.c.H * blocks * p.t.B), dim3(64), 0, stream, p);
+        return hipGetLastError();
+    });
+}
+hipError_t launch_paged_copy(const PagedCopyParams &p, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_copy_kernel, dim3((unsigned)p.n * p.c.H), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+hipError_t launch_paged_fork(const PagedForkParams &p, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_fork_kernel, dim3((unsigned)p.n * p.c.H), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+hipError_t launch_paged_plan(const PagedPlanParams &p, hipStream_t stream) {
+    const int smem = ((p.pages + 31) / 32) * 4;
+    static unsigned long long attr_done = 0;
+    if (const hipError_t e = allow_dynamic_smem(paged_plan_kernel, kPagedMostPages / 8, attr_done); e != hipSuccess) return e;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), smem, stream, p);
+    return hipGetLastError();
+}
+hipError_t launch_paged_compact(const PagedCompactParams &p, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_compact_kernel, dim3(2048), dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+}  // namespace sa

@@ -6,12 +6,15 @@
 
 #include <chrono>
 
+#include "api_common.h"
 #include "kernels.h"
 #include "sparseattn.h"
 
 namespace {
-
 thread_local char g_error[512] = "";
+}
+
+namespace sa {
 
 int fail(int code, const char *fmt, ...) {
     va_list ap;
@@ -21,16 +24,6 @@ int fail(int code, const char *fmt, ...) {
     return code;
 }
 
-int log2_exact(int x) {  // -1 unless x is a power of two
-    if (x <= 0 || (x & (x - 1))) return -1;
-    int l = 0;
-    while ((1 << l) < x) l++;
-    return l;
-}
-
-// The number of a launch whose workgroups count their arrivals (arrives_last): its upper 56 bits, no two in a process alike.
-// The first one depends on the time the process took it and on where it lies in memory, so that memory which another
-// process left behind holds none of them.
 uint64_t next_launch_tag() {
     static uint64_t last = [] {
         uint64_t x = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() ^ (uint64_t)(uintptr_t)&g_error;
@@ -38,6 +31,20 @@ uint64_t next_launch_tag() {
         return x << 8;
     }();
     return __atomic_add_fetch(&last, 256, __ATOMIC_RELAXED);
+}
+
+}  // namespace sa
+
+namespace {
+
+using sa::fail;
+using sa::next_launch_tag;
+
+int log2_exact(int x) {  // -1 unless x is a power of two
+    if (x <= 0 || (x & (x - 1))) return -1;
+    int l = 0;
+    while ((1 << l) < x) l++;
+    return l;
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
