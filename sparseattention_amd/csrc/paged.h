@@ -6,7 +6,7 @@
 // Inside a block the codes lie in the order in which the attention's matrix instructions take them, so that a wave reads a
 // block with D / 32 loads of 1 KiB each, straight into their operands:
 //   K  16 bytes of lane (key = lane % 32, hh = lane / 32) of piece c: d = 32 c + 16 hh ..+15 of that key
-//   V  16 bytes of lane (d % 32 = lane % 32, hh) of piece d / 32: keys 16 (j / 8) + 8 (j % 8 / 4) + 4 hh + j % 4, j = 0..15
+//   V  16 bytes of lane (d % 32 = lane % 32, hh) of piece d / 32: keys 16 (j / 4 % 2) + 8 (j / 8) + 4 hh + j % 4, j = 0..15
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -92,7 +92,7 @@ struct PagedDecodeParams {
     float *lse;  // or null
     int64_t qs[3], os[3], lses[3];  // b, h, row strides in elements
     const int32_t *counts;  // valid query rows of each sequence, or null: Sq
-    int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT tiles of 32
+    int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT tiles of 16 (all of them) or 32
     int window;             // or 0
     // tile lists, tile = page, all null: every key that causality and window leave
     const int32_t *full_ids, *full_lens, *part_ids, *part_lens;
@@ -101,7 +101,20 @@ struct PagedDecodeParams {
     int64_t pks[2];
     int nK;
     float scale;  // softmax scale / ln 2
+    // The launch's workgroups, the fewest chunks that one of them takes, and what planes that several of them share are added up by:
+    //   ws        [groups][2][part_rows][D + 2] floats: unnormalised rows, reference value and sum of each
+    //   arrivals  [planes + groups] words (all_arrived), the number of the launch
+    int groups, least, part_rows;
+    float *ws;
+    uint64_t *arrivals;
+    uint64_t tag;
 };
+constexpr int kPagedMostParts = 64;  // of a plane (all_arrived looks at one word per lane)
+struct PagedDecodePlan {
+    int groups, least, part_rows;
+    size_t parts_bytes, bytes;
+};
+PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus);
 hipError_t launch_paged_decode(const PagedDecodeParams &p, int dtype, hipStream_t stream);
 
 }  // namespace sa

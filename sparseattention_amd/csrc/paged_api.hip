@@ -57,6 +57,18 @@ int grid_fits(const char *who, int64_t workgroups) {
     return workgroups <= 0x7fffffff ? SA_OK : fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 workgroups", who);
 }
 
+constexpr int kMostRows = 1 << 20;
+
+// Compute units of the current device.
+int compute_units() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    return n;
+}
+
 #define SA_TRY(x)                              \
     do {                                       \
         if (const int rc_ = (x)) return rc_;   \
@@ -187,7 +199,13 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
     return launched(who, sa::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
 }
 
-size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) { return 0; }
+size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
+    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > 32 || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
+        (int64_t)Hq / H * Sq > kMostRows)
+        return 0;
+    const int R = Hq / H * Sq;
+    return sa::paged_decode_plan((int64_t)B * H * ((R + 31) / 32), R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units()).bytes;
+}
 
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
                                      const int64_t page_table_strides[2], const int32_t *lens, const int32_t *counts, int pages_per_sequence, void *o,
@@ -244,12 +262,23 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     p.counts = counts;
     p.G = Hq / p.c.H;
     p.Sq = Sq;
-    if ((int64_t)p.G * Sq > (1 << 24)) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^24 rows per K/V head", who);
+    if ((int64_t)p.G * Sq > kMostRows) return fail(SA_ERR_UNSUPPORTED, "%s: more than %d rows per K/V head", who, kMostRows);
     p.R = p.G * Sq;
     p.RT = (p.R + 31) / 32;
     p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
     p.scale = sm_scale_log2;
-    SA_TRY(grid_fits(who, (int64_t)B * p.c.H * p.RT));
+    const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)pages_per_sequence << p.c.lper;
+    if (planes > (1 << 24) || (int64_t)p.c.H * p.RT * chunks > 0x7fffffff)
+        return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
+    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
+        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, plan.bytes, workspace ? workspace_bytes : (size_t)0);
+    p.groups = plan.groups;
+    p.least = plan.least;
+    p.part_rows = plan.part_rows;
+    p.ws = static_cast<float *>(workspace);
+    p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + plan.parts_bytes);
+    p.tag = sa::next_launch_tag() | 1;
     return launched(who, sa::launch_paged_decode(p, dtype, static_cast<hipStream_t>(stream)));
 }
 

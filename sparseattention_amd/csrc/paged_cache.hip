@@ -144,7 +144,7 @@ __global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParam
         for (int g = 0; g < NG; g++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                const int t = 16 * (j >> 3) + 8 * ((j >> 2) & 1) + 4 * hh + (j & 3);
+                const int t = 16 * ((j >> 2) & 1) + 8 * (j >> 3) + 4 * hh + (j & 3);
                 w[16 * g + j] = t >= a && t < z ? *(const uint32_t *)(x + t * row + 64 * g + 2 * l32) : 0u;
             }
     }
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParam
         uint32_t isnew[4], isold[4], any = 0u, all = ~0u;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int base = 16 * (i >> 1) + 8 * (i & 1) + 4 * hh;
+            const int base = 16 * (i & 1) + 8 * (i >> 1) + 4 * hh;
             isnew[i] = bytes_in(base, a, z);
             isold[i] = grows ? bytes_in(base, 0, held) : 0u;
             any |= isnew[i] | isold[i];
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64) void paged_gather_kernel(const PagedGatherParam
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int base = 16 * (i >> 1) + 8 * (i & 1) + 4 * hh;
+                const int base = 16 * (i & 1) + 8 * (i >> 1) + 4 * hh;
                 const uint32_t a0 = X::cvt_lo(u[0][i], scale), a1 = X::cvt_hi(u[0][i], scale);
                 const uint32_t b0 = X::cvt_lo(u[1][i], scale), b1 = X::cvt_hi(u[1][i], scale);
                 const uint32_t v[4] = {(a0 & 0xffffu) | (b0 << 16), (a0 >> 16) | (b0 & 0xffff0000u), (a1 & 0xffffu) | (b1 << 16),

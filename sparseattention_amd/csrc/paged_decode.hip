@@ -18,6 +18,9 @@ namespace {
 
 constexpr int kWaves = 4;
 
+// Workgroups that a compute unit holds (a wave of each per SIMD).
+constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 4 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : rows == 16 ? 2 : 1; }
+
 template <int DT>
 struct Codes;  // eight codes as an operand, times a power of two
 template <>
@@ -41,241 +44,561 @@ struct Codes<1> {
 
 // 0x80 in every byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t nan_ones(uint32_t w) { return (nan_bytes(w) >> 7) * 0x38u; }  // the code of 1 for NaN, else 0
+__device__ __forceinline__ uint32_t no_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); }
 
 __device__ __forceinline__ float scale_of(float s) {  // (as the cache's kernels write them; anything else is brought into range)
     const int e = (int)((__float_as_uint(s) >> 23) & 0xffu);
     return __uint_as_float((uint32_t)min(max(e, 127 + kScaleExpMin), 127 + kScaleExpMax) << 23);
 }
 
-template <int DT, int ND, bool LISTS>
-__global__ __launch_bounds__(kWaves * 64, ND == 8 ? 1 : 2) void paged_decode_kernel(const PagedDecodeParams p) {
-    using E = Elem<DT>;
-    constexpr int D = 32 * ND, NC = 2 * ND, PST = D + 2;
-    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][32][PST]
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int plane = (int)(blockIdx.x / (unsigned)p.RT), rt = (int)(blockIdx.x - (unsigned)plane * (unsigned)p.RT);
-    const int b = plane / p.c.H, h = plane - b * p.c.H;
+// ---- who does what ----
+// The work is a row of chunks: units (a sequence, with lists a sequence and K/V head) one behind the other, of every unit its planes (head,
+// tile of 32 rows), of every plane its T chunks, at least one, so that planes without keys are written too.  Every workgroup takes
+// an equal piece of the row, whatever the lengths: segments, each of one plane.  A plane that lies in several workgroups' pieces is
+// added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself, by a sum over the units.
+struct Unit {
+    int T0, T;  // first chunk, chunks (0: none)
+};
+template <bool LISTS>
+__device__ __forceinline__ Unit unit_of(const PagedDecodeParams &p, int u) {
+    const int b = LISTS ? u / p.c.H : u;
     const int lP = p.c.lper + 5;
-
     const int len = min(max(p.t.lens[b], 0), p.t.width << lP);
     const int cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.Sq) : p.Sq;
-    // this lane's row: query i of query head g
-    const int row = 32 * rt + l32, g = row / p.Sq, i = row - g * p.Sq;
-    const bool live = row < p.R && i < cnt;
-    // without lists it sees the keys from `lo` to `hi`
-    const int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
-
-    u32x4 qf[NC];
-    {
-        const uint16_t *qp = p.q + b * p.qs[0] + (live ? (h * p.G + g) * p.qs[1] + i * p.qs[2] : 0) + 16 * hh;
-#pragma unroll
-        for (int c = 0; c < NC; c++) qf[c] = live ? *(const u32x4 *)(qp + 32 * (c >> 1) + 8 * (c & 1)) : u32x4{0u, 0u, 0u, 0u};
-    }
-
-    const int32_t *fid = nullptr, *pid = nullptr;
-    int F = 0, T0 = 0, T1 = 0;  // chunks [T0, T1): of the sequence, or of the list
+    if (cnt == 0 || len == 0) return {0, 0};
     if constexpr (LISTS) {
-        fid = p.full_ids + b * p.fis[0] + h * p.fis[1];
-        pid = p.part_ids + b * p.pis[0] + h * p.pis[1];
-        F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
-        T1 = (F + min(max(p.part_lens[b * p.pls[0] + h * p.pls[1]], 0), p.nK - F)) << p.c.lper;
-        if (cnt == 0) T1 = 0;
-    } else if (cnt > 0) {
-        T1 = (len + 31) >> 5;
-        if (p.window > 0) T0 = max(len - cnt - p.window + 1, 0) >> 5;
+        const int h = u - b * p.c.H;
+        const int F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
+        return {0, (F + min(max(p.part_lens[b * p.pls[0] + h * p.pls[1]], 0), p.nK - F)) << p.c.lper};
+    } else {
+        const int T0 = p.window > 0 ? max(len - cnt - p.window + 1, 0) >> 5 : 0;
+        return {T0, ((len + 31) >> 5) - T0};
     }
-    const uint8_t *const bits = LISTS ? p.packed + b * p.pks[0] + h * p.pks[1] + ((int64_t)i << (lP - 3)) : nullptr;
+}
 
-    float m_ref = 0.f, raise_above = -3.0e38f, l = 0.f;
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {  // (wave-uniform)
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)((uint64_t)x >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t sum_up_to(int64_t x, int lane) {  // over lanes 0 .. lane
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)x, s), hi = (uint32_t)__shfl_up((int)((uint64_t)x >> 32), s);
+        if (lane >= s) x += (int64_t)(((uint64_t)hi << 32) | lo);
+    }
+    return x;
+}
+
+// The products of a tile of ROWS query rows, S^T = K Q^T (32 keys) and O^T += V^T P^T, on 32 x 32 or 16 x 16 matrix instructions.
+// A lane has its row's share: row lane % ROWS, group lane / ROWS.
+template <int DT, int ND, int ROWS>
+struct Tile;
+template <int DT, int ND>
+struct Tile<DT, ND, 32> {
+    using E = Elem<DT>;
+    static constexpr int NS = 16, NQ = 2 * ND, NA = 16 * ND;  // scores, registers of 8 queries' elements, output elements
+    static __device__ __forceinline__ int d_of_q(int i, int g) { return 32 * (i >> 1) + 16 * g + 8 * (i & 1); }
+    static __device__ __forceinline__ int key(int e, int g) { return 8 * (e >> 2) + 4 * g + (e & 3); }
+    static __device__ __forceinline__ int d_of(int e, int g) { return 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * g + (e & 3); }
+    struct Operands {
+        u32x4 k[ND], v[ND];
+    };
+    static __device__ __forceinline__ void load_k(Operands &c, const uint8_t *k, int lane) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) c.k[d] = __builtin_nontemporal_load((const u32x4 *)(k + 1024 * d + 16 * lane));
+    }
+    static __device__ __forceinline__ void load_v(Operands &c, const uint8_t *v, int lane) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) c.v[d] = __builtin_nontemporal_load((const u32x4 *)(v + 1024 * d + 16 * lane));
+    }
+    static __device__ __forceinline__ void scores(const Operands &c, const u32x4 (&q)[NQ], float (&s)[NS]) {
+        f32x16 x;
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) x = E::mfma(Codes<DT>::take(c.k[i >> 1][2 * (i & 1)], c.k[i >> 1][2 * (i & 1) + 1], 1.0f), q[i], x);
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = x[e];
+    }
     f32x16 acc[ND];
+    // f(register of four codes) for every one
+    template <class F>
+    static __device__ __forceinline__ void each_v(Operands &c, F &&f) {
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
-
-    for (int t = T0 + wave; t < T1; t += kWaves) {
-        int key0, slot = -1;  // first key of the chunk; slot of a PARTIAL tile
-        if constexpr (LISTS) {
-            const int e = t >> p.c.lper;
-            const int tile = __builtin_amdgcn_readfirstlane(e < F ? fid[(int64_t)e * p.fis[2]] : pid[(int64_t)(e - F) * p.pis[2]]);
-            if (tile < 0 || tile >= p.nK) continue;
-            if (e >= F) slot = e - F;
-            key0 = (tile << lP) + ((t & ((1 << p.c.lper) - 1)) << 5);
-        } else {
-            key0 = t << 5;
-        }
-        if (key0 >= len) continue;
-        const int page = __builtin_amdgcn_readfirstlane(p.t.ids[b * p.t.s0 + (key0 >> lP) * p.t.s1]);
-        if (page < 0 || page >= p.c.pages) continue;  // nothing attends to keys of a page that does not exist
-        const int64_t at = (((int64_t)page * p.c.H + h) << p.c.lper) + ((key0 >> 5) & ((1 << p.c.lper) - 1));
-        const u32x4 *const kp = (const u32x4 *)(p.c.k + at * (1024 * ND)) + lane, *const vp = (const u32x4 *)(p.c.v + at * (1024 * ND)) + lane;
-        u32x4 kf[ND], vf[ND];
+            for (int e = 0; e < 4; e++) f(c.v[d], e);
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int c = 0; c < ND; c++) kf[c] = kp[64 * c];
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int c = 0; c < ND; c++) vf[c] = vp[64 * c];
-        const float ks = scale_of(p.c.k_scales[at]) * p.scale, vs = scale_of(p.c.v_scales[at]);
-
-        f32x16 s;
+            for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
+    }
+    __device__ __forceinline__ void scale(float a) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = 0.f;
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int c = 0; c < NC; c++) s = E::mfma(Codes<DT>::take(kf[c >> 1][2 * (c & 1)], kf[c >> 1][2 * (c & 1) + 1], 1.0f), qf[c], s);
-
-        // which keys the lane's row attends to, key k in bit k; `cut`: not all of them for every row
-        uint32_t see = ~0u;
-        bool cut = key0 + 32 > len;
-        if (cut) see = (1u << (len - key0)) - 1u;
-        if constexpr (LISTS) {
-            if (slot >= 0) {
-                cut = true;
-                see &= *(const uint32_t *)(bits + ((int64_t)slot * p.Sq << (lP - 3)) + (((key0 >> 5) & ((1 << p.c.lper) - 1)) << 2));
-            }
-        } else {
-            if (key0 + 31 > len - cnt || (p.window > 0 && key0 <= len - 1 - p.window)) {
-                cut = true;
-                const int upto = hi - key0, from = lo - key0;  // bits from .. upto
-                see = upto < 0 ? 0u : see & (upto >= 31 ? ~0u : (2u << upto) - 1u);
-                see = from > 31 ? 0u : from > 0 ? see & ~((1u << from) - 1u) : see;
-            }
-        }
-        if (cut) {
-            const uint32_t w = see >> (4 * hh);
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                if (((w >> (8 * (e >> 2) + (e & 3))) & 1u) == 0u) s[e] = kNegInf;
-        }
-        float mx = kNegInf;
-#pragma unroll
-        for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[e]);
-        mx = half_swap_max(mx) * ks;
-        const float rel = mx - m_ref;
-        const bool raise = rel > raise_above;  // false for rows without an attended key so far (mx = -inf)
-        if (__builtin_amdgcn_ballot_w64(raise) != 0ull) {
-            const float a = raise ? (raise_above == kMaxSlack ? __builtin_amdgcn_exp2f(-rel) : 0.f) : 1.f;
-            m_ref = raise ? mx : m_ref;
-            raise_above = raise ? kMaxSlack : raise_above;
-            l *= a;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[d][e] *= a;
-        }
-        uint32_t pw[8];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], ks, -m_ref)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], ks, -m_ref));
-            l += x + y;
-            pw[e >> 1] = E::pack2(x, y);
-        }
-        // A value that is NaN reaches the rows that attend to it and no others: 0 * NaN would be NaN in the product.  Looked for
-        // where some row leaves a key out.
-        if (cut) {
-            uint32_t any = 0u;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) any |= nan_bytes(vf[d][e]);
-            if (__builtin_amdgcn_ballot_w64(any != 0u) != 0ull) {
-                const uint32_t w = see >> (4 * hh);
-                uint32_t att[8];  // 1 where the row attends to the key
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int at0 = 8 * (e >> 2) + (e & 3);
-                    att[e >> 1] = E::pack2((w >> at0) & 1u ? 1.f : 0.f, (w >> (at0 + 1)) & 1u ? 1.f : 0.f);
-                }
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    f32x16 hits;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) hits[e] = 0.f;
-#pragma unroll
-                    for (int kc = 0; kc < 2; kc++) {
-                        uint32_t one[2];
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const uint32_t n = nan_bytes(vf[d][2 * kc + e]) >> 7;  // 1 in every NaN byte
-                            one[e] = n * 0x38u;                                    // (the code of 1)
-                            vf[d][2 * kc + e] &= ~(n * 0xffu);
-                        }
-                        hits = E::mfma(Codes<DT>::take(one[0], one[1], 1.0f), u32x4{att[4 * kc], att[4 * kc + 1], att[4 * kc + 2], att[4 * kc + 3]}, hits);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; e++) acc[d][e] = hits[e] > 0.f ? __builtin_nanf("") : acc[d][e];
-                }
-            }
-        }
+            for (int e = 0; e < 16; e++) acc[d][e] *= a;
+    }
+    __device__ __forceinline__ void add(const Operands &c, const uint32_t (&pw)[NS / 2], float vs) {
 #pragma unroll
         for (int kc = 0; kc < 2; kc++) {
             const u32x4 pk4 = u32x4{pw[4 * kc], pw[4 * kc + 1], pw[4 * kc + 2], pw[4 * kc + 3]};
 #pragma unroll
-            for (int d = 0; d < ND; d++) acc[d] = E::mfma(Codes<DT>::take(vf[d][2 * kc], vf[d][2 * kc + 1], vs), pk4, acc[d]);
+            for (int d = 0; d < ND; d++) acc[d] = E::mfma(Codes<DT>::take(c.v[d][kc], c.v[d][2 + kc], vs), pk4, acc[d]);
+        }
+    }
+    // Rows that attend to a NaN become NaN, the NaN codes 0.  att: 1 where the row attends.
+    __device__ __forceinline__ void poison(Operands &c, const uint32_t (&att)[NS / 2]) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            f32x16 hits;
+#pragma unroll
+            for (int e = 0; e < 16; e++) hits[e] = 0.f;
+#pragma unroll
+            for (int kc = 0; kc < 2; kc++) {
+                const u32x4 at4 = u32x4{att[4 * kc], att[4 * kc + 1], att[4 * kc + 2], att[4 * kc + 3]};
+                hits = E::mfma(Codes<DT>::take(nan_ones(c.v[d][kc]), nan_ones(c.v[d][2 + kc]), 1.0f), at4, hits);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[d][e] = hits[e] > 0.f ? __builtin_nanf("") : acc[d][e];
+#pragma unroll
+            for (int e = 0; e < 4; e++) c.v[d][e] = no_nan(c.v[d][e]);
+            __builtin_amdgcn_sched_barrier(0);  // (one tile's registers at a time)
+        }
+    }
+    __device__ __forceinline__ float get(int e) const { return acc[e >> 4][e & 15]; }
+    static __device__ __forceinline__ float row_max(float x) { return half_swap_max(x); }
+    static __device__ __forceinline__ float row_sum(float x) { return x + __shfl_xor(x, 32); }
+};
+template <int DT, int ND>
+struct Tile<DT, ND, 16> {
+    using E = Elem<DT>;
+    static constexpr int NS = 8, NQ = ND, NA = 8 * ND;
+    static __device__ __forceinline__ int d_of_q(int i, int g) { return 64 * (i >> 1) + 16 * g + 8 * (i & 1); }
+    static __device__ __forceinline__ int key(int e, int g) { return 16 * (e >> 2) + 4 * g + (e & 3); }
+    static __device__ __forceinline__ int d_of(int e, int g) { return 16 * (e >> 2) + 4 * g + (e & 3); }
+    struct Operands {
+        u32x4 k[ND];      // [16 keys][64 d]
+        u32x2 v[2 * ND];  // [16 d]
+    };
+    static __device__ __forceinline__ void load_k(Operands &c, const uint8_t *k, int lane) {
+        const int l = lane & 15, g = lane >> 4;
+        k += 1024 * (g >> 1) + 16 * (32 * (g & 1) + l);
+#pragma unroll
+        for (int i = 0; i < ND; i++) c.k[i] = __builtin_nontemporal_load((const u32x4 *)(k + 2048 * (i >> 1) + 256 * (i & 1)));
+    }
+    static __device__ __forceinline__ void load_v(Operands &c, const uint8_t *v, int lane) {
+        const int l = lane & 15, g = lane >> 4;
+        v += 16 * (32 * (g & 1) + l) + 8 * (g >> 1);
+#pragma unroll
+        for (int i = 0; i < 2 * ND; i++) c.v[i] = __builtin_nontemporal_load((const u32x2 *)(v + 1024 * (i >> 1) + 256 * (i & 1)));
+    }
+    static __device__ __forceinline__ void scores(const Operands &c, const u32x4 (&q)[NQ], float (&s)[NS]) {
+        f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const u32x4 k = c.k[2 * (i >> 1) + t];
+                x[t] = E::mfma16(Codes<DT>::take(k[2 * (i & 1)], k[2 * (i & 1) + 1], 1.0f), q[i], x[t]);
+            }
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] = x[e >> 2][e & 3];
+    }
+    f32x4 acc[2 * ND];
+    template <class F>
+    static __device__ __forceinline__ void each_v(Operands &c, F &&f) {
+#pragma unroll
+        for (int d = 0; d < 2 * ND; d++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) f(c.v[d], e);
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int d = 0; d < 2 * ND; d++) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void scale(float a) {
+#pragma unroll
+        for (int d = 0; d < 2 * ND; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[d][e] *= a;
+    }
+    __device__ __forceinline__ void add(const Operands &c, const uint32_t (&pw)[NS / 2], float vs) {
+        const u32x4 pk4 = u32x4{pw[0], pw[1], pw[2], pw[3]};
+#pragma unroll
+        for (int d = 0; d < 2 * ND; d++) acc[d] = E::mfma16(Codes<DT>::take(c.v[d].x, c.v[d].y, vs), pk4, acc[d]);
+    }
+    __device__ __forceinline__ void poison(Operands &c, const uint32_t (&att)[NS / 2]) {
+        const u32x4 at4 = u32x4{att[0], att[1], att[2], att[3]};
+#pragma unroll
+        for (int d = 0; d < 2 * ND; d++) {
+            const f32x4 hits = E::mfma16(Codes<DT>::take(nan_ones(c.v[d].x), nan_ones(c.v[d].y), 1.0f), at4, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[d][e] = hits[e] > 0.f ? __builtin_nanf("") : acc[d][e];
+            c.v[d].x = no_nan(c.v[d].x);
+            c.v[d].y = no_nan(c.v[d].y);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __device__ __forceinline__ float get(int e) const { return acc[e >> 2][e & 3]; }
+    static __device__ __forceinline__ float row_max(float x) {
+        const uint32_t u = __float_as_uint(x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+    }
+    static __device__ __forceinline__ float row_sum(float x) {
+        x += __shfl_xor(x, 16);
+        return x + __shfl_xor(x, 32);
+    }
+};
+
+template <int DT, int ND, int ROWS, bool LISTS>
+__global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
+    using E = Elem<DT>;
+    using X = Tile<DT, ND, ROWS>;
+    constexpr int D = 32 * ND, PST = D + 2;
+    extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][ROWS][PST]
+    const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lP = p.c.lper + 5, sub_mask = (1 << p.c.lper) - 1;
+
+    // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in ----
+    const int U = LISTS ? p.t.B * p.c.H : p.t.B, M = LISTS ? p.RT : p.c.H * p.RT;  // units, planes of each
+    const int per_lane = (U + 63) >> 6;
+    int64_t mine = 0;
+    int longest = 0;
+    for (int j = 0; j < per_lane; j++) {
+        const int u = lane * per_lane + j;
+        const int T = u < U ? max(unit_of<LISTS>(p, u).T, 1) : 0;
+        mine += T;
+        longest = max(longest, T);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) longest = max(longest, __shfl_xor(longest, s));
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    const int64_t upto = sum_up_to(mine, lane), total = of_lane(upto, 63) * M;
+    int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    share = max(max(share, (int64_t)p.least), (int64_t)((longest + kPagedMostParts - 3) / (kPagedMostParts - 2)));
+    const int64_t x0 = share * blockIdx.x, x1 = min(x0 + share, total);
+    if (x0 >= x1) return;
+    int u;
+    int64_t base;  // of unit u
+    {
+        const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < upto * M)) - 1;  // the lane whose units hold x0
+        base = of_lane(upto - mine, at) * M;
+        u = at * per_lane;
+        for (;; u++) {  // (U <= 64: at once)
+            const int64_t next = base + (int64_t)max(unit_of<LISTS>(p, u).T, 1) * M;
+            if (x0 < next) break;
+            base = next;
         }
     }
 
-    // ---- the waves' parts ----
-    l += __shfl_xor(l, 32);
-    {
-        float *mine = part + (wave * 32 + l32) * PST;
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) mine[32 * d + 8 * (e >> 2) + 4 * hh + (e & 3)] = acc[d][e];
-        if (hh == 0) {
-            // (a row whose only scores are NaN has a sum and no reference value)
-            mine[D] = raise_above == kMaxSlack ? m_ref : l == 0.f ? kNegInf : 0.f;
-            mine[D + 1] = l;
+    int64_t x = x0;
+    while (x < x1) {
+        const Unit unit = unit_of<LISTS>(p, u);
+        const int T = max(unit.T, 1);
+        const int m = (int)((x - base) / T), off = (int)(x - base - (int64_t)m * T);
+        const int n = (int)min((int64_t)(T - off), x1 - x);  // chunks off .. off + n - 1 of this plane
+        const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + m : m;
+        const int h = hr / p.RT, rt = hr - h * p.RT;
+        const int plane = (b * p.c.H + h) * p.RT + rt;
+        const int64_t plane_at = x - off;
+        x += n;
+        if (m + 1 == M && off + n == T) {
+            base += (int64_t)T * M;
+            u++;
         }
-    }
-    __syncthreads();
-    constexpr int LPR = D / 4;  // lanes per row
-    for (int x = tid; x < 32 * LPR; x += kWaves * 64) {
-        const int r = x / LPR, d0 = 4 * (x - r * LPR), at = 32 * rt + r;
-        if (at >= p.R) break;
-        float M = kNegInf, L = 0.f;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < kWaves; w++) M = fmaxf(M, part[(w * 32 + r) * PST + D]);
-        if (M != kNegInf)
-            for (int w = 0; w < kWaves; w++) {
-                const float *pp = part + (w * 32 + r) * PST;
-                const float a = pp[D] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(pp[D] - M);
-                L += a * pp[D + 1];
+
+        const int len = min(max(p.t.lens[b], 0), p.t.width << lP);
+        const int cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.Sq) : p.Sq;
+        // this lane's row: query i of query head g
+        const int row = ROWS * rt + lrow, g = row / p.Sq, i = row - g * p.Sq;
+        const bool live = row < p.R && i < cnt;
+        // without lists it sees the keys from `lo` to `hi`
+        const int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
+
+        u32x4 qf[X::NQ];
+        {
+            const uint16_t *qp = p.q + b * p.qs[0] + (live ? (h * p.G + g) * p.qs[1] + i * p.qs[2] : 0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum[e] += a * pp[d0 + e];
+            for (int c = 0; c < X::NQ; c++) qf[c] = live ? *(const u32x4 *)(qp + X::d_of_q(c, lgrp)) : u32x4{0u, 0u, 0u, 0u};
+        }
+        const int32_t *fid = nullptr, *pid = nullptr;
+        int F = 0;
+        if constexpr (LISTS) {
+            fid = p.full_ids + b * p.fis[0] + h * p.fis[1];
+            pid = p.part_ids + b * p.pis[0] + h * p.pis[1];
+            F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
+        }
+        const uint8_t *const bits = LISTS ? p.packed + b * p.pks[0] + h * p.pks[1] + ((int64_t)i << (lP - 3)) : nullptr;
+
+        float m_ref = 0.f, raise_above = -3.0e38f, l = 0.f;
+        X out_rows;
+        out_rows.clear();
+
+        // This wave's chunks are off + wave + 4 j, j < nw.  Lane j of a round of 64 of them finds where chunk j lies.
+        const int nw = (n - wave + kWaves - 1) / kWaves;
+        struct Places {
+            int block, tile, slot;  // block of the pool or -1; with lists the tile, and the slot of a PARTIAL one or -1
+            float ks, vs;
+        };
+        auto places = [&](int j0) {
+            Places r{-1, 0, -1, 0.f, 0.f};
+            const int j = j0 + lane;
+            const int t = unit.T0 + off + wave + kWaves * j;
+            if (j < nw && unit.T > 0) {
+                int tile = t >> p.c.lper;
+                if constexpr (LISTS) {
+                    if (tile >= F) r.slot = tile - F;
+                    tile = tile < F ? fid[(int64_t)tile * p.fis[2]] : pid[(int64_t)(tile - F) * p.pis[2]];
+                    if (tile < 0 || tile >= p.nK) tile = p.t.width;
+                }
+                const int sub = t & sub_mask;
+                if (tile < p.t.width) {
+                    r.tile = tile;
+                    const int page = p.t.ids[b * p.t.s0 + tile * p.t.s1];
+                    // (nothing attends to keys of a page that does not exist)
+                    if ((tile << lP) + (sub << 5) < len && page >= 0 && page < p.c.pages) r.block = ((page * p.c.H + h) << p.c.lper) + sub;
+                }
             }
-        const int gg = at / p.Sq, ii = at - gg * p.Sq, head = h * p.G + gg;
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        if (ii >= cnt) sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p.lse != nullptr && d0 == 0)
-            p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
-                ii >= cnt || L == 0.f ? kNegInf : (M + __builtin_amdgcn_logf(L)) * 0.69314718056f;
-        *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(sum.x * inv, sum.y * inv), E::pack2(sum.z * inv, sum.w * inv)};
+            const int at = max(r.block, 0);
+            r.ks = p.c.k_scales[at];
+            r.vs = p.c.v_scales[at];
+            return r;
+        };
+        // What is requested next takes the registers of what has just gone into a product: K of the next chunk is on its way during
+        // the softmax and the second product, V behind it.  More registers for that would cost waves, which hide as much.
+        struct Chunk {
+            int block, key0, slot;
+            uint32_t bits;
+        };
+        auto chunk = [&](const Places &at, int j) {
+            const int t = unit.T0 + off + wave + kWaves * j;
+            Chunk c{__builtin_amdgcn_readlane(at.block, j & 63), t << 5, -1, 0u};
+            if constexpr (LISTS) {
+                c.key0 = (__builtin_amdgcn_readlane(at.tile, j & 63) << lP) + ((t & sub_mask) << 5);
+                c.slot = __builtin_amdgcn_readlane(at.slot, j & 63);
+                c.bits = *(const uint32_t *)(bits + ((int64_t)max(c.slot, 0) * p.Sq << (lP - 3)) + ((t & sub_mask) << 2));
+            }
+            return c;
+        };
+        typename X::Operands x;
+        auto request_k = [&](const Chunk &c) { X::load_k(x, p.c.k + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
+        auto request_v = [&](const Chunk &c) { X::load_v(x, p.c.v + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
+        // (of a round of 64 chunks: their places; of the round behind it, on their way)
+        Places here = places(0), next = places(64);
+        Chunk c = chunk(here, 0);
+        if (nw > 0) {
+            request_k(c);
+            request_v(c);
+        }
+        for (int j = 0; j < nw; j++) {
+            const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.ks), j & 63))) * p.scale;
+            const float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.vs), j & 63)));
+            if (((j + 1) & 63) == 0 && j + 1 < nw) {
+                here = next;
+                next = places(j + 65);  // (none behind the last chunk)
+            }
+            const Chunk nc = chunk(here, min(j + 1, nw - 1));  // (behind the last one: that one again)
+            const int key0 = c.key0;
+            float s[X::NS];
+            X::scores(x, qf, s);
+            request_k(nc);
+
+            // which keys the lane's row attends to, key k in bit k; `cut`: not all of them for every row
+            // (a chunk that does not exist goes through as one that no row attends to: a way around it doubles the registers)
+            const int left = c.block < 0 ? 0 : len - key0;
+            uint32_t see = ~0u;
+            bool cut = left < 32;
+            if (cut) see = (1u << left) - 1u;
+            if constexpr (LISTS) {
+                if (c.slot >= 0) {
+                    cut = true;
+                    see &= c.bits;
+                }
+            } else {
+                if (key0 + 31 > len - cnt || (p.window > 0 && key0 <= len - 1 - p.window)) {
+                    cut = true;
+                    const int last = hi - key0, from = lo - key0;  // bits from .. last
+                    see = last < 0 ? 0u : see & (last >= 31 ? ~0u : (2u << last) - 1u);
+                    see = from > 31 ? 0u : from > 0 ? see & ~((1u << from) - 1u) : see;
+                }
+            }
+            if (cut) {
+#pragma unroll
+                for (int e = 0; e < X::NS; e++)
+                    if (((see >> X::key(e, lgrp)) & 1u) == 0u) s[e] = kNegInf;
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int e = 0; e < X::NS; e++) mx = fmaxf(mx, s[e]);
+            mx = X::row_max(mx) * ks;
+            const float rel = mx - m_ref;
+            const bool raise = rel > raise_above;  // false for rows without an attended key so far (mx = -inf)
+            if (__builtin_amdgcn_ballot_w64(raise) != 0ull) {
+                const float a = raise ? (raise_above == kMaxSlack ? __builtin_amdgcn_exp2f(-rel) : 0.f) : 1.f;
+                m_ref = raise ? mx : m_ref;
+                raise_above = raise ? kMaxSlack : raise_above;
+                l *= a;
+                out_rows.scale(a);
+            }
+            uint32_t pw[X::NS / 2];
+#pragma unroll
+            for (int e = 0; e < X::NS; e += 2) {
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], ks, -m_ref)), z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], ks, -m_ref));
+                l += y + z;
+                pw[e >> 1] = E::pack2(y, z);
+            }
+            // A value that is NaN reaches the rows that attend to it and no others: 0 * NaN would be NaN in the product.  Looked
+            // for where some row leaves a key out.
+            if (cut) {
+                uint32_t any = 0u;
+                X::each_v(x, [&](auto &v, int e) { any |= nan_bytes(v[e]); });
+                if (__builtin_amdgcn_ballot_w64(any != 0u) != 0ull) {
+                    uint32_t att[X::NS / 2];  // 1 where the row attends to the key
+#pragma unroll
+                    for (int e = 0; e < X::NS; e += 2)
+                        att[e >> 1] = E::pack2((see >> X::key(e, lgrp)) & 1u ? 1.f : 0.f, (see >> X::key(e + 1, lgrp)) & 1u ? 1.f : 0.f);
+                    out_rows.poison(x, att);
+                }
+            }
+            out_rows.add(x, pw, vs);
+            request_v(nc);
+            c = nc;
+        }
+
+        // ---- the waves' parts, added up in LDS ----
+        l = X::row_sum(l);
+        {
+            float *to = part + (wave * ROWS + lrow) * PST;
+#pragma unroll
+            for (int e = 0; e < X::NA; e++) to[X::d_of(e, lgrp)] = out_rows.get(e);
+            if (lgrp == 0) {
+                // (a row whose only scores are NaN has a sum and no reference value)
+                to[D] = raise_above == kMaxSlack ? m_ref : l == 0.f ? kNegInf : 0.f;
+                to[D + 1] = l;
+            }
+        }
+        __syncthreads();
+        constexpr int LPR = D / 4;  // lanes per row
+        const int rows = min(p.R - ROWS * rt, ROWS);
+        // `leave` gets a row's sum of `parts` parts in LDS or memory
+        auto finish = [&](int r, int d0, f32x4 sum, float Mx, float L) {
+            const int at = ROWS * rt + r, gg = at / p.Sq, ii = at - gg * p.Sq, head = h * p.G + gg;
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            if (ii >= cnt) sum = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p.lse != nullptr && d0 == 0)
+                p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
+                    ii >= cnt || L == 0.f ? kNegInf : (Mx + __builtin_amdgcn_logf(L)) * 0.69314718056f;
+            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(sum.x * inv, sum.y * inv), E::pack2(sum.z * inv, sum.w * inv)};
+        };
+        const bool whole = n == T;
+        const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
+        const int g0 = (int)(plane_at / share), g1 = (int)((plane_at + T - 1) / share);  // workgroups of the plane
+        uint8_t *const ws = reinterpret_cast<uint8_t *>(p.ws);
+        // a workgroup has at most two parts: of the plane that its piece starts inside of, and of the one that goes on behind it
+        const HandOver out(ws + (int64_t)(2 * blockIdx.x + (off == 0 ? 1 : 0)) * part_bytes, whole ? 0u : part_bytes);
+        for (int it = tid; it < rows * LPR; it += kWaves * 64) {
+            const int r = it / LPR, d0 = 4 * (it - r * LPR);
+            float Mx = kNegInf, L = 0.f;
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < kWaves; w++) Mx = fmaxf(Mx, part[(w * ROWS + r) * PST + D]);
+            if (Mx != kNegInf)
+                for (int w = 0; w < kWaves; w++) {
+                    const float *pp = part + (w * ROWS + r) * PST;
+                    const float a = pp[D] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(pp[D] - Mx);
+                    L += a * pp[D + 1];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[e] += a * pp[d0 + e];
+                }
+            if (whole) {
+                finish(r, d0, sum, Mx, L);
+            } else {
+                out.put(r * row_bytes + 4 * d0, f32x2{sum.x, sum.y});
+                out.put(r * row_bytes + 4 * d0 + 8, f32x2{sum.z, sum.w});
+                if (d0 == 0) out.put(r * row_bytes + 4 * D, f32x2{Mx, L});
+            }
+        }
+        if (!whole) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();  // every wave's rows have been handed over, and LDS has been read
+            int *const told = reinterpret_cast<int *>(part);
+            if (wave == 0) {
+                const bool last = all_arrived(p.arrivals + plane + g0, p.tag, (int)blockIdx.x - g0, g1 - g0 + 1);
+                if (lane == 0) *told = last;
+            }
+            __syncthreads();
+            const bool last = __builtin_amdgcn_readfirstlane(*told) != 0;
+            if (last) {
+                const HandOver in(ws + (int64_t)2 * g0 * part_bytes, (uint32_t)(2 * (g1 - g0 + 1)) * part_bytes);
+                auto part_at = [&](int k) { return (uint32_t)(k == 0 ? 1 : 2 * k) * part_bytes; };
+                const int parts = g1 - g0 + 1;
+                for (int it = tid; it < rows * LPR; it += kWaves * 64) {
+                    const int r = it / LPR, d0 = 4 * (it - r * LPR);
+                    float Mx = kNegInf, L = 0.f;
+                    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+                    for (int k = 0; k < parts; k++) Mx = fmaxf(Mx, in.get2(part_at(k) + r * row_bytes + 4 * D).x);
+                    if (Mx != kNegInf)
+                        for (int k = 0; k < parts; k++) {
+                            const f32x2 ml = in.get2(part_at(k) + r * row_bytes + 4 * D);
+                            const f32x2 v0 = in.get2(part_at(k) + r * row_bytes + 4 * d0), v1 = in.get2(part_at(k) + r * row_bytes + 4 * d0 + 8);
+                            const float a = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mx);
+                            L += a * ml.y;
+                            sum.x += a * v0.x;
+                            sum.y += a * v0.y;
+                            sum.z += a * v1.x;
+                            sum.w += a * v1.y;
+                        }
+                    finish(r, d0, sum, Mx, L);
+                }
+            }
+        }
+        __syncthreads();  // LDS is free for the next segment
     }
 }
 
-template <int DT, int ND, bool LISTS>
+template <int DT, int ND, int ROWS, bool LISTS>
 hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
-    constexpr int smem = kWaves * 32 * (32 * ND + 2) * 4;
-    auto kern = paged_decode_kernel<DT, ND, LISTS>;
+    constexpr int smem = kWaves * ROWS * (32 * ND + 2) * 4;
+    auto kern = paged_decode_kernel<DT, ND, ROWS, LISTS>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.t.B * p.c.H * p.RT), dim3(kWaves * 64), smem, stream, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.groups), dim3(kWaves * 64), smem, stream, p);
     return hipGetLastError();
 }
-template <int DT, int ND>
+template <int DT, int ND, int ROWS>
 hipError_t launch_lists(const PagedDecodeParams &p, hipStream_t stream) {
-    return p.full_ids != nullptr ? launch_kind<DT, ND, true>(p, stream) : launch_kind<DT, ND, false>(p, stream);
+    return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, true>(p, stream) : launch_kind<DT, ND, ROWS, false>(p, stream);
+}
+template <int DT, int ND>
+hipError_t launch_rows(const PagedDecodeParams &p, hipStream_t stream) {
+    return p.R <= 16 ? launch_lists<DT, ND, 16>(p, stream) : launch_lists<DT, ND, 32>(p, stream);
 }
 template <int DT>
 hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {
-    if (p.c.D == 64) return launch_lists<DT, 2>(p, stream);
-    if (p.c.D == 128) return launch_lists<DT, 4>(p, stream);
-    if (p.c.D == 256) return launch_lists<DT, 8>(p, stream);
+    if (p.c.D == 64) return launch_rows<DT, 2>(p, stream);
+    if (p.c.D == 128) return launch_rows<DT, 4>(p, stream);
+    if (p.c.D == 256) return launch_rows<DT, 8>(p, stream);
     return hipErrorInvalidValue;
 }
 
 }  // namespace
+
+PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus) {
+    PagedDecodePlan r;
+    r.least = 4;
+    const int64_t most = (planes * chunks + r.least - 1) / r.least, resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
+    r.groups = (int)(most < resident ? most : resident);
+    r.part_rows = R < 32 ? R : 32;
+    r.parts_bytes = (size_t)r.groups * 2 * r.part_rows * (D + 2) * 4;
+    r.parts_bytes = (r.parts_bytes + 15) / 16 * 16;
+    r.bytes = r.parts_bytes + (size_t)(planes + r.groups) * 8;
+    return r;
+}
 
 hipError_t launch_paged_decode(const PagedDecodeParams &p, int dtype, hipStream_t stream) {
     if (dtype == 0) return launch_dim<0>(p, stream);
