@@ -102,16 +102,16 @@ struct PagedDecodeParams {
     int nK;
     float scale;  // softmax scale / ln 2
     // The launch's workgroups, the fewest chunks that one of them takes, and what planes that several of them share are added up by:
-    //   ws        [groups][2][part_rows][D + 2] floats: unnormalised rows, reference value and sum of each
+    //   ws        [groups][2][part_rows][D + 4] floats: unnormalised rows, reference value and sum of each
     //   arrivals  [planes + groups] words (all_arrived), the number of the launch
-    int groups, least, part_rows;
+    int groups, least, parts, cuts, part_rows;
     float *ws;
     uint64_t *arrivals;
     uint64_t tag;
 };
 constexpr int kPagedMostParts = 64;  // of a plane (all_arrived looks at one word per lane)
 struct PagedDecodePlan {
-    int groups, least, part_rows;
+    int groups, least, parts, cuts, part_rows;
     size_t parts_bytes, bytes;
 };
 PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus);

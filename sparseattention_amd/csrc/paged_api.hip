@@ -268,13 +268,15 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
     p.scale = sm_scale_log2;
     const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)pages_per_sequence << p.c.lper;
-    if (planes > (1 << 24) || (int64_t)p.c.H * p.RT * chunks > 0x7fffffff)
+    if (planes > (1 << 24) || planes * chunks > (1 << 30))
         return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
     if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
         return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, plan.bytes, workspace ? workspace_bytes : (size_t)0);
     p.groups = plan.groups;
     p.least = plan.least;
+    p.parts = plan.parts;
+    p.cuts = plan.cuts;
     p.part_rows = plan.part_rows;
     p.ws = static_cast<float *>(workspace);
     p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + plan.parts_bytes);

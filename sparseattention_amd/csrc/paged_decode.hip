@@ -17,9 +17,10 @@ namespace sa {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kPagedRowPad = 4;  // floats behind a row of a part: reference value and sum, and two that keep rows 16-byte aligned
 
 // Workgroups that a compute unit holds (a wave of each per SIMD).
-constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 4 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : rows == 16 ? 2 : 1; }
+constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 4 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
 
 template <int DT>
 struct Codes;  // eight codes as an operand, times a power of two
@@ -77,16 +78,17 @@ __device__ __forceinline__ Unit unit_of(const PagedDecodeParams &p, int u) {
     }
 }
 
-__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {  // (wave-uniform)
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)((uint64_t)x >> 32), lane);
-    return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ int64_t sum_up_to(int64_t x, int lane) {  // over lanes 0 .. lane
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)x, s), hi = (uint32_t)__shfl_up((int)((uint64_t)x >> 32), s);
-        if (lane >= s) x += (int64_t)(((uint64_t)hi << 32) | lo);
-    }
+// Over the lanes up to this one: inside rows of 16, then from row to row.
+template <class Op>
+__device__ __forceinline__ int scan(int x, Op &&op) {  // op(0, x) == x for x >= 0
+#define SA_SCAN_STEP(ctrl, rows) x = op(__builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false), x)
+    SA_SCAN_STEP(0x111, 0xf);  // row_shr:1
+    SA_SCAN_STEP(0x112, 0xf);
+    SA_SCAN_STEP(0x114, 0xf);
+    SA_SCAN_STEP(0x118, 0xf);
+    SA_SCAN_STEP(0x142, 0xa);  // row_bcast:15 to rows 1 and 3
+    SA_SCAN_STEP(0x143, 0xc);  // row_bcast:31 to rows 2 and 3
+#undef SA_SCAN_STEP
     return x;
 }
 
@@ -259,57 +261,84 @@ template <int DT, int ND, int ROWS, bool LISTS>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
     using E = Elem<DT>;
     using X = Tile<DT, ND, ROWS>;
-    constexpr int D = 32 * ND, PST = D + 2;
+    constexpr int D = 32 * ND, PST = D + kPagedRowPad;
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][ROWS][PST]
     const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lP = p.c.lper + 5, sub_mask = (1 << p.c.lper) - 1;
 
-    // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in ----
-    const int U = LISTS ? p.t.B * p.c.H : p.t.B, M = LISTS ? p.RT : p.c.H * p.RT;  // units, planes of each
+    // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in (the host: a row is less than 2^31 chunks) ----
+    const int U = LISTS ? p.t.B * p.c.H : p.t.B;                // units
+    const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;  // planes of each
     const int per_lane = (U + 63) >> 6;
-    int64_t mine = 0;
-    int longest = 0;
+    int mine = 0, longest = 0;
+#pragma unroll 1
     for (int j = 0; j < per_lane; j++) {
         const int u = lane * per_lane + j;
         const int T = u < U ? max(unit_of<LISTS>(p, u).T, 1) : 0;
         mine += T;
         longest = max(longest, T);
     }
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) longest = max(longest, __shfl_xor(longest, s));
-    longest = __builtin_amdgcn_readfirstlane(longest);
-    const int64_t upto = sum_up_to(mine, lane), total = of_lane(upto, 63) * M;
-    int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    share = max(max(share, (int64_t)p.least), (int64_t)((longest + kPagedMostParts - 3) / (kPagedMostParts - 2)));
-    const int64_t x0 = share * blockIdx.x, x1 = min(x0 + share, total);
-    if (x0 >= x1) return;
-    int u;
-    int64_t base;  // of unit u
-    {
-        const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < upto * M)) - 1;  // the lane whose units hold x0
-        base = of_lane(upto - mine, at) * M;
-        u = at * per_lane;
-        for (;; u++) {  // (U <= 64: at once)
-            const int64_t next = base + (int64_t)max(unit_of<LISTS>(p, u).T, 1) * M;
-            if (x0 < next) break;
-            base = next;
+    const auto plus = [](int a, int x) { return a + x; };
+    int upto = scan(mine, plus);
+    longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
+    unsigned total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
+    // Few planes: a plane is cut into equal parts of up to `share` chunks, a workgroup each, so that none has two planes' latencies.
+    // The row is then one of parts.  Many: equal pieces of a row of chunks.
+    const bool cuts = p.cuts != 0;
+    unsigned share = (total + gridDim.x - 1) / gridDim.x;
+    if (cuts) share = (total + gridDim.x - U * M - 1) / (gridDim.x - U * M);
+    share = max(max(share, (unsigned)p.least), ((unsigned)longest + p.parts - 1) / p.parts);
+    auto length = [&](int u) { // of a plane of the unit in the row
+        const unsigned T = (unsigned)max(unit_of<LISTS>(p, u).T, 1);
+        return cuts ? (T + share - 1) / share : T;
+    };
+    if (cuts) {
+        mine = 0;
+#pragma unroll 1
+        for (int j = 0; j < per_lane; j++) {
+            const int u = lane * per_lane + j;
+            if (u < U) mine += (int)length(u);
         }
+        upto = scan(mine, plus);
+        total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
+    }
+    const unsigned piece = cuts ? 1u : share;
+    const unsigned x0 = piece * blockIdx.x, x1 = min(x0 + piece, total);
+    if (x0 >= total) return;
+    int u;
+    unsigned base;  // of unit u
+    {
+        const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < (unsigned)upto * M)) - 1;  // the lane whose units hold x0
+        base = (unsigned)__builtin_amdgcn_readlane(upto - mine, at) * M;
+        u = at * per_lane;
+        if (per_lane > 1)
+#pragma unroll 1
+            for (;; u++) {
+                const unsigned next = base + length(u) * M;
+                if (x0 < next) break;
+                base = next;
+            }
     }
 
-    int64_t x = x0;
+    // Of the workgroups of a compute unit the oldest goes first and is done when others have a third of their piece left; so the
+    // further a workgroup is, the lower its priority.
+    __builtin_amdgcn_s_setprio(3);
+    unsigned x = x0, lower_at = share / 4;
     while (x < x1) {
+        const unsigned done = cuts ? 0u : x - x0;
         const Unit unit = unit_of<LISTS>(p, u);
-        const int T = max(unit.T, 1);
-        const int m = (int)((x - base) / T), off = (int)(x - base - (int64_t)m * T);
-        const int n = (int)min((int64_t)(T - off), x1 - x);  // chunks off .. off + n - 1 of this plane
-        const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + m : m;
+        const unsigned T = (unsigned)max(unit.T, 1), row_T = cuts ? (T + share - 1) / share : T;
+        const unsigned m = (x - base) / row_T, at_row = x - base - m * row_T;
+        const unsigned plane_at = x - at_row;  // in the row
+        // chunks off .. off + n - 1 of this plane
+        const int off = (int)(cuts ? T * at_row / row_T : at_row), n = (int)(cuts ? T * (at_row + 1) / row_T - off : min(T - at_row, x1 - x));
+        const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + (int)m : (int)m;
         const int h = hr / p.RT, rt = hr - h * p.RT;
         const int plane = (b * p.c.H + h) * p.RT + rt;
-        const int64_t plane_at = x - off;
-        x += n;
-        if (m + 1 == M && off + n == T) {
-            base += (int64_t)T * M;
+        x += cuts ? 1 : n;
+        if (m + 1 == M && x - plane_at == row_T) {
+            base += row_T * M;
             u++;
         }
 
@@ -397,6 +426,13 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             request_v(c);
         }
         for (int j = 0; j < nw; j++) {
+            if (done + 4u * j >= lower_at) {
+                const unsigned quarter = (done + 4u * j) * 4u / share;
+                lower_at = (quarter + 1) * share / 4;
+                if (quarter == 1) __builtin_amdgcn_s_setprio(2);
+                else if (quarter == 2) __builtin_amdgcn_s_setprio(1);
+                else if (quarter >= 3) __builtin_amdgcn_s_setprio(0);
+            }
             const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.ks), j & 63))) * p.scale;
             const float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.vs), j & 63)));
             if (((j + 1) & 63) == 0 && j + 1 < nw) {
@@ -476,84 +512,132 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         {
             float *to = part + (wave * ROWS + lrow) * PST;
 #pragma unroll
-            for (int e = 0; e < X::NA; e++) to[X::d_of(e, lgrp)] = out_rows.get(e);
-            if (lgrp == 0) {
-                // (a row whose only scores are NaN has a sum and no reference value)
-                to[D] = raise_above == kMaxSlack ? m_ref : l == 0.f ? kNegInf : 0.f;
-                to[D + 1] = l;
-            }
+            for (int e = 0; e < X::NA; e += 4) *(f32x4 *)(to + X::d_of(e, lgrp)) = f32x4{out_rows.get(e), out_rows.get(e + 1), out_rows.get(e + 2), out_rows.get(e + 3)};
+            // (a row whose only scores are NaN has a sum and no reference value)
+            if (lgrp == 0) *(f32x2 *)(to + D) = f32x2{raise_above == kMaxSlack ? m_ref : l == 0.f ? kNegInf : 0.f, l};
         }
         __syncthreads();
         constexpr int LPR = D / 4;  // lanes per row
         const int rows = min(p.R - ROWS * rt, ROWS);
-        // `leave` gets a row's sum of `parts` parts in LDS or memory
-        auto finish = [&](int r, int d0, f32x4 sum, float Mx, float L) {
+        struct Sum {
+            float M = kNegInf, L = 0.f;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        };
+        // parts k = 0 .. N - 1 to the sum: their rows' values, reference values and sums
+        auto add_to = [](Sum &s, const auto &v, const auto &ml) __attribute__((always_inline)) {
+            constexpr int N = sizeof(ml) / sizeof(ml[0]);
+            float M = s.M;
+#pragma unroll
+            for (int k = 0; k < N; k++) M = fmaxf(M, ml[k].x);
+            const float a = s.M == kNegInf ? 0.f : __builtin_amdgcn_exp2f(s.M - M);
+            s.L *= a;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s.x[e] *= a;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const float w = ml[k].x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - M);
+                s.L += w * ml[k].y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) s.x[e] += w * v[k][e];
+            }
+            s.M = M;
+        };
+        auto finish = [&](int r, int d0, Sum s) {
             const int at = ROWS * rt + r, gg = at / p.Sq, ii = at - gg * p.Sq, head = h * p.G + gg;
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            if (ii >= cnt) sum = f32x4{0.f, 0.f, 0.f, 0.f};
+            const float inv = s.L == 0.f ? 0.f : 1.f / s.L;
+            if (ii >= cnt) s.x = f32x4{0.f, 0.f, 0.f, 0.f};
             if (p.lse != nullptr && d0 == 0)
                 p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
-                    ii >= cnt || L == 0.f ? kNegInf : (Mx + __builtin_amdgcn_logf(L)) * 0.69314718056f;
-            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(sum.x * inv, sum.y * inv), E::pack2(sum.z * inv, sum.w * inv)};
+                    ii >= cnt || s.L == 0.f ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
+            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(s.x.x * inv, s.x.y * inv), E::pack2(s.x.z * inv, s.x.w * inv)};
         };
-        const bool whole = n == T;
+        const bool whole = n == (int)T;
         const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
-        const int g0 = (int)(plane_at / share), g1 = (int)((plane_at + T - 1) / share);  // workgroups of the plane
         uint8_t *const ws = reinterpret_cast<uint8_t *>(p.ws);
         // a workgroup has at most two parts: of the plane that its piece starts inside of, and of the one that goes on behind it
         const HandOver out(ws + (int64_t)(2 * blockIdx.x + (off == 0 ? 1 : 0)) * part_bytes, whole ? 0u : part_bytes);
         for (int it = tid; it < rows * LPR; it += kWaves * 64) {
             const int r = it / LPR, d0 = 4 * (it - r * LPR);
-            float Mx = kNegInf, L = 0.f;
-            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < kWaves; w++) Mx = fmaxf(Mx, part[(w * ROWS + r) * PST + D]);
-            if (Mx != kNegInf)
-                for (int w = 0; w < kWaves; w++) {
-                    const float *pp = part + (w * ROWS + r) * PST;
-                    const float a = pp[D] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(pp[D] - Mx);
-                    L += a * pp[D + 1];
+            f32x4 v[kWaves];
+            f32x2 ml[kWaves];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sum[e] += a * pp[d0 + e];
-                }
+            for (int w = 0; w < kWaves; w++) {
+                v[w] = *(const f32x4 *)(part + (w * ROWS + r) * PST + d0);
+                ml[w] = *(const f32x2 *)(part + (w * ROWS + r) * PST + D);
+            }
+            Sum s;
+            add_to(s, v, ml);
             if (whole) {
-                finish(r, d0, sum, Mx, L);
+                finish(r, d0, s);
             } else {
-                out.put(r * row_bytes + 4 * d0, f32x2{sum.x, sum.y});
-                out.put(r * row_bytes + 4 * d0 + 8, f32x2{sum.z, sum.w});
-                if (d0 == 0) out.put(r * row_bytes + 4 * D, f32x2{Mx, L});
+                out.put(r * row_bytes + 4 * d0, s.x);
+                if (d0 == 0) out.put(r * row_bytes + 4 * D, f32x2{s.M, s.L});
             }
         }
         if (!whole) {
+            const int g0 = (int)(plane_at / piece), parts = (int)((plane_at + row_T - 1) / piece) - g0 + 1;  // workgroups of the plane
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();  // every wave's rows have been handed over, and LDS has been read
-            int *const told = reinterpret_cast<int *>(part);
+            int *const told = reinterpret_cast<int *>(part + D + 2);  // (behind a row: the sum below leaves it alone)
             if (wave == 0) {
-                const bool last = all_arrived(p.arrivals + plane + g0, p.tag, (int)blockIdx.x - g0, g1 - g0 + 1);
+                const bool last = all_arrived(p.arrivals + plane + g0, p.tag, (int)blockIdx.x - g0, parts);
                 if (lane == 0) *told = last;
             }
             __syncthreads();
             const bool last = __builtin_amdgcn_readfirstlane(*told) != 0;
             if (last) {
-                const HandOver in(ws + (int64_t)2 * g0 * part_bytes, (uint32_t)(2 * (g1 - g0 + 1)) * part_bytes);
-                auto part_at = [&](int k) { return (uint32_t)(k == 0 ? 1 : 2 * k) * part_bytes; };
-                const int parts = g1 - g0 + 1;
-                for (int it = tid; it < rows * LPR; it += kWaves * 64) {
-                    const int r = it / LPR, d0 = 4 * (it - r * LPR);
-                    float Mx = kNegInf, L = 0.f;
-                    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-                    for (int k = 0; k < parts; k++) Mx = fmaxf(Mx, in.get2(part_at(k) + r * row_bytes + 4 * D).x);
-                    if (Mx != kNegInf)
-                        for (int k = 0; k < parts; k++) {
-                            const f32x2 ml = in.get2(part_at(k) + r * row_bytes + 4 * D);
-                            const f32x2 v0 = in.get2(part_at(k) + r * row_bytes + 4 * d0), v1 = in.get2(part_at(k) + r * row_bytes + 4 * d0 + 8);
-                            const float a = ml.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mx);
-                            L += a * ml.y;
-                            sum.x += a * v0.x;
-                            sum.y += a * v0.y;
-                            sum.z += a * v1.x;
-                            sum.w += a * v1.y;
+                const HandOver in(ws + (int64_t)2 * g0 * part_bytes, (uint32_t)(2 * parts) * part_bytes);
+                // Every `teams`-th part by the same threads where there are some to spare, 8 parts on their way at a time.
+                const int items = rows * LPR, teams = items <= 64 ? 4 : items <= 128 ? 2 : 1;
+                for (int it = tid; it < teams * items; it += kWaves * 64) {
+                    const int team = it / items, it0 = it - team * items, r = it0 / LPR, d0 = 4 * (it0 - r * LPR);
+                    Sum s;
+                    for (int k0 = team; k0 < parts; k0 += 8 * teams) {
+                        f32x4 v[8];
+                        f32x2 ml[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int at = min(k0 + k * teams, parts - 1);
+                            const uint32_t from = (uint32_t)(at == 0 ? 1 : 2 * at) * part_bytes + r * row_bytes;
+                            v[k] = in.get4(from + 4 * d0);
+                            ml[k] = in.get2(from + 4 * D);
                         }
-                    finish(r, d0, sum, Mx, L);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (k0 + k * teams >= parts) {  // (none there: the last one again, left out)
+                                ml[k] = f32x2{kNegInf, 0.f};
+                                v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                            }
+                        add_to(s, v, ml);
+                    }
+                    if (teams == 1) {
+                        finish(r, d0, s);
+                    } else {
+                        float *const to = part + (team * ROWS + r) * PST;
+                        *(f32x4 *)(to + d0) = s.x;
+                        if (d0 == 0) *(f32x2 *)(to + D) = f32x2{s.M, s.L};
+                    }
+                }
+                if (teams > 1) {
+                    __syncthreads();
+                    if (tid < items) {
+                        const int r = tid / LPR, d0 = 4 * (tid - r * LPR);
+                        f32x4 v[4];
+                        f32x2 ml[4];
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            const float *const from = part + (min(w, teams - 1) * ROWS + r) * PST;
+                            v[w] = *(const f32x4 *)(from + d0);
+                            ml[w] = *(const f32x2 *)(from + D);
+                            if (w >= teams) {
+                                v[w] = f32x4{0.f, 0.f, 0.f, 0.f};
+                                ml[w] = f32x2{kNegInf, 0.f};
+                            }
+                        }
+                        Sum s;
+                        add_to(s, v, ml);
+                        finish(r, d0, s);
+                    }
                 }
             }
         }
@@ -563,7 +647,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
 
 template <int DT, int ND, int ROWS, bool LISTS>
 hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
-    constexpr int smem = kWaves * ROWS * (32 * ND + 2) * 4;
+    constexpr int smem = kWaves * ROWS * (32 * ND + kPagedRowPad) * 4;
     auto kern = paged_decode_kernel<DT, ND, ROWS, LISTS>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
@@ -588,14 +672,24 @@ hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {
 
 }  // namespace
 
+// As many workgroups as the device holds at once: with more, the pieces of a workgroup that starts late do not make up for its start
+// (32 sequences of up to 32768 keys: 294 us; twice as many workgroups 304, four times 324).
+// Planes are cut where they are few, so that a plane is many parts and their ends are even: at 8 parts a plane (64 planes of 129 chunks)
+// 21.5 -> 18.3 us, 8 planes of 63 chunks 12.1 -> 9.1; at 3 (256 planes of 700 ... 1024) it would be 290 -> 319.
+// Parts are added up by one workgroup, 8 to 32 at a time, so there are no more of them than give every compute unit one, but at
+// least 16: 16 planes of 1000 chunks with 16 | 32 | 62 parts 32.3 | 37.9 | 41.6 us.
 PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus) {
     PagedDecodePlan r;
-    r.least = 4;
-    const int64_t most = (planes * chunks + r.least - 1) / r.least, resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
+    r.least = kWaves;
+    const int64_t even = cus / planes;
+    r.parts = (int)(even < 16 ? 16 : even < kPagedMostParts - 2 ? even : kPagedMostParts - 2);
+    const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
+    r.cuts = 8 * planes <= resident;
+    const int64_t fine = (chunks + r.least - 1) / r.least;  // parts of a plane of that many chunks each
+    const int64_t most = r.cuts ? planes * ((fine < r.parts ? fine : r.parts) + 1) : planes * fine;
     r.groups = (int)(most < resident ? most : resident);
     r.part_rows = R < 32 ? R : 32;
-    r.parts_bytes = (size_t)r.groups * 2 * r.part_rows * (D + 2) * 4;
-    r.parts_bytes = (r.parts_bytes + 15) / 16 * 16;
+    r.parts_bytes = (size_t)r.groups * 2 * r.part_rows * (D + kPagedRowPad) * 4;
     r.bytes = r.parts_bytes + (size_t)(planes + r.groups) * 8;
     return r;
 }
