@@ -91,18 +91,50 @@ __device__ __forceinline__ int64_t block_at(const PagedPool &c, int page, int h,
     return (((int64_t)page * c.H + h) << c.lper) + sub;
 }
 
-// One wave stores the new tokens of one block of one head, K or V.
+// The largest of the wave's x >= 0, in all lanes.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#define SA_MAX_STEP(ctrl, rows) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))
+    SA_MAX_STEP(0x111, 0xf);  // row_shr:1
+    SA_MAX_STEP(0x112, 0xf);
+    SA_MAX_STEP(0x114, 0xf);
+    SA_MAX_STEP(0x118, 0xf);
+    SA_MAX_STEP(0x142, 0xa);  // row_bcast:15
+    SA_MAX_STEP(0x143, 0xc);  // row_bcast:31
+#undef SA_MAX_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// Rows of a block in LDS, a wave's own: 16 bytes apart from the banks' period, so that the same piece of 16 rows and a row's own
+// pieces both fall into different banks.  A wave's operations on LDS take effect in their order; the fence keeps the compiler, which
+// sees one lane, to it.
+constexpr int kCacheWaves = 4;
+template <int ND>
+constexpr int row_bytes = 64 * ND + 16;
+__device__ __forceinline__ void in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// One wave stores the new tokens of one block of one head, K or V.  The rows come from memory as they lie there, 1 KiB a load, and
+// cross the lanes through LDS, 16 at a time.
 template <int DT, int ND>
-__global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParams p) {
+__global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_append_kernel(const PagedAppendParams p) {
     using X = Half16<DT>;
-    constexpr int NG = ND / 2;  // groups of 64 d
-    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5;
-    unsigned item = blockIdx.x;
+    constexpr int NG = ND / 2;                        // groups of 64 d
+    constexpr int PPR = 4 * ND, RPI = 64 / PPR;       // 16-byte pieces of a row, rows of a load
+    constexpr int NL = 32 / RPI;                      // loads of a block
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kCacheWaves * 16 * row_bytes<ND>];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t *const mine = smem + wave * 16 * row_bytes<ND>;
+    const int l32 = lane & 31, hh = lane >> 5;
+    unsigned item = blockIdx.x * kCacheWaves + wave;
     const bool values = item & 1u;
     item >>= 1;
     const int h = (int)(item % (unsigned)p.c.H);
     item /= (unsigned)p.c.H;
     const int nb = (int)(item % (unsigned)p.blocks), b = (int)(item / (unsigned)p.blocks);
+    if (b >= p.t.B) return;
     const int room = p.t.width << (p.c.lper + 5);  // tokens that the table has place for
     const int len = max(p.t.lens[b], 0);
     if (len >= room) return;
@@ -114,49 +146,80 @@ __global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParam
     const int held = max(len - first, 0), a = held, z = min(len + n - first, 32);
     if (a >= z) return;
     const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
+    // row t of the block is token first + t of the sequence, first + t - len of the new ones
+    const int64_t *const xs = values ? p.vs : p.ks;
+    const int64_t row = xs[2];
+    const uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)(first - len) * row;
+    u32x4 in[NL];
+    const int r0 = lane / PPR, piece = lane % PPR;
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int r = RPI * i + r0;
+        in[i] = u32x4{0u, 0u, 0u, 0u};
+        if (r >= a && r < z) in[i] = __builtin_nontemporal_load((const u32x4 *)(x + r * row + 8 * piece));
+    }
     if (page < 0) return;
     const int64_t at = block_at(p.c, page, h, blk & ((1 << p.c.lper) - 1));
     uint8_t *const out = (values ? p.c.v : p.c.k) + at * (ND * 1024);
     float *const scale = (values ? p.c.v_scales : p.c.k_scales) + at;
-    const int64_t *const xs = values ? p.vs : p.ks;
-    // row t of the block is token first + t of the sequence, first + t - len of the new ones
-    const uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)(first - len) * xs[2];
-    const int64_t row = xs[2];
     const int e_old = held > 0 ? exp_of_scale(*scale) : kScaleExpMin;
-
-    // the new values: K as 16 of one token per piece, V as two neighbouring d of 16 tokens per group
-    uint32_t w[16 * NG];
-    uint32_t m = 0u;
-    if (!values) {
+    // V of a block that is not all new: what there is, d = 64 g + 2 l32 and the next one
+    u32x4 was[2 * NG];
+    const bool mixed = values && z - a < 32;
+    auto v_at = [&](int g) { return (u32x4 *)(out + 1024 * (2 * g + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15))); };
+    if (mixed) {
 #pragma unroll
-        for (int c = 0; c < ND; c++) {
-            u32x4 u[2] = {};
-            if (l32 >= a && l32 < z) {
-                const uint16_t *src = x + l32 * row + 32 * c + 16 * hh;
-                u[0] = *(const u32x4 *)src;
-                u[1] = *(const u32x4 *)(src + 8);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[8 * c + i] = u[i >> 2][i & 3];
+        for (int g = 0; g < NG; g++) {
+            was[2 * g] = v_at(g)[0];
+            was[2 * g + 1] = v_at(g)[1];
         }
-    } else {
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int t = 16 * ((j >> 2) & 1) + 8 * (j >> 3) + 4 * hh + (j & 3);
-                w[16 * g + j] = t >= a && t < z ? *(const uint32_t *)(x + t * row + 64 * g + 2 * l32) : 0u;
-            }
     }
+
+    uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < 16 * NG; i++) m = amax2<DT>(m, w[i]);
+    for (int i = 0; i < NL; i++)
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, s));
+        for (int j = 0; j < 4; j++) m = amax2<DT>(m, in[i][j]);
+    m = wave_max(m);
     const int e = max(e_old, scale_exp(DT == 0 ? __uint_as_float(m << 16) : X::lo(m)));
     const float inv = exp2i(-e);
     const bool grows = held > 0 && e > e_old;
     const float f = exp2i(max(e_old - e, -126));
     if (lane == 0 && (grows || held == 0)) *scale = exp2i(e);
+
+    u32x4 made[2 * NG];  // codes: of 16 d of a token per piece (K), of 16 tokens of two d (V)
+#pragma unroll
+    for (int half = 0; half < 2; half++) {  // rows 16 half ..
+        if (a >= 16 * half + 16 || z <= 16 * half) continue;
+#pragma unroll
+        for (int i = 0; i < NL / 2; i++) *(u32x4 *)(mine + (RPI * i + r0) * row_bytes<ND> + 16 * piece) = in[NL / 2 * half + i];
+        in_order();
+        if (!values) {
+            if ((l32 >> 4) == half) {
+#pragma unroll
+                for (int c = 0; c < ND; c++) {
+                    const u32x4 *const from = (const u32x4 *)(mine + (l32 & 15) * row_bytes<ND> + 64 * c + 32 * hh);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t lo = from[i >> 1][2 * (i & 1)], hi = from[i >> 1][2 * (i & 1) + 1];
+                        made[c][i] = codes4(scaled(X::lo(lo), inv), scaled(X::hi(lo), inv), scaled(X::lo(hi), inv), scaled(X::hi(hi), inv));
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int i = half; i < 4; i += 2) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) q[j] = *(const uint32_t *)(mine + (8 * (i >> 1) + 4 * hh + j) * row_bytes<ND> + 128 * g + 4 * l32);
+                    made[2 * g][i] = codes4(scaled(X::lo(q[0]), inv), scaled(X::lo(q[1]), inv), scaled(X::lo(q[2]), inv), scaled(X::lo(q[3]), inv));
+                    made[2 * g + 1][i] = codes4(scaled(X::hi(q[0]), inv), scaled(X::hi(q[1]), inv), scaled(X::hi(q[2]), inv), scaled(X::hi(q[3]), inv));
+                }
+        }
+        in_order();
+    }
 
     if (!values) {
         const bool fresh = l32 >= a && l32 < z, old = grows && l32 < held;
@@ -164,13 +227,7 @@ __global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParam
         for (int c = 0; c < ND; c++) {
             u32x4 *const to = (u32x4 *)(out + 1024 * c + 16 * lane);
             if (fresh) {
-                u32x4 u;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t lo = w[8 * c + 2 * i], hi = w[8 * c + 2 * i + 1];
-                    u[i] = codes4(scaled(X::lo(lo), inv), scaled(X::hi(lo), inv), scaled(X::lo(hi), inv), scaled(X::hi(hi), inv));
-                }
-                *to = u;
+                *to = made[c];
             } else if (old) {
                 u32x4 u = *to;
 #pragma unroll
@@ -179,98 +236,108 @@ __global__ __launch_bounds__(64) void paged_append_kernel(const PagedAppendParam
             }
         }
     } else {
-        uint32_t isnew[4], isold[4], any = 0u, all = ~0u;
+        uint32_t isnew[4], isold[4], any = 0u;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int base = 16 * (i & 1) + 8 * (i >> 1) + 4 * hh;
             isnew[i] = bytes_in(base, a, z);
             isold[i] = grows ? bytes_in(base, 0, held) : 0u;
             any |= isnew[i] | isold[i];
-            all &= isnew[i];
         }
         if (any == 0u) return;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            // d = 64 g + 2 l32 and the next one
-            u32x4 *const to = (u32x4 *)(out + 1024 * (2 * g + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15)));
-            u32x4 u[2] = {};
-            if (all != ~0u) {
-                u[0] = to[0];
-                u[1] = to[1];
-            }
+        for (int g = 0; g < NG; g++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t *const q = &w[16 * g + 4 * i];
-                const uint32_t lo = codes4(scaled(X::lo(q[0]), inv), scaled(X::lo(q[1]), inv), scaled(X::lo(q[2]), inv), scaled(X::lo(q[3]), inv));
-                const uint32_t hi = codes4(scaled(X::hi(q[0]), inv), scaled(X::hi(q[1]), inv), scaled(X::hi(q[2]), inv), scaled(X::hi(q[3]), inv));
-                if (grows) {
-                    u[0][i] = (u[0][i] & ~isold[i]) | (again4(u[0][i], f) & isold[i]);
-                    u[1][i] = (u[1][i] & ~isold[i]) | (again4(u[1][i], f) & isold[i]);
+            for (int k = 0; k < 2; k++) {
+                u32x4 u = made[2 * g + k];
+                if (mixed) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t w = was[2 * g + k][i];
+                        if (grows) w = (w & ~isold[i]) | (again4(w, f) & isold[i]);
+                        u[i] = isnew[i] == 0u ? w : (w & ~isnew[i]) | (u[i] & isnew[i]);
+                    }
                 }
-                u[0][i] = (u[0][i] & ~isnew[i]) | (lo & isnew[i]);
-                u[1][i] = (u[1][i] & ~isnew[i]) | (hi & isnew[i]);
+                v_at(g)[k] = u;
             }
-            to[0] = u[0];
-            to[1] = u[1];
-        }
     }
 }
 
-// One wave reads one block of one head, K or V, into rows; rows that hold nothing become zero.
-template <int DT, int ND>
-__global__ __launch_bounds__(64) void paged_gather_kernel(const PagedGatherParams p) {
+// One wave reads one block of one head, K or V, into rows; rows that hold nothing become zero.  The rows cross the lanes in LDS and leave
+// 1 KiB a store, 16 rows at a time, so that all the waves that a compute unit holds have their place there.  FAR: the stores pass the
+// caches by, for outputs larger than those.
+template <int DT, int ND, bool FAR>
+__global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const PagedGatherParams p) {
     using X = Half16<DT>;
-    constexpr int NG = ND / 2;
-    const int lane = threadIdx.x, l32 = lane & 31, hh = lane >> 5;
+    constexpr int NG = ND / 2, PPR = 4 * ND, RPI = 64 / PPR, NL = 16 / RPI;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kCacheWaves * 16 * row_bytes<ND>];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t *const mine = smem + wave * 16 * row_bytes<ND>;
+    const int l32 = lane & 31, hh = lane >> 5;
     const unsigned blocks = ((unsigned)p.length + 31) / 32;
-    unsigned item = blockIdx.x;
+    unsigned item = blockIdx.x * kCacheWaves + wave;
     const bool values = item & 1u;
     item >>= 1;
     const int blk = (int)(item % blocks);
     item /= blocks;
     const int h = (int)(item % (unsigned)p.c.H), b = (int)(item / (unsigned)p.c.H);
-    const int first = 32 * blk;
-    const int rows = min(p.length - first, 32);
-    int n = min(max(p.t.lens[b] - first, 0), rows);  // rows that hold something
-    const int page = n > 0 ? page_at(p.t, b, blk >> p.c.lper, p.c.pages) : -1;
-    if (page < 0) n = 0;
+    if (b >= p.t.B) return;
+    const int first = 32 * blk, rows = min(p.length - first, 32);
+    const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
+    const int n = page < 0 ? 0 : min(max(p.t.lens[b] - first, 0), rows);  // rows that hold something
     const int64_t at = block_at(p.c, max(page, 0), h, blk & ((1 << p.c.lper) - 1));
     const uint8_t *const in = (values ? p.c.v : p.c.k) + at * (ND * 1024);
-    const float scale = n > 0 ? exp2i(exp_of_scale((values ? p.c.v_scales : p.c.k_scales)[at])) : 0.f;
+    u32x4 u[ND];
+    float scale = 0.f;
+    if (n > 0) {
+#pragma unroll
+        for (int c = 0; c < ND; c++)
+            u[c] = *(const u32x4 *)(in + (values ? 1024 * (2 * (c >> 1) + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15) + (c & 1)) : 1024 * c + 16 * lane));
+        scale = exp2i(exp_of_scale((values ? p.c.v_scales : p.c.k_scales)[at]));
+    }
     const int64_t *const xs = values ? p.vs : p.ks;
     uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)first * xs[2];
-    const int64_t row = xs[2];
-    if (!values) {
-        if (l32 >= rows) return;
+    const int r0 = lane / PPR, piece = lane % PPR;
 #pragma unroll
-        for (int c = 0; c < ND; c++) {
-            u32x4 u = {};
-            if (l32 < n) u = *(const u32x4 *)(in + 1024 * c + 16 * lane);
-            uint16_t *const to = x + l32 * row + 32 * c + 16 * hh;
-            *(u32x4 *)to = u32x4{X::cvt_lo(u.x, scale), X::cvt_hi(u.x, scale), X::cvt_lo(u.y, scale), X::cvt_hi(u.y, scale)};
-            *(u32x4 *)(to + 8) = u32x4{X::cvt_lo(u.z, scale), X::cvt_hi(u.z, scale), X::cvt_lo(u.w, scale), X::cvt_hi(u.w, scale)};
-        }
-    } else {
+    for (int half = 0; half < 2; half++) {  // rows 16 half ..
+        if (n > 16 * half) {
+            if (!values) {
+                if ((l32 >> 4) == half) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            u32x4 u[2] = {};
-            if (n > 0) {
-                const u32x4 *const from = (const u32x4 *)(in + 1024 * (2 * g + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15)));
-                u[0] = from[0];
-                u[1] = from[1];
+                    for (int c = 0; c < ND; c++) {
+                        u32x4 *const to = (u32x4 *)(mine + (l32 & 15) * row_bytes<ND> + 64 * c + 32 * hh);
+                        to[0] = u32x4{X::cvt_lo(u[c].x, scale), X::cvt_hi(u[c].x, scale), X::cvt_lo(u[c].y, scale), X::cvt_hi(u[c].y, scale)};
+                        to[1] = u32x4{X::cvt_lo(u[c].z, scale), X::cvt_hi(u[c].z, scale), X::cvt_lo(u[c].w, scale), X::cvt_hi(u[c].w, scale)};
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; g++)  // d = 64 g + 2 l32 and the next one
+#pragma unroll
+                    for (int i = half; i < 4; i += 2) {
+                        uint32_t *const to = (uint32_t *)(mine + (8 * (i >> 1) + 4 * hh) * row_bytes<ND> + 128 * g + 4 * l32);
+                        const uint32_t a0 = X::cvt_lo(u[2 * g][i], scale), a1 = X::cvt_hi(u[2 * g][i], scale);
+                        const uint32_t b0 = X::cvt_lo(u[2 * g + 1][i], scale), b1 = X::cvt_hi(u[2 * g + 1][i], scale);
+                        to[0] = (a0 & 0xffffu) | (b0 << 16);
+                        to[row_bytes<ND> / 4] = (a0 >> 16) | (b0 & 0xffff0000u);
+                        to[2 * row_bytes<ND> / 4] = (a1 & 0xffffu) | (b1 << 16);
+                        to[3 * row_bytes<ND> / 4] = (a1 >> 16) | (b1 & 0xffff0000u);
+                    }
             }
+            in_order();
+        }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int base = 16 * (i & 1) + 8 * (i >> 1) + 4 * hh;
-                const uint32_t a0 = X::cvt_lo(u[0][i], scale), a1 = X::cvt_hi(u[0][i], scale);
-                const uint32_t b0 = X::cvt_lo(u[1][i], scale), b1 = X::cvt_hi(u[1][i], scale);
-                const uint32_t v[4] = {(a0 & 0xffffu) | (b0 << 16), (a0 >> 16) | (b0 & 0xffff0000u), (a1 & 0xffffu) | (b1 << 16),
-                                       (a1 >> 16) | (b1 & 0xffff0000u)};
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (base + j < rows) *(uint32_t *)(x + (base + j) * row + 64 * g + 2 * l32) = base + j < n ? v[j] : 0u;
+        for (int i = 0; i < NL; i++) {
+            const int r = RPI * i + r0, t = 16 * half + r;
+            u32x4 y = u32x4{0u, 0u, 0u, 0u};
+            if (t < n) y = *(const u32x4 *)(mine + r * row_bytes<ND> + 16 * piece);
+            if (t < rows) {
+                u32x4 *const to = (u32x4 *)(x + t * xs[2] + 8 * piece);
+                if constexpr (FAR) __builtin_nontemporal_store(y, to);
+                else *to = y;
             }
         }
+        in_order();
     }
 }
 
@@ -336,25 +403,27 @@ __global__ __launch_bounds__(256) void paged_fork_kernel(const PagedForkParams p
 }
 
 constexpr int kPlanThreads = 1024;
-// Sum over the threads in front of this one, and of all.
+// Sum over the lanes up to this one, and over the threads in front of this one (and of all).
+__device__ __forceinline__ int lanes_up_to(int x) {
+#define SA_SUM_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+    SA_SUM_STEP(0x111, 0xf);
+    SA_SUM_STEP(0x112, 0xf);
+    SA_SUM_STEP(0x114, 0xf);
+    SA_SUM_STEP(0x118, 0xf);
+    SA_SUM_STEP(0x142, 0xa);
+    SA_SUM_STEP(0x143, 0xc);
+#undef SA_SUM_STEP
+    return x;
+}
 __device__ __forceinline__ int before_me(int x, int *waves, int &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = x;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int up = __shfl_up(sum, s);
-        if (lane >= s) sum += up;
-    }
+    const int sum = lanes_up_to(x);
     __syncthreads();
     if (lane == 63) waves[wave] = sum;
     __syncthreads();
-    int base = 0;
-    total = 0;
-    for (int w = 0; w < kPlanThreads / 64; w++) {
-        if (w < wave) base += waves[w];
-        total += waves[w];
-    }
-    return base + sum - x;
+    const int up = lanes_up_to(lane < kPlanThreads / 64 ? waves[lane] : 0);
+    total = __builtin_amdgcn_readlane(up, 63);
+    return sum - x + (wave == 0 ? 0 : __shfl(up, wave - 1));
 }
 
 // One workgroup: a bit per page that a sequence uses, then the pairs of the compaction or the free list.  The table is read
@@ -365,12 +434,21 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPla
     const int tid = threadIdx.x, words = (p.pages + 31) >> 5;
     for (int i = tid; i < words; i += kPlanThreads) bits[i] = 0u;
     __syncthreads();
+    // four entries and their lengths on their way at a time
     const int64_t entries = (int64_t)p.t.B * p.t.width;
-    for (int64_t i = tid; i < entries; i += kPlanThreads) {
-        const int b = (int)(i / p.t.width), j = (int)(i - (int64_t)b * p.t.width);
-        if (((int64_t)j << p.lP) >= p.t.lens[b]) continue;
-        const int page = p.t.ids[b * p.t.s0 + j * p.t.s1];
-        if (page >= 0 && page < p.pages) atomicOr(&bits[page >> 5], 1u << (page & 31));
+    for (int64_t i0 = tid; i0 < entries; i0 += 4 * kPlanThreads) {
+        int page[4], len[4], at[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t i = min(i0 + k * kPlanThreads, entries - 1);
+            const int b = (int)(i / p.t.width);
+            at[k] = (int)(i - (int64_t)b * p.t.width);
+            len[k] = p.t.lens[b];
+            page[k] = p.t.ids[b * p.t.s0 + at[k] * p.t.s1];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (((int64_t)at[k] << p.lP) < len[k] && page[k] >= 0 && page[k] < p.pages) atomicOr(&bits[page[k] >> 5], 1u << (page[k] & 31));
     }
     __syncthreads();
     // this thread's words
@@ -444,14 +522,20 @@ hipError_t with_sizes(int dtype, int D, F &&f) {
 
 hipError_t launch_paged_append(const PagedAppendParams &p, int dtype, hipStream_t stream) {
     return with_sizes(dtype, p.c.D, [&](auto dt, auto nd) {
-        hipLaunchKernelGGL((paged_append_kernel<decltype(dt)::value, decltype(nd)::value>), dim3(2u * p.c.H * p.blocks * p.t.B), dim3(64), 0, stream, p);
+        hipLaunchKernelGGL((paged_append_kernel<decltype(dt)::value, decltype(nd)::value>), dim3((2u * p.c.H * p.blocks * p.t.B + kCacheWaves - 1) / kCacheWaves), dim3(64 * kCacheWaves), 0, stream, p);
         return hipGetLastError();
     });
 }
+// Outputs of that many bytes go past the caches (L2 and the memory-side cache hold 288 MiB, what reads the output brings its own).
+// us, through them | past them: 64 MiB 24.4 | 27.1 (with the fork in front), 192 MiB 58.4 | 55.3, 768 MiB (with the compaction) 296 | 278.
+constexpr int64_t kGatherFar = 128ll << 20;
+
 hipError_t launch_paged_gather(const PagedGatherParams &p, int dtype, hipStream_t stream) {
     const unsigned blocks = ((unsigned)p.length + 31) / 32;
+    const bool far = (int64_t)p.t.B * p.c.H * p.length * p.c.D * 4 >= kGatherFar;
     return with_sizes(dtype, p.c.D, [&](auto dt, auto nd) {
-        hipLaunchKernelGGL((paged_gather_kernel<decltype(dt)::value, decltype(nd)::value>), dim3(2u * p.c.H * blocks * p.t.B), dim3(64), 0, stream, p);
+        constexpr int DT = decltype(dt)::value, ND = decltype(nd)::value;
+        hipLaunchKernelGGL((far ? paged_gather_kernel<DT, ND, true> : paged_gather_kernel<DT, ND, false>), dim3((2u * p.c.H * blocks * p.t.B + kCacheWaves - 1) / kCacheWaves), dim3(64 * kCacheWaves), 0, stream, p);
         return hipGetLastError();
     });
 }
