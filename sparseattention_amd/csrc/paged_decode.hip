@@ -59,23 +59,32 @@ __device__ __forceinline__ float scale_of(float s) {  // (as the cache's kernels
 // an equal piece of the row, whatever the lengths: segments, each of one plane.  A plane that lies in several workgroups' pieces is
 // added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself, by a sum over the units.
 struct Unit {
-    int T0, T;  // first chunk, chunks (0: none)
+    int len, cnt;  // keys and query rows of its sequence
+    int T0, T;     // first chunk, chunks (0: none)
+    int F;         // with lists: FULL entries
 };
 template <bool LISTS>
 __device__ __forceinline__ Unit unit_of(const PagedDecodeParams &p, int u) {
     const int b = LISTS ? u / p.c.H : u;
     const int lP = p.c.lper + 5;
-    const int len = min(max(p.t.lens[b], 0), p.t.width << lP);
-    const int cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.Sq) : p.Sq;
-    if (cnt == 0 || len == 0) return {0, 0};
+    Unit r{p.t.lens[b], p.counts != nullptr ? p.counts[b] : p.Sq, 0, 0, 0};
     if constexpr (LISTS) {
         const int h = u - b * p.c.H;
-        const int F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
-        return {0, (F + min(max(p.part_lens[b * p.pls[0] + h * p.pls[1]], 0), p.nK - F)) << p.c.lper};
-    } else {
-        const int T0 = p.window > 0 ? max(len - cnt - p.window + 1, 0) >> 5 : 0;
-        return {T0, ((len + 31) >> 5) - T0};
+        r.F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
+        r.T = (r.F + min(max(p.part_lens[b * p.pls[0] + h * p.pls[1]], 0), p.nK - r.F)) << p.c.lper;
     }
+    r.len = min(max(r.len, 0), p.t.width << lP);
+    r.cnt = min(max(r.cnt, 0), p.Sq);
+    if constexpr (!LISTS) {
+        r.T0 = p.window > 0 ? max(r.len - r.cnt - p.window + 1, 0) >> 5 : 0;
+        r.T = ((r.len + 31) >> 5) - r.T0;
+    }
+    if (r.cnt == 0 || r.len == 0) r.T = 0;
+    return r;
+}
+__device__ __forceinline__ Unit of_lane(const Unit &r, int lane) {  // (wave-uniform)
+    return {__builtin_amdgcn_readlane(r.len, lane), __builtin_amdgcn_readlane(r.cnt, lane), __builtin_amdgcn_readlane(r.T0, lane),
+            __builtin_amdgcn_readlane(r.T, lane), __builtin_amdgcn_readlane(r.F, lane)};
 }
 
 // Over the lanes up to this one: inside rows of 16, then from row to row.
@@ -272,10 +281,12 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;  // planes of each
     const int per_lane = (U + 63) >> 6;
     int mine = 0, longest = 0;
+    Unit own{0, 0, 0, 0, 0};  // the lane's last unit (the only one of up to 64 units)
 #pragma unroll 1
     for (int j = 0; j < per_lane; j++) {
         const int u = lane * per_lane + j;
-        const int T = u < U ? max(unit_of<LISTS>(p, u).T, 1) : 0;
+        own = unit_of<LISTS>(p, min(u, U - 1));
+        const int T = u < U ? max(own.T, 1) : 0;
         mine += T;
         longest = max(longest, T);
     }
@@ -289,17 +300,20 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     unsigned share = (total + gridDim.x - 1) / gridDim.x;
     if (cuts) share = (total + gridDim.x - U * M - 1) / (gridDim.x - U * M);
     share = max(max(share, (unsigned)p.least), ((unsigned)longest + p.parts - 1) / p.parts);
-    auto length = [&](int u) { // of a plane of the unit in the row
-        const unsigned T = (unsigned)max(unit_of<LISTS>(p, u).T, 1);
+    auto length = [&](int chunks) __attribute__((always_inline)) {  // of a plane of so many, in the row
+        const unsigned T = (unsigned)max(chunks, 1);
         return cuts ? (T + share - 1) / share : T;
     };
     if (cuts) {
         mine = 0;
+        if (per_lane == 1)
+            mine = lane < U ? (int)length(own.T) : 0;
+        else
 #pragma unroll 1
-        for (int j = 0; j < per_lane; j++) {
-            const int u = lane * per_lane + j;
-            if (u < U) mine += (int)length(u);
-        }
+            for (int j = 0; j < per_lane; j++) {
+                const int u = lane * per_lane + j;
+                if (u < U) mine += (int)length(unit_of<LISTS>(p, u).T);
+            }
         upto = scan(mine, plus);
         total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
     }
@@ -308,17 +322,22 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     if (x0 >= total) return;
     int u;
     unsigned base;  // of unit u
+    Unit unit;
     {
         const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < (unsigned)upto * M)) - 1;  // the lane whose units hold x0
         base = (unsigned)__builtin_amdgcn_readlane(upto - mine, at) * M;
         u = at * per_lane;
-        if (per_lane > 1)
+        if (per_lane == 1) {
+            unit = of_lane(own, at);
+        } else {
 #pragma unroll 1
             for (;; u++) {
-                const unsigned next = base + length(u) * M;
+                unit = of_lane(unit_of<LISTS>(p, u), 0);
+                const unsigned next = base + length(unit.T) * M;
                 if (x0 < next) break;
                 base = next;
             }
+        }
     }
 
     // Of the workgroups of a compute unit the oldest goes first and is done when others have a third of their piece left; so the
@@ -327,7 +346,6 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     unsigned x = x0, lower_at = share / 4;
     while (x < x1) {
         const unsigned done = cuts ? 0u : x - x0;
-        const Unit unit = unit_of<LISTS>(p, u);
         const unsigned T = (unsigned)max(unit.T, 1), row_T = cuts ? (T + share - 1) / share : T;
         const unsigned m = (x - base) / row_T, at_row = x - base - m * row_T;
         const unsigned plane_at = x - at_row;  // in the row
@@ -341,9 +359,9 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             base += row_T * M;
             u++;
         }
-
-        const int len = min(max(p.t.lens[b], 0), p.t.width << lP);
-        const int cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.Sq) : p.Sq;
+        const int len = unit.len, cnt = unit.cnt, T0 = unit.T0, F = unit.F;
+        const bool keys = unit.T > 0;
+        if (x < x1 && x == base) unit = of_lane(unit_of<LISTS>(p, u), 0);  // (the next segment's)
         // this lane's row: query i of query head g
         const int row = ROWS * rt + lrow, g = row / p.Sq, i = row - g * p.Sq;
         const bool live = row < p.R && i < cnt;
@@ -356,14 +374,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
 #pragma unroll
             for (int c = 0; c < X::NQ; c++) qf[c] = live ? *(const u32x4 *)(qp + X::d_of_q(c, lgrp)) : u32x4{0u, 0u, 0u, 0u};
         }
-        const int32_t *fid = nullptr, *pid = nullptr;
-        int F = 0;
-        if constexpr (LISTS) {
-            fid = p.full_ids + b * p.fis[0] + h * p.fis[1];
-            pid = p.part_ids + b * p.pis[0] + h * p.pis[1];
-            F = min(max(p.full_lens[b * p.fls[0] + h * p.fls[1]], 0), p.nK);
-        }
-        const uint8_t *const bits = LISTS ? p.packed + b * p.pks[0] + h * p.pks[1] + ((int64_t)i << (lP - 3)) : nullptr;
+        const uint32_t bits_i = (uint32_t)i << (lP - 3);
 
         float m_ref = 0.f, raise_above = -3.0e38f, l = 0.f;
         X out_rows;
@@ -375,29 +386,31 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             int block, tile, slot;  // block of the pool or -1; with lists the tile, and the slot of a PARTIAL one or -1
             float ks, vs;
         };
-        auto places = [&](int j0) {
-            Places r{-1, 0, -1, 0.f, 0.f};
+        auto places = [&](int j0) __attribute__((always_inline)) {
+            int block = -1, at_tile = 0, slot = -1;
+            float ks = 0.f, vs = 0.f;
             const int j = j0 + lane;
-            const int t = unit.T0 + off + wave + kWaves * j;
-            if (j < nw && unit.T > 0) {
+            const int t = T0 + off + wave + kWaves * j;
+            if (j < nw && keys) {
                 int tile = t >> p.c.lper;
                 if constexpr (LISTS) {
-                    if (tile >= F) r.slot = tile - F;
-                    tile = tile < F ? fid[(int64_t)tile * p.fis[2]] : pid[(int64_t)(tile - F) * p.pis[2]];
+                    if (tile >= F) slot = tile - F;
+                    tile = tile < F ? p.full_ids[b * p.fis[0] + h * p.fis[1] + (int64_t)tile * p.fis[2]] : p.part_ids[b * p.pis[0] + h * p.pis[1] + (int64_t)(tile - F) * p.pis[2]];
                     if (tile < 0 || tile >= p.nK) tile = p.t.width;
                 }
                 const int sub = t & sub_mask;
                 if (tile < p.t.width) {
-                    r.tile = tile;
+                    at_tile = tile;
                     const int page = p.t.ids[b * p.t.s0 + tile * p.t.s1];
                     // (nothing attends to keys of a page that does not exist)
-                    if ((tile << lP) + (sub << 5) < len && page >= 0 && page < p.c.pages) r.block = ((page * p.c.H + h) << p.c.lper) + sub;
+                    if ((tile << lP) + (sub << 5) < len && page >= 0 && page < p.c.pages) block = ((page * p.c.H + h) << p.c.lper) + sub;
                 }
             }
-            const int at = max(r.block, 0);
-            r.ks = p.c.k_scales[at];
-            r.vs = p.c.v_scales[at];
-            return r;
+            if (block >= 0) {
+                ks = p.c.k_scales[block];
+                vs = p.c.v_scales[block];
+            }
+            return Places{block, at_tile, slot, ks, vs};
         };
         // What is requested next takes the registers of what has just gone into a product: K of the next chunk is on its way during
         // the softmax and the second product, V behind it.  More registers for that would cost waves, which hide as much.
@@ -405,13 +418,13 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             int block, key0, slot;
             uint32_t bits;
         };
-        auto chunk = [&](const Places &at, int j) {
-            const int t = unit.T0 + off + wave + kWaves * j;
+        auto chunk = [&](const Places &at, int j) __attribute__((always_inline)) {
+            const int t = T0 + off + wave + kWaves * j;
             Chunk c{__builtin_amdgcn_readlane(at.block, j & 63), t << 5, -1, 0u};
             if constexpr (LISTS) {
                 c.key0 = (__builtin_amdgcn_readlane(at.tile, j & 63) << lP) + ((t & sub_mask) << 5);
                 c.slot = __builtin_amdgcn_readlane(at.slot, j & 63);
-                c.bits = *(const uint32_t *)(bits + ((int64_t)max(c.slot, 0) * p.Sq << (lP - 3)) + ((t & sub_mask) << 2));
+                c.bits = *(const uint32_t *)(p.packed + b * p.pks[0] + h * p.pks[1] + ((int64_t)max(c.slot, 0) * p.Sq << (lP - 3)) + ((t & sub_mask) << 2) + bits_i);
             }
             return c;
         };
@@ -542,14 +555,14 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             }
             s.M = M;
         };
-        auto finish = [&](int r, int d0, Sum s) {
+        auto finish = [&](int r, int d0, const Sum &s) __attribute__((always_inline)) {
             const int at = ROWS * rt + r, gg = at / p.Sq, ii = at - gg * p.Sq, head = h * p.G + gg;
             const float inv = s.L == 0.f ? 0.f : 1.f / s.L;
-            if (ii >= cnt) s.x = f32x4{0.f, 0.f, 0.f, 0.f};
+            const f32x4 y = ii >= cnt ? f32x4{0.f, 0.f, 0.f, 0.f} : s.x;
             if (p.lse != nullptr && d0 == 0)
                 p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
                     ii >= cnt || s.L == 0.f ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
-            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(s.x.x * inv, s.x.y * inv), E::pack2(s.x.z * inv, s.x.w * inv)};
+            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x * inv, y.y * inv), E::pack2(y.z * inv, y.w * inv)};
         };
         const bool whole = n == (int)T;
         const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
