@@ -499,7 +499,7 @@ int sa_sparse_attention_decode_mask(const void *q, const int64_t q_strides[4], c
  * A pool of pages of page_size tokens (32, 64, 128 or 256) of all H K/V heads; a sequence's tokens lie in the pages that its row of a
  * page table names.  Blocks of 32 consecutive tokens of one head are held as e4m3 codes (float8_e4m3fn) with a scale 2^e: e is the least
  * integer with max|x| <= 448 * 2^e over the block's finite values, from -96 to 119; x is held as round(x / 2^e) * 2^e, NaN and infinities
- * as NaN.  D is 64, 128 or 256.
+ * as NaN.  D is 64, 128 or 256; the callers' tensors have head_dim columns, a multiple of 8 up to D, the pool's further ones are zero.
  *   k, v               uint8 [num_pages, H, page_size / 32, 32 * D], contiguous, 16-byte aligned; the order inside a block is the kernels' own
  *                      (csrc/paged.h): sa_paged_cache_gather gives the values
  *   k_scales, v_scales float32 [num_pages, H, page_size / 32], contiguous
@@ -514,11 +514,11 @@ typedef struct sa_paged_cache {
     uint8_t *k, *v;
     float *k_scales, *v_scales;
     int num_pages; /* 1 .. 2^20 */
-    int H, page_size, D;
+    int H, page_size, D, head_dim;
 } sa_paged_cache;
 
 /*
- * Stores new tokens: the first counts[b] (NULL: all S) rows of k, v [B,H,S,D] (bf16 or fp16, strides multiples of 8 elements, last dimension
+ * Stores new tokens: the first counts[b] (NULL: all S) rows of k, v [B,H,S,head_dim] (bf16 or fp16, strides multiples of 8 elements, last dimension
  * contiguous, 16-byte aligned) become tokens lens[b] .. lens[b] + counts[b] - 1 of sequence b.  lens is not changed.  Tokens past the
  * table are not stored.  A block that holds tokens keeps its scale or takes a larger one, with which what it holds is rounded again.
  */
@@ -527,7 +527,7 @@ int sa_paged_cache_append(const sa_paged_cache *cache, const void *k, const int6
                           const int32_t *lens, const int32_t *counts, int B, int S, int pages_per_sequence, int dtype,
                           void *stream);
 
-/* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,D] (bf16 or fp16, as above); rows from lens[b] on are zero. */
+/* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,head_dim] (bf16 or fp16, as above); rows from lens[b] on are zero. */
 int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_strides[4], void *v, const int64_t v_strides[4],
                           const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, int B, int length,
                           int pages_per_sequence, int dtype, void *stream);
@@ -568,7 +568,7 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
                               void *stream);
 
 /*
- * sa_sparse_attention_decode over the cache: q, o [B,Hq,Sq,D], Sq <= 32, Hq a multiple of H (query heads h * Hq/H .. of K/V head h).
+ * sa_sparse_attention_decode over the cache: q, o [B,Hq,Sq,head_dim], Sq <= 32, Hq a multiple of H (query heads h * Hq/H .. of K/V head h).
  *   lens      the keys of every sequence, the call's own tokens among them (append, then attend)
  *   counts    device int32 [B], valid query rows of every sequence, or NULL for Sq; the rows behind give 0 and -inf
  *   without lists (all NULL) row i of sequence b attends to keys 0 .. lens[b] - counts[b] + i, with window > 0 to the last `window` of these

@@ -88,7 +88,7 @@ class PagedCacheStruct(ctypes.Structure):
     """sa_paged_cache of the C ABI."""
 
     _fields_ = ([(n, _vp) for n in ("k", "v", "k_scales", "v_scales")]
-                + [(n, ctypes.c_int) for n in ("num_pages", "H", "page_size", "D")])
+                + [(n, ctypes.c_int) for n in ("num_pages", "H", "page_size", "D", "head_dim")])
 
 
 class SparseAttnError(RuntimeError):

@@ -376,7 +376,7 @@ struct Cache {
     sa_paged_cache c;
     int64_t H() const { return c.H; }
     int64_t page() const { return c.page_size; }
-    int64_t Dk() const { return c.D; }
+    int64_t cols() const { return c.head_dim; }  // D, or the next multiple of 8, which the callers' tensors are brought to
 };
 // (read under the interpreter's lock)
 Cache cache_of(py::handle o) {
@@ -403,7 +403,7 @@ Cache cache_of(py::handle o) {
             value_error("cache scales must be contiguous float32 [pages, H, page_size / 32] on the cache's device, got " + str(*t));
     if (N > (1 << 20) || per > 8 || H > 0x7fffffff) value_error("cache of " + std::to_string(N) + " pages of " + std::to_string(32 * per) + " tokens");
     if (x.D < 1 || kernel_head_dim(x.D, true) != Dk) value_error("cache.head_dim " + std::to_string(x.D) + " does not belong to a pool of " + std::to_string(Dk));
-    x.c = {ptr<uint8_t>(x.k), ptr<uint8_t>(x.v), ptr<float>(x.k_scales), ptr<float>(x.v_scales), (int)N, (int)H, (int)(32 * per), (int)Dk};
+    x.c = {ptr<uint8_t>(x.k), ptr<uint8_t>(x.v), ptr<float>(x.k_scales), ptr<float>(x.v_scales), (int)N, (int)H, (int)(32 * per), (int)Dk, (int)((x.D + 7) / 8 * 8)};
     return x;
 }
 
@@ -445,7 +445,7 @@ void paged_append(py::object cache, const Tensor &k, const Tensor &v, const Tens
         if (t->device() != c.k.device()) value_error("k, v must be on the cache's device " + c.k.device().str() + ", got " + t->device().str());
     const int64_t S = k.size(2);
     if (B == 0 || S == 0) return;
-    const Tensor kc = kernel_ready(pad_head_dim(k, c.Dk())), vc = kernel_ready(pad_head_dim(v, c.Dk()));
+    const Tensor kc = kernel_ready(pad_head_dim(k, c.cols())), vc = kernel_ready(pad_head_dim(v, c.cols()));
     check_rc(sa_paged_cache_append(&c.c, kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), ptr<int32_t>(table), st(table), ptr<int32_t>(lens),
                                    ptr<int32_t>(counts), as_int(B, "B"), as_int(S, "S"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
 }
@@ -461,7 +461,7 @@ py::tuple paged_gather(py::object cache, const Tensor &table, const Tensor &lens
         const int dt = cache_dtype(dtype, "dtype");
         const int64_t n = length.value_or(table.size(1) * c.page());
         if (n < 0) value_error("length must not be negative (got " + std::to_string(n) + ")");
-        for (Tensor &t : out) t = at::empty({B, c.H(), n, c.Dk()}, at::TensorOptions().dtype(dtype).device(c.k.device()));
+        for (Tensor &t : out) t = at::empty({B, c.H(), n, c.cols()}, at::TensorOptions().dtype(dtype).device(c.k.device()));
         if (B > 0 && n > 0)
             check_rc(sa_paged_cache_gather(&c.c, out[0].data_ptr(), st(out[0]), out[1].data_ptr(), st(out[1]), ptr<int32_t>(table), st(table),
                                            ptr<int32_t>(lens), as_int(B, "B"), as_int(n, "length"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
@@ -588,13 +588,13 @@ py::object decode_paged(const Tensor &q, py::object cache, const Tensor &table, 
             tiles = Sk / P;
             l = classify_lists(mask->expand({B, H, Sq, Sk}), Sq, P, true);
         }
-        const Tensor qc = kernel_ready(pad_head_dim(q, c.Dk()));
+        const Tensor qc = kernel_ready(pad_head_dim(q, c.cols()));
         const Tensor o = at::empty_like(qc);
         const auto f32 = at::TensorOptions().dtype(at::kFloat).device(q.device());
         if (return_lse) r.lse = at::empty({B, Hq, Sq}, f32);
         if (B > 0 && Sq > 0) {
             const int Bi = as_int(B, "B"), pages = as_int(table.size(1), "pages"), w = window ? (int)std::min<int64_t>(*window, 1 << 30) : 0;
-            const size_t bytes = sa_decode_paged_workspace_bytes(Bi, as_int(Hq, "Hq"), (int)H, (int)Sq, (int)c.Dk(), pages, (int)P);
+            const size_t bytes = sa_decode_paged_workspace_bytes(Bi, as_int(Hq, "Hq"), (int)H, (int)Sq, c.c.D, pages, (int)P);
             Tensor ws;
             if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
             const bool lists = l.fid.defined();

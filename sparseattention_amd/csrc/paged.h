@@ -21,6 +21,7 @@ struct PagedPool {
     uint8_t *k, *v;            // [pages, H, per, 32 * D]
     float *k_scales, *v_scales;  // [pages, H, per]
     int pages, H, lper, D;     // per = page_size / 32 = 2^lper
+    int cols;                  // of the caller's tensors: a multiple of 8, at most D; the pool's others are zero
 };
 struct PageTable {
     const int32_t *ids;
@@ -101,17 +102,17 @@ struct PagedDecodeParams {
     int64_t pks[2];
     int nK;
     float scale;  // softmax scale / ln 2
-    // The launch's workgroups, the fewest chunks that one of them takes, and what planes that several of them share are added up by:
+    // The launch's workgroups, the most parts a plane has, and what planes that several workgroups share are added up by:
     //   ws        [groups][2][part_rows][D + 4] floats: unnormalised rows, reference value and sum of each
     //   arrivals  [planes + groups] words (all_arrived), the number of the launch
-    int groups, least, parts, cuts, part_rows;
+    int groups, parts, part_rows;
     float *ws;
     uint64_t *arrivals;
     uint64_t tag;
 };
 constexpr int kPagedMostParts = 64;  // of a plane (all_arrived looks at one word per lane)
 struct PagedDecodePlan {
-    int groups, least, parts, cuts, part_rows;
+    int groups, parts, part_rows;
     size_t parts_bytes, bytes;
 };
 PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus);

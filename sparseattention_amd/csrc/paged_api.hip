@@ -19,13 +19,15 @@ int pool_of(const char *who, const sa_paged_cache *c, sa::PagedPool &out) {
     if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
         return fail(SA_ERR_UNSUPPORTED, "%s: page_size must be 32, 64, 128 or 256 (got %d)", who, c->page_size);
     if (c->D != 64 && c->D != 128 && c->D != 256) return fail(SA_ERR_UNSUPPORTED, "%s: head dim %d not supported (64, 128 and 256 are)", who, c->D);
+    if (c->head_dim <= 0 || c->head_dim > c->D || c->head_dim % 8)
+        return fail(SA_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 up to %d (got %d)", who, c->D, c->head_dim);
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scales, 4) || !aligned(c->v_scales, 4))
         return fail(SA_ERR_UNSUPPORTED, "%s: the cache's codes must be 16-byte aligned", who);
     const int per = c->page_size / 32;
     if ((int64_t)c->num_pages * c->H * per > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 blocks in the cache", who);
     int lper = 0;
     while ((1 << lper) < per) lper++;
-    out = {c->k, c->v, c->k_scales, c->v_scales, c->num_pages, c->H, lper, c->D};
+    out = {c->k, c->v, c->k_scales, c->v_scales, c->num_pages, c->H, lper, c->D, c->head_dim};
     return SA_OK;
 }
 
@@ -274,9 +276,7 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
         return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, plan.bytes, workspace ? workspace_bytes : (size_t)0);
     p.groups = plan.groups;
-    p.least = plan.least;
     p.parts = plan.parts;
-    p.cuts = plan.cuts;
     p.part_rows = plan.part_rows;
     p.ws = static_cast<float *>(workspace);
     p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + plan.parts_bytes);

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_appen
     for (int i = 0; i < NL; i++) {
         const int r = RPI * i + r0;
         in[i] = u32x4{0u, 0u, 0u, 0u};
-        if (r >= a && r < z) in[i] = __builtin_nontemporal_load((const u32x4 *)(x + r * row + 8 * piece));
+        if (r >= a && r < z && 8 * piece < p.c.cols) in[i] = __builtin_nontemporal_load((const u32x4 *)(x + r * row + 8 * piece));
     }
     if (page < 0) return;
     const int64_t at = block_at(p.c, page, h, blk & ((1 << p.c.lper) - 1));
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const Pa
             const int r = RPI * i + r0, t = 16 * half + r;
             u32x4 y = u32x4{0u, 0u, 0u, 0u};
             if (t < n) y = *(const u32x4 *)(mine + r * row_bytes<ND> + 16 * piece);
-            if (t < rows) {
+            if (t < rows && 8 * piece < p.c.cols) {
                 u32x4 *const to = (u32x4 *)(x + t * xs[2] + 8 * piece);
                 if constexpr (FAR) __builtin_nontemporal_store(y, to);
                 else *to = y;
@@ -532,7 +532,7 @@ constexpr int64_t kGatherFar = 128ll << 20;
 
 hipError_t launch_paged_gather(const PagedGatherParams &p, int dtype, hipStream_t stream) {
     const unsigned blocks = ((unsigned)p.length + 31) / 32;
-    const bool far = (int64_t)p.t.B * p.c.H * p.length * p.c.D * 4 >= kGatherFar;
+    const bool far = (int64_t)p.t.B * p.c.H * p.length * p.c.cols * 4 >= kGatherFar;
     return with_sizes(dtype, p.c.D, [&](auto dt, auto nd) {
         constexpr int DT = decltype(dt)::value, ND = decltype(nd)::value;
         hipLaunchKernelGGL((far ? paged_gather_kernel<DT, ND, true> : paged_gather_kernel<DT, ND, false>), dim3((2u * p.c.H * blocks * p.t.B + kCacheWaves - 1) / kCacheWaves), dim3(64 * kCacheWaves), 0, stream, p);

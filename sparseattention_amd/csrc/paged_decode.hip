@@ -103,10 +103,17 @@ __device__ __forceinline__ int scan(int x, Op &&op) {  // op(0, x) == x for x >=
 
 // The products of a tile of ROWS query rows, S^T = K Q^T (32 keys) and O^T += V^T P^T, on 32 x 32 or 16 x 16 matrix instructions.
 // A lane has its row's share: row lane % ROWS, group lane / ROWS.
-template <int DT, int ND, int ROWS>
+// FAR: K and V are read once by the launch, past the caches (6.3 against 5.7 TB/s at 32 sequences of up to 32768 keys); not where
+// several tiles of rows read them.
+template <bool FAR, class T>
+__device__ __forceinline__ T load(const uint8_t *at) {
+    if constexpr (FAR) return __builtin_nontemporal_load((const T *)at);
+    else return *(const T *)at;
+}
+template <int DT, int ND, int ROWS, bool FAR>
 struct Tile;
-template <int DT, int ND>
-struct Tile<DT, ND, 32> {
+template <int DT, int ND, bool FAR>
+struct Tile<DT, ND, 32, FAR> {
     using E = Elem<DT>;
     static constexpr int NS = 16, NQ = 2 * ND, NA = 16 * ND;  // scores, registers of 8 queries' elements, output elements
     static __device__ __forceinline__ int d_of_q(int i, int g) { return 32 * (i >> 1) + 16 * g + 8 * (i & 1); }
@@ -117,11 +124,11 @@ struct Tile<DT, ND, 32> {
     };
     static __device__ __forceinline__ void load_k(Operands &c, const uint8_t *k, int lane) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) c.k[d] = __builtin_nontemporal_load((const u32x4 *)(k + 1024 * d + 16 * lane));
+        for (int d = 0; d < ND; d++) c.k[d] = load<FAR, u32x4>(k + 1024 * d + 16 * lane);
     }
     static __device__ __forceinline__ void load_v(Operands &c, const uint8_t *v, int lane) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) c.v[d] = __builtin_nontemporal_load((const u32x4 *)(v + 1024 * d + 16 * lane));
+        for (int d = 0; d < ND; d++) c.v[d] = load<FAR, u32x4>(v + 1024 * d + 16 * lane);
     }
     static __device__ __forceinline__ void scores(const Operands &c, const u32x4 (&q)[NQ], float (&s)[NS]) {
         f32x16 x;
@@ -184,8 +191,8 @@ struct Tile<DT, ND, 32> {
     static __device__ __forceinline__ float row_max(float x) { return half_swap_max(x); }
     static __device__ __forceinline__ float row_sum(float x) { return x + __shfl_xor(x, 32); }
 };
-template <int DT, int ND>
-struct Tile<DT, ND, 16> {
+template <int DT, int ND, bool FAR>
+struct Tile<DT, ND, 16, FAR> {
     using E = Elem<DT>;
     static constexpr int NS = 8, NQ = ND, NA = 8 * ND;
     static __device__ __forceinline__ int d_of_q(int i, int g) { return 64 * (i >> 1) + 16 * g + 8 * (i & 1); }
@@ -199,13 +206,13 @@ struct Tile<DT, ND, 16> {
         const int l = lane & 15, g = lane >> 4;
         k += 1024 * (g >> 1) + 16 * (32 * (g & 1) + l);
 #pragma unroll
-        for (int i = 0; i < ND; i++) c.k[i] = __builtin_nontemporal_load((const u32x4 *)(k + 2048 * (i >> 1) + 256 * (i & 1)));
+        for (int i = 0; i < ND; i++) c.k[i] = load<FAR, u32x4>(k + 2048 * (i >> 1) + 256 * (i & 1));
     }
     static __device__ __forceinline__ void load_v(Operands &c, const uint8_t *v, int lane) {
         const int l = lane & 15, g = lane >> 4;
         v += 16 * (32 * (g & 1) + l) + 8 * (g >> 1);
 #pragma unroll
-        for (int i = 0; i < 2 * ND; i++) c.v[i] = __builtin_nontemporal_load((const u32x2 *)(v + 1024 * (i >> 1) + 256 * (i & 1)));
+        for (int i = 0; i < 2 * ND; i++) c.v[i] = load<FAR, u32x2>(v + 1024 * (i >> 1) + 256 * (i & 1));
     }
     static __device__ __forceinline__ void scores(const Operands &c, const u32x4 (&q)[NQ], float (&s)[NS]) {
         f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -266,10 +273,10 @@ struct Tile<DT, ND, 16> {
     }
 };
 
-template <int DT, int ND, int ROWS, bool LISTS>
+template <int DT, int ND, int ROWS, bool FAR, bool LISTS>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
     using E = Elem<DT>;
-    using X = Tile<DT, ND, ROWS>;
+    using X = Tile<DT, ND, ROWS, FAR>;
     constexpr int D = 32 * ND, PST = D + kPagedRowPad;
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][ROWS][PST]
     const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
@@ -294,12 +301,15 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     int upto = scan(mine, plus);
     longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
     unsigned total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
-    // Few planes: a plane is cut into equal parts of up to `share` chunks, a workgroup each, so that none has two planes' latencies.
-    // The row is then one of parts.  Many: equal pieces of a row of chunks.
-    const bool cuts = p.cuts != 0;
-    unsigned share = (total + gridDim.x - 1) / gridDim.x;
-    if (cuts) share = (total + gridDim.x - U * M - 1) / (gridDim.x - U * M);
-    share = max(max(share, (unsigned)p.least), ((unsigned)longest + p.parts - 1) / p.parts);
+    // Either pieces of a row of chunks, wherever they begin and end; or every plane cut into equal parts of up to `share` chunks, a
+    // workgroup each, so that none has two planes' latencies (the row is then one of parts).  The second where there are several
+    // parts a plane, whose ends are then even, or where a part is short, so that latencies are all there is (the rule: paged_decode_plan).
+    const unsigned planes = U * M, groups = gridDim.x;
+    const unsigned parts = min((unsigned)p.parts, max(16u, (unsigned)__builtin_amdgcn_sqrtf(2.f * (float)longest)));
+    unsigned share = (total + groups - 1) / groups, even_share = planes < groups ? (total + groups - planes - 1) / (groups - planes) : total;
+    const bool cuts = planes < groups && (8 * planes <= groups || even_share <= 2 * kWaves);
+    if (cuts) share = max(even_share, (unsigned)kWaves);
+    share = max(share, ((unsigned)longest + parts - 1) / parts);
     auto length = [&](int chunks) __attribute__((always_inline)) {  // of a plane of so many, in the row
         const unsigned T = (unsigned)max(chunks, 1);
         return cuts ? (T + share - 1) / share : T;
@@ -372,7 +382,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         {
             const uint16_t *qp = p.q + b * p.qs[0] + (live ? (h * p.G + g) * p.qs[1] + i * p.qs[2] : 0);
 #pragma unroll
-            for (int c = 0; c < X::NQ; c++) qf[c] = live ? *(const u32x4 *)(qp + X::d_of_q(c, lgrp)) : u32x4{0u, 0u, 0u, 0u};
+            for (int c = 0; c < X::NQ; c++) qf[c] = live && X::d_of_q(c, lgrp) < p.c.cols ? *(const u32x4 *)(qp + X::d_of_q(c, lgrp)) : u32x4{0u, 0u, 0u, 0u};
         }
         const uint32_t bits_i = (uint32_t)i << (lP - 3);
 
@@ -562,7 +572,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             if (p.lse != nullptr && d0 == 0)
                 p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
                     ii >= cnt || s.L == 0.f ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
-            *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x * inv, y.y * inv), E::pack2(y.z * inv, y.w * inv)};
+            if (d0 < p.c.cols) *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x * inv, y.y * inv), E::pack2(y.z * inv, y.w * inv)};
         };
         const bool whole = n == (int)T;
         const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
@@ -658,22 +668,23 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     }
 }
 
-template <int DT, int ND, int ROWS, bool LISTS>
+template <int DT, int ND, int ROWS, bool FAR, bool LISTS>
 hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
     constexpr int smem = kWaves * ROWS * (32 * ND + kPagedRowPad) * 4;
-    auto kern = paged_decode_kernel<DT, ND, ROWS, LISTS>;
+    auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, LISTS>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)p.groups), dim3(kWaves * 64), smem, stream, p);
     return hipGetLastError();
 }
-template <int DT, int ND, int ROWS>
+template <int DT, int ND, int ROWS, bool FAR>
 hipError_t launch_lists(const PagedDecodeParams &p, hipStream_t stream) {
-    return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, true>(p, stream) : launch_kind<DT, ND, ROWS, false>(p, stream);
+    return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, FAR, true>(p, stream) : launch_kind<DT, ND, ROWS, FAR, false>(p, stream);
 }
 template <int DT, int ND>
 hipError_t launch_rows(const PagedDecodeParams &p, hipStream_t stream) {
-    return p.R <= 16 ? launch_lists<DT, ND, 16>(p, stream) : launch_lists<DT, ND, 32>(p, stream);
+    if (p.R <= 16) return launch_lists<DT, ND, 16, true>(p, stream);
+    return p.RT == 1 ? launch_lists<DT, ND, 32, true>(p, stream) : launch_lists<DT, ND, 32, false>(p, stream);
 }
 template <int DT>
 hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {
@@ -687,19 +698,18 @@ hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {
 
 // As many workgroups as the device holds at once: with more, the pieces of a workgroup that starts late do not make up for its start
 // (32 sequences of up to 32768 keys: 294 us; twice as many workgroups 304, four times 324).
-// Planes are cut where they are few, so that a plane is many parts and their ends are even: at 8 parts a plane (64 planes of 129 chunks)
-// 21.5 -> 18.3 us, 8 planes of 63 chunks 12.1 -> 9.1; at 3 (256 planes of 700 ... 1024) it would be 290 -> 319.
-// Parts are added up by one workgroup, 8 to 32 at a time, so there are no more of them than give every compute unit one, but at
-// least 16: 16 planes of 1000 chunks with 16 | 32 | 62 parts 32.3 | 37.9 | 41.6 us.
+// Planes are cut evenly where they are few, so that a plane is many parts and their ends are even: at 8 parts a plane (64 planes of
+// 129 chunks) 21.5 -> 18.3 us, 8 planes of 63 chunks 12.1 -> 9.1; at 3 (256 planes of 700 ... 1024) it would be 290 -> 319.
+// One workgroup adds a plane's parts up, 8 to 32 at a time.  So there are no more of them than let every compute unit read at full speed (a
+// chunk of 8 KiB a wave, one workgroup each, or two of 4 KiB), but at least 16: 16 planes of 1000 chunks with 16 | 32 | 62 parts 32.3 |
+// 37.9 | 41.6 us; and no more than balance the chunks a wave has one after the other (1.15 us each) with the sum: sqrt(2 T) of T chunks.
 PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus) {
     PagedDecodePlan r;
-    r.least = kWaves;
-    const int64_t even = cus / planes;
+    const int64_t even = (int64_t)cus * (D == 64 ? 2 : 1) / planes;
     r.parts = (int)(even < 16 ? 16 : even < kPagedMostParts - 2 ? even : kPagedMostParts - 2);
     const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
-    r.cuts = 8 * planes <= resident;
-    const int64_t fine = (chunks + r.least - 1) / r.least;  // parts of a plane of that many chunks each
-    const int64_t most = r.cuts ? planes * ((fine < r.parts ? fine : r.parts) + 1) : planes * fine;
+    const int64_t fine = (chunks + kWaves - 1) / kWaves;  // parts of a plane of a chunk a wave
+    const int64_t most = planes * ((fine < r.parts ? fine : r.parts) + 1);
     r.groups = (int)(most < resident ? most : resident);
     r.part_rows = R < 32 ? R : 32;
     r.parts_bytes = (size_t)r.groups * 2 * r.part_rows * (D + kPagedRowPad) * 4;

@@ -14,8 +14,8 @@ S3 = _native.strides((8, 8, 1))
 S4 = _native.strides((1024, 128, 128, 1))
 
 
-def pool(k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, pages=8, H=2, page=64, D=128):
-    return ctypes.byref(_native.PagedCacheStruct(k, v, ks, vs, pages, H, page, D))
+def pool(k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, pages=8, H=2, page=64, D=128, cols=128):
+    return ctypes.byref(_native.PagedCacheStruct(k, v, ks, vs, pages, H, page, D, cols))
 
 
 def append(c=None, k=FAKE, ks=S4, table=FAKE, lens=FAKE, B=1, S=4, pages=4, dtype=0):
@@ -37,6 +37,7 @@ def test_pools(call):
     assert call(pool(k=None)) == BAD and call(pool(vs=None)) == BAD
     assert call(pool(pages=0)) == BAD and call(pool(pages=(1 << 20) + 1)) == BAD and call(pool(H=0)) == BAD
     assert call(pool(page=16)) == UNSUPPORTED and call(pool(page=48)) == UNSUPPORTED and call(pool(page=512)) == UNSUPPORTED
+    assert call(pool(cols=0)) == UNSUPPORTED and call(pool(cols=132)) == UNSUPPORTED and call(pool(cols=60)) == UNSUPPORTED
     assert call(pool(D=80)) == UNSUPPORTED and call(pool(k=FAKE + 8)) == UNSUPPORTED
     assert call(pool(pages=1 << 20, H=1024, page=256)) == UNSUPPORTED
     assert call(B=0) == BAD and call(dtype=2) == UNSUPPORTED
