@@ -20,7 +20,7 @@ constexpr int kWaves = 4;
 constexpr int kPagedRowPad = 4;  // floats behind a row of a part: reference value and sum, and two that keep rows 16-byte aligned
 
 // Workgroups that a compute unit holds (a wave of each per SIMD).
-constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 4 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
+constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
 
 template <int DT>
 struct Codes;  // eight codes as an operand, times a power of two
@@ -427,8 +427,10 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             }
             return Places{block, at_tile, slot, ks, vs};
         };
-        // What is requested next takes the registers of what has just gone into a product: K of the next chunk is on its way during
-        // the softmax and the second product, V behind it.  More registers for that would cost waves, which hide as much.
+        // What is requested next takes the registers of what has just gone into a product: K of a later chunk is on its way during the
+        // softmax and the second product, V behind it.  At D = 64 two chunks are under way, as their bytes are half as many; with
+        // more registers for more there would be fewer waves, which hide as much.
+        constexpr int PRE = ND == 2 ? 2 : 1;
         struct Chunk {
             int block, key0, slot;
             uint32_t bits;
@@ -443,17 +445,20 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             }
             return c;
         };
-        typename X::Operands x;
-        auto request_k = [&](const Chunk &c) { X::load_k(x, p.c.k + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
-        auto request_v = [&](const Chunk &c) { X::load_v(x, p.c.v + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
-        // (of a round of 64 chunks: their places; of the round behind it, on their way)
+        auto request_k = [&](const Chunk &c, typename X::Operands &x) { X::load_k(x, p.c.k + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
+        auto request_v = [&](const Chunk &c, typename X::Operands &x) { X::load_v(x, p.c.v + (int64_t)max(c.block, 0) * (1024 * ND), lane); };
+        // (of the round of 64 chunks that is requested: their places; of the round behind it, on their way; of the round at hand: scales)
         Places here = places(0), next = places(64);
-        Chunk c = chunk(here, 0);
-        if (nw > 0) {
-            request_k(c);
-            request_v(c);
-        }
-        for (int j = 0; j < nw; j++) {
+        float ks_at = 0.f, vs_at = 0.f;
+        typename X::Operands ops[PRE];
+        Chunk under_way[PRE];
+        if (nw > 0)
+            static_for<PRE>([&](auto i) {
+                under_way[i] = chunk(here, min((int)i, nw - 1));  // (behind the last chunk: that one again)
+                request_k(under_way[i], ops[i]);
+                request_v(under_way[i], ops[i]);
+            });
+        auto step = [&](int j, Chunk &c, typename X::Operands &x) __attribute__((always_inline)) {
             if (done + 4u * j >= lower_at) {
                 const unsigned quarter = (done + 4u * j) * 4u / share;
                 lower_at = (quarter + 1) * share / 4;
@@ -461,17 +466,22 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 else if (quarter == 2) __builtin_amdgcn_s_setprio(1);
                 else if (quarter >= 3) __builtin_amdgcn_s_setprio(0);
             }
-            const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.ks), j & 63))) * p.scale;
-            const float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(here.vs), j & 63)));
-            if (((j + 1) & 63) == 0 && j + 1 < nw) {
-                here = next;
-                next = places(j + 65);  // (none behind the last chunk)
+            if ((j & 63) == 0) {
+                ks_at = here.ks;
+                vs_at = here.vs;
             }
-            const Chunk nc = chunk(here, min(j + 1, nw - 1));  // (behind the last one: that one again)
+            const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_at), j & 63))) * p.scale;
+            const float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_at), j & 63)));
+            const int jn = j + PRE;
+            if ((jn & 63) == 0 && jn < nw) {
+                here = next;
+                next = places(jn + 64);  // (none behind the last chunk)
+            }
+            const Chunk nc = chunk(here, min(jn, nw - 1));
             const int key0 = c.key0;
             float s[X::NS];
             X::scores(x, qf, s);
-            request_k(nc);
+            request_k(nc, x);
 
             // which keys the lane's row attends to, key k in bit k; `cut`: not all of them for every row
             // (a chunk that does not exist goes through as one that no row attends to: a way around it doubles the registers)
@@ -531,9 +541,13 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 }
             }
             out_rows.add(x, pw, vs);
-            request_v(nc);
+            request_v(nc, x);
             c = nc;
-        }
+        };
+        for (int j0 = 0; j0 < nw; j0 += PRE)
+            static_for<PRE>([&](auto i) {
+                if (j0 + i < nw) step(j0 + i, under_way[i], ops[i]);
+            });
 
         // ---- the waves' parts, added up in LDS ----
         l = X::row_sum(l);
