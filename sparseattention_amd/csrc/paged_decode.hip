@@ -282,21 +282,22 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lP = p.c.lper + 5, sub_mask = (1 << p.c.lper) - 1;
+    auto by_rows = [&](int row) { return p.Sq == 1 ? row : row / p.Sq; };  // (a division costs as much as a step of the scan)
 
     // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in (the host: a row is less than 2^31 chunks) ----
     const int U = LISTS ? p.t.B * p.c.H : p.t.B;                // units
     const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;  // planes of each
     const int per_lane = (U + 63) >> 6;
-    int mine = 0, longest = 0;
-    Unit own{0, 0, 0, 0, 0};  // the lane's last unit (the only one of up to 64 units)
-#pragma unroll 1
-    for (int j = 0; j < per_lane; j++) {
-        const int u = lane * per_lane + j;
-        own = unit_of<LISTS>(p, min(u, U - 1));
-        const int T = u < U ? max(own.T, 1) : 0;
-        mine += T;
-        longest = max(longest, T);
-    }
+    Unit own = unit_of<LISTS>(p, min(lane * per_lane, U - 1));  // the lane's first unit (the only one of up to 64 units)
+    int mine = lane * per_lane < U ? max(own.T, 1) : 0, longest = mine;
+    if (per_lane > 1)
+#pragma unroll 4
+        for (int j = 1; j < per_lane; j++) {
+            const int u = lane * per_lane + j;
+            const int T = u < U ? max(unit_of<LISTS>(p, min(u, U - 1)).T, 1) : 0;
+            mine += T;
+            longest = max(longest, T);
+        }
     const auto plus = [](int a, int x) { return a + x; };
     int upto = scan(mine, plus);
     longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
@@ -306,10 +307,12 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     // parts a plane, whose ends are then even, or where a part is short, so that latencies are all there is (the rule: paged_decode_plan).
     const unsigned planes = U * M, groups = gridDim.x;
     const unsigned parts = min((unsigned)p.parts, max(16u, (unsigned)__builtin_amdgcn_sqrtf(2.f * (float)longest)));
-    unsigned share = (total + groups - 1) / groups, even_share = planes < groups ? (total + groups - planes - 1) / (groups - planes) : total;
-    const bool cuts = planes < groups && (8 * planes <= groups || even_share <= 2 * kWaves);
-    if (cuts) share = max(even_share, (unsigned)kWaves);
-    share = max(share, ((unsigned)longest + parts - 1) / parts);
+    // (divisions cost a step of the scan each: as few as can be)
+    const bool cuts = planes < groups && (8 * planes <= groups || total <= 2 * kWaves * (groups - planes));
+    const unsigned among = cuts ? groups - planes : groups;
+    unsigned share = (total + among - 1) / among;
+    if (cuts) share = max(share, (unsigned)kWaves);
+    if ((uint64_t)longest > (uint64_t)share * parts) share = ((unsigned)longest + parts - 1) / parts;
     auto length = [&](int chunks) __attribute__((always_inline)) {  // of a plane of so many, in the row
         const unsigned T = (unsigned)max(chunks, 1);
         return cuts ? (T + share - 1) / share : T;
@@ -319,10 +322,11 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         if (per_lane == 1)
             mine = lane < U ? (int)length(own.T) : 0;
         else
-#pragma unroll 1
+#pragma unroll 4
             for (int j = 0; j < per_lane; j++) {
                 const int u = lane * per_lane + j;
-                if (u < U) mine += (int)length(unit_of<LISTS>(p, u).T);
+                const int n = (int)length(unit_of<LISTS>(p, min(u, U - 1)).T);
+                mine += u < U ? n : 0;
             }
         upto = scan(mine, plus);
         total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
@@ -342,16 +346,21 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < (unsigned)upto * M)) - 1;  // the lane whose units hold x0
         base = (unsigned)__builtin_amdgcn_readlane(upto - mine, at) * M;
         u = at * per_lane;
-        if (per_lane == 1) {
-            unit = of_lane(own, at);
-        } else {
-#pragma unroll 1
-            for (;; u++) {
-                unit = of_lane(unit_of<LISTS>(p, u), 0);
-                const unsigned next = base + length(unit.T) * M;
-                if (x0 < next) break;
-                base = next;
+        if (per_lane == 1) unit = of_lane(own, at);
+        // its units by 64, a lane each
+        for (int j0 = 0; per_lane > 1; j0 += 64) {
+            own = unit_of<LISTS>(p, min(u + j0 + lane, U - 1));
+            const int n = j0 + lane < per_lane && u + j0 + lane < U ? (int)length(own.T) : 0;
+            const int to = scan(n, plus);
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(x0 < base + (unsigned)to * M);
+            if (hit != 0ull) {
+                const int in = __ffsll((unsigned long long)hit) - 1;
+                unit = of_lane(own, in);
+                base += (unsigned)__builtin_amdgcn_readlane(to - n, in) * M;
+                u += j0 + in;
+                break;
             }
+            base += (unsigned)__builtin_amdgcn_readlane(to, 63) * M;
         }
     }
 
@@ -359,15 +368,17 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     // further a workgroup is, the lower its priority.
     __builtin_amdgcn_s_setprio(3);
     unsigned x = x0, lower_at = share / 4;
+    int quarter = 0;
     while (x < x1) {
         const unsigned done = cuts ? 0u : x - x0;
-        const unsigned T = (unsigned)max(unit.T, 1), row_T = cuts ? (T + share - 1) / share : T;
-        const unsigned m = (x - base) / row_T, at_row = x - base - m * row_T;
+        const unsigned T = (unsigned)max(unit.T, 1), row_T = length(unit.T);
+        const unsigned m = M == 1 ? 0u : (x - base) / row_T, at_row = x - base - m * row_T;
         const unsigned plane_at = x - at_row;  // in the row
         // chunks off .. off + n - 1 of this plane
-        const int off = (int)(cuts ? T * at_row / row_T : at_row), n = (int)(cuts ? T * (at_row + 1) / row_T - off : min(T - at_row, x1 - x));
+        const unsigned even = cuts ? (T + row_T - 1) / row_T : 0u;  // (at most `share`, and row_T of them are no fewer than needed)
+        const int off = (int)(cuts ? at_row * even : at_row), n = (int)min(T - off, cuts ? even : x1 - x);
         const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + (int)m : (int)m;
-        const int h = hr / p.RT, rt = hr - h * p.RT;
+        const int h = p.RT == 1 ? hr : hr / p.RT, rt = hr - h * p.RT;
         const int plane = (b * p.c.H + h) * p.RT + rt;
         x += cuts ? 1 : n;
         if (m + 1 == M && x - plane_at == row_T) {
@@ -378,7 +389,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         const bool keys = unit.T > 0;
         if (x < x1 && x == base) unit = of_lane(unit_of<LISTS>(p, u), 0);  // (the next segment's)
         // this lane's row: query i of query head g
-        const int row = ROWS * rt + lrow, g = row / p.Sq, i = row - g * p.Sq;
+        const int row = ROWS * rt + lrow, g = by_rows(row), i = row - g * p.Sq;
         const bool live = row < p.R && i < cnt;
         // without lists it sees the keys from `lo` to `hi`
         const int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
@@ -460,11 +471,11 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             });
         auto step = [&](int j, Chunk &c, typename X::Operands &x) __attribute__((always_inline)) {
             if (done + 4u * j >= lower_at) {
-                const unsigned quarter = (done + 4u * j) * 4u / share;
-                lower_at = (quarter + 1) * share / 4;
+                lower_at += share / 4;
+                quarter++;
                 if (quarter == 1) __builtin_amdgcn_s_setprio(2);
                 else if (quarter == 2) __builtin_amdgcn_s_setprio(1);
-                else if (quarter >= 3) __builtin_amdgcn_s_setprio(0);
+                else if (quarter == 3) __builtin_amdgcn_s_setprio(0);
             }
             if ((j & 63) == 0) {
                 ks_at = here.ks;
@@ -585,13 +596,14 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             s.M = M;
         };
         auto finish = [&](int r, int d0, const Sum &s) __attribute__((always_inline)) {
-            const int at = ROWS * rt + r, gg = at / p.Sq, ii = at - gg * p.Sq, head = h * p.G + gg;
-            const float inv = s.L == 0.f ? 0.f : 1.f / s.L;
-            const f32x4 y = ii >= cnt ? f32x4{0.f, 0.f, 0.f, 0.f} : s.x;
+            const int at = ROWS * rt + r, gg = by_rows(at), ii = at - gg * p.Sq, head = h * p.G + gg;
+            const bool none = ii >= cnt || s.L == 0.f;  // (a row of padding may have met a NaN)
+            const float inv = 1.f / s.L;
+            const f32x4 y = none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{s.x.x * inv, s.x.y * inv, s.x.z * inv, s.x.w * inv};
             if (p.lse != nullptr && d0 == 0)
                 p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
-                    ii >= cnt || s.L == 0.f ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
-            if (d0 < p.c.cols) *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x * inv, y.y * inv), E::pack2(y.z * inv, y.w * inv)};
+                    none ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
+            if (d0 < p.c.cols) *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x, y.y), E::pack2(y.z, y.w)};
         };
         const bool whole = n == (int)T;
         const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
@@ -617,7 +629,8 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             }
         }
         if (!whole) {
-            const int g0 = (int)(plane_at / piece), parts = (int)((plane_at + row_T - 1) / piece) - g0 + 1;  // workgroups of the plane
+            // workgroups of the plane
+            const int g0 = (int)(cuts ? plane_at : plane_at / piece), parts = cuts ? (int)row_T : (int)((plane_at + row_T - 1) / piece) - g0 + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();  // every wave's rows have been handed over, and LDS has been read
             int *const told = reinterpret_cast<int *>(part + D + 2);  // (behind a row: the sum below leaves it alone)

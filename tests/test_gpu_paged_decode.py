@@ -88,6 +88,9 @@ def check(cache, table, lens, q, o, lse=None, see=None, counts=None, window=None
     (1, 2, 4, 128, 64, 1, [20011], torch.bfloat16),
     (1, 1, 1, 64, 32, 17, [9000], torch.float16),
     (40, 8, 1, 64, 64, 1, [37 * i % 1501 for i in range(40)], torch.bfloat16),
+    (130, 1, 3, 64, 32, 1, [53 * i % 200 for i in range(130)], torch.float16),
+    (300, 8, 1, 64, 32, 1, [7 * i % 90 for i in range(300)], torch.bfloat16),
+    (6, 2, 5, 128, 64, 32, [900, 33, 0, 400, 2500, 1], torch.bfloat16),
 ])
 def test_causal(gpu, B, H, G, D, P, Sq, lens, dtype):
     cache, table = make(B, H, D, P, lens, dtype, 0, gpu)
@@ -115,6 +118,13 @@ def test_padded_batch(gpu):
     for window in (None, 40):
         o, lse = sa.sparse_attention_decode_paged(q, cache, table, ints(lens, gpu), counts=ints(counts, gpu), window=window, return_lse=True)
         check(cache, table, lens, q, o, lse, counts=counts, window=window)
+    # a NaN that rows of padding meet
+    k = torch.full((7, 2, 1, 128), float("nan"), dtype=torch.bfloat16, device=gpu)
+    sa.paged_cache_append(cache, k, k, table, ints([2] * 7, gpu))
+    for window in (None, 40):
+        o, lse = sa.sparse_attention_decode_paged(q, cache, table, ints(lens, gpu), counts=ints(counts, gpu), window=window, return_lse=True)
+        check(cache, table, lens, q, o, lse, counts=counts, window=window)
+    cache, table = make(7, 2, 128, 32, [128] * 7, torch.bfloat16, 4, gpu)
     seen = torch.rand(7, 2, 3, 128, generator=torch.Generator().manual_seed(0)) < 0.5
     o, lse = sa.sparse_attention_decode_paged(q, cache, table, ints(lens, gpu), seen.to(gpu), counts=ints(counts, gpu), return_lse=True)
     check(cache, table, lens, q, o, lse, see=seen, counts=counts)
@@ -138,9 +148,10 @@ def masks(kind, B, H, Sq, Sk, P, seed):
 @pytest.mark.parametrize("kind", ["tiles", "rows", "none", "all"])
 @pytest.mark.parametrize("B,H,G,D,P,Sq,Sk,dtype", [(2, 2, 1, 128, 32, 1, 320, torch.bfloat16), (2, 3, 2, 64, 64, 5, 1024, torch.float16),
                                                    (1, 2, 4, 128, 128, 32, 512, torch.bfloat16), (2, 1, 3, 256, 256, 2, 768, torch.bfloat16),
-                                                   (3, 2, 5, 128, 32, 9, 4096, torch.float16)])
+                                                   (3, 2, 5, 128, 32, 9, 4096, torch.float16), (70, 3, 1, 64, 32, 2, 192, torch.bfloat16),
+                                                   (24, 40, 1, 64, 32, 1, 96, torch.float16)])
 def test_lists(gpu, kind, B, H, G, D, P, Sq, Sk, dtype):
-    lens = [Sk - 7, Sk // 2 + 3, Sk][:B]
+    lens = [(Sk - 7, Sk // 2 + 3, Sk)[b % 3] for b in range(B)]
     cache, table = make(B, H, D, P, lens, dtype, 6, gpu, width=Sk // P + 1)
     q = queries(B, H * G, Sq, D, dtype, 7, gpu)
     see = masks(kind, B, H, Sq, Sk, P, 8)
