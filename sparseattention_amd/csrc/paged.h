@@ -103,6 +103,7 @@ struct PagedDecodeParams {
     int nK;
     float scale;  // softmax scale / ln 2
     // The launch's workgroups, the most parts a plane has, and what planes that several workgroups share are added up by:
+    // (paged_pieces.h)
     //   ws        [groups][2][part_rows][D + 4] floats: unnormalised rows, reference value and sum of each
     //   arrivals  [planes + groups] words (all_arrived), the number of the launch
     int groups, parts, part_rows;
@@ -110,12 +111,8 @@ struct PagedDecodeParams {
     uint64_t *arrivals;
     uint64_t tag;
 };
-constexpr int kPagedMostParts = 64;  // of a plane (all_arrived looks at one word per lane)
-struct PagedDecodePlan {
-    int groups, parts, part_rows;
-    size_t parts_bytes, bytes;
-};
-PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus);
+// Bytes of ws.
+size_t paged_decode_parts_bytes(int groups, int part_rows, int D);
 hipError_t launch_paged_decode(const PagedDecodeParams &p, int dtype, hipStream_t stream);
 
 }  // namespace sa

@@ -4,6 +4,7 @@
 
 #include "api_common.h"
 #include "paged.h"
+#include "paged_pieces.h"
 #include "sparseattn.h"
 
 namespace {
@@ -206,7 +207,9 @@ size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int 
         (int64_t)Hq / H * Sq > kMostRows)
         return 0;
     const int R = Hq / H * Sq;
-    return sa::paged_decode_plan((int64_t)B * H * ((R + 31) / 32), R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units()).bytes;
+    const int64_t planes = (int64_t)B * H * ((R + 31) / 32);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units());
+    return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8;
 }
 
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
@@ -273,13 +276,14 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     if (planes > (1 << 24) || planes * chunks > (1 << 30))
         return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
-    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
-        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, plan.bytes, workspace ? workspace_bytes : (size_t)0);
+    const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), need = parts_bytes + (size_t)(planes + plan.groups) * 8;
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
     p.groups = plan.groups;
     p.parts = plan.parts;
     p.part_rows = plan.part_rows;
     p.ws = static_cast<float *>(workspace);
-    p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + plan.parts_bytes);
+    p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + parts_bytes);
     p.tag = sa::next_launch_tag() | 1;
     return launched(who, sa::launch_paged_decode(p, dtype, static_cast<hipStream_t>(stream)));
 }

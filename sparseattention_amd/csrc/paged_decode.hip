@@ -11,16 +11,14 @@
 //   * computes S^T = K . Q^T (32 keys x 32 rows), masks, P = exp2(S^T - m), O^T += V^T . P^T.
 #include "fwd_common.h"
 #include "paged.h"
+#include "paged_pieces.h"
 
 namespace sa {
 
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = kPagedWaves;
 constexpr int kPagedRowPad = 4;  // floats behind a row of a part: reference value and sum, and two that keep rows 16-byte aligned
-
-// Workgroups that a compute unit holds (a wave of each per SIMD).
-constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
 
 template <int DT>
 struct Codes;  // eight codes as an operand, times a power of two
@@ -53,11 +51,10 @@ __device__ __forceinline__ float scale_of(float s) {  // (as the cache's kernels
     return __uint_as_float((uint32_t)min(max(e, 127 + kScaleExpMin), 127 + kScaleExpMax) << 23);
 }
 
-// ---- who does what ----
-// The work is a row of chunks: units (a sequence, with lists a sequence and K/V head) one behind the other, of every unit its planes (head,
-// tile of 32 rows), of every plane its T chunks, at least one, so that planes without keys are written too.  Every workgroup takes
-// an equal piece of the row, whatever the lengths: segments, each of one plane.  A plane that lies in several workgroups' pieces is
-// added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself, by a sum over the units.
+// ---- who does what (paged_pieces.h) ----
+// Every workgroup takes an equal piece of the row of chunks, whatever the lengths: segments, each of one plane.  A plane that lies in several
+// workgroups' pieces is added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself,
+// by a sum over the units.
 struct Unit {
     int len, cnt;  // keys and query rows of its sequence
     int T0, T;     // first chunk, chunks (0: none)
@@ -282,9 +279,17 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lP = p.c.lper + 5, sub_mask = (1 << p.c.lper) - 1;
+    // What is read from the argument block where it is used: hoisted out of the loop over the segments, the strides of everything had
+    // the inner loop's scalars spilled.
+    typedef const __attribute__((address_space(4))) PagedDecodeParams *ArgPtr;
+    auto late = [] {
+        ArgPtr a = (ArgPtr)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
+    };
     auto by_rows = [&](int row) { return p.Sq == 1 ? row : row / p.Sq; };  // (a division costs as much as a step of the scan)
 
-    // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in (the host: a row is less than 2^31 chunks) ----
+    // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in (the host: a row is at most 2^30 chunks) ----
     const int U = LISTS ? p.t.B * p.c.H : p.t.B;                // units
     const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;  // planes of each
     const int per_lane = (U + 63) >> 6;
@@ -302,21 +307,9 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     int upto = scan(mine, plus);
     longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
     unsigned total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
-    // Either pieces of a row of chunks, wherever they begin and end; or every plane cut into equal parts of up to `share` chunks, a
-    // workgroup each, so that none has two planes' latencies (the row is then one of parts).  The second where there are several
-    // parts a plane, whose ends are then even, or where a part is short, so that latencies are all there is (the rule: paged_decode_plan).
-    const unsigned planes = U * M, groups = gridDim.x;
-    const unsigned parts = min((unsigned)p.parts, max(16u, (unsigned)__builtin_amdgcn_sqrtf(2.f * (float)longest)));
-    // (divisions cost a step of the scan each: as few as can be)
-    const bool cuts = planes < groups && (8 * planes <= groups || total <= 2 * kWaves * (groups - planes));
-    const unsigned among = cuts ? groups - planes : groups;
-    unsigned share = (total + among - 1) / among;
-    if (cuts) share = max(share, (unsigned)kWaves);
-    if ((uint64_t)longest > (uint64_t)share * parts) share = ((unsigned)longest + parts - 1) / parts;
-    auto length = [&](int chunks) __attribute__((always_inline)) {  // of a plane of so many, in the row
-        const unsigned T = (unsigned)max(chunks, 1);
-        return cuts ? (T + share - 1) / share : T;
-    };
+    const PagedShare share = paged_share(total, U * M, gridDim.x, (unsigned)longest, (unsigned)p.parts);
+    const bool cuts = share.cuts;
+    auto length = [&](int chunks) __attribute__((always_inline)) { return paged_row_length(share, (unsigned)max(chunks, 1)); };  // in the row
     if (cuts) {
         mine = 0;
         if (per_lane == 1)
@@ -331,13 +324,9 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         upto = scan(mine, plus);
         total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
     }
-    const unsigned piece = cuts ? 1u : share;
-    // Consecutive workgroups go to the 8 XCDs in turn, consecutive pieces of the row to one (the host: groups are eights), so that row
-    // tiles of a head read K and V from one L2: 224 rows over a window of 4955 111 -> 76 us, one row or few 0 ... 3 % less.
-    const unsigned pieces = cuts ? total : groups, per_xcd = (pieces + 7) >> 3;
-    const unsigned me = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per_xcd) return;
-    const unsigned x0 = piece * me, x1 = min(x0 + piece, total);
+    const int me = paged_piece(blockIdx.x, cuts ? total : gridDim.x);
+    if (me < 0) return;
+    const unsigned piece = cuts ? 1u : share.share, x0 = piece * me, x1 = min(x0 + piece, total);
     if (x0 >= total) return;
     int u;
     unsigned base;  // of unit u
@@ -367,16 +356,15 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     // Of the workgroups of a compute unit the oldest goes first and is done when others have a third of their piece left; so the
     // further a workgroup is, the lower its priority.
     __builtin_amdgcn_s_setprio(3);
-    unsigned x = x0, lower_at = share / 4;
+    unsigned x = x0, lower_at = share.share / 4;
     int quarter = 0;
     while (x < x1) {
         const unsigned done = cuts ? 0u : x - x0;
         const unsigned T = (unsigned)max(unit.T, 1), row_T = length(unit.T);
         const unsigned m = M == 1 ? 0u : (x - base) / row_T, at_row = x - base - m * row_T;
         const unsigned plane_at = x - at_row;  // in the row
-        // chunks off .. off + n - 1 of this plane
-        const unsigned even = cuts ? (T + row_T - 1) / row_T : 0u;  // (at most `share`, and row_T of them are no fewer than needed)
-        const int off = (int)(cuts ? at_row * even : at_row), n = (int)min(T - off, cuts ? even : x1 - x);
+        const PagedSegment seg = paged_segment(share, T, row_T, at_row, x1 - x);
+        const int off = seg.off, n = seg.n;  // chunks off .. off + n - 1 of this plane
         const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + (int)m : (int)m;
         const int h = p.RT == 1 ? hr : hr / p.RT, rt = hr - h * p.RT;
         const int plane = (b * p.c.H + h) * p.RT + rt;
@@ -396,7 +384,8 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
 
         u32x4 qf[X::NQ];
         {
-            const uint16_t *qp = p.q + b * p.qs[0] + (live ? (h * p.G + g) * p.qs[1] + i * p.qs[2] : 0);
+            const ArgPtr a = late();
+            const uint16_t *qp = a->q + b * a->qs[0] + (live ? (h * a->G + g) * a->qs[1] + i * a->qs[2] : 0);
 #pragma unroll
             for (int c = 0; c < X::NQ; c++) qf[c] = live && X::d_of_q(c, lgrp) < p.c.cols ? *(const u32x4 *)(qp + X::d_of_q(c, lgrp)) : u32x4{0u, 0u, 0u, 0u};
         }
@@ -413,6 +402,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             float ks, vs;
         };
         auto places = [&](int j0) __attribute__((always_inline)) {
+            const ArgPtr a = late();
             int block = -1, at_tile = 0, slot = -1;
             float ks = 0.f, vs = 0.f;
             const int j = j0 + lane;
@@ -421,20 +411,21 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 int tile = t >> p.c.lper;
                 if constexpr (LISTS) {
                     if (tile >= F) slot = tile - F;
-                    tile = tile < F ? p.full_ids[b * p.fis[0] + h * p.fis[1] + (int64_t)tile * p.fis[2]] : p.part_ids[b * p.pis[0] + h * p.pis[1] + (int64_t)(tile - F) * p.pis[2]];
-                    if (tile < 0 || tile >= p.nK) tile = p.t.width;
+                    tile = tile < F ? a->full_ids[b * a->fis[0] + h * a->fis[1] + (int64_t)tile * a->fis[2]]
+                                    : a->part_ids[b * a->pis[0] + h * a->pis[1] + (int64_t)(tile - F) * a->pis[2]];
+                    if (tile < 0 || tile >= a->nK) tile = a->t.width;
                 }
                 const int sub = t & sub_mask;
-                if (tile < p.t.width) {
+                if (tile < a->t.width) {
                     at_tile = tile;
-                    const int page = p.t.ids[b * p.t.s0 + tile * p.t.s1];
+                    const int page = a->t.ids[b * a->t.s0 + tile * a->t.s1];
                     // (nothing attends to keys of a page that does not exist)
-                    if ((tile << lP) + (sub << 5) < len && page >= 0 && page < p.c.pages) block = ((page * p.c.H + h) << p.c.lper) + sub;
+                    if ((tile << lP) + (sub << 5) < len && page >= 0 && page < a->c.pages) block = ((page * a->c.H + h) << p.c.lper) + sub;
                 }
             }
             if (block >= 0) {
-                ks = p.c.k_scales[block];
-                vs = p.c.v_scales[block];
+                ks = a->c.k_scales[block];
+                vs = a->c.v_scales[block];
             }
             return Places{block, at_tile, slot, ks, vs};
         };
@@ -471,7 +462,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             });
         auto step = [&](int j, Chunk &c, typename X::Operands &x) __attribute__((always_inline)) {
             if (done + 4u * j >= lower_at) {
-                lower_at += share / 4;
+                lower_at += share.share / 4;
                 quarter++;
                 if (quarter == 1) __builtin_amdgcn_s_setprio(2);
                 else if (quarter == 2) __builtin_amdgcn_s_setprio(1);
@@ -571,7 +562,8 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         }
         __syncthreads();
         constexpr int LPR = D / 4;  // lanes per row
-        const int rows = min(p.R - ROWS * rt, ROWS);
+        const ArgPtr a = late();
+        const int rows = min(a->R - ROWS * rt, ROWS);
         struct Sum {
             float M = kNegInf, L = 0.f;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -596,18 +588,18 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             s.M = M;
         };
         auto finish = [&](int r, int d0, const Sum &s) __attribute__((always_inline)) {
-            const int at = ROWS * rt + r, gg = by_rows(at), ii = at - gg * p.Sq, head = h * p.G + gg;
+            const int at = ROWS * rt + r, gg = by_rows(at), ii = at - gg * p.Sq, head = h * a->G + gg;
             const bool none = ii >= cnt || s.L == 0.f;  // (a row of padding may have met a NaN)
             const float inv = 1.f / s.L;
             const f32x4 y = none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{s.x.x * inv, s.x.y * inv, s.x.z * inv, s.x.w * inv};
-            if (p.lse != nullptr && d0 == 0)
-                p.lse[b * p.lses[0] + head * p.lses[1] + ii * p.lses[2]] =
+            if (a->lse != nullptr && d0 == 0)
+                a->lse[b * a->lses[0] + head * a->lses[1] + ii * a->lses[2]] =
                     none ? kNegInf : (s.M + __builtin_amdgcn_logf(s.L)) * 0.69314718056f;
-            if (d0 < p.c.cols) *(u32x2 *)(p.o + b * p.os[0] + head * p.os[1] + ii * p.os[2] + d0) = u32x2{E::pack2(y.x, y.y), E::pack2(y.z, y.w)};
+            if (d0 < a->c.cols) *(u32x2 *)(a->o + b * a->os[0] + head * a->os[1] + ii * a->os[2] + d0) = u32x2{E::pack2(y.x, y.y), E::pack2(y.z, y.w)};
         };
         const bool whole = n == (int)T;
-        const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)p.part_rows * row_bytes;
-        uint8_t *const ws = reinterpret_cast<uint8_t *>(p.ws);
+        const uint32_t row_bytes = PST * 4, part_bytes = (uint32_t)a->part_rows * row_bytes;
+        uint8_t *const ws = reinterpret_cast<uint8_t *>(a->ws);
         // a workgroup has at most two parts: of the plane that its piece starts inside of, and of the one that goes on behind it
         const HandOver out(ws + (int64_t)(2 * me + (off == 0 ? 1 : 0)) * part_bytes, whole ? 0u : part_bytes);
         for (int it = tid; it < rows * LPR; it += kWaves * 64) {
@@ -629,13 +621,13 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             }
         }
         if (!whole) {
-            // workgroups of the plane
-            const int g0 = (int)(cuts ? plane_at : plane_at / piece), parts = cuts ? (int)row_T : (int)((plane_at + row_T - 1) / piece) - g0 + 1;
+            const PagedRange range = paged_range(share, plane_at, row_T);  // the plane's workgroups
+            const int g0 = range.first, parts = range.parts;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();  // every wave's rows have been handed over, and LDS has been read
             int *const told = reinterpret_cast<int *>(part + D + 2);  // (behind a row: the sum below leaves it alone)
             if (wave == 0) {
-                const bool last = all_arrived(p.arrivals + plane + g0, p.tag, (int)me - g0, parts);
+                const bool last = all_arrived(a->arrivals + plane + g0, a->tag, (int)me - g0, parts);
                 if (lane == 0) *told = last;
             }
             __syncthreads();
@@ -728,26 +720,7 @@ hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {
 
 }  // namespace
 
-// As many workgroups as the device holds at once: with more, the pieces of a workgroup that starts late do not make up for its start
-// (32 sequences of up to 32768 keys: 294 us; twice as many workgroups 304, four times 324).
-// Planes are cut evenly where they are few, so that a plane is many parts and their ends are even: at 8 parts a plane (64 planes of
-// 129 chunks) 21.5 -> 18.3 us, 8 planes of 63 chunks 12.1 -> 9.1; at 3 (256 planes of 700 ... 1024) it would be 290 -> 319.
-// One workgroup adds a plane's parts up, 8 to 32 at a time.  So there are no more of them than let every compute unit read at full speed (a
-// chunk of 8 KiB a wave, one workgroup each, or two of 4 KiB), but at least 16: 16 planes of 1000 chunks with 16 | 32 | 62 parts 32.3 |
-// 37.9 | 41.6 us; and no more than balance the chunks a wave has one after the other (1.15 us each) with the sum: sqrt(2 T) of T chunks.
-PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus) {
-    PagedDecodePlan r;
-    const int64_t even = (int64_t)cus * (D == 64 ? 2 : 1) / planes;
-    r.parts = (int)(even < 16 ? 16 : even < kPagedMostParts - 2 ? even : kPagedMostParts - 2);
-    const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
-    const int64_t fine = (chunks + kWaves - 1) / kWaves;  // parts of a plane of a chunk a wave
-    const int64_t most = planes * ((fine < r.parts ? fine : r.parts) + 1);
-    r.groups = ((int)(most < resident ? most : resident) + 7) / 8 * 8;
-    r.part_rows = R < 32 ? R : 32;
-    r.parts_bytes = (size_t)r.groups * 2 * r.part_rows * (D + kPagedRowPad) * 4;
-    r.bytes = r.parts_bytes + (size_t)(planes + r.groups) * 8;
-    return r;
-}
+size_t paged_decode_parts_bytes(int groups, int part_rows, int D) { return (size_t)groups * 2 * part_rows * (D + kPagedRowPad) * 4; }
 
 hipError_t launch_paged_decode(const PagedDecodeParams &p, int dtype, hipStream_t stream) {
     if (dtype == 0) return launch_dim<0>(p, stream);
