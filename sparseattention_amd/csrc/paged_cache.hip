@@ -16,9 +16,18 @@ namespace {
 
 template <int DT>
 struct Half16;  // what a pair of input values is, as bits
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
 template <>
 struct Half16<0> {
     static constexpr uint32_t kInf = 0x7f80u;
+    // the codes of two pairs, divided by a power of two, in range and finite
+    static __device__ __forceinline__ uint32_t codes(uint32_t a, uint32_t b, float scale) {
+        i16x2 r = {0, 0};
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, a), scale, false);
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, b), scale, true));
+    }
     static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
     static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
     static __device__ __forceinline__ uint32_t cvt_lo(uint32_t w, float s) {
@@ -31,6 +40,11 @@ struct Half16<0> {
 template <>
 struct Half16<1> {
     static constexpr uint32_t kInf = 0x7c00u;
+    static __device__ __forceinline__ uint32_t codes(uint32_t a, uint32_t b, float scale) {
+        i16x2 r = {0, 0};
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, a), scale, false);
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, b), scale, true));
+    }
     static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w).x; }
     static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w).y; }
     static __device__ __forceinline__ uint32_t cvt_lo(uint32_t w, float s) {
@@ -59,6 +73,10 @@ __device__ __forceinline__ uint32_t amax2(uint32_t m, uint32_t w) {
     const uint32_t a = w & 0x7fffu, b = (w >> 16) & 0x7fffu;
     m = max(m, a < Half16<DT>::kInf ? a : 0u);
     return max(m, b < Half16<DT>::kInf ? b : 0u);
+}
+// The larger magnitudes of two pairs, as bits, infinities and NaN among them.
+__device__ __forceinline__ uint32_t larger2(uint32_t m, uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
 }
 // What a value becomes before it is rounded to a code: in range (beyond it only at the largest scale), infinities NaN.
 __device__ __forceinline__ float scaled(float x, float inv) {
@@ -175,17 +193,32 @@ __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_appen
         }
     }
 
+    // (finite values, as nearly always, go the short way)
     uint32_t m = 0u;
 #pragma unroll
     for (int i = 0; i < NL; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) m = amax2<DT>(m, in[i][j]);
-    m = wave_max(m);
+        for (int j = 0; j < 4; j++) m = larger2(m, in[i][j]);
+    m = wave_max(max(m & 0xffffu, m >> 16));
+    const bool finite = m < X::kInf;
+    if (!finite) {
+        m = 0u;
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = amax2<DT>(m, in[i][j]);
+        m = wave_max(m);
+    }
     const int e = max(e_old, scale_exp(DT == 0 ? __uint_as_float(m << 16) : X::lo(m)));
-    const float inv = exp2i(-e);
+    const float up = exp2i(e), inv = exp2i(-e);
+    const bool plain = finite && e < kScaleExpMax;
+    // codes of four values in two pairs
+    auto code = [&](uint32_t a, uint32_t b) {
+        return plain ? X::codes(a, b, up) : codes4(scaled(X::lo(a), inv), scaled(X::hi(a), inv), scaled(X::lo(b), inv), scaled(X::hi(b), inv));
+    };
     const bool grows = held > 0 && e > e_old;
     const float f = exp2i(max(e_old - e, -126));
-    if (lane == 0 && (grows || held == 0)) *scale = exp2i(e);
+    if (lane == 0 && (grows || held == 0)) *scale = up;
 
     u32x4 made[2 * NG];  // codes: of 16 d of a token per piece (K), of 16 tokens of two d (V)
 #pragma unroll
@@ -201,8 +234,7 @@ __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_appen
                     const u32x4 *const from = (const u32x4 *)(mine + (l32 & 15) * row_bytes<ND> + 64 * c + 32 * hh);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint32_t lo = from[i >> 1][2 * (i & 1)], hi = from[i >> 1][2 * (i & 1) + 1];
-                        made[c][i] = codes4(scaled(X::lo(lo), inv), scaled(X::hi(lo), inv), scaled(X::lo(hi), inv), scaled(X::hi(hi), inv));
+                        made[c][i] = code(from[i >> 1][2 * (i & 1)], from[i >> 1][2 * (i & 1) + 1]);
                     }
                 }
             }
@@ -214,8 +246,10 @@ __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_appen
                     uint32_t q[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) q[j] = *(const uint32_t *)(mine + (8 * (i >> 1) + 4 * hh + j) * row_bytes<ND> + 128 * g + 4 * l32);
-                    made[2 * g][i] = codes4(scaled(X::lo(q[0]), inv), scaled(X::lo(q[1]), inv), scaled(X::lo(q[2]), inv), scaled(X::lo(q[3]), inv));
-                    made[2 * g + 1][i] = codes4(scaled(X::hi(q[0]), inv), scaled(X::hi(q[1]), inv), scaled(X::hi(q[2]), inv), scaled(X::hi(q[3]), inv));
+                    // two tokens of a d in a pair
+                    constexpr uint32_t lows = 0x05040100u, highs = 0x07060302u;
+                    made[2 * g][i] = code(__builtin_amdgcn_perm(q[1], q[0], lows), __builtin_amdgcn_perm(q[3], q[2], lows));
+                    made[2 * g + 1][i] = code(__builtin_amdgcn_perm(q[1], q[0], highs), __builtin_amdgcn_perm(q[3], q[2], highs));
                 }
         }
         in_order();
