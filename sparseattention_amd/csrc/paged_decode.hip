@@ -322,8 +322,12 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 mine += u < U ? n : 0;
             }
         upto = scan(mine, plus);
-        total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
+    } else {
+        const int before = min(lane * per_lane, U), after = min((lane + 1) * per_lane, U);  // the lane's units
+        mine += (after - before) * (int)kPagedComing;
+        upto += after * (int)kPagedComing;
     }
+    total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
     const int me = paged_piece(blockIdx.x, cuts ? total : gridDim.x);
     if (me < 0) return;
     const unsigned piece = cuts ? 1u : share.share, x0 = piece * me, x1 = min(x0 + piece, total);
@@ -361,8 +365,10 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     while (x < x1) {
         const unsigned done = cuts ? 0u : x - x0;
         const unsigned T = (unsigned)max(unit.T, 1), row_T = length(unit.T);
-        const unsigned m = M == 1 ? 0u : (x - base) / row_T, at_row = x - base - m * row_T;
-        const unsigned plane_at = x - at_row;  // in the row
+        const unsigned m = M == 1 ? 0u : (x - base) / row_T, plane_at = base + m * row_T;  // in the row
+        x += paged_coming(share, x - plane_at);
+        if (x >= x1) break;
+        const unsigned at_row = x - plane_at;
         const PagedSegment seg = paged_segment(share, T, row_T, at_row, x1 - x);
         const int off = seg.off, n = seg.n;  // chunks off .. off + n - 1 of this plane
         const int b = LISTS ? u / p.c.H : u, hr = LISTS ? (u - b * p.c.H) * p.RT + (int)m : (int)m;

@@ -18,6 +18,10 @@ namespace sa {
 
 constexpr int kPagedWaves = 4;       // of a workgroup, which take chunks in turn
 constexpr int kPagedMostParts = 64;  // of a plane (all_arrived looks at one word per lane)
+// Where pieces begin and end anywhere, what it costs a workgroup to come to a plane (queries, places and the first chunk to wait for, rows to
+// hand over) stands in the row in front of the plane, as so many chunks: 64 ragged sequences of up to 8192 keys 103.7 us with none, 103.4 with
+// 2, 102.9 with 4, 102.0 with 8, 103.6 with 16; 16 sequences at D = 256 75.8 -> 73.6 with 8.
+constexpr unsigned kPagedComing = 8;
 
 // Workgroups that a compute unit holds (a wave of each per SIMD), by D / 32 and the rows of a tile.
 constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
@@ -65,6 +69,7 @@ SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned gr
     PagedShare r;
     r.cuts = planes < groups && (8 * planes <= groups || total <= 2 * kPagedWaves * (groups - planes));
     const unsigned among = r.cuts ? groups - planes : groups;  // (a part of each plane may be short)
+    if (!r.cuts) total += planes * kPagedComing;  // (the host: at most 2^24 planes)
     r.share = (total + among - 1) / among;
     if (r.cuts && r.share < (unsigned)kPagedWaves) r.share = kPagedWaves;
     if ((uint64_t)longest > (uint64_t)r.share * parts) r.share = (longest + parts - 1) / parts;
@@ -72,7 +77,9 @@ SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned gr
 }
 
 // A plane of T chunks in the row.
-SA_PIECES_FN unsigned paged_row_length(PagedShare s, unsigned T) { return s.cuts ? (T + s.share - 1) / s.share : T; }
+SA_PIECES_FN unsigned paged_row_length(PagedShare s, unsigned T) { return s.cuts ? (T + s.share - 1) / s.share : T + kPagedComing; }
+// What of a plane's place in the row, from at_row on, is not its chunks.
+SA_PIECES_FN unsigned paged_coming(PagedShare s, unsigned at_row) { return s.cuts || at_row >= kPagedComing ? 0u : kPagedComing - at_row; }
 
 // The piece of workgroup `block`, of `pieces` in all, or -1.  Consecutive workgroups go to the 8 XCDs in turn, consecutive pieces of the row
 // to one, so that row tiles of a head read K and V from one L2: 224 rows over a window of 4955 111 -> 76 us, one row or few 0 ... 3 % less.
@@ -87,7 +94,7 @@ struct PagedSegment {
 };
 SA_PIECES_FN PagedSegment paged_segment(PagedShare s, unsigned T, unsigned row_T, unsigned at_row, unsigned left) {
     // (even parts: at most `share`, and no fewer than row_T of them hold the plane)
-    const unsigned step = s.cuts ? (T + row_T - 1) / row_T : left, off = s.cuts ? at_row * step : at_row;
+    const unsigned step = s.cuts ? (T + row_T - 1) / row_T : left, off = s.cuts ? at_row * step : at_row - kPagedComing;
     return {(int)off, (int)(T - off < step ? T - off : step)};
 }
 
@@ -97,7 +104,7 @@ struct PagedRange {
 };
 SA_PIECES_FN PagedRange paged_range(PagedShare s, unsigned plane_at, unsigned row_T) {
     if (s.cuts) return {(int)plane_at, (int)row_T};
-    const unsigned first = plane_at / s.share;
+    const unsigned first = (plane_at + kPagedComing) / s.share;
     return {(int)first, (int)((plane_at + row_T - 1) / s.share - first + 1)};
 }
 

@@ -35,7 +35,10 @@ int main(int n, char **a) {
         for (unsigned x = x0; x < x1;) {
             unsigned base = 0, u = 0;
             while (x >= base + sa::paged_row_length(s, T[u]) * M) base += sa::paged_row_length(s, T[u++]) * M;
-            const unsigned row_T = sa::paged_row_length(s, T[u]), m = (x - base) / row_T, at = x - base - m * row_T;
+            const unsigned row_T = sa::paged_row_length(s, T[u]), m = (x - base) / row_T;
+            x += sa::paged_coming(s, x - base - m * row_T);
+            if (x >= x1) break;
+            const unsigned at = x - base - m * row_T;
             const sa::PagedSegment g = sa::paged_segment(s, T[u], row_T, at, x1 - x);
             const sa::PagedRange r = sa::paged_range(s, x - at, row_T);
             printf("%d %u %u %d %d %d %d\n", me, u, m, g.off, g.n, r.first, r.parts);
