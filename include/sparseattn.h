@@ -527,7 +527,8 @@ int sa_paged_cache_append(const sa_paged_cache *cache, const void *k, const int6
                           const int32_t *lens, const int32_t *counts, int B, int S, int pages_per_sequence, int dtype,
                           void *stream);
 
-/* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,head_dim] (bf16 or fp16, as above); rows from lens[b] on are zero. */
+/* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,head_dim] (bf16 or fp16, as above); rows from lens[b] on are zero.
+ * bf16 holds the values exactly; fp16 rounds those below its normal numbers and has 61440 for those beyond its 65504. */
 int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_strides[4], void *v, const int64_t v_strides[4],
                           const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, int B, int length,
                           int pages_per_sequence, int dtype, void *stream);
@@ -576,8 +577,8 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
  *             [B,H,1], packed tiles with strides in bytes along B and H.  The mask alone says who attends, among the keys below
  *             lens[b]; window must be 0.  Tile indices out of range are skipped.
  * workspace, lse, dtype, sm_scale_log2: as for sa_sparse_attention_decode; sa_decode_paged_workspace_bytes(...) bytes, 16-byte aligned (of
- * the current device).  K and V are read as they are held, exactly; a value beyond fp16's range is infinite there.  A masked NaN or
- * infinity has no effect.
+ * the current device).  K and V are read as they are held, exactly; in fp16 V as sa_paged_cache_gather gives it.  A masked NaN has no
+ * effect.
  */
 size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size);
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache,

@@ -17,6 +17,20 @@ constexpr int kPagedBlock = 32;                  // tokens that share a scale
 constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^119 is the largest that bf16 and float32 hold
 constexpr int kPagedMostPages = 1 << 20;         // (compaction keeps a bit per page in LDS)
 
+// In fp16 a code times 2^e, e > 7, may be beyond the type: fp16 tokens up to 65504 make blocks of the scale 2^8, where 65504 itself is held as 65536,
+// and codes that no token has, or that a row leaves out, stand for up to 114688 and more; times a weight of 0 these must be 0.  There codes stop at
+// the largest one within the type, 1.875 * 2^15 up to e = 21; four codes at a time, NaN as it is.
+constexpr float kFp16Scale = 128.f;  // (448 * 2^7 is within)
+__device__ __forceinline__ uint32_t most_fp16_code(float scale) {
+    const int e = (int)(__float_as_uint(scale) >> 23) - 127;
+    return (uint32_t)(e <= 21 ? 0x77 - 8 * (e - 8) : 15 >> (e - 21 < 4 ? e - 21 : 4)) * 0x01010101u;
+}
+__device__ __forceinline__ uint32_t within_fp16(uint32_t w, uint32_t most) {
+    const uint32_t size = w & 0x7f7f7f7fu, nan = (size + 0x01010101u) & 0x80808080u;
+    const uint32_t over = (((size + (0x7f7f7f7fu - most)) & 0x80808080u & ~nan) >> 7) * 0x7fu;
+    return (w & ~over) | (most & over);
+}
+
 struct PagedPool {
     uint8_t *k, *v;            // [pages, H, per, 32 * D]
     float *k_scales, *v_scales;  // [pages, H, per]

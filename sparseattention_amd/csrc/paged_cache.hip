@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const Pa
     if (b >= p.t.B) return;
     const int first = 32 * blk, rows = min(p.length - first, 32);
     const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
-    const int n = page < 0 ? 0 : min(max(p.t.lens[b] - first, 0), rows);  // rows that hold something
+    const int n = page < 0 ? 0 : min(max(max(p.t.lens[b], 0) - first, 0), rows);  // rows that hold something
     const int64_t at = block_at(p.c, max(page, 0), h, blk & ((1 << p.c.lper) - 1));
     const uint8_t *const in = (values ? p.c.v : p.c.k) + at * (ND * 1024);
     u32x4 u[ND];
@@ -328,6 +328,13 @@ __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const Pa
         for (int c = 0; c < ND; c++)
             u[c] = *(const u32x4 *)(in + (values ? 1024 * (2 * (c >> 1) + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15) + (c & 1)) : 1024 * c + 16 * lane));
         scale = exp2i(exp_of_scale((values ? p.c.v_scales : p.c.k_scales)[at]));
+        if (DT == 1 && scale > kFp16Scale) {
+            const uint32_t most = most_fp16_code(scale);
+#pragma unroll
+            for (int c = 0; c < ND; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) u[c][i] = within_fp16(u[c][i], most);
+        }
     }
     const int64_t *const xs = values ? p.vs : p.ks;
     uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)first * xs[2];

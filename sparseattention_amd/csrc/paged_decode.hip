@@ -548,6 +548,10 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                     out_rows.poison(x, att);
                 }
             }
+            if (DT == 1 && vs > kFp16Scale) {
+                const uint32_t most = most_fp16_code(vs);
+                X::each_v(x, [&](auto &v, int e) { v[e] = within_fp16(v[e], most); });
+            }
             out_rows.add(x, pw, vs);
             request_v(nc, x);
             c = nc;

@@ -90,7 +90,8 @@ def paged_cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page
 
 def paged_cache_gather(cache: PagedCache, page_table: torch.Tensor, lens: torch.Tensor, length: Optional[int] = None,
                        dtype: torch.dtype = torch.bfloat16):
-    """``(k, v)`` [B,H,length,D] in ``dtype`` (bf16: exactly what the cache holds; fp16: exactly, within its range): the first
+    """``(k, v)`` [B,H,length,D] in ``dtype`` (bf16: exactly what the cache holds; fp16: rounded below its normal numbers, and
+    61440 where the cache holds more than its 65504): the first
     ``lens[b]`` tokens of every sequence, zeros behind them and where the table names no page.  ``length`` defaults to the
     tokens the table has place for.  Any window of the table's columns reads those pages (with lengths that count from there)."""
     return _native.host().paged_gather(cache, page_table, lens, length, dtype)
@@ -137,5 +138,8 @@ def sparse_attention_decode_paged(q: torch.Tensor, cache: PagedCache, page_table
     are padding and give 0 (``lse`` -inf).
     ``mask``: bool broadcastable to [B,H,Sq,Sk], H the K/V heads, Sk whole pages, True = attend; it replaces causality, and keys from
     ``lens[b]`` on are left out whatever it says.  ``mask_metadata``: ``compute_mask_kernel(mask, Sq, page_size)``, with which no mask is
-    needed; only the pages it lists are read."""
+    needed; only the pages it lists are read.
+
+    Probabilities and values meet in q's type, sums are float32; with fp16 queries the values are those that
+    ``paged_cache_gather(..., dtype=torch.float16)`` gives."""
     return _native.host().decode_paged(q, cache, page_table, lens, mask, mask_metadata, counts, window, return_lse)

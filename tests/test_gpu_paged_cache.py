@@ -159,6 +159,67 @@ def test_what_has_no_page_is_not_stored(gpu):
     same(sa.paged_cache_gather(cache, ints([[3]], gpu), ints([20], gpu))[0][0, 0, :20], s.x)
 
 
+@pytest.mark.parametrize("e", [-96, -24, -1, 7, 8, 9, 20, 21, 22, 23, 24, 25, 40, 119])
+def test_every_code_in_fp16(gpu, e):
+    cache = sa.empty_paged_cache(1, 1, 64, page_size=32, device=gpu)
+    codes = torch.arange(256, dtype=torch.uint8, device=gpu).repeat(8)
+    for t in (cache.k, cache.v):
+        t.copy_(codes.view(t.shape))
+    for t in (cache.k_scales, cache.v_scales):
+        t.fill_(2.0 ** e)
+    args = cache, ints([[0]], gpu), ints([32], gpu)
+    for wide, got in zip(sa.paged_cache_gather(*args), sa.paged_cache_gather(*args, dtype=torch.float16)):
+        wide = wide.double()
+        held = torch.unique(wide[wide.abs() <= 65504.0].abs())
+        want = torch.where(wide.abs() > 65504.0, torch.sign(wide) * held.max(), wide)
+        same(got, (torch.round(want * 2.0 ** 24) * 2.0 ** -24 if e < 0 else want).half())
+
+
+def test_lengths_far_out_of_range(gpu):
+    """Lengths below 0 count as 0, down to the type's lowest; those past the table as what it has place for."""
+    D, P, H = 64, 32, 1
+    cache = filled(12, H, D, P, 30, gpu)
+    table = ints([[0, 1, 2], [3, 4, 5], [6, 7, 8]], gpu)
+    lens = ints([-(1 << 31), 2 ** 31 - 1, -1], gpu)
+    k, v = sa.paged_cache_gather(cache, table, lens)
+    whole = sa.paged_cache_gather(cache, table, ints([0, 96, 0], gpu))
+    same(k, whole[0]), same(v, whole[1])
+    assert not k[0].any() and not v[2].any()
+    new, n = sa.paged_cache_fork(cache, table, lens, ints([0, 1, 2], gpu), ints([9, 10, 11], gpu))
+    assert n.tolist() == [0, 96, 0] and new.tolist() == [[-1] * 3, [3, 4, 5], [-1] * 3]
+    pages, count = sa.paged_cache_free_pages(cache, table, lens)
+    assert int(count) == 9 and pages[:9].tolist() == [0, 1, 2, 6, 7, 8, 9, 10, 11]
+    new, used = sa.paged_cache_compact(cache, table, lens)
+    assert int(used) == 3 and new.tolist() == [[-1] * 3, [0, 1, 2], [-1] * 3]  # (3, 4, 5 to the free 0, 1, 2)
+    got = sa.paged_cache_gather(cache, new, lens)
+    same(got[0], whole[0]), same(got[1], whole[1])
+
+
+def test_what_fp16_does_not_hold(gpu):
+    """Read back as fp16, what the cache holds beyond its 65504 (65504 itself is held as 65536) becomes 61440, the largest code within the
+    type, and what is below its normal numbers is rounded (to even) to its steps of 2^-24."""
+    D, P = 64, 32
+    cache = sa.empty_paged_cache(1, 1, D, page_size=P, device=gpu)
+    x = torch.zeros(1, 1, 32, D, dtype=torch.bfloat16, device=gpu)
+    x[0, 0, 0] = 2.0 ** 17
+    x[0, 0, 1] = -2.0 ** 16
+    x[0, 0, 2] = -448.0
+    x[0, 0, 3] = float("nan")
+    sa.paged_cache_append(cache, x, x, ints([[0]], gpu), ints([0], gpu))
+    for got in sa.paged_cache_gather(cache, ints([[0]], gpu), ints([32], gpu), dtype=torch.float16):
+        assert (got[0, 0, 0] == 61440.0).all() and (got[0, 0, 1] == -61440.0).all() and (got[0, 0, 2] == -448.0).all()
+        assert torch.isnan(got[0, 0, 3]).all() and not got[0, 0, 4:].any()
+    x[0, 0, 0] = 1.0 * 2.0 ** -14
+    x[0, 0, 1] = -1.125 * 2.0 ** -22  # (4.5 steps of 2^-24: 4)
+    x[0, 0, 2] = 1.0 * 2.0 ** -25     # (half a step: 0)
+    x[0, 0, 3] = 1.5 * 2.0 ** -24     # (1.5 steps: 2)
+    cache = sa.empty_paged_cache(1, 1, D, page_size=P, device=gpu)
+    sa.paged_cache_append(cache, x, x, ints([[0]], gpu), ints([0], gpu))
+    held = sa.paged_cache_gather(cache, ints([[0]], gpu), ints([32], gpu))[0].double()
+    for got in sa.paged_cache_gather(cache, ints([[0]], gpu), ints([32], gpu), dtype=torch.float16):
+        same(got, torch.round(held * 2.0 ** 24) * 2.0 ** -24)
+
+
 def test_empty_calls(gpu):
     cache = sa.empty_paged_cache(4, 2, 64, page_size=32, device=gpu)
     none = torch.empty(0, dtype=torch.int32, device=gpu)

@@ -226,6 +226,33 @@ def test_lists_out_of_range(gpu):
         sa.sparse_attention_decode_paged(q, cache, table, ints([256], gpu), mask_metadata=md)
 
 
+@pytest.mark.parametrize("D,G,Sq", [(64, 1, 3), (128, 4, 8), (256, 2, 1)])
+def test_values_at_the_end_of_fp16(gpu, D, G, Sq):
+    """Values near fp16's largest, among codes that stand for more than it: behind a sequence, and at keys that rows leave out."""
+    cache = sa.empty_paged_cache(3, 1, D, page_size=64, device=gpu)
+    cache.k.fill_(0x7E), cache.v.fill_(0xFE)  # (+-448 times the block's scale)
+    cache.k_scales.fill_(1.0), cache.v_scales.fill_(1.0)
+    g = torch.Generator().manual_seed(40)
+    k = torch.randn(1, 1, 70, D, generator=g).half().to(gpu)
+    v = (6e4 * (2 * torch.rand(1, 1, 70, D, generator=g) - 1)).half().to(gpu)
+    v[0, 0, 69], v[0, 0, 68] = 60000.0, -60000.0
+    table = ints([[2, 0]], gpu)
+    sa.paged_cache_append(cache, k, v, table, ints([0], gpu))
+    assert (cache.v_scales[2] == 256.0).all()  # 448 * 256 > 65504
+    q = queries(1, G, Sq, D, torch.float16, 41, gpu)
+    o, lse = sa.sparse_attention_decode_paged(q, cache, table, ints([70], gpu), return_lse=True)
+    check(cache, table, [70], q, o, lse)
+    # a token of 2^17, which the first rows do not see
+    x = torch.zeros(1, 1, 1, D, dtype=torch.bfloat16, device=gpu)
+    x[...] = 2.0 ** 17
+    sa.paged_cache_append(cache, x, x, table, ints([70], gpu))
+    see = torch.ones(1, 1, Sq, 128, dtype=torch.bool)
+    see[:, :, :, 70] = False
+    o, lse = sa.sparse_attention_decode_paged(q, cache, table, ints([71], gpu), see.to(gpu), return_lse=True)
+    assert torch.isfinite(o).all()
+    check(cache, table, [71], q, o, lse, see=see)
+
+
 def test_wide_scores(gpu):
     """Scores of several hundred either way: weights that vanish, a reference value that rises late."""
     for dtype in (torch.bfloat16, torch.float16):
@@ -330,6 +357,59 @@ def test_another_stream(gpu):
         got = sa.sparse_attention_decode_paged(q, cache, table, n)
     stream.synchronize()
     assert torch.equal(got, want)
+
+
+def test_calls_side_by_side(gpu):
+    """Threads with streams of their own, at the same time over one cache, each of whose calls shares planes between workgroups."""
+    import threading
+
+    lens = [3000, 77, 1500]
+    cache, table = make(3, 2, 128, 64, lens, torch.bfloat16, 23, gpu)
+    n = ints(lens, gpu)
+    qs = [queries(3, 8, 1 + t, 128, torch.bfloat16, 24 + t, gpu) for t in range(4)]
+    want = [sa.sparse_attention_decode_paged(q, cache, table, n, return_lse=True) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(t):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(25):
+                o, lse = sa.sparse_attention_decode_paged(qs[t], cache, table, n, return_lse=True)
+                stream.synchronize()
+                if not (torch.equal(o, want[t][0]) and torch.equal(lse, want[t][1])):
+                    wrong.append(t)
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_two_graphs_of_one_pool(gpu):
+    """Graphs that share their memory, replayed in turn with lengths that change between the replays."""
+    lens = [900, 33]
+    cache, table = make(2, 2, 64, 32, [1000, 1000], torch.float16, 28, gpu)
+    n = ints(lens, gpu)
+    qs = [queries(2, 4, 2, 64, torch.float16, 29 + t, gpu) for t in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sa.sparse_attention_decode_paged(qs[0], cache, table, n)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g, q in zip(graphs, qs):
+        with torch.cuda.graph(g, pool=graphs[0].pool() if outs else None):
+            outs.append(sa.sparse_attention_decode_paged(q, cache, table, n, return_lse=True))
+    for step in range(6):
+        n.copy_(ints([(0, 1, 900, 1000, 33, 640)[step], (1000, 5, 700, 0, 1, 65)[step]], gpu))
+        for g, q, (o, lse) in zip(graphs, qs, outs):
+            g.replay()
+            want = sa.sparse_attention_decode_paged(q, cache, table, n, return_lse=True)
+            torch.cuda.synchronize()
+            assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
 
 
 def test_refusals(gpu):
