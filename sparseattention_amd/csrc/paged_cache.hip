@@ -515,14 +515,13 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPla
         movers += __popc(bits[w] & ~below(w));
     }
     int hole_at = before_me(holes, waves, hole_total), mover_at = before_me(movers, waves, mover_total);
-    const int mover_first = mover_at;
     for (int w = w0; w < w1; w++) {
         for (uint32_t left = ~bits[w] & below(w); left != 0u; left &= left - 1u) p.holes[hole_at++] = 32 * w + __ffs(left) - 1;
         for (uint32_t left = bits[w] & ~below(w); left != 0u; left &= left - 1u) p.movers[mover_at++] = 32 * w + __ffs(left) - 1;
     }
     __threadfence_block();
     __syncthreads();
-    for (int i = mover_first; i < mover_at; i++) p.to[p.movers[i]] = p.holes[i];
+    for (int i = tid; i < mover_total; i += kPlanThreads) p.to[p.movers[i]] = p.holes[i];
     if (tid == 0) {
         *p.count = L;
         *p.moves = mover_total;
