@@ -98,6 +98,24 @@ __device__ __forceinline__ int scan(int x, Op &&op) {  // op(0, x) == x for x >=
     return x;
 }
 
+// all_arrived for up to kPagedMostParts workgroups, whose words a wave looks at 64 at a time.
+__device__ __forceinline__ bool parts_arrived(uint64_t *words, uint64_t tag, int mine, int n) {
+    if (n <= 64) return all_arrived(words, tag, mine, n);
+    const int lane = threadIdx.x & 63;
+    const HandOver h(words, 8u * (uint32_t)n);
+    const u32x2 set = {(uint32_t)tag, (uint32_t)(tag >> 32)};
+    if (lane == 0) h.put(8u * (uint32_t)mine, __builtin_bit_cast(f32x2, set));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool there = true;
+    for (int at = 0; at < n; at += 64) {
+        const u32x2 seen = __builtin_bit_cast(u32x2, h.get2(8u * (uint32_t)min(at + lane, n - 1)));
+        there = there && seen.x == set.x && seen.y == set.y;
+    }
+    const bool all = __builtin_amdgcn_ballot_w64(there) == ~0ull;
+    for (int at = lane; all && at < n; at += 64) h.put(8u * (uint32_t)at, f32x2{0.f, 0.f});
+    return all;
+}
+
 // The products of a tile of ROWS query rows, S^T = K Q^T (32 keys) and O^T += V^T P^T, on 32 x 32 or 16 x 16 matrix instructions.
 // A lane has its row's share: row lane % ROWS, group lane / ROWS.
 // FAR: K and V are read once by the launch, past the caches (6.3 against 5.7 TB/s at 32 sequences of up to 32768 keys); not where
@@ -646,7 +664,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             __syncthreads();  // every wave's rows have been handed over, and LDS has been read
             int *const told = reinterpret_cast<int *>(part + D + 2);  // (behind a row: the sum below leaves it alone)
             if (wave == 0) {
-                const bool last = all_arrived(a->arrivals + plane + g0, a->tag, (int)me - g0, parts);
+                const bool last = parts_arrived(a->arrivals + plane + g0, a->tag, (int)me - g0, parts);
                 if (lane == 0) *told = last;
             }
             __syncthreads();

@@ -87,6 +87,7 @@ def check(cache, table, lens, q, o, lse=None, see=None, counts=None, window=None
     (1, 1, 2, 36, 32, 2, [70], torch.float16),
     (1, 2, 4, 128, 64, 1, [20011], torch.bfloat16),
     (1, 1, 1, 64, 32, 17, [9000], torch.float16),
+    (1, 1, 2, 64, 64, 3, [131077], torch.bfloat16),  # (a plane of more than 64 parts)
     (40, 8, 1, 64, 64, 1, [37 * i % 1501 for i in range(40)], torch.bfloat16),
     (130, 1, 3, 64, 32, 1, [53 * i % 200 for i in range(130)], torch.float16),
     (300, 8, 1, 64, 32, 1, [7 * i % 90 for i in range(300)], torch.bfloat16),

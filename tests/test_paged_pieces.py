@@ -73,7 +73,7 @@ def check(pieces, cus, R, D, chunks, M, T):
         of_group[me] = of_group.get(me, 0) + n
         if n < t:  # a part: two at most of a workgroup, each in a place of its own, its word in the plane's row of words
             slot = 2 * me + (off == 0)
-            assert 0 <= me - first < parts <= 64 and slot not in slots
+            assert 0 <= me - first < parts <= 128 and slot not in slots
             slots.add(slot)
             word = u * M + m + me
             assert word not in words and word < len(T) * M + groups
