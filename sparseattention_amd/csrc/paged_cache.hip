@@ -6,7 +6,8 @@
 // max|x| <= 448 * 2^e over the finite values.  Tokens that come to a block that holds some take
 //     e' = max(e, e of the new ones),   c = round(x / 2^e'),   and the old ones   c' = round(c * 2^(e - e')),
 // which changes nothing but codes that fall below 2^-6.  NaN and infinities are held as NaN.
-// All of it moves memory: per element 2 bytes read and 1 written (append) or the reverse (gather).
+// All of it moves memory: per element 2 bytes read and 1 written (append) or the reverse (gather).  A copy of 2 GiB runs at 4.86 TB/s
+// of bytes read and written, 7 where little is read.
 #include "fwd_common.h"
 #include "paged.h"
 
@@ -136,6 +137,8 @@ __device__ __forceinline__ void in_order() {
 
 // One wave stores the new tokens of one block of one head, K or V.  The rows come from memory as they lie there, 1 KiB a load, and
 // cross the lanes through LDS, 16 at a time.
+// Bound by memory: 32 prompts of 32768 tokens, 8 heads, D = 128 1.17 ms, 4.7 TB/s; by latency: one token of 64 sequences 5.8 us (length,
+// table, scale, block).  Loads of a lane's own pieces instead of rows, without LDS: ragged prompts with their read-back 62 us, now 45.
 template <int DT, int ND>
 __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_append_kernel(const PagedAppendParams p) {
     using X = Half16<DT>;
@@ -300,6 +303,8 @@ __global__ __launch_bounds__(64 * kCacheWaves, ND == 8 ? 2 : 4) void paged_appen
 // One wave reads one block of one head, K or V, into rows; rows that hold nothing become zero.  The rows cross the lanes in LDS and leave
 // 1 KiB a store, 16 rows at a time, so that all the waves that a compute unit holds have their place there.  FAR: the stores pass the
 // caches by, for outputs larger than those.
+// 192 MiB of zeros and tokens of 16 ragged sequences, D = 64 36 us, 7.3 TB/s; 768 MiB, D = 128 204 us, 5.3 TB/s.  One or two waves a
+// workgroup are no faster, streaming loads slower (37 -> 51 us).
 template <int DT, int ND, bool FAR>
 __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const PagedGatherParams p) {
     using X = Half16<DT>;
@@ -382,7 +387,8 @@ __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const Pa
     }
 }
 
-// The first `blocks` blocks of head h of page `src` to page `dst`, by a workgroup of 256.
+// The first `blocks` blocks of head h of page `src` to page `dst`, by a workgroup of 256.  Half of a pool of 3000 pages of 64 tokens, 8 heads,
+// D = 128 in a compaction: 366 MB read and written in 68 us, 5.3 TB/s.
 __device__ __forceinline__ void copy_head(const PagedPool &c, int src, int dst, int h, int blocks) {
     const int64_t from = block_at(c, src, h, 0), to = block_at(c, dst, h, 0);
     const int pieces = blocks * c.D * 2;  // of 16 bytes
@@ -468,7 +474,8 @@ __device__ __forceinline__ int before_me(int x, int *waves, int &total) {
 }
 
 // One workgroup: a bit per page that a sequence uses, then the pairs of the compaction or the free list.  The table is read
-// once and the bits stay in LDS (2^20 pages: 128 KiB), which beats launches over them in memory by what a launch costs.
+// once and the bits stay in LDS (2^20 pages: 128 KiB), which beats launches over them in memory by what a launch costs: 7 us for 24 sequences of
+// up to 128 pages.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPlanParams p) {
     extern __shared__ uint32_t bits[];
     __shared__ int waves[kPlanThreads / 64];
