@@ -85,8 +85,8 @@ struct PagedPlanParams {
     int pages, lP;
     int32_t *count;  // pages in use (compaction) or free (free list)
     // compaction: the j-th lowest free page below `count` and the j-th lowest page in use from `count` on, how many such pairs
-    // there are, and where a page in use from `count` on goes
-    int32_t *holes, *movers, *moves, *to;
+    // there are, and the j of a page in use from `count` on
+    int32_t *holes, *movers, *moves, *rank;
     int32_t *free_list;  // or the free pages in rising order, -1 behind the last
 };
 hipError_t launch_paged_plan(const PagedPlanParams &p, hipStream_t stream);
@@ -94,7 +94,7 @@ hipError_t launch_paged_plan(const PagedPlanParams &p, hipStream_t stream);
 struct PagedCompactParams {
     PagedPool c;
     PageTable t;
-    const int32_t *count, *holes, *movers, *moves, *to;
+    const int32_t *count, *holes, *movers, *moves, *rank;
     int32_t *new_ids;  // [B, width]
 };
 hipError_t launch_paged_compact(const PagedCompactParams &p, hipStream_t stream);

@@ -174,13 +174,13 @@ int sa_paged_cache_compact(const sa_paged_cache *cache, const int32_t *page_tabl
     plan.moves = ws;
     plan.holes = ws + 4;
     plan.movers = plan.holes + p.c.pages;
-    plan.to = plan.movers + p.c.pages;
+    plan.rank = plan.movers + p.c.pages;
     SA_TRY(launched(who, sa::launch_paged_plan(plan, static_cast<hipStream_t>(stream))));
     p.count = used;
     p.moves = plan.moves;
     p.holes = plan.holes;
     p.movers = plan.movers;
-    p.to = plan.to;
+    p.rank = plan.rank;
     p.new_ids = new_table;
     return launched(who, sa::launch_paged_compact(p, static_cast<hipStream_t>(stream)));
 }

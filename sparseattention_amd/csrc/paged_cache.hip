@@ -450,6 +450,7 @@ __global__ __launch_bounds__(256) void paged_fork_kernel(const PagedForkParams p
 }
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanPages = 8192;  // whose lists a workgroup writes (16384: 29 -> 30 us, 11 -> 13 at 32768 used of 40000)
 // Sum over the lanes up to this one, and over the threads in front of this one (and of all).
 __device__ __forceinline__ int lanes_up_to(int x) {
 #define SA_SUM_STEP(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
@@ -473,65 +474,97 @@ __device__ __forceinline__ int before_me(int x, int *waves, int &total) {
     return sum - x + (wave == 0 ? 0 : __shfl(up, wave - 1));
 }
 
-// One workgroup: a bit per page that a sequence uses, then the pairs of the compaction or the free list.  The table is read
-// once and the bits stay in LDS (2^20 pages: 128 KiB), which beats launches over them in memory by what a launch costs: 7 us for 24 sequences of
-// up to 128 pages.
+// A bit per page that a sequence uses, then the pairs of a compaction or the free list.  Every workgroup reads the whole table and has all bits in
+// LDS (2^20 pages: 128 KiB), which beats more launches over bits in memory; each writes the lists of its own part of the pages, 64 pages
+// a step of a wave.  Free list, us, by one workgroup whose threads write the pages of their own words | so: 64 sequences in 2048 columns, 70000
+// pages 61 | 29; in 8192 columns, 2^20 pages 709 | 117; 24 in 128 columns, 6147 pages 5.8 | 6.3.  Most of it is a table entry's VALU work, 20 instructions.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPlanParams p) {
-    extern __shared__ uint32_t bits[];
-    __shared__ int waves[kPlanThreads / 64];
-    const int tid = threadIdx.x, words = (p.pages + 31) >> 5;
+    extern __shared__ __attribute__((aligned(8))) uint32_t bits[];
+    __shared__ int waves[kPlanThreads / 64], before[kPlanThreads];  // before: pages in use in front of a thread's words
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pairs = (p.pages + 63) >> 6, words = 2 * pairs;
     for (int i = tid; i < words; i += kPlanThreads) bits[i] = 0u;
     __syncthreads();
-    // four entries and their lengths on their way at a time
-    const int64_t entries = (int64_t)p.t.B * p.t.width;
-    for (int64_t i0 = tid; i0 < entries; i0 += 4 * kPlanThreads) {
-        int page[4], len[4], at[4];
+    // a thread's entries, kPlanThreads apart: slot `at` of sequence b, `off` in the table
+    constexpr int kEntries = 8;  // and their lengths, on their way at a time
+    const int width = p.t.width, step_b = kPlanThreads / width, step_at = kPlanThreads - step_b * width;
+    const int64_t step = step_b * p.t.s0 + step_at * p.t.s1, wrap = p.t.s0 - width * p.t.s1;
+    unsigned b = (unsigned)(tid / width);
+    int at = tid - (int)b * width;
+    int64_t off = b * p.t.s0 + at * p.t.s1;
+    while (b < (unsigned)p.t.B) {
+        int page[kEntries], len[kEntries], first[kEntries];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int64_t i = min(i0 + k * kPlanThreads, entries - 1);
-            const int b = (int)(i / p.t.width);
-            at[k] = (int)(i - (int64_t)b * p.t.width);
-            len[k] = p.t.lens[b];
-            page[k] = p.t.ids[b * p.t.s0 + at[k] * p.t.s1];
+        for (int k = 0; k < kEntries; k++) {
+            page[k] = -1;
+            len[k] = 0;
+            if (b < (unsigned)p.t.B) {
+                len[k] = p.t.lens[b];
+                page[k] = p.t.ids[off];
+            }
+            first[k] = at << p.lP;  // (a table has at most 2^30 tokens a sequence)
+            b += step_b;
+            at += step_at;
+            off += step;
+            if (at >= width) {
+                at -= width;
+                b++;
+                off += wrap;
+            }
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (((int64_t)at[k] << p.lP) < len[k] && page[k] >= 0 && page[k] < p.pages) atomicOr(&bits[page[k] >> 5], 1u << (page[k] & 31));
+        for (int k = 0; k < kEntries; k++)
+            if (first[k] < len[k] && (unsigned)page[k] < (unsigned)p.pages) atomicOr(&bits[page[k] >> 5], 1u << (page[k] & 31));
     }
     __syncthreads();
-    // this thread's words
-    const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-    auto valid = [&](int w) { return 32 * w + 32 <= p.pages ? ~0u : (1u << (p.pages & 31)) - 1u; };
+    const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);  // (per: at most 32)
     int used = 0, total;
     for (int w = w0; w < w1; w++) used += __popc(bits[w]);
-    const int used_before = before_me(used, waves, total);
+    before[tid] = before_me(used, waves, total);
+    __syncthreads();
+    // pages in use below page x, by a whole wave
+    auto used_below = [&](int x) {
+        if (x >= p.pages) return total;
+        const int w = x >> 5, t = w / per, in = w - t * per;  // (word `in` of thread t's)
+        const uint32_t mine = lane <= in ? bits[t * per + lane] : 0u;
+        return before[t] + __builtin_amdgcn_readlane(lanes_up_to(__popc(lane < in ? mine : mine & ((1u << (x & 31)) - 1u))), 63);
+    };
+    // this wave's pairs of words
+    const int all_waves = (int)gridDim.x * (kPlanThreads / 64), per_wave = (pairs + all_waves - 1) / all_waves;
+    const int q0 = min(((int)blockIdx.x * (kPlanThreads / 64) + wave) * per_wave, pairs), q1 = min(q0 + per_wave, pairs);
+    auto in_use = [&](int q) { return *(const uint64_t *)(bits + 2 * q); };
+    auto below = [&](int q, int x) { return x >= 64 * q + 64 ? ~0ull : x <= 64 * q ? 0ull : (1ull << (x - 64 * q)) - 1ull; };
+    // put(place, page) for the pages that of(pair) gives, their places from `place` on
+    auto each = [&](auto &&of, int place, auto &&put) {
+        for (int q = q0; q < q1; q += 64) {
+            const uint64_t m = q + lane < q1 ? of(q + lane) : 0ull;
+            const int n = __popcll(m), up = lanes_up_to(n);
+            for (int j = 0; j < min(64, q1 - q); j++) {
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)m, j), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(m >> 32), j);
+                const int first = place + __builtin_amdgcn_readlane(up - n, j);
+                if (((lane < 32 ? lo : hi) >> (lane & 31)) & 1u) put(first + (int)__builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u)), 64 * (q + j) + lane);
+            }
+            place += __builtin_amdgcn_readlane(up, 63);
+        }
+    };
+    const int start = min(64 * q0, p.pages), used_before = used_below(start);
+    const bool first_thread = blockIdx.x == 0 && tid == 0;
     if (p.free_list != nullptr) {
         const int free_total = p.pages - total;
-        int at = min(32 * w0, p.pages) - used_before;
-        for (int w = w0; w < w1; w++)
-            for (uint32_t left = ~bits[w] & valid(w); left != 0u; left &= left - 1u) p.free_list[at++] = 32 * w + __ffs(left) - 1;
-        for (int i = free_total + tid; i < p.pages; i += kPlanThreads) p.free_list[i] = -1;
-        if (tid == 0) *p.count = free_total;
+        each([&](int q) { return ~in_use(q) & below(q, p.pages); }, start - used_before, [&](int i, int page) { p.free_list[i] = page; });
+        for (int i = free_total + (int)blockIdx.x * kPlanThreads + tid; i < p.pages; i += (int)gridDim.x * kPlanThreads) p.free_list[i] = -1;
+        if (first_thread) *p.count = free_total;
         return;
     }
-    const int L = total;
-    auto below = [&](int w) { return 32 * w + 32 <= L ? ~0u : 32 * w >= L ? 0u : (1u << (L & 31)) - 1u; };  // pages < L
-    int holes = 0, movers = 0, hole_total, mover_total;
-    for (int w = w0; w < w1; w++) {
-        holes += __popc(~bits[w] & below(w));
-        movers += __popc(bits[w] & ~below(w));
-    }
-    int hole_at = before_me(holes, waves, hole_total), mover_at = before_me(movers, waves, mover_total);
-    for (int w = w0; w < w1; w++) {
-        for (uint32_t left = ~bits[w] & below(w); left != 0u; left &= left - 1u) p.holes[hole_at++] = 32 * w + __ffs(left) - 1;
-        for (uint32_t left = bits[w] & ~below(w); left != 0u; left &= left - 1u) p.movers[mover_at++] = 32 * w + __ffs(left) - 1;
-    }
-    __threadfence_block();
-    __syncthreads();
-    for (int i = tid; i < mover_total; i += kPlanThreads) p.to[p.movers[i]] = p.holes[i];
-    if (tid == 0) {
+    const int L = total, stay = used_below(L);  // pages in use below L: those that are where they are to be
+    each([&](int q) { return ~in_use(q) & below(q, L); }, min(start, L) - min(used_before, stay), [&](int i, int page) { p.holes[i] = page; });
+    each([&](int q) { return in_use(q) & ~below(q, L); }, max(used_before - stay, 0), [&](int i, int page) {
+        p.movers[i] = page;
+        p.rank[page] = i;
+    });
+    if (first_thread) {
         *p.count = L;
-        *p.moves = mover_total;
+        *p.moves = L - stay;
     }
 }
 
@@ -543,7 +576,7 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const PagedCompactPa
         const int b = (int)(i / p.t.width), j = (int)(i - (int64_t)b * p.t.width);
         int page = -1;
         if (((int64_t)j << lP) < p.t.lens[b]) page = page_at(p.t, b, j, p.c.pages);
-        p.new_ids[i] = page >= L ? p.to[page] : page;
+        p.new_ids[i] = page >= L ? p.holes[p.rank[page]] : page;
     }
     const int64_t items = (int64_t)*p.moves * p.c.H;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
@@ -595,10 +628,11 @@ hipError_t launch_paged_fork(const PagedForkParams &p, hipStream_t stream) {
     return hipGetLastError();
 }
 hipError_t launch_paged_plan(const PagedPlanParams &p, hipStream_t stream) {
-    const int smem = ((p.pages + 31) / 32) * 4;
+    const int smem = ((p.pages + 63) / 64) * 8;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(paged_plan_kernel, kPagedMostPages / 8, attr_done); e != hipSuccess) return e;
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), smem, stream, p);
+    const int groups = (p.pages + kPlanPages - 1) / kPlanPages;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(groups), dim3(kPlanThreads), smem, stream, p);
     return hipGetLastError();
 }
 hipError_t launch_paged_compact(const PagedCompactParams &p, hipStream_t stream) {

@@ -319,7 +319,8 @@ def test_fork(gpu):
         assert torch.equal(got, w)
 
 
-@pytest.mark.parametrize("pool,B,width,P", [(1, 1, 1, 32), (31, 2, 3, 64), (33, 5, 6, 32), (1000, 7, 60, 32), (40000, 33, 700, 64), (1 << 20, 64, 512, 32)])
+@pytest.mark.parametrize("pool,B,width,P", [(1, 1, 1, 32), (31, 2, 3, 64), (33, 5, 6, 32), (1000, 7, 60, 32), (40000, 33, 700, 64), (1 << 20, 64, 512, 32),
+                                            (8193, 5000, 1, 32), (20000, 3, 2500, 32), (16385, 40, 1024, 64)])
 def test_compact_and_free(gpu, pool, B, width, P):
     g = torch.Generator().manual_seed(pool)
     H, D = 1, 64
