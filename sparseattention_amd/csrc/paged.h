@@ -67,8 +67,9 @@ struct PagedCopyParams {
     PagedPool c;
     const int32_t *src, *dst;
     int n;
+    int heads;  // of a workgroup (set by the launch)
 };
-hipError_t launch_paged_copy(const PagedCopyParams &p, hipStream_t stream);
+hipError_t launch_paged_copy(PagedCopyParams p, hipStream_t stream);
 
 struct PagedForkParams {
     PagedPool c;
@@ -76,8 +77,9 @@ struct PagedForkParams {
     const int32_t *parents, *new_pages;
     int n;
     int32_t *new_ids, *new_lens;  // [n, width], [n]
+    int heads;
 };
-hipError_t launch_paged_fork(const PagedForkParams &p, hipStream_t stream);
+hipError_t launch_paged_fork(PagedForkParams p, hipStream_t stream);
 
 // Which pages are in use, by a bit per page in LDS, and what follows from it.
 struct PagedPlanParams {

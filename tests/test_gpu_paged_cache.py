@@ -267,9 +267,10 @@ def test_copy(gpu, H, D, P):
         assert torch.equal(got, w)
 
 
-def test_copy_of_many(gpu):
+@pytest.mark.parametrize("H", [2, 5])
+def test_copy_of_many(gpu, H):
     n = 700
-    cache = filled(2 * n, 2, 64, 32, 1, gpu)
+    cache = filled(2 * n, H, 64, 32, 1, gpu)
     order = torch.randperm(2 * n, generator=torch.Generator().manual_seed(2)).to(torch.int32).to(gpu)
     src, dst = order[:n], order[n:].clone()
     dst[:300] = dst[300:600]  # named again
@@ -313,6 +314,23 @@ def test_fork(gpu):
     for new, (old, blocks) in copies.items():
         for t in want:
             t[new, :, :blocks] = t[old, :, :blocks]
+    new_table, new_lens = sa.paged_cache_fork(cache, ints(table, gpu), ints(lens, gpu), ints(parents, gpu), ints(new_pages, gpu))
+    assert new_table.tolist() == rows and new_lens.tolist() == out
+    for got, w in zip(parts(cache), want):
+        assert torch.equal(got, w)
+
+
+def test_fork_of_many(gpu):
+    P, width, B, n = 32, 3, 6, 900
+    cache = filled(2000, 5, 64, P, 31, gpu)
+    table = torch.arange(B * width).view(B, width).tolist()
+    lens = [70, 33, 1, 0, 96, 64]
+    parents = [(7 * i) % 8 - 1 for i in range(n)]
+    new_pages = [100 + (i if i % 9 else i // 2) for i in range(n)]  # some of them twice
+    rows, out, copies = plain_fork(cache, table, lens, parents, new_pages)
+    want = [t.clone() for t in parts(cache)]
+    for t in want:
+        t[list(copies)] = t[[old for old, _ in copies.values()]]  # (a page is one block)
     new_table, new_lens = sa.paged_cache_fork(cache, ints(table, gpu), ints(lens, gpu), ints(parents, gpu), ints(new_pages, gpu))
     assert new_table.tolist() == rows and new_lens.tolist() == out
     for got, w in zip(parts(cache), want):
