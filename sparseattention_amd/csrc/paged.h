@@ -101,6 +101,11 @@ struct PagedCompactParams {
 };
 hipError_t launch_paged_compact(const PagedCompactParams &p, hipStream_t stream);
 
+// Where the units of a launch's row begin (paged_decode.hip), found by a launch in front.
+struct PagedUnits {
+    unsigned cuts, share, total, pad;
+    unsigned first[1];  // [units]
+};
 struct PagedDecodeParams {
     PagedPool c;
     PageTable t;
@@ -126,6 +131,7 @@ struct PagedDecodeParams {
     float *ws;
     uint64_t *arrivals;
     uint64_t tag;
+    PagedUnits *units;  // or null: every workgroup finds them itself
 };
 // Bytes of ws.
 size_t paged_decode_parts_bytes(int groups, int part_rows, int D);

@@ -202,6 +202,8 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
     return launched(who, sa::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
 }
 
+static size_t units_bytes(int64_t units) { return (sizeof(sa::PagedUnits) + (size_t)units * 4 + 15) / 16 * 16; }
+
 size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > 32 || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
         (int64_t)Hq / H * Sq > kMostRows)
@@ -209,7 +211,7 @@ size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int 
     const int R = Hq / H * Sq;
     const int64_t planes = (int64_t)B * H * ((R + 31) / 32);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units());
-    return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8;
+    return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8 + units_bytes((int64_t)B * H);
 }
 
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
@@ -276,7 +278,8 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     if (planes > (1 << 24) || planes * chunks > (1 << 30))
         return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
-    const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), need = parts_bytes + (size_t)(planes + plan.groups) * 8;
+    const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
+                 need = units_at + units_bytes((int64_t)B * p.c.H);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
     p.groups = plan.groups;
@@ -285,6 +288,7 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     p.ws = static_cast<float *>(workspace);
     p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + parts_bytes);
     p.tag = sa::next_launch_tag() | 1;
+    if ((p.full_ids != nullptr ? (int64_t)B * p.c.H : B) > sa::kPagedFewUnits(p.full_ids != nullptr)) p.units = reinterpret_cast<sa::PagedUnits *>(static_cast<uint8_t *>(workspace) + units_at);
     return launched(who, sa::launch_paged_decode(p, dtype, static_cast<hipStream_t>(stream)));
 }
 

@@ -294,6 +294,53 @@ struct Tile<DT, ND, 16, FAR> {
     }
 };
 
+// Where there are many units (kPagedFewUnits), a launch in front finds the share and where every unit begins in the row, divided by the unit's planes.
+constexpr int kUnitThreads = 1024;
+template <bool LISTS>
+__global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDecodeParams p, const int groups) {
+    __shared__ int sums[2][kUnitThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int U = LISTS ? p.t.B * p.c.H : p.t.B;
+    const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;
+    const int per = (U + kUnitThreads - 1) / kUnitThreads, u0 = min(tid * per, U), u1 = min(u0 + per, U);
+    const auto plus = [](int a, int x) { return a + x; };
+    const auto most = [](int a, int x) { return max(a, x); };
+    // (of all threads, and of those in front of this one)
+    auto over = [&](int x, auto &&op, int *all, int &total) {
+        const int up = scan(x, op);
+        if (lane == 63) all[wave] = up;
+        __syncthreads();
+        const int waves = scan(lane < kUnitThreads / 64 ? all[lane] : 0, op);
+        total = __builtin_amdgcn_readlane(waves, 63);
+        __syncthreads();
+        return up - x + (wave == 0 ? 0 : __builtin_amdgcn_readlane(waves, max(wave - 1, 0)));
+    };
+    int sum = 0, longest = 0, total;
+#pragma unroll 8
+    for (int u = u0; u < u1; u++) {
+        const int T = max(unit_of<LISTS>(p, u).T, 1);
+        p.units->first[u] = (unsigned)T;
+        sum += T;
+        longest = max(longest, T);
+    }
+    over(sum, plus, sums[0], total);
+    over(longest, most, sums[1], longest);
+    const PagedShare share = paged_share((unsigned)total * M, U * M, groups, (unsigned)longest, (unsigned)p.parts);
+    sum = 0;
+    for (int u = u0; u < u1; u++) sum += (int)paged_row_length(share, p.units->first[u]);
+    unsigned at = (unsigned)over(sum, plus, sums[0], total);
+    for (int u = u0; u < u1; u++) {
+        const unsigned n = paged_row_length(share, p.units->first[u]);
+        p.units->first[u] = at;
+        at += n;
+    }
+    if (tid == 0) {
+        p.units->cuts = share.cuts;
+        p.units->share = share.share;
+        p.units->total = (unsigned)total * M;
+    }
+}
+
 template <int DT, int ND, int ROWS, bool FAR, bool LISTS>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
     using E = Elem<DT>;
@@ -316,69 +363,88 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     // ---- this workgroup's piece [x0, x1) of the row, and the unit it starts in (the host: a row is at most 2^30 chunks) ----
     const int U = LISTS ? p.t.B * p.c.H : p.t.B;                // units
     const unsigned M = LISTS ? p.RT : (unsigned)p.c.H * p.RT;  // planes of each
-    const int per_lane = (U + 63) >> 6;
-    Unit own = unit_of<LISTS>(p, min(lane * per_lane, U - 1));  // the lane's first unit (the only one of up to 64 units)
-    int mine = lane * per_lane < U ? max(own.T, 1) : 0, longest = mine;
-    if (per_lane > 1)
-#pragma unroll 4
-        for (int j = 1; j < per_lane; j++) {
-            const int u = lane * per_lane + j;
-            const int T = u < U ? max(unit_of<LISTS>(p, min(u, U - 1)).T, 1) : 0;
-            mine += T;
-            longest = max(longest, T);
-        }
-    const auto plus = [](int a, int x) { return a + x; };
-    int upto = scan(mine, plus);
-    longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
-    unsigned total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
-    const PagedShare share = paged_share(total, U * M, gridDim.x, (unsigned)longest, (unsigned)p.parts);
-    const bool cuts = share.cuts;
+    PagedShare share;
+    unsigned total;
     auto length = [&](int chunks) __attribute__((always_inline)) { return paged_row_length(share, (unsigned)max(chunks, 1)); };  // in the row
-    if (cuts) {
-        mine = 0;
-        if (per_lane == 1)
-            mine = lane < U ? (int)length(own.T) : 0;
-        else
-#pragma unroll 4
-            for (int j = 0; j < per_lane; j++) {
-                const int u = lane * per_lane + j;
-                const int n = (int)length(unit_of<LISTS>(p, min(u, U - 1)).T);
-                mine += u < U ? n : 0;
+    // (few units: lane l has units l, 64 + l, ...; in the row: a unit, the units up to it)
+    constexpr int NB = kPagedFewUnits(LISTS) / 64;
+    Unit own[NB], unit;
+    int mine[NB], upto[NB];
+    const bool few = p.units == nullptr;
+    if (few) {
+        int sum = 0, longest = 0;
+        const auto plus = [](int a, int x) { return a + x; };
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+            if (k == 0 || 64 * k < U) own[k] = unit_of<LISTS>(p, min(64 * k + lane, U - 1));
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+            if (k == 0 || 64 * k < U) {
+                mine[k] = 64 * k + lane < U ? max(own[k].T, 1) : 0;
+                upto[k] = sum + scan(mine[k], plus);
+                sum = __builtin_amdgcn_readlane(upto[k], 63);
+                longest = max(longest, mine[k]);
             }
-        upto = scan(mine, plus);
+        longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
+        share = paged_share((unsigned)sum * M, U * M, gridDim.x, (unsigned)longest, (unsigned)p.parts);
+        if (share.cuts) {
+            sum = 0;
+#pragma unroll
+            for (int k = 0; k < NB; k++)
+                if (k == 0 || 64 * k < U) {
+                    mine[k] = 64 * k + lane < U ? (int)length(own[k].T) : 0;
+                    upto[k] = sum + scan(mine[k], plus);
+                    sum = __builtin_amdgcn_readlane(upto[k], 63);
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                mine[k] += 64 * k + lane < U ? (int)kPagedComing : 0;
+                upto[k] += min(64 * k + lane + 1, U) * (int)kPagedComing;
+            }
+            sum += U * (int)kPagedComing;
+        }
+        total = (unsigned)sum * M;
     } else {
-        const int before = min(lane * per_lane, U), after = min((lane + 1) * per_lane, U);  // the lane's units
-        mine += (after - before) * (int)kPagedComing;
-        upto += after * (int)kPagedComing;
+        share = {p.units->cuts != 0u, p.units->share};
+        total = p.units->total;
     }
-    total = (unsigned)__builtin_amdgcn_readlane(upto, 63) * M;
+    const bool cuts = share.cuts;
     const int me = paged_piece(blockIdx.x, cuts ? total : gridDim.x);
     if (me < 0) return;
     const unsigned piece = cuts ? 1u : share.share, x0 = piece * me, x1 = min(x0 + piece, total);
     if (x0 >= total) return;
-    int u;
+    int u = 0;
     unsigned base;  // of unit u
-    Unit unit;
-    {
-        const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < (unsigned)upto * M)) - 1;  // the lane whose units hold x0
-        base = (unsigned)__builtin_amdgcn_readlane(upto - mine, at) * M;
-        u = at * per_lane;
-        if (per_lane == 1) unit = of_lane(own, at);
-        // its units by 64, a lane each
-        for (int j0 = 0; per_lane > 1; j0 += 64) {
-            own = unit_of<LISTS>(p, min(u + j0 + lane, U - 1));
-            const int n = j0 + lane < per_lane && u + j0 + lane < U ? (int)length(own.T) : 0;
-            const int to = scan(n, plus);
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(x0 < base + (unsigned)to * M);
-            if (hit != 0ull) {
-                const int in = __ffsll((unsigned long long)hit) - 1;
-                unit = of_lane(own, in);
-                base += (unsigned)__builtin_amdgcn_readlane(to - n, in) * M;
-                u += j0 + in;
-                break;
+    if (few) {
+        // the block of 64 units and the lane whose unit holds x0
+        int k = 0;
+#pragma unroll
+        for (int i = 1; i < NB; i++)
+            if (64 * i < U && x0 >= (unsigned)__builtin_amdgcn_readlane(upto[i - 1], 63) * M) k = i;
+        unit = own[0];
+        int to = upto[0], n = mine[0];
+#pragma unroll
+        for (int i = 1; i < NB; i++)
+            if (k == i) {
+                unit = own[i];
+                to = upto[i];
+                n = mine[i];
             }
-            base += (unsigned)__builtin_amdgcn_readlane(to, 63) * M;
+        const int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(x0 < (unsigned)to * M)) - 1;
+        u = 64 * k + at;
+        base = (unsigned)__builtin_amdgcn_readlane(to - n, at) * M;
+        unit = of_lane(unit, at);
+    } else {
+        for (int left = U; left > 1;) {  // of the units u .. u + left - 1, every step-th by a lane
+            const int step = (left + 63) >> 6;
+            const int skip = (__popcll(__builtin_amdgcn_ballot_w64(lane * step < left && p.units->first[min(u + lane * step, U - 1)] * M <= x0)) - 1) * step;
+            u += skip;
+            left = min(step, left - skip);
         }
+        u = __builtin_amdgcn_readfirstlane(u);
+        base = (unsigned)__builtin_amdgcn_readfirstlane((int)p.units->first[u]) * M;
+        unit = of_lane(unit_of<LISTS>(p, u), 0);
     }
 
     // Of the workgroups of a compute unit the oldest goes first and is done when others have a third of their piece left; so the
@@ -741,6 +807,10 @@ hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
     auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, LISTS>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
+    if (p.units != nullptr) {
+        hipLaunchKernelGGL(paged_units_kernel<LISTS>, dim3(1), dim3(kUnitThreads), 0, stream, p, p.groups);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL(kern, dim3((unsigned)p.groups), dim3(kWaves * 64), smem, stream, p);
     return hipGetLastError();
 }

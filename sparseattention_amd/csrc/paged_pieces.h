@@ -23,6 +23,10 @@ constexpr int kPagedMostParts = 128;  // of a plane (131072 keys of one K/V head
 // 2, 102.9 with 4, 102.0 with 8, 103.6 with 16; 16 sequences at D = 256 75.8 -> 73.6 with 8.
 constexpr unsigned kPagedComing = 8;
 
+// Up to that many units (sequences, with lists their K/V heads) every wave finds its piece itself, of more a launch in front finds where they
+// begin.  us, by every wave | by a launch: lists of 256 sequences x 8 heads 61 | 41, of 1024 x 8 191 | 89; 256 sequences without lists 31.6 | 34,
+// 16384 164 | 122.
+constexpr int kPagedFewUnits(bool lists) { return lists ? 64 : 256; }
 // Workgroups that a compute unit holds (a wave of each per SIMD), by D / 32 and the rows of a tile.
 constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
 

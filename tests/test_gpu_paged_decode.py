@@ -91,6 +91,8 @@ def check(cache, table, lens, q, o, lse=None, see=None, counts=None, window=None
     (40, 8, 1, 64, 64, 1, [37 * i % 1501 for i in range(40)], torch.bfloat16),
     (130, 1, 3, 64, 32, 1, [53 * i % 200 for i in range(130)], torch.float16),
     (300, 8, 1, 64, 32, 1, [7 * i % 90 for i in range(300)], torch.bfloat16),
+    (256, 3, 1, 64, 32, 1, [31 * i % 400 for i in range(256)], torch.float16),
+    (1300, 1, 2, 64, 32, 1, [11 * i % 70 for i in range(1300)], torch.bfloat16),
     (6, 2, 5, 128, 64, 32, [900, 33, 0, 400, 2500, 1], torch.bfloat16),
 ])
 def test_causal(gpu, B, H, G, D, P, Sq, lens, dtype):
@@ -150,7 +152,7 @@ def masks(kind, B, H, Sq, Sk, P, seed):
 @pytest.mark.parametrize("B,H,G,D,P,Sq,Sk,dtype", [(2, 2, 1, 128, 32, 1, 320, torch.bfloat16), (2, 3, 2, 64, 64, 5, 1024, torch.float16),
                                                    (1, 2, 4, 128, 128, 32, 512, torch.bfloat16), (2, 1, 3, 256, 256, 2, 768, torch.bfloat16),
                                                    (3, 2, 5, 128, 32, 9, 4096, torch.float16), (70, 3, 1, 64, 32, 2, 192, torch.bfloat16),
-                                                   (24, 40, 1, 64, 32, 1, 96, torch.float16)])
+                                                   (24, 40, 1, 64, 32, 1, 96, torch.float16), (420, 3, 1, 64, 32, 1, 64, torch.bfloat16)])
 def test_lists(gpu, kind, B, H, G, D, P, Sq, Sk, dtype):
     lens = [(Sk - 7, Sk // 2 + 3, Sk)[b % 3] for b in range(B)]
     cache, table = make(B, H, D, P, lens, dtype, 6, gpu, width=Sk // P + 1)
