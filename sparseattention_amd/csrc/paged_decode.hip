@@ -4,12 +4,12 @@
 // the reference names decode kernels as future work, README.md:65) with K and V read from pages of e4m3 codes
 // (paged.h), several query heads per K/V head, and sequences of their own lengths:
 //     s = q . k / sqrt(D),  p = exp2(s - m),  o = sum p v / sum p     over the keys that a row attends to.
-// The R = G * Sq rows of a K/V head go through the matrix unit together, 32 a tile; codes become bf16 or fp16 (exactly,
-// V with its scale) on their way from registers into the products, the scale of K joins the softmax's.  Bound by the
+// The R = G * Sq rows of a K/V head go through the matrix unit together, 16 or 32 a tile; codes become bf16 or fp16 (exactly,
+// V with its scale, which in fp16 rounds below its normal numbers) on their way from registers into the products, the scale of K joins the softmax's.  Bound by the
 // bytes of K and V, each read once.  Per chunk of 32 keys a wave
 //   * has K and V as operands straight from memory (D / 32 loads of 1 KiB each for both: paged.h has the order),
 //   * computes S^T = K . Q^T (32 keys x 32 rows), masks, P = exp2(S^T - m), O^T += V^T . P^T.
-// P is rounded to q's type for the second product, by half a step (bf16 2^-9, fp16 2^-12) of each weight, as in this library's other
+// P is rounded to q's type for the second product, by up to half a step (bf16 2^-8, fp16 2^-11) of each weight, as in this library's other
 // attention kernels: a split of P in two would double that product and still leave the output's own rounding.  Scores, reference values, sums and
 // accumulators are float32.
 // Measured (bf16 and one row per query head where nothing else is said): 32 sequences of up to 32768 keys, 8 x 8 heads, D = 128 286 us, 6.4 TB/s
@@ -60,7 +60,7 @@ __device__ __forceinline__ float scale_of(float s) {  // (as the cache's kernels
 // ---- who does what (paged_pieces.h) ----
 // Every workgroup takes an equal piece of the row of chunks, whatever the lengths: segments, each of one plane.  A plane that lies in several
 // workgroups' pieces is added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself,
-// by a sum over the units.
+// by a sum over the units, or a launch in front does it for all.
 struct Unit {
     int len, cnt;  // keys and query rows of its sequence
     int T0, T;     // first chunk, chunks (0: none)
