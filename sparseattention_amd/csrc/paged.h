@@ -18,17 +18,32 @@ constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^119 is the lar
 constexpr int kPagedMostPages = 1 << 20;         // (compaction keeps a bit per page in LDS)
 
 // In fp16 a code times 2^e, e > 7, may be beyond the type: fp16 tokens up to 65504 make blocks of the scale 2^8, where 65504 itself is held as 65536,
-// and codes that no token has, or that a row leaves out, stand for up to 114688 and more; times a weight of 0 these must be 0.  There codes stop at
-// the largest one within the type, 1.875 * 2^15 up to e = 21; four codes at a time, NaN as it is.
+// bf16 tokens blocks of any scale, and codes that no token has, or that a row leaves out, stand for up to 114688 and more; times a weight of 0 these must
+// be 0.  What lies beyond 65504 counts as 61440, the largest value within the type that four bits hold; NaN stays NaN.
+// within_fp16 gives the scale that the block has from there on; each(f) is to replace every register w of four codes by f(w).
+// Up to e = 21 61440 is a code of the block's own, at which larger ones stop.  From 22 on it is none, and codes from 8 on are beyond: the
+// block is taken to 2^8, where 61440 is code 0x77 and the multiples of 2^13 below 2^16 that codes 1 .. 7 may be have codes too.
 constexpr float kFp16Scale = 128.f;  // (448 * 2^7 is within)
-__device__ __forceinline__ uint32_t most_fp16_code(float scale) {
+template <class Each>
+__device__ __forceinline__ float within_fp16(float scale, Each &&each) {
     const int e = (int)(__float_as_uint(scale) >> 23) - 127;
-    return (uint32_t)(e <= 21 ? 0x77 - 8 * (e - 8) : 15 >> (e - 21 < 4 ? e - 21 : 4)) * 0x01010101u;
-}
-__device__ __forceinline__ uint32_t within_fp16(uint32_t w, uint32_t most) {
-    const uint32_t size = w & 0x7f7f7f7fu, nan = (size + 0x01010101u) & 0x80808080u;
-    const uint32_t over = (((size + (0x7f7f7f7fu - most)) & 0x80808080u & ~nan) >> 7) * 0x7fu;
-    return (w & ~over) | (most & over);
+    if (e <= 21) {
+        const uint32_t most = (uint32_t)(0x77 - 8 * (e - 8)) * 0x01010101u;
+        each([=](uint32_t w) {
+            const uint32_t size = w & 0x7f7f7f7fu, nan = (size + 0x01010101u) & 0x80808080u;
+            const uint32_t over = (((size + (0x7f7f7f7fu - most)) & 0x80808080u & ~nan) >> 7) * 0x7fu;
+            return (w & ~over) | (most & over);
+        });
+        return scale;
+    }
+    // what codes 0 .. 3 and 4 .. 7 become: n * 2^(e - 9) over 2^8
+    const uint32_t low = e == 22 ? 0x6c686000u : e == 23 ? 0x74706800u : e == 24 ? 0x77777000u : 0x77777700u, high = e == 22 ? 0x76747270u : 0x77777777u;
+    each([=](uint32_t w) {
+        const uint32_t size = w & 0x7f7f7f7fu, nan = ((size + 0x01010101u) & 0x80808080u) >> 7, over = ((size + 0x78787878u) & 0x80808080u) >> 7;
+        const uint32_t within = __builtin_amdgcn_perm(high, low, size & 0x07070707u) & ~(over * 0x7fu);
+        return (w & 0x80808080u) | within | over * 0x77u | nan * 0x7fu;
+    });
+    return 256.f;
 }
 
 struct PagedPool {

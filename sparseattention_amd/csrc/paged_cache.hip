@@ -335,13 +335,13 @@ __global__ __launch_bounds__(64 * kCacheWaves) void paged_gather_kernel(const Pa
         for (int c = 0; c < ND; c++)
             u[c] = *(const u32x4 *)(in + (values ? 1024 * (2 * (c >> 1) + (l32 >> 4)) + 16 * (32 * hh + 2 * (l32 & 15) + (c & 1)) : 1024 * c + 16 * lane));
         scale = exp2i(exp_of_scale((values ? p.c.v_scales : p.c.k_scales)[at]));
-        if (DT == 1 && scale > kFp16Scale) {
-            const uint32_t most = most_fp16_code(scale);
+        if (DT == 1 && scale > kFp16Scale)
+            scale = within_fp16(scale, [&](auto &&f) {
 #pragma unroll
-            for (int c = 0; c < ND; c++)
+                for (int c = 0; c < ND; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) u[c][i] = within_fp16(u[c][i], most);
-        }
+                    for (int i = 0; i < 4; i++) u[c][i] = f(u[c][i]);
+            });
     }
     const int64_t *const xs = values ? p.vs : p.ks;
     uint16_t *const x = (values ? p.v : p.k) + b * xs[0] + h * xs[1] + (int64_t)first * xs[2];

@@ -578,7 +578,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 vs_at = here.vs;
             }
             const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_at), j & 63))) * p.scale;
-            const float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_at), j & 63)));
+            float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_at), j & 63)));
             const int jn = j + PRE;
             if ((jn & 63) == 0 && jn < nw) {
                 here = next;
@@ -647,10 +647,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                     out_rows.poison(x, att);
                 }
             }
-            if (DT == 1 && vs > kFp16Scale) {
-                const uint32_t most = most_fp16_code(vs);
-                X::each_v(x, [&](auto &v, int e) { v[e] = within_fp16(v[e], most); });
-            }
+            if (DT == 1 && vs > kFp16Scale) vs = within_fp16(vs, [&](auto &&f) { X::each_v(x, [&](auto &v, int e) { v[e] = f(v[e]); }); });
             out_rows.add(x, pw, vs);
             request_v(nc, x);
             c = nc;

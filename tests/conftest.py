@@ -12,6 +12,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a ROCm GPU (run on the MI355X box)")
 
 
+# Cases whose expectation is not what the operator promises.  They run as they are, and are expected to fail.
+HOLD_A_WRONG_VALUE = {
+    "test_gpu_paged_cache.py": ({f"test_every_code_in_fp16[{e}]" for e in (22, 23, 24, 25, 40, 119)},
+                                "expects the largest code of the block within fp16 (57344, 49152, 32768, 0) where the cache holds more "
+                                "than 65504; documented is 61440, which test_gpu_paged_fp16_range.py checks"),
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        names, reason = HOLD_A_WRONG_VALUE.get(os.path.basename(str(item.path)), ((), ""))
+        if item.name in names:
+            item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
+
+
 @pytest.fixture(scope="session")
 def gpu():
     import torch
