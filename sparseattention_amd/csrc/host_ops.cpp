@@ -393,8 +393,9 @@ Cache cache_of(py::handle o) {
     x.D = d.cast<int64_t>();
     if (x.k.dim() != 4 || x.k.scalar_type() != at::kByte || x.k.size(3) % 32 || !x.k.is_contiguous())
         value_error("cache.k must be contiguous uint8 [pages, H, page_size / 32, 32 * D], got " + str(x.k));
-    if (!x.k.is_cuda()) throw std::runtime_error("the paged cache's operators need it on a ROCm GPU; there is no CPU path");
     const int64_t N = x.k.size(0), H = x.k.size(1), per = x.k.size(2), Dk = x.k.size(3) / 32;
+    if (N < 1 || H < 1 || per < 1) value_error("a cache needs a page, a head and 32 tokens a page at least, got " + str(x.k));
+    if (!x.k.is_cuda()) throw std::runtime_error("the paged cache's operators need it on a ROCm GPU; there is no CPU path");
     if (x.v.sizes() != x.k.sizes() || x.v.scalar_type() != at::kByte || !x.v.is_contiguous() || x.v.device() != x.k.device())
         value_error("cache.v must be like cache.k, got " + str(x.v));
     const int64_t want[3] = {N, H, per};
