@@ -77,12 +77,13 @@ void same_device(const Tensor &ref, const char *name, const OptTensor &t) {
     if (t) same_device(ref, name, *t);
 }
 
-// The kernels want a unit stride in D and 16-byte aligned rows; copied only when that does not hold.
+// The kernels want a unit stride in D and 16-byte aligned rows; copied only when that does not hold.  (A clone: contiguous() would give back a
+// contiguous tensor as it is, at whatever address and, in dimensions of size 1, with whatever strides.)
 Tensor kernel_ready(const Tensor &t) {
     const int64_t per16 = 16 / t.element_size();
     bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
     for (int64_t d = 0; d + 1 < t.dim(); d++) ok = ok && t.stride(d) % per16 == 0;
-    return ok ? t : t.contiguous();
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 // The head dim the kernels run a request for D with: the smallest that holds it (q, k, v are then padded with zero columns,
 // which change neither the scores nor the first D columns of the result; the softmax scale stays that of D).  A D beyond
