@@ -487,7 +487,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         }
         const uint32_t bits_i = (uint32_t)i << (lP - 3);
 
-        float m_ref = 0.f, raise_above = -3.0e38f, l = 0.f;
+        float m_ref = 0.f, raise_above = kNegInf, l = 0.f;
         X out_rows;
         out_rows.clear();
 
@@ -627,10 +627,18 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 l *= a;
                 out_rows.scale(a);
             }
+            // The reference value is a rounded score, the fma's product is not: beyond 2^24 they differ by more than 1, and the weight of a row's largest
+            // score would be anything.  There the products are rounded too.
+            float by = ks;
+            if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(m_ref) > 16777216.f) != 0ull) {
+                by = 1.f;
+#pragma unroll
+                for (int e = 0; e < X::NS; e++) s[e] *= ks;
+            }
             uint32_t pw[X::NS / 2];
 #pragma unroll
             for (int e = 0; e < X::NS; e += 2) {
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], ks, -m_ref)), z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], ks, -m_ref));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], by, -m_ref)), z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], by, -m_ref));
                 l += y + z;
                 pw[e >> 1] = E::pack2(y, z);
             }
