@@ -578,7 +578,7 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
  *             lens[b]; window must be 0.  Tile indices out of range are skipped.
  * workspace, lse, dtype, sm_scale_log2: as for sa_sparse_attention_decode; sa_decode_paged_workspace_bytes(...) bytes, 16-byte aligned (of
  * the current device).  K and V are read as they are held, exactly; in fp16 V as sa_paged_cache_gather gives it.  A masked NaN has no
- * effect.
+ * effect.  The product of sm_scale_log2 and a block's scale is at least float32's least number and at most its largest.
  */
 size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size);
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache,

@@ -57,6 +57,10 @@ __device__ __forceinline__ float scale_of(float s) {  // (as the cache's kernels
     return __uint_as_float((uint32_t)min(max(e, 127 + kScaleExpMin), 127 + kScaleExpMax) << 23);
 }
 
+// A product of positive factors that is 0 or infinite, as the least or the largest number: 0 times the -inf of a masked key and infinity times a score
+// of 0 would be NaN.
+__device__ __forceinline__ float positive(float x) { return __uint_as_float(min(max(__float_as_uint(x), 1u), 0x7f7fffffu)); }
+
 // ---- who does what (paged_pieces.h) ----
 // Every workgroup takes an equal piece of the row of chunks, whatever the lengths: segments, each of one plane.  A plane that lies in several
 // workgroups' pieces is added up by the last of them.  T is known on the device only, so every wave finds its workgroup's piece itself,
@@ -577,7 +581,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 ks_at = here.ks;
                 vs_at = here.vs;
             }
-            const float ks = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_at), j & 63))) * p.scale;
+            const float ks = positive(scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_at), j & 63))) * p.scale);
             float vs = scale_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_at), j & 63)));
             const int jn = j + PRE;
             if ((jn & 63) == 0 && jn < nw) {
