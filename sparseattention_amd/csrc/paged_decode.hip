@@ -440,12 +440,9 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         base = (unsigned)__builtin_amdgcn_readlane(to - n, at) * M;
         unit = of_lane(unit, at);
     } else {
-        for (int left = U; left > 1;) {  // of the units u .. u + left - 1, every step-th by a lane
-            const int step = (left + 63) >> 6;
-            const int skip = (__popcll(__builtin_amdgcn_ballot_w64(lane * step < left && p.units->first[min(u + lane * step, U - 1)] * M <= x0)) - 1) * step;
-            u += skip;
-            left = min(step, left - skip);
-        }
+        u = paged_find_unit(U, [&](int from, int step, int left) {
+            return __popcll(__builtin_amdgcn_ballot_w64(lane * step < left && p.units->first[min(from + lane * step, U - 1)] * M <= x0));
+        });
         u = __builtin_amdgcn_readfirstlane(u);
         base = (unsigned)__builtin_amdgcn_readfirstlane((int)p.units->first[u]) * M;
         unit = of_lane(unit_of<LISTS>(p, u), 0);

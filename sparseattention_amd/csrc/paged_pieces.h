@@ -80,6 +80,19 @@ SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned gr
     return r;
 }
 
+// The last of U units that begins at a place of the row or in front of it, as a wave finds it, which looks at 64 at a time: count(u, step, left) is how
+// many of the units u, u + step, ... (64 at most, below u + left) do, and the first of them does.
+template <class Count>
+SA_PIECES_FN int paged_find_unit(int U, Count &&count) {
+    int u = 0;
+    for (int left = U; left > 1;) {
+        const int step = (left + 63) >> 6, skip = (count(u, step, left) - 1) * step;
+        u += skip;
+        left = step < left - skip ? step : left - skip;
+    }
+    return u;
+}
+
 // A plane of T chunks in the row.
 SA_PIECES_FN unsigned paged_row_length(PagedShare s, unsigned T) { return s.cuts ? (T + s.share - 1) / s.share : T + kPagedComing; }
 // What of a plane's place in the row, from at_row on, is not its chunks.
