@@ -13,9 +13,8 @@
 
 namespace sa {
 
-constexpr int kPagedBlock = 32;                  // tokens that share a scale
-constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^119 is the largest that bf16 and float32 hold
-constexpr int kPagedMostPages = 1 << 20;         // (compaction keeps a bit per page in LDS)
+constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^120 would be beyond bf16 and float32
+constexpr int kPagedMostPages = 1 << 20;               // (compaction keeps a bit per page in LDS)
 
 // In fp16 a code times 2^e, e > 7, may be beyond the type: fp16 tokens up to 65504 make blocks of the scale 2^8, where 65504 itself is held as 65536,
 // bf16 tokens blocks of any scale, and codes that no token has, or that a row leaves out, stand for up to 114688 and more; times a weight of 0 these must
