@@ -498,8 +498,8 @@ int sa_sparse_attention_decode_mask(const void *q, const int64_t q_strides[4], c
  *
  * A pool of pages of page_size tokens (32, 64, 128 or 256) of all H K/V heads; a sequence's tokens lie in the pages that its row of a
  * page table names.  Blocks of 32 consecutive tokens of one head are held as e4m3 codes (float8_e4m3fn) with a scale 2^e: e is the least
- * integer with max|x| <= 448 * 2^e over the block's finite values, from -96 to 119; x is held as round(x / 2^e) * 2^e, NaN and infinities
- * as NaN.  D is 64, 128 or 256; the callers' tensors have head_dim columns, a multiple of 8 up to D, the pool's further ones are zero.
+ * integer with max|x| <= 448 * 2^e over the block's finite values, from -96 to 119; x is held as round(x / 2^e) * 2^e (as +-448 * 2^119
+ * beyond that), NaN and infinities as NaN.  D is 64, 128 or 256; the callers' tensors have head_dim columns, a multiple of 8 up to D, the pool's further ones are zero.
  *   k, v               uint8 [num_pages, H, page_size / 32, 32 * D], contiguous, 16-byte aligned; the order inside a block is the kernels' own
  *                      (csrc/paged.h): sa_paged_cache_gather gives the values
  *   k_scales, v_scales float32 [num_pages, H, page_size / 32], contiguous

@@ -32,7 +32,9 @@ MOST_PAGES = 1 << 20
 class PagedCache:
     """A pool of pages (:func:`empty_paged_cache`).  Blocks of 32 consecutive tokens of one head are e4m3 codes with one scale
     2^e each, e the least integer for which the block's largest finite magnitude is at most 448 * 2^e (-96 <= e <= 119): a
-    value is off by at most 2^-4 of itself, or by 2^-10 * 2^e where it is smaller than 2^-6 * 2^e.  NaN and infinities are held as NaN.
+    value is off by at most 2^-4 of itself, or by 2^-10 * 2^e where it is smaller than 2^-6 * 2^e.  Where later tokens made the
+    scale grow it was rounded again each time, and is off by less than 2^-4 of itself and 2^-9 * 2^e together.  What is larger than 448 * 2^119
+    (2.98e38; bf16 ends at 3.39e38) is held as that.  NaN and infinities are held as NaN.
 
     ``k``, ``v``: uint8 [pages, H, page_size / 32, 32 * D], in the order the kernels read (:func:`paged_cache_gather` gives
     the values); ``k_scales``, ``v_scales``: float32 [pages, H, page_size / 32].  Head dims that the kernels do not have (they have
