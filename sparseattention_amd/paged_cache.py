@@ -10,7 +10,10 @@ and a prompt's later chunk, which has more than 32 rows, reads its keys back:
 
     paged_cache_append(cache, k, v, page_table, lens)
     K, V = paged_cache_gather(cache, page_table, lens + n)
+    K, V = (x.repeat_interleave(q.shape[1] // cache.num_heads, 1) for x in (K, V))
     o = sparse_attention(q, K, V, mask, BLOCK_Q, BLOCK_K)
+
+(sparse_attention has a K/V head per query head: with grouped heads the third line copies K and V for each of a group.)
 
 All calls enqueue work on the current stream of the cache's device and read no tensor on the host, so they can be captured
 into a graph.  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip and csrc/paged_decode.hip."""
