@@ -508,7 +508,8 @@ int sa_sparse_attention_decode_mask(const void *q, const int64_t q_strides[4], c
  *                      An entry that is no page (outside [0, num_pages)) is as if nothing were there: nothing is stored, read as zeros,
  *                      attended to.
  *   lens               device int32 [B]: tokens that each sequence holds; below 0 counts as 0.
- * Pages may be shared by sequences that read them.  Two sequences of one call that store into the same block leave it undefined.
+ * Pages may be shared by sequences that read them.  Two sequences of one call, or two entries of one, that store into the same block leave it
+ * undefined.
  */
 typedef struct sa_paged_cache {
     uint8_t *k, *v;

@@ -486,7 +486,7 @@ __device__ __forceinline__ int before_me(int x, int *waves, int &total) {
 }
 
 // A bit per page that a sequence uses, then the pairs of a compaction or the free list.  Every workgroup reads the whole table and has all bits in
-// LDS (2^20 pages: 128 KiB), which beats more launches over bits in memory; each writes the lists of its own part of the pages, 64 pages
+// LDS (2^20 pages: 128 KiB), in one launch: what the small tables of most programs cost is that.  Each writes the lists of its own part of the pages, 64 pages
 // a step of a wave.  Free list, us, by one workgroup whose threads write the pages of their own words | so: 64 sequences in 2048 columns, 70000
 // pages 61 | 29; in 8192 columns, 2^20 pages 709 | 117; 24 in 128 columns, 6147 pages 5.8 | 6.3.  Most of it is a table entry's VALU work, 20 instructions.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PagedPlanParams p) {

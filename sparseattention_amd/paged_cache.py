@@ -16,7 +16,7 @@ and a prompt's later chunk, which has more than 32 rows, reads its keys back:
 (sparse_attention has a K/V head per query head: with grouped heads the third line copies K and V for each of a group.)
 
 All calls enqueue work on the current stream of the cache's device and read no tensor on the host, so they can be captured
-into a graph.  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip and csrc/paged_decode.hip."""
+into a graph (tile lists that a caller wrote or changed are looked at on the host, once, by the first call that gets them).  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip and csrc/paged_decode.hip."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -88,8 +88,8 @@ def paged_cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page
     ``page_table`` int32 [B, pages], ``lens``, ``counts`` int32 [B], on the cache's device; ``lens`` is what the sequences hold before and
     is not changed.  Tokens past the table, and those whose entry is no page, are not stored.  The 32 tokens of a block
     share a scale: one that holds some keeps its scale or takes a larger one, with which what it holds is rounded again;
-    what a block held before its first token of the sequence does not count.  Sequences of one call must not store into
-    the same page (fork it first: :func:`paged_cache_fork`)."""
+    what a block held before its first token of the sequence does not count.  Sequences of one call, or two entries of one, must not
+    store into the same page (fork it first: :func:`paged_cache_fork`)."""
     _native.host().paged_append(cache, k, v, page_table, lens, counts)
 
 
