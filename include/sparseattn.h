@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define SA_ABI_VERSION 19
+#define SA_ABI_VERSION 20
 
 enum sa_status {
     SA_OK = 0,
@@ -591,6 +591,49 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
                                      const int64_t packed_strides[2], int tiles, int B, int Hq, int Sq, int window, int dtype,
                                      float sm_scale_log2, void *workspace, size_t workspace_bytes, float *lse,
                                      const int64_t lse_strides[3], void *stream);
+
+/*
+ * Norm and position rotation of queries and keys in front of attention, in one pass.  No counterpart in the reference, whose attention takes q and
+ * k as they are (sparseattention/sparse_attn_kernel.py:149).  A row x of D values (a multiple of 8 up to 256):
+ *   y = x / sqrt(mean(x^2) + eps) * weight    with a weight [D]; y = x without
+ *   of the first R columns (a multiple of 8 up to D) the pairs (a, b) at (j, j + R/2), or interleaved (2j, 2j + 1), j < R/2, become
+ *   (a cos t - b sin t, a sin t + b cos t),   t = positions[axes[j]][b][s] * frequencies[j]
+ * t is taken to a part of a turn in 64 bits, the rest is float32, rounded once to the output's type.
+ *   frequencies  device float64 [R/2], radians per position
+ *   axes         device int32 [R/2], which row of positions each pair turns by (one out of range is taken as the nearest), or NULL: row 0
+ *   positions    device int32, or int64 (positions_64 != 0), [num_axes, B, S], strides in elements (0 allowed)
+ *   weights      of the rows' type or float32, or NULL each
+ */
+typedef struct sa_rotation {
+    const double *frequencies;
+    const int32_t *axes;
+    const void *positions;
+    int64_t position_strides[3];
+    int positions_64, num_axes;
+    int R, interleaved;
+    const void *q_weight, *k_weight;
+    int weight_dtype;
+    float eps;
+} sa_rotation;
+
+/* q [B,Hq,S,D], k [B,H,S,D] (bf16, fp16 or float32; last dimension contiguous, other strides and addresses multiples of 16 bytes) to q_out, k_out
+ * of the same kind.  Outputs must not overlap inputs other than being exactly them. */
+int sa_rotate_heads(const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *q_out,
+                    const int64_t q_out_strides[4], void *k_out, const int64_t k_out_strides[4], const sa_rotation *rotation, int B, int Hq,
+                    int H, int S, int D, int dtype, void *stream);
+
+/*
+ * Its gradients: dq, dk (and of weights that are there dq_weight, dk_weight [D], in the weights' type, NULL: not wanted) from those of the
+ * outputs, dq_out, dk_out.  q, k: the forward's inputs, read only where there is a weight (else they may be NULL).  Sums for the weights are
+ * float32 in each workgroup and float64 over these, in a fixed order.
+ * workspace: sa_rotate_heads_bwd_workspace_bytes(B, Hq, H, S, D) bytes of device memory where a weight's gradient is wanted, 4-byte aligned.
+ */
+size_t sa_rotate_heads_bwd_workspace_bytes(int B, int Hq, int H, int S, int D);
+int sa_rotate_heads_bwd(const void *dq_out, const int64_t dq_out_strides[4], const void *dk_out, const int64_t dk_out_strides[4],
+                        const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *dq,
+                        const int64_t dq_strides[4], void *dk, const int64_t dk_strides[4], void *dq_weight, void *dk_weight,
+                        const sa_rotation *rotation, void *workspace, size_t workspace_bytes, int B, int Hq, int H, int S, int D,
+                        int dtype, void *stream);
 
 /*
  * Merge of n attention results over disjoint key ranges of the same queries (what sharding the key axis over

@@ -20,6 +20,7 @@ from .mask_utils import (MaskMetadata, MaskTerm, block_term, causal_term, comput
                          with_list_stats)
 from .paged_cache import (PagedCache, empty_paged_cache, paged_cache_append, paged_cache_compact, paged_cache_copy,
                           paged_cache_fork, paged_cache_free_pages, paged_cache_gather, sparse_attention_decode_paged)
+from .rotary import Rotary, rotary_frequencies, rotate_heads, rotate_heads_backward, rotate_heads_trainable
 from .sparse_attn_kernel import (BackwardMetadata, compute_backward_metadata, compute_backward_metadata_terms,
                                  merge_attention_parts, sparse_attention,
                                  sparse_attention_backward, sparse_attention_decode, sparse_attention_kv_split,
@@ -31,4 +32,5 @@ __all__ = ["MaskMetadata", "compute_mask_kernel", "compute_mask_slow", "select_b
            "block_term", "compute_mask_terms", "materialize_mask_terms", "compute_backward_metadata_terms", "select_tiling",
            "Tiling", "sparse_attention_tiled", "with_list_stats", "PagedCache", "empty_paged_cache", "paged_cache_append",
            "paged_cache_gather", "paged_cache_copy", "paged_cache_fork", "paged_cache_compact", "paged_cache_free_pages",
-           "sparse_attention_decode_paged"]
+           "sparse_attention_decode_paged", "Rotary", "rotary_frequencies", "rotate_heads", "rotate_heads_backward",
+           "rotate_heads_trainable"]

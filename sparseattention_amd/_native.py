@@ -10,7 +10,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsparseattn_hip.so")
 
-SA_ABI_VERSION = 19
+SA_ABI_VERSION = 20
 SA_OK = 0
 SA_ERR_INVALID_ARGUMENT = -1
 SA_ERR_UNSUPPORTED = -2
@@ -75,6 +75,9 @@ EXPORTS = (
     "sa_paged_cache_free_pages",
     "sa_decode_paged_workspace_bytes",
     "sa_sparse_attention_decode_paged",
+    "sa_rotate_heads",
+    "sa_rotate_heads_bwd_workspace_bytes",
+    "sa_rotate_heads_bwd",
 )
 
 _lib = None
@@ -89,6 +92,14 @@ class PagedCacheStruct(ctypes.Structure):
 
     _fields_ = ([(n, _vp) for n in ("k", "v", "k_scales", "v_scales")]
                 + [(n, ctypes.c_int) for n in ("num_pages", "H", "page_size", "D", "head_dim")])
+
+
+class RotationStruct(ctypes.Structure):
+    """sa_rotation of the C ABI."""
+
+    _fields_ = ([(n, _vp) for n in ("frequencies", "axes", "positions")] + [("position_strides", ctypes.c_int64 * 3)]
+                + [(n, ctypes.c_int) for n in ("positions_64", "num_axes", "R", "interleaved")]
+                + [(n, _vp) for n in ("q_weight", "k_weight")] + [("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float)])
 
 
 class SparseAttnError(RuntimeError):
@@ -234,6 +245,13 @@ def load() -> ctypes.CDLL:
         [_vp, _i64p, cache] + table + [_vp, ctypes.c_int] + [_vp, _i64p] + [_vp, _i64p] * 4 + [_vp, _i64p]
         + [ctypes.c_int] * 6 + [ctypes.c_float] + [_vp, ctypes.c_size_t] + [_vp, _i64p] + [_vp]
     )
+    rotation = ctypes.POINTER(RotationStruct)
+    lib.sa_rotate_heads.restype = ctypes.c_int
+    lib.sa_rotate_heads.argtypes = [_vp, _i64p] * 4 + [rotation] + [ctypes.c_int] * 6 + [_vp]
+    lib.sa_rotate_heads_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.sa_rotate_heads_bwd_workspace_bytes.argtypes = [ctypes.c_int] * 5
+    lib.sa_rotate_heads_bwd.restype = ctypes.c_int
+    lib.sa_rotate_heads_bwd.argtypes = [_vp, _i64p] * 6 + [_vp] * 2 + [rotation] + [_vp, ctypes.c_size_t] + [ctypes.c_int] * 6 + [_vp]
     if lib.sa_abi_version() != SA_ABI_VERSION:
         raise RuntimeError(f"libsparseattn_hip ABI {lib.sa_abi_version()} != expected {SA_ABI_VERSION}")
     _lib = lib

@@ -1,0 +1,153 @@
+// Norm and position rotation of the rows of heads: what rotate.hip and paged_rotated.hip share.
+//
+// A row x of D values:  y = x * r * w,  r = 1 / sqrt(mean(x^2) + eps)  (or y = x), then of its first R columns the pairs (a, b) at columns
+// (j, j + R/2) or, interleaved, (2j, 2j + 1) become  (a cos t - b sin t, a sin t + b cos t),  t = position * frequency of j.
+//
+// A row is held by LPR lanes, 8 columns each in two runs of 4: columns 4l .. and R/2 + 4l .. where pairs lie R/2 apart, so that a lane has both
+// of its four pairs and nothing crosses the lanes but the norm's sum; else 8l .. and 8l + 4 ...  Rows of other tokens are in the wave's other lanes.
+#pragma once
+#include "fwd_common.h"
+#include "rotation.h"
+
+namespace sa {
+namespace {
+
+// cos and sin of position * frequency.  Positions reach 2^31 and angles 2^31 radians, of which float32 would keep nothing: the product and its
+// remainder of quarter turns are 64 bits wide (off by 2^-24 of a turn at most up to 2^31), what is left of it, an eighth of a turn x at most, 32.
+// There the series of sine and cosine end with x^9 and x^10: what follows is less than 2^-28.
+__device__ __forceinline__ void turn(double position, double frequency, float &c, float &s) {
+    const double t = position * frequency * 0.15915494309189533577;  // in turns
+    const double quarters = __builtin_rint(4.0 * t);
+    const float x = (float)(t - 0.25 * quarters) * 6.283185307f, z = x * x;
+    const float sine = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
+    const float cosine = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+    const int turned = (int)(quarters - 4.0 * __builtin_floor(0.25 * quarters));  // 0 .. 3
+    const float a = turned & 1 ? sine : cosine, b = turned & 1 ? cosine : sine;
+    c = turned == 1 || turned == 2 ? -a : a;
+    s = turned & 2 ? -b : b;
+}
+
+template <int DT>
+struct Run4 {  // four values in memory
+    typedef u32x2 T;
+    static __device__ __forceinline__ void floats(T w, float (&x)[4]) {
+        if constexpr (DT == 0) {
+            x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u);
+            x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
+        } else {
+            const uint32_t lo = w.x, hi = w.y;  // (of an element of a vector the bit cast would take the first one)
+            const f16x2 a = __builtin_bit_cast(f16x2, lo), b = __builtin_bit_cast(f16x2, hi);
+            x[0] = (float)a.x, x[1] = (float)a.y, x[2] = (float)b.x, x[3] = (float)b.y;
+        }
+    }
+    static __device__ __forceinline__ T rounded(const float (&x)[4]) { return T{Elem<DT>::pack2(x[0], x[1]), Elem<DT>::pack2(x[2], x[3])}; }
+};
+template <>
+struct Run4<2> {
+    typedef f32x4 T;
+    static __device__ __forceinline__ void floats(T w, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = w[i];
+    }
+    static __device__ __forceinline__ T rounded(const float (&x)[4]) { return T{x[0], x[1], x[2], x[3]}; }
+};
+template <int DT>
+using RowElem = std::conditional_t<DT == 2, float, uint16_t>;
+
+// The columns of a lane, l of LPR of its row.
+struct Columns {
+    bool live, rot;  // whether it has any; whether they are rotated
+    int at[2];       // where its two runs of 4 begin
+};
+__device__ __forceinline__ Columns columns_of(int l, int D, int R, bool interleaved) {
+    Columns c;
+    c.live = 8 * l < D;
+    c.rot = 8 * l < R;
+    const bool apart = c.rot && !interleaved;
+    c.at[0] = apart ? 4 * l : 8 * l;
+    c.at[1] = apart ? R / 2 + 4 * l : 8 * l + 4;
+    return c;
+}
+
+// The sum over the LPR lanes of a row, in all of them.
+template <int LPR>
+__device__ __forceinline__ float row_total(float x) {
+#define SA_ROW_STEP(ctrl) x += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), ctrl, 0xf, 0xf, true))
+    SA_ROW_STEP(0xb1);   // with the neighbour
+    SA_ROW_STEP(0x4e);   // in fours
+    SA_ROW_STEP(0x141);  // in eights (mirrored)
+    if constexpr (LPR >= 16) SA_ROW_STEP(0x140);
+#undef SA_ROW_STEP
+    if constexpr (LPR == 32) {
+        const uint32_t u = __float_as_uint(x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return x;
+}
+
+// The weights of a lane's columns in float32.
+__device__ __forceinline__ void weights_of(const void *w, int dtype, const Columns &c, float (&out)[2][4]) {
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = c.at[k] + i;
+            float x = 0.f;
+            if (w != nullptr && c.live) {
+                if (dtype == 2) x = ((const float *)w)[at];
+                else if (dtype == 1) x = (float)((const _Float16 *)w)[at];
+                else x = __uint_as_float((uint32_t)((const uint16_t *)w)[at] << 16);
+            }
+            out[k][i] = x;
+        }
+}
+
+// cos and sin of the four pairs of a lane.
+struct Turns {
+    float c[4], s[4];
+};
+// y in a lane's two runs turned by t; back: by -t.
+// (INTER as a number of the kernel: chosen at run time, the runs went through scratch memory)
+template <bool INTER, bool BACK>
+__device__ __forceinline__ void rotate(float (&y)[2][4], const Turns &t) {
+    auto pair = [&](float &a, float &b, float c, float s) __attribute__((always_inline)) {
+        const float a0 = a, b0 = b;
+        if constexpr (BACK) s = -s;
+        a = a0 * c - b0 * s;
+        b = a0 * s + b0 * c;
+    };
+    if constexpr (!INTER) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) pair(y[0][i], y[1][i], t.c[i], t.s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) pair(y[i >> 1][2 * (i & 1)], y[i >> 1][2 * (i & 1) + 1], t.c[i], t.s[i]);
+    }
+}
+
+__device__ __forceinline__ double position_at(const Rotation &r, int axis, int64_t b, int64_t s) {
+    const int64_t at = axis * r.position_strides[0] + b * r.position_strides[1] + s * r.position_strides[2];
+    return r.positions_64 ? (double)((const int64_t *)r.positions)[at] : (double)((const int32_t *)r.positions)[at];
+}
+__device__ __forceinline__ int axis_of(const Rotation &r, int j) { return r.axes != nullptr ? min(max(r.axes[j], 0), r.num_axes - 1) : 0; }
+
+// Node `lane` of a tree of n <= 64 nodes given by their parents (an entry that is not below its own index and at least 0: none): a bit for itself
+// and for each of its ancestors.  The ways up double in six steps.
+__device__ __forceinline__ uint64_t tree_ancestors(const int32_t *parents, int64_t stride, int n, int lane) {
+    int up = lane < n ? parents[lane * stride] : -1;
+    if (up < 0 || up >= lane) up = -1;
+    uint64_t bits = 1ull << lane;
+#pragma unroll
+    for (int step = 0; step < 6; step++) {
+        const int from = up < 0 ? lane : up;
+        const uint64_t more = __shfl((unsigned long long)bits, from);
+        const int next = __shfl(up, from);
+        bits |= more;
+        up = up < 0 ? -1 : next;
+    }
+    return bits;
+}
+
+}  // namespace
+}  // namespace sa
