@@ -493,6 +493,49 @@ int sa_sparse_attention_decode_mask(const void *q, const int64_t q_strides[4], c
                                     float *lse, const int64_t lse_strides[3], void *stream);
 
 /*
+ * Norm and position rotation of queries and keys in front of attention, in one pass.  No counterpart in the reference, whose attention takes q and
+ * k as they are (sparseattention/sparse_attn_kernel.py:149).  A row x of D values (a multiple of 8 up to 256):
+ *   y = x / sqrt(mean(x^2) + eps) * weight    with a weight [D]; y = x without
+ *   of the first R columns (a multiple of 8 up to D) the pairs (a, b) at (j, j + R/2), or interleaved (2j, 2j + 1), j < R/2, become
+ *   (a cos t - b sin t, a sin t + b cos t),   t = positions[axes[j]][b][s] * frequencies[j]
+ * t is taken to a part of a turn in 64 bits, the rest is float32, rounded once to the output's type.
+ *   frequencies  device float64 [R/2], radians per position
+ *   axes         device int32 [R/2], which row of positions each pair turns by (one out of range is taken as the nearest), or NULL: row 0
+ *   positions    device int32, or int64 (positions_64 != 0), [num_axes, B, S], strides in elements (0 allowed)
+ *   weights      of the rows' type or float32, or NULL each
+ */
+typedef struct sa_rotation {
+    const double *frequencies;
+    const int32_t *axes;
+    const void *positions;
+    int64_t position_strides[3];
+    int positions_64, num_axes;
+    int R, interleaved;
+    const void *q_weight, *k_weight;
+    int weight_dtype;
+    float eps;
+} sa_rotation;
+
+/* q [B,Hq,S,D], k [B,H,S,D] (bf16, fp16 or float32; last dimension contiguous, other strides and addresses multiples of 16 bytes) to q_out, k_out
+ * of the same kind.  Outputs must not overlap inputs other than being exactly them. */
+int sa_rotate_heads(const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *q_out,
+                    const int64_t q_out_strides[4], void *k_out, const int64_t k_out_strides[4], const sa_rotation *rotation, int B, int Hq,
+                    int H, int S, int D, int dtype, void *stream);
+
+/*
+ * Its gradients: dq, dk (and of weights that are there dq_weight, dk_weight [D], in the weights' type, NULL: not wanted) from those of the
+ * outputs, dq_out, dk_out.  q, k: the forward's inputs, read only where there is a weight (else they may be NULL).  Sums for the weights are
+ * float32 in each workgroup and float64 over these, in a fixed order.
+ * workspace: sa_rotate_heads_bwd_workspace_bytes(B, Hq, H, S, D) bytes of device memory where a weight's gradient is wanted, 4-byte aligned.
+ */
+size_t sa_rotate_heads_bwd_workspace_bytes(int B, int Hq, int H, int S, int D);
+int sa_rotate_heads_bwd(const void *dq_out, const int64_t dq_out_strides[4], const void *dk_out, const int64_t dk_out_strides[4],
+                        const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *dq,
+                        const int64_t dq_strides[4], void *dk, const int64_t dk_strides[4], void *dq_weight, void *dk_weight,
+                        const sa_rotation *rotation, void *workspace, size_t workspace_bytes, int B, int Hq, int H, int S, int D,
+                        int dtype, void *stream);
+
+/*
  * 8-bit paged K/V cache.  No counterpart in the reference, which keeps no cache; the attention over it
  * (sa_sparse_attention_decode_paged) is the function of its forward (sparseattention/sparse_attn_kernel.py:149-185).
  *
@@ -527,6 +570,20 @@ int sa_paged_cache_append(const sa_paged_cache *cache, const void *k, const int6
                           const int64_t v_strides[4], const int32_t *page_table, const int64_t page_table_strides[2],
                           const int32_t *lens, const int32_t *counts, int B, int S, int pages_per_sequence, int dtype,
                           void *stream);
+
+/*
+ * sa_paged_cache_append with queries and keys normed and rotated on the way: of q [B,Hq,S,head_dim], k and v [B,H,S,head_dim] (strides as above; Hq
+ * any) the first counts[b] rows; q_out [B,Hq,S,head_dim] gets the queries, rounded to their type, zeros in the rows behind; the keys go to
+ * the cache, rounded once; v as it is.  Queries are written for tokens that are not stored, too.
+ *   rotation   as for sa_rotate_heads with D = head_dim; positions NULL: token s of sequence b has position max(lens[b], 0) + s
+ *   parents    device int32 [B,S], S <= 64, or NULL: the tokens are a tree (sa_sparse_attention_decode_tree) and have position lens[b] + depth,
+ *              0 for a node without a parent; positions must then be NULL
+ */
+int sa_paged_cache_append_rotated(const sa_paged_cache *cache, const void *q, const int64_t q_strides[4], void *q_out,
+                                  const int64_t q_out_strides[4], const void *k, const int64_t k_strides[4], const void *v,
+                                  const int64_t v_strides[4], const int32_t *page_table, const int64_t page_table_strides[2],
+                                  const int32_t *lens, const int32_t *counts, const int32_t *parents, const int64_t parents_strides[2],
+                                  const sa_rotation *rotation, int B, int Hq, int S, int pages_per_sequence, int dtype, void *stream);
 
 /* Reads tokens 0 .. length - 1 of every sequence into k, v [B,H,length,head_dim] (bf16 or fp16, as above); rows from lens[b] on are zero.
  * bf16 holds the values exactly; fp16 rounds those below its normal numbers and has 61440 for those beyond its 65504. */
@@ -591,49 +648,6 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
                                      const int64_t packed_strides[2], int tiles, int B, int Hq, int Sq, int window, int dtype,
                                      float sm_scale_log2, void *workspace, size_t workspace_bytes, float *lse,
                                      const int64_t lse_strides[3], void *stream);
-
-/*
- * Norm and position rotation of queries and keys in front of attention, in one pass.  No counterpart in the reference, whose attention takes q and
- * k as they are (sparseattention/sparse_attn_kernel.py:149).  A row x of D values (a multiple of 8 up to 256):
- *   y = x / sqrt(mean(x^2) + eps) * weight    with a weight [D]; y = x without
- *   of the first R columns (a multiple of 8 up to D) the pairs (a, b) at (j, j + R/2), or interleaved (2j, 2j + 1), j < R/2, become
- *   (a cos t - b sin t, a sin t + b cos t),   t = positions[axes[j]][b][s] * frequencies[j]
- * t is taken to a part of a turn in 64 bits, the rest is float32, rounded once to the output's type.
- *   frequencies  device float64 [R/2], radians per position
- *   axes         device int32 [R/2], which row of positions each pair turns by (one out of range is taken as the nearest), or NULL: row 0
- *   positions    device int32, or int64 (positions_64 != 0), [num_axes, B, S], strides in elements (0 allowed)
- *   weights      of the rows' type or float32, or NULL each
- */
-typedef struct sa_rotation {
-    const double *frequencies;
-    const int32_t *axes;
-    const void *positions;
-    int64_t position_strides[3];
-    int positions_64, num_axes;
-    int R, interleaved;
-    const void *q_weight, *k_weight;
-    int weight_dtype;
-    float eps;
-} sa_rotation;
-
-/* q [B,Hq,S,D], k [B,H,S,D] (bf16, fp16 or float32; last dimension contiguous, other strides and addresses multiples of 16 bytes) to q_out, k_out
- * of the same kind.  Outputs must not overlap inputs other than being exactly them. */
-int sa_rotate_heads(const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *q_out,
-                    const int64_t q_out_strides[4], void *k_out, const int64_t k_out_strides[4], const sa_rotation *rotation, int B, int Hq,
-                    int H, int S, int D, int dtype, void *stream);
-
-/*
- * Its gradients: dq, dk (and of weights that are there dq_weight, dk_weight [D], in the weights' type, NULL: not wanted) from those of the
- * outputs, dq_out, dk_out.  q, k: the forward's inputs, read only where there is a weight (else they may be NULL).  Sums for the weights are
- * float32 in each workgroup and float64 over these, in a fixed order.
- * workspace: sa_rotate_heads_bwd_workspace_bytes(B, Hq, H, S, D) bytes of device memory where a weight's gradient is wanted, 4-byte aligned.
- */
-size_t sa_rotate_heads_bwd_workspace_bytes(int B, int Hq, int H, int S, int D);
-int sa_rotate_heads_bwd(const void *dq_out, const int64_t dq_out_strides[4], const void *dk_out, const int64_t dk_out_strides[4],
-                        const void *q, const int64_t q_strides[4], const void *k, const int64_t k_strides[4], void *dq,
-                        const int64_t dq_strides[4], void *dk, const int64_t dk_strides[4], void *dq_weight, void *dk_weight,
-                        const sa_rotation *rotation, void *workspace, size_t workspace_bytes, int B, int Hq, int H, int S, int D,
-                        int dtype, void *stream);
 
 /*
  * Merge of n attention results over disjoint key ranges of the same queries (what sharding the key axis over

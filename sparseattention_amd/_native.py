@@ -78,6 +78,7 @@ EXPORTS = (
     "sa_rotate_heads",
     "sa_rotate_heads_bwd_workspace_bytes",
     "sa_rotate_heads_bwd",
+    "sa_paged_cache_append_rotated",
 )
 
 _lib = None
@@ -252,6 +253,10 @@ def load() -> ctypes.CDLL:
     lib.sa_rotate_heads_bwd_workspace_bytes.argtypes = [ctypes.c_int] * 5
     lib.sa_rotate_heads_bwd.restype = ctypes.c_int
     lib.sa_rotate_heads_bwd.argtypes = [_vp, _i64p] * 6 + [_vp] * 2 + [rotation] + [_vp, ctypes.c_size_t] + [ctypes.c_int] * 6 + [_vp]
+    lib.sa_paged_cache_append_rotated.restype = ctypes.c_int
+    lib.sa_paged_cache_append_rotated.argtypes = (
+        [cache] + [_vp, _i64p] * 4 + table + [_vp] + [_vp, _i64p] + [rotation] + [ctypes.c_int] * 5 + [_vp]
+    )
     if lib.sa_abi_version() != SA_ABI_VERSION:
         raise RuntimeError(f"libsparseattn_hip ABI {lib.sa_abi_version()} != expected {SA_ABI_VERSION}")
     _lib = lib

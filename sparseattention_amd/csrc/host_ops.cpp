@@ -369,6 +369,160 @@ py::object decode(const Tensor &q, const Tensor &k, const Tensor &v, const OptTe
     return as_object(decode_impl(q, k, v, mask, BK, md, num_splits, return_lse));
 }
 
+int as_int(int64_t x, const char *name) {
+    if (x < 0 || x > 0x7fffffff) value_error(std::string(name) + " out of range: " + std::to_string(x));
+    return (int)x;
+}
+
+// ---- norm and position rotation of queries and keys -----------------------------------------------------------------
+const Name kFrequencies{"frequencies"}, kAxes{"axes"}, kInterleaved{"interleaved"};
+struct Rotary {
+    Tensor frequencies;
+    OptTensor axes;
+    bool interleaved;
+};
+// (read under the interpreter's lock)
+Rotary rotary_of(py::handle o) {
+    Rotary r;
+    const py::object f = attr(o, kFrequencies), a = attr(o, kAxes);
+    if (!f || !THPVariable_Check(f.ptr())) type_error("rotary.frequencies is not a tensor");
+    if (a && !THPVariable_Check(a.ptr())) type_error("rotary.axes is not a tensor");
+    r.frequencies = THPVariable_Unpack(f.ptr());
+    if (a) r.axes = THPVariable_Unpack(a.ptr());
+    const py::object inter = attr(o, kInterleaved);
+    r.interleaved = inter && inter.cast<bool>();
+    return r;
+}
+
+struct RotationIn {
+    Rotary rotary;
+    OptTensor positions, q_weight, k_weight;  // positions as [axes, B, S]
+    sa_rotation c;
+};
+// ref: rows [B, heads, S, D] whose device, type and sizes the rest has to fit.
+RotationIn rotation_in(const Tensor &ref, const Rotary &rotary, const OptTensor &positions, const OptTensor &q_weight, const OptTensor &k_weight, double eps) {
+    const int64_t B = ref.size(0), S = ref.size(2), D = ref.size(3);
+    const auto dev = ref.device().str();
+    if (D % 8 || D > 256 || D < 8) value_error("the rotation takes head dims of multiples of 8 up to 256 (got " + std::to_string(D) + ")");
+    RotationIn r{rotary, std::nullopt, std::nullopt, std::nullopt, {}};
+    Tensor &f = r.rotary.frequencies;
+    if (f.dim() != 1 || f.scalar_type() != at::kDouble || f.device() != ref.device()) value_error("rotary.frequencies: expected float64 [R/2] on " + dev + ", got " + str(f));
+    const int64_t R = 2 * f.size(0);
+    if (R < 8 || R % 8 || R > D) value_error("rotary.frequencies: expected a multiple of 4 up to D / 2 = " + std::to_string(D / 2) + " of them, got " + str(f));
+    f = f.contiguous();
+    if (r.rotary.axes) {
+        Tensor &a = *r.rotary.axes;
+        if (a.dim() != 1 || a.size(0) != R / 2 || a.scalar_type() != at::kInt || a.device() != ref.device())
+            value_error("rotary.axes: expected int32 (" + std::to_string(R / 2) + ",) on " + dev + ", got " + str(a));
+        a = a.contiguous();
+    }
+    if (positions) {
+        const Tensor &p = *positions;
+        const int64_t want = r.rotary.axes ? 3 : 2;
+        const bool fits = r.rotary.axes ? p.dim() == 3 && p.size(0) > 0 && (p.size(1) == B || p.size(1) == 1) && p.size(2) == S
+                                        : (p.dim() == 1 && p.size(0) == S) || (p.dim() == 2 && (p.size(0) == B || p.size(0) == 1) && p.size(1) == S);
+        if (!fits || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || p.device() != ref.device())
+            value_error(std::string("positions: expected int32 or int64 ") + (want == 3 ? "[axes, " : "[") + std::to_string(B) + ", " + std::to_string(S) + "] on " + dev +
+                        ", got " + str(p));
+        r.positions = want == 3 ? p.expand({p.size(0), B, S}) : p.expand({B, S}).unsqueeze(0);
+    } else if (r.rotary.axes) {
+        value_error("rotary.axes needs positions [axes, B, S]");
+    }
+    at::ScalarType wt = at::kFloat;
+    for (auto [name, from, to] : {std::tuple{"q_weight", &q_weight, &r.q_weight}, std::tuple{"k_weight", &k_weight, &r.k_weight}}) {
+        if (!*from) continue;
+        const Tensor &w = **from;
+        if (w.dim() != 1 || w.size(0) != D || w.device() != ref.device()) value_error(std::string(name) + ": expected (" + std::to_string(D) + ",) on " + dev + ", got " + str(w));
+        if (w.scalar_type() != ref.scalar_type() && w.scalar_type() != at::kFloat)
+            type_error(std::string(name) + " must be " + c10::toString(ref.scalar_type()) + " or float32 (got " + c10::toString(w.scalar_type()) + ")");
+        *to = w.contiguous();
+        wt = w.scalar_type();
+    }
+    if (r.q_weight && r.k_weight && r.q_weight->scalar_type() != r.k_weight->scalar_type()) type_error("q_weight and k_weight must share a dtype");
+    if (!(eps >= 0.0) || !std::isfinite((float)eps)) value_error("eps must be finite and not negative (got " + std::to_string(eps) + ")");
+    r.c = {ptr<double>(f), ptr<int32_t>(r.rotary.axes), r.positions ? r.positions->data_ptr() : nullptr, {0, 0, 0}, r.positions && r.positions->scalar_type() == at::kLong,
+           r.positions ? as_int(r.positions->size(0), "axes") : 1, (int)R, r.rotary.interleaved, r.q_weight ? r.q_weight->data_ptr() : nullptr,
+           r.k_weight ? r.k_weight->data_ptr() : nullptr, dtype_code(wt), (float)eps};
+    if (r.positions)
+        for (int i = 0; i < 3; i++) r.c.position_strides[i] = r.positions->stride(i);
+    return r;
+}
+
+void check_heads(const Tensor &q, const Tensor &k, const char *what) {
+    if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(3) != k.size(3) || q.size(1) < 1 || k.size(1) < 1)
+        value_error(std::string(what) + " takes q [B,Hq,S,D] and k [B,H,S,D] (got " + str(q.sizes()) + ", " + str(k.sizes()) + ")");
+    if (dtype_code(q.scalar_type()) < 0) type_error(std::string("q and k must be bfloat16, float16 or float32 (got ") + c10::toString(q.scalar_type()) + ")");
+    if (k.scalar_type() != q.scalar_type()) type_error("q and k must share a dtype");
+    if (!q.is_cuda()) throw std::runtime_error(std::string(what) + " needs tensors on a ROCm GPU; there is no CPU path");
+    same_device(q, "k", k);
+}
+
+std::pair<Tensor, Tensor> rotate_impl(const Tensor &q, const Tensor &k, const OptTensor &positions, const Rotary &rotary, const OptTensor &qw, const OptTensor &kw,
+                                      double eps) {
+    check_heads(q, k, "rotate_heads");
+    const c10::DeviceGuard guard(q.device());
+    const RotationIn r = rotation_in(q, rotary, positions, qw, kw, eps);
+    const Tensor qc = kernel_ready(q), kc = kernel_ready(k);
+    const Tensor qo = at::empty_like(qc), ko = at::empty_like(kc);
+    if (q.size(0) > 0 && q.size(2) > 0)
+        check_rc(sa_rotate_heads(qc.data_ptr(), st(qc), kc.data_ptr(), st(kc), qo.data_ptr(), st(qo), ko.data_ptr(), st(ko), &r.c, as_int(q.size(0), "B"),
+                                 as_int(q.size(1), "Hq"), as_int(k.size(1), "H"), as_int(q.size(2), "S"), as_int(q.size(3), "D"), dtype_code(q.scalar_type()),
+                                 stream_of(q)));
+    return {qo, ko};
+}
+py::tuple rotate_heads(const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw, const OptTensor &kw, double eps) {
+    const Rotary r = rotary_of(rotary);
+    std::pair<Tensor, Tensor> out;
+    {
+        const py::gil_scoped_release unlocked;
+        const at::NoGradGuard no_grad;
+        out = rotate_impl(q, k, positions, r, qw, kw, eps);
+    }
+    return py::make_tuple(out.first, out.second);
+}
+
+struct RotateGrads {
+    Tensor dq, dk;
+    OptTensor dqw, dkw;
+};
+RotateGrads rotate_backward_impl(const Tensor &dqo, const Tensor &dko, const Tensor &q, const Tensor &k, const OptTensor &positions, const Rotary &rotary,
+                                 const OptTensor &qw, const OptTensor &kw, double eps) {
+    check_heads(q, k, "rotate_heads_backward");
+    for (auto [name, d, x] : {std::tuple{"dq", &dqo, &q}, std::tuple{"dk", &dko, &k}})
+        if (d->sizes() != x->sizes() || d->scalar_type() != x->scalar_type() || d->device() != x->device())
+            value_error(std::string(name) + ": expected " + str(*x) + ", got " + str(*d));
+    const c10::DeviceGuard guard(q.device());
+    const RotationIn r = rotation_in(q, rotary, positions, qw, kw, eps);
+    const Tensor qc = kernel_ready(q), kc = kernel_ready(k), dqc = kernel_ready(dqo), dkc = kernel_ready(dko);
+    RotateGrads g{at::empty_like(qc), at::empty_like(kc), std::nullopt, std::nullopt};
+    const bool some = q.size(0) > 0 && q.size(2) > 0;
+    if (qw) g.dqw = some ? at::empty_like(*r.q_weight) : at::zeros_like(*r.q_weight);
+    if (kw) g.dkw = some ? at::empty_like(*r.k_weight) : at::zeros_like(*r.k_weight);
+    if (!some) return g;
+    const int B = as_int(q.size(0), "B"), Hq = as_int(q.size(1), "Hq"), H = as_int(k.size(1), "H"), S = as_int(q.size(2), "S"), D = (int)q.size(3);
+    size_t bytes = 0;
+    Tensor ws;
+    if (qw || kw) {
+        bytes = sa_rotate_heads_bwd_workspace_bytes(B, Hq, H, S, D);
+        ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+    }
+    check_rc(sa_rotate_heads_bwd(dqc.data_ptr(), st(dqc), dkc.data_ptr(), st(dkc), qc.data_ptr(), st(qc), kc.data_ptr(), st(kc), g.dq.data_ptr(), st(g.dq),
+                                 g.dk.data_ptr(), st(g.dk), g.dqw ? g.dqw->data_ptr() : nullptr, g.dkw ? g.dkw->data_ptr() : nullptr, &r.c,
+                                 bytes ? ws.data_ptr() : nullptr, bytes, B, Hq, H, S, D, dtype_code(q.scalar_type()), stream_of(q)));
+    return g;
+}
+py::tuple rotate_heads_backward(const Tensor &dqo, const Tensor &dko, const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw,
+                                const OptTensor &kw, double eps) {
+    const Rotary r = rotary_of(rotary);
+    RotateGrads g;
+    {
+        const py::gil_scoped_release unlocked;
+        const at::NoGradGuard no_grad;
+        g = rotate_backward_impl(dqo, dko, q, k, positions, r, qw, kw, eps);
+    }
+    return py::make_tuple(g.dq, g.dk, g.dqw ? py::cast(*g.dqw) : py::none(), g.dkw ? py::cast(*g.dkw) : py::none());
+}
+
 // ---- the 8-bit paged K/V cache ------------------------------------------------------------------------------------
 const Name kCacheK{"k"}, kCacheV{"v"}, kCacheKScales{"k_scales"}, kCacheVScales{"v_scales"}, kHeadDim{"head_dim"};
 struct Cache {
@@ -425,11 +579,6 @@ int cache_dtype(at::ScalarType t, const char *what) {
     if (dt != SA_DTYPE_BF16 && dt != SA_DTYPE_FP16) type_error(std::string(what) + " must be bfloat16 or float16 (got " + c10::toString(t) + ")");
     return dt;
 }
-int as_int(int64_t x, const char *name) {
-    if (x < 0 || x > 0x7fffffff) value_error(std::string(name) + " out of range: " + std::to_string(x));
-    return (int)x;
-}
-
 void paged_append(py::object cache, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens_in, const OptTensor &counts_in) {
     const Cache c = cache_of(cache);
     const py::gil_scoped_release unlocked;
@@ -450,6 +599,48 @@ void paged_append(py::object cache, const Tensor &k, const Tensor &v, const Tens
     const Tensor kc = kernel_ready(pad_head_dim(k, c.cols())), vc = kernel_ready(pad_head_dim(v, c.cols()));
     check_rc(sa_paged_cache_append(&c.c, kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), ptr<int32_t>(table), st(table), ptr<int32_t>(lens),
                                    ptr<int32_t>(counts), as_int(B, "B"), as_int(S, "S"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
+}
+
+// [B, n] int32 with any strides
+const Tensor &tree_parents(const Tensor &ref, const Tensor &t, int64_t B, int64_t n) {
+    if (t.dim() != 2 || t.size(0) != B || t.size(1) != n || t.scalar_type() != at::kInt || t.device() != ref.device())
+        value_error("parents: expected int32 (" + std::to_string(B) + ", " + std::to_string(n) + ") on " + ref.device().str() + ", got " + str(t));
+    if (n > 64) value_error("trees of at most 64 nodes (got " + std::to_string(n) + ")");
+    return t;
+}
+
+Tensor paged_append_rotated(py::object cache, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens_in, py::object rotary,
+                            const OptTensor &counts_in, const OptTensor &positions, const OptTensor &parents, const OptTensor &qw, const OptTensor &kw, double eps) {
+    const Cache c = cache_of(cache);
+    const Rotary rot = rotary_of(rotary);
+    const py::gil_scoped_release unlocked;
+    const at::NoGradGuard no_grad;
+    const int64_t B = check_table(c, table);
+    const c10::DeviceGuard guard(c.k.device());
+    const Tensor lens = cache_ints(c, "lens", lens_in, B);
+    OptTensor counts;
+    if (counts_in) counts = cache_ints(c, "counts", *counts_in, B);
+    if (k.dim() != 4 || k.size(0) != B || k.size(1) != c.H() || k.size(3) != c.D || v.sizes() != k.sizes() || q.dim() != 4 || q.size(0) != B || q.size(1) < 1 ||
+        q.size(2) != k.size(2) || q.size(3) != c.D)
+        value_error("k, v must be [" + std::to_string(B) + ", " + std::to_string(c.H()) + ", S, " + std::to_string(c.D) + "] and q [" + std::to_string(B) + ", Hq, S, " +
+                    std::to_string(c.D) + "] (got " + str(k.sizes()) + ", " + str(v.sizes()) + ", " + str(q.sizes()) + ")");
+    const int dt = cache_dtype(k.scalar_type(), "q, k, v");
+    if (v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) type_error("q, k and v must share a dtype");
+    for (const Tensor *t : {&q, &k, &v})
+        if (t->device() != c.k.device()) value_error("q, k, v must be on the cache's device " + c.k.device().str() + ", got " + t->device().str());
+    const int64_t S = k.size(2);
+    if (parents) {
+        tree_parents(c.k, *parents, B, S);
+        if (positions) value_error("positions come from the parents or are given, not both");
+    }
+    const RotationIn r = rotation_in(q, rot, positions, qw, kw, eps);
+    const Tensor qc = kernel_ready(q), kc = kernel_ready(k), vc = kernel_ready(v);
+    const Tensor qo = at::empty_like(qc);
+    if (B == 0 || S == 0) return qo;
+    check_rc(sa_paged_cache_append_rotated(&c.c, qc.data_ptr(), st(qc), qo.data_ptr(), st(qo), kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), ptr<int32_t>(table), st(table),
+                                           ptr<int32_t>(lens), ptr<int32_t>(counts), ptr<int32_t>(parents), st(parents), &r.c, as_int(B, "B"), as_int(q.size(1), "Hq"),
+                                           as_int(S, "S"), as_int(table.size(1), "pages"), dt, stream_of(c.k)));
+    return qo;
 }
 
 py::tuple paged_gather(py::object cache, const Tensor &table, const Tensor &lens_in, std::optional<int64_t> length, at::ScalarType dtype) {
@@ -1100,155 +1291,6 @@ py::object trainable(const Tensor &q, const Tensor &k, const Tensor &v, const Op
     return py::cast(AttentionFunction::apply(q, k, v, mask, *r, bmd));
 }
 
-// ---- norm and position rotation of queries and keys -----------------------------------------------------------------
-const Name kFrequencies{"frequencies"}, kAxes{"axes"}, kInterleaved{"interleaved"};
-struct Rotary {
-    Tensor frequencies;
-    OptTensor axes;
-    bool interleaved;
-};
-// (read under the interpreter's lock)
-Rotary rotary_of(py::handle o) {
-    Rotary r;
-    const py::object f = attr(o, kFrequencies), a = attr(o, kAxes);
-    if (!f || !THPVariable_Check(f.ptr())) type_error("rotary.frequencies is not a tensor");
-    if (a && !THPVariable_Check(a.ptr())) type_error("rotary.axes is not a tensor");
-    r.frequencies = THPVariable_Unpack(f.ptr());
-    if (a) r.axes = THPVariable_Unpack(a.ptr());
-    const py::object inter = attr(o, kInterleaved);
-    r.interleaved = inter && inter.cast<bool>();
-    return r;
-}
-
-struct RotationIn {
-    Rotary rotary;
-    OptTensor positions, q_weight, k_weight;  // positions as [axes, B, S]
-    sa_rotation c;
-};
-// ref: rows [B, heads, S, D] whose device, type and sizes the rest has to fit.
-RotationIn rotation_in(const Tensor &ref, const Rotary &rotary, const OptTensor &positions, const OptTensor &q_weight, const OptTensor &k_weight, double eps) {
-    const int64_t B = ref.size(0), S = ref.size(2), D = ref.size(3);
-    const auto dev = ref.device().str();
-    if (D % 8 || D > 256 || D < 8) value_error("the rotation takes head dims of multiples of 8 up to 256 (got " + std::to_string(D) + ")");
-    RotationIn r{rotary, std::nullopt, std::nullopt, std::nullopt, {}};
-    Tensor &f = r.rotary.frequencies;
-    if (f.dim() != 1 || f.scalar_type() != at::kDouble || f.device() != ref.device()) value_error("rotary.frequencies: expected float64 [R/2] on " + dev + ", got " + str(f));
-    const int64_t R = 2 * f.size(0);
-    if (R < 8 || R % 8 || R > D) value_error("rotary.frequencies: expected a multiple of 4 up to D / 2 = " + std::to_string(D / 2) + " of them, got " + str(f));
-    f = f.contiguous();
-    if (r.rotary.axes) {
-        Tensor &a = *r.rotary.axes;
-        if (a.dim() != 1 || a.size(0) != R / 2 || a.scalar_type() != at::kInt || a.device() != ref.device())
-            value_error("rotary.axes: expected int32 (" + std::to_string(R / 2) + ",) on " + dev + ", got " + str(a));
-        a = a.contiguous();
-    }
-    if (positions) {
-        const Tensor &p = *positions;
-        const int64_t want = r.rotary.axes ? 3 : 2;
-        const bool fits = r.rotary.axes ? p.dim() == 3 && p.size(0) > 0 && (p.size(1) == B || p.size(1) == 1) && p.size(2) == S
-                                        : (p.dim() == 1 && p.size(0) == S) || (p.dim() == 2 && (p.size(0) == B || p.size(0) == 1) && p.size(1) == S);
-        if (!fits || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || p.device() != ref.device())
-            value_error(std::string("positions: expected int32 or int64 ") + (want == 3 ? "[axes, " : "[") + std::to_string(B) + ", " + std::to_string(S) + "] on " + dev +
-                        ", got " + str(p));
-        r.positions = want == 3 ? p.expand({p.size(0), B, S}) : p.expand({B, S}).unsqueeze(0);
-    } else if (r.rotary.axes) {
-        value_error("rotary.axes needs positions [axes, B, S]");
-    }
-    at::ScalarType wt = at::kFloat;
-    for (auto [name, from, to] : {std::tuple{"q_weight", &q_weight, &r.q_weight}, std::tuple{"k_weight", &k_weight, &r.k_weight}}) {
-        if (!*from) continue;
-        const Tensor &w = **from;
-        if (w.dim() != 1 || w.size(0) != D || w.device() != ref.device()) value_error(std::string(name) + ": expected (" + std::to_string(D) + ",) on " + dev + ", got " + str(w));
-        if (w.scalar_type() != ref.scalar_type() && w.scalar_type() != at::kFloat)
-            type_error(std::string(name) + " must be " + c10::toString(ref.scalar_type()) + " or float32 (got " + c10::toString(w.scalar_type()) + ")");
-        *to = w.contiguous();
-        wt = w.scalar_type();
-    }
-    if (r.q_weight && r.k_weight && r.q_weight->scalar_type() != r.k_weight->scalar_type()) type_error("q_weight and k_weight must share a dtype");
-    if (!(eps >= 0.0) || !std::isfinite((float)eps)) value_error("eps must be finite and not negative (got " + std::to_string(eps) + ")");
-    r.c = {ptr<double>(f), ptr<int32_t>(r.rotary.axes), r.positions ? r.positions->data_ptr() : nullptr, {0, 0, 0}, r.positions && r.positions->scalar_type() == at::kLong,
-           r.positions ? as_int(r.positions->size(0), "axes") : 1, (int)R, r.rotary.interleaved, r.q_weight ? r.q_weight->data_ptr() : nullptr,
-           r.k_weight ? r.k_weight->data_ptr() : nullptr, dtype_code(wt), (float)eps};
-    if (r.positions)
-        for (int i = 0; i < 3; i++) r.c.position_strides[i] = r.positions->stride(i);
-    return r;
-}
-
-void check_heads(const Tensor &q, const Tensor &k, const char *what) {
-    if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(3) != k.size(3) || q.size(1) < 1 || k.size(1) < 1)
-        value_error(std::string(what) + " takes q [B,Hq,S,D] and k [B,H,S,D] (got " + str(q.sizes()) + ", " + str(k.sizes()) + ")");
-    if (dtype_code(q.scalar_type()) < 0) type_error(std::string("q and k must be bfloat16, float16 or float32 (got ") + c10::toString(q.scalar_type()) + ")");
-    if (k.scalar_type() != q.scalar_type()) type_error("q and k must share a dtype");
-    if (!q.is_cuda()) throw std::runtime_error(std::string(what) + " needs tensors on a ROCm GPU; there is no CPU path");
-    same_device(q, "k", k);
-}
-
-std::pair<Tensor, Tensor> rotate_impl(const Tensor &q, const Tensor &k, const OptTensor &positions, const Rotary &rotary, const OptTensor &qw, const OptTensor &kw,
-                                      double eps) {
-    check_heads(q, k, "rotate_heads");
-    const c10::DeviceGuard guard(q.device());
-    const RotationIn r = rotation_in(q, rotary, positions, qw, kw, eps);
-    const Tensor qc = kernel_ready(q), kc = kernel_ready(k);
-    const Tensor qo = at::empty_like(qc), ko = at::empty_like(kc);
-    if (q.size(0) > 0 && q.size(2) > 0)
-        check_rc(sa_rotate_heads(qc.data_ptr(), st(qc), kc.data_ptr(), st(kc), qo.data_ptr(), st(qo), ko.data_ptr(), st(ko), &r.c, as_int(q.size(0), "B"),
-                                 as_int(q.size(1), "Hq"), as_int(k.size(1), "H"), as_int(q.size(2), "S"), as_int(q.size(3), "D"), dtype_code(q.scalar_type()),
-                                 stream_of(q)));
-    return {qo, ko};
-}
-py::tuple rotate_heads(const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw, const OptTensor &kw, double eps) {
-    const Rotary r = rotary_of(rotary);
-    std::pair<Tensor, Tensor> out;
-    {
-        const py::gil_scoped_release unlocked;
-        const at::NoGradGuard no_grad;
-        out = rotate_impl(q, k, positions, r, qw, kw, eps);
-    }
-    return py::make_tuple(out.first, out.second);
-}
-
-struct RotateGrads {
-    Tensor dq, dk;
-    OptTensor dqw, dkw;
-};
-RotateGrads rotate_backward_impl(const Tensor &dqo, const Tensor &dko, const Tensor &q, const Tensor &k, const OptTensor &positions, const Rotary &rotary,
-                                 const OptTensor &qw, const OptTensor &kw, double eps) {
-    check_heads(q, k, "rotate_heads_backward");
-    for (auto [name, d, x] : {std::tuple{"dq", &dqo, &q}, std::tuple{"dk", &dko, &k}})
-        if (d->sizes() != x->sizes() || d->scalar_type() != x->scalar_type() || d->device() != x->device())
-            value_error(std::string(name) + ": expected " + str(*x) + ", got " + str(*d));
-    const c10::DeviceGuard guard(q.device());
-    const RotationIn r = rotation_in(q, rotary, positions, qw, kw, eps);
-    const Tensor qc = kernel_ready(q), kc = kernel_ready(k), dqc = kernel_ready(dqo), dkc = kernel_ready(dko);
-    RotateGrads g{at::empty_like(qc), at::empty_like(kc), std::nullopt, std::nullopt};
-    const bool some = q.size(0) > 0 && q.size(2) > 0;
-    if (qw) g.dqw = some ? at::empty_like(*r.q_weight) : at::zeros_like(*r.q_weight);
-    if (kw) g.dkw = some ? at::empty_like(*r.k_weight) : at::zeros_like(*r.k_weight);
-    if (!some) return g;
-    const int B = as_int(q.size(0), "B"), Hq = as_int(q.size(1), "Hq"), H = as_int(k.size(1), "H"), S = as_int(q.size(2), "S"), D = (int)q.size(3);
-    size_t bytes = 0;
-    Tensor ws;
-    if (qw || kw) {
-        bytes = sa_rotate_heads_bwd_workspace_bytes(B, Hq, H, S, D);
-        ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
-    }
-    check_rc(sa_rotate_heads_bwd(dqc.data_ptr(), st(dqc), dkc.data_ptr(), st(dkc), qc.data_ptr(), st(qc), kc.data_ptr(), st(kc), g.dq.data_ptr(), st(g.dq),
-                                 g.dk.data_ptr(), st(g.dk), g.dqw ? g.dqw->data_ptr() : nullptr, g.dkw ? g.dkw->data_ptr() : nullptr, &r.c,
-                                 bytes ? ws.data_ptr() : nullptr, bytes, B, Hq, H, S, D, dtype_code(q.scalar_type()), stream_of(q)));
-    return g;
-}
-py::tuple rotate_heads_backward(const Tensor &dqo, const Tensor &dko, const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw,
-                                const OptTensor &kw, double eps) {
-    const Rotary r = rotary_of(rotary);
-    RotateGrads g;
-    {
-        const py::gil_scoped_release unlocked;
-        const at::NoGradGuard no_grad;
-        g = rotate_backward_impl(dqo, dko, q, k, positions, r, qw, kw, eps);
-    }
-    return py::make_tuple(g.dq, g.dk, g.dqw ? py::cast(*g.dqw) : py::none(), g.dkw ? py::cast(*g.dkw) : py::none());
-}
-
 struct RotateFunction : public torch::autograd::Function<RotateFunction> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const OptTensor &qw, const OptTensor &kw,
                                                   const Tensor &positions, const Tensor &frequencies, const OptTensor &axes, bool interleaved, double eps) {
@@ -1288,6 +1330,7 @@ PYBIND11_MODULE(_host, m) {
     m.def("decode", &decode);
     m.def("decode_paged", &decode_paged);
     m.def("paged_append", &paged_append);
+    m.def("paged_append_rotated", &paged_append_rotated);
     m.def("paged_gather", &paged_gather);
     m.def("paged_copy", &paged_copy);
     m.def("paged_fork", &paged_fork);

@@ -11,6 +11,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "rotation.h"
+
 namespace sa {
 
 constexpr int kScaleExpMin = -96, kScaleExpMax = 119;  // 448 * 2^120 would be beyond bf16 and float32
@@ -67,6 +69,22 @@ struct PagedAppendParams {
     int S, blocks;          // blocks: the most that S tokens touch
 };
 hipError_t launch_paged_append(const PagedAppendParams &p, int dtype, hipStream_t stream);
+
+struct PagedRotatedParams {
+    PagedPool c;
+    PageTable t;
+    Rotation r;  // positions null: those of the tokens in their sequence, of trees the depth in it
+    const uint16_t *q, *k, *v;
+    uint16_t *qo;
+    int64_t qs[3], ks[3], vs[3], qos[3];  // b, h, token strides in elements (d stride 1)
+    const int32_t *counts;                // or null: S of every sequence
+    const int32_t *parents;               // or null: a chain
+    int64_t parents_stride[2];
+    int Hq, S, blocks;
+    int splits, steps;  // workgroups that share a block; steps of an item of queries
+};
+int paged_rotated_splits(int B, int blocks, int H, int Hq, int S);
+hipError_t launch_paged_rotated(const PagedRotatedParams &p, int dtype, hipStream_t stream);
 
 struct PagedGatherParams {
     PagedPool c;

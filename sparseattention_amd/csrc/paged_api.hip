@@ -5,6 +5,7 @@
 #include "api_common.h"
 #include "paged.h"
 #include "paged_pieces.h"
+#include "rotation_api.h"
 #include "sparseattn.h"
 
 namespace {
@@ -61,6 +62,7 @@ int grid_fits(const char *who, int64_t workgroups) {
 }
 
 constexpr int kMostRows = 1 << 20;
+constexpr int kTreeNodes = 64;
 
 // Compute units of the current device.
 int compute_units() {
@@ -100,6 +102,46 @@ int sa_paged_cache_append(const sa_paged_cache *cache, const void *k, const int6
     p.blocks = (S + 62) / 32;  // the first one may have room for one token only
     SA_TRY(grid_fits(who, (int64_t)2 * p.c.H * p.blocks * B));
     return launched(who, sa::launch_paged_append(p, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int sa_paged_cache_append_rotated(const sa_paged_cache *cache, const void *q, const int64_t q_strides[4], void *q_out, const int64_t q_out_strides[4],
+                                  const void *k, const int64_t k_strides[4], const void *v, const int64_t v_strides[4], const int32_t *page_table,
+                                  const int64_t page_table_strides[2], const int32_t *lens, const int32_t *counts, const int32_t *parents,
+                                  const int64_t parents_strides[2], const sa_rotation *rotation, int B, int Hq, int S, int pages_per_sequence, int dtype,
+                                  void *stream) {
+    const char *who = "sa_paged_cache_append_rotated";
+    sa::PagedRotatedParams p{};
+    SA_TRY(pool_of(who, cache, p.c));
+    SA_TRY(table_of(who, page_table, page_table_strides, lens, B, pages_per_sequence, cache->page_size, p.t));
+    SA_TRY(rows_of(who, "q", q, q_strides));
+    SA_TRY(rows_of(who, "q_out", q_out, q_out_strides));
+    SA_TRY(rows_of(who, "k", k, k_strides));
+    SA_TRY(rows_of(who, "v", v, v_strides));
+    SA_TRY(half_dtype(who, dtype));
+    SA_TRY(sa::rotation_of(who, rotation, p.c.cols, dtype, true, p.r));
+    if (S <= 0 || S > (1 << 30)) return fail(SA_ERR_INVALID_ARGUMENT, "%s: S must be 1 .. 2^30 (got %d)", who, S);
+    if (Hq <= 0 || Hq > kMostRows) return fail(SA_ERR_INVALID_ARGUMENT, "%s: Hq must be 1 .. %d (got %d)", who, kMostRows, Hq);
+    if (p.r.axes && !p.r.positions) return fail(SA_ERR_INVALID_ARGUMENT, "%s: axes need positions", who);
+    if (parents) {
+        if (!parents_strides) return fail(SA_ERR_INVALID_ARGUMENT, "%s: null strides of the parents", who);
+        if (p.r.positions) return fail(SA_ERR_INVALID_ARGUMENT, "%s: positions come from the parents or are given, not both", who);
+        if (S > kTreeNodes) return fail(SA_ERR_UNSUPPORTED, "%s: trees of at most %d nodes (got %d)", who, kTreeNodes, S);
+        p.parents = parents;
+        for (int i = 0; i < 2; i++) p.parents_stride[i] = parents_strides[i];
+    }
+    p.q = static_cast<const uint16_t *>(q);
+    p.k = static_cast<const uint16_t *>(k);
+    p.v = static_cast<const uint16_t *>(v);
+    p.qo = static_cast<uint16_t *>(q_out);
+    for (int i = 0; i < 3; i++) p.qs[i] = q_strides[i], p.ks[i] = k_strides[i], p.vs[i] = v_strides[i], p.qos[i] = q_out_strides[i];
+    p.counts = counts;
+    p.Hq = Hq;
+    p.S = S;
+    p.blocks = (S + 62) / 32;
+    p.steps = S == 1 ? 1 : 8;
+    p.splits = sa::paged_rotated_splits(B, p.blocks, p.c.H, Hq, S);
+    SA_TRY(grid_fits(who, (int64_t)p.splits * p.blocks * B));
+    return launched(who, sa::launch_paged_rotated(p, dtype, static_cast<hipStream_t>(stream)));
 }
 
 int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_strides[4], void *v, const int64_t v_strides[4],

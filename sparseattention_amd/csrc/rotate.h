@@ -16,11 +16,13 @@ namespace {
 // remainder of quarter turns are 64 bits wide (off by 2^-24 of a turn at most up to 2^31), what is left of it, an eighth of a turn x at most, 32.
 // There the series of sine and cosine end with x^9 and x^10: what follows is less than 2^-28.
 __device__ __forceinline__ void turn(double position, double frequency, float &c, float &s) {
+#pragma clang fp contract(off)
     const double t = position * frequency * 0.15915494309189533577;  // in turns
     const double quarters = __builtin_rint(4.0 * t);
     const float x = (float)(t - 0.25 * quarters) * 6.283185307f, z = x * x;
-    const float sine = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
-    const float cosine = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+    auto fma = [](float a, float b, float c) { return __builtin_fmaf(a, b, c); };
+    const float sine = fma(x * z, fma(z, fma(z, fma(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+    const float cosine = fma(z, fma(z, fma(z, fma(z, fma(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
     const int turned = (int)(quarters - 4.0 * __builtin_floor(0.25 * quarters));  // 0 .. 3
     const float a = turned & 1 ? sine : cosine, b = turned & 1 ? cosine : sine;
     c = turned == 1 || turned == 2 ? -a : a;
@@ -103,6 +105,22 @@ __device__ __forceinline__ void weights_of(const void *w, int dtype, const Colum
         }
 }
 
+// A row over its root mean square times its weights.  Here and below the fused products are written out, so that kernels that share these functions give
+// the same to the bit.
+template <int LPR>
+__device__ __forceinline__ float row_factor(const float (&x)[2][4], float share, float eps) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum = __builtin_fmaf(x[i >> 2][i & 3], x[i >> 2][i & 3], sum);
+    return __builtin_amdgcn_rsqf(__builtin_fmaf(row_total<LPR>(sum), share, eps));
+}
+template <int LPR>
+__device__ __forceinline__ void norm_row(float (&x)[2][4], const float (&w)[2][4], float share, float eps) {
+    const float n = row_factor<LPR>(x, share, eps);
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = x[i >> 2][i & 3] * n * w[i >> 2][i & 3];
+}
+
 // cos and sin of the four pairs of a lane.
 struct Turns {
     float c[4], s[4];
@@ -114,8 +132,8 @@ __device__ __forceinline__ void rotate(float (&y)[2][4], const Turns &t) {
     auto pair = [&](float &a, float &b, float c, float s) __attribute__((always_inline)) {
         const float a0 = a, b0 = b;
         if constexpr (BACK) s = -s;
-        a = a0 * c - b0 * s;
-        b = a0 * s + b0 * c;
+        a = __builtin_fmaf(a0, c, -(b0 * s));
+        b = __builtin_fmaf(a0, s, b0 * c);
     };
     if constexpr (!INTER) {
 #pragma unroll

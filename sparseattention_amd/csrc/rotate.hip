@@ -69,14 +69,7 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_kernel(const RotateP
                 float f[2][4];
                 X::floats(in[u][0], f[0]);
                 X::floats(in[u][1], f[1]);
-                if (weight != nullptr) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum += f[i >> 2][i & 3] * f[i >> 2][i & 3];
-                    const float n = __builtin_amdgcn_rsqf(row_total<LPR>(sum) * share + p.r.eps);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) f[i >> 2][i & 3] = f[i >> 2][i & 3] * n * ww[i >> 2][i & 3];
-                }
+                if (weight != nullptr) norm_row<LPR>(f, ww, share, p.r.eps);
                 if (w.c.rot) rotate<INTER, false>(f, w.t);
                 if (w.live) {
                     *(typename X::T *)(y + (h + u) * r.ys[1] + w.c.at[0]) = X::rounded(f[0]);
@@ -134,14 +127,10 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_backward_kernel(cons
                         float f[2][4];
                         X::floats(in[u][0], f[0]);
                         X::floats(in[u][1], f[1]);
-                        float square = 0.f, along = 0.f;
+                        float along = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float xi = f[i >> 2][i & 3];
-                            square += xi * xi;
-                            along += xi * (ww[i >> 2][i & 3] * g[i >> 2][i & 3]);
-                        }
-                        const float n = __builtin_amdgcn_rsqf(row_total<LPR>(square) * share + p.r.eps);
+                        for (int i = 0; i < 8; i++) along += f[i >> 2][i & 3] * (ww[i >> 2][i & 3] * g[i >> 2][i & 3]);
+                        const float n = row_factor<LPR>(f, share, p.r.eps);
                         const float m = row_total<LPR>(along) * share * n * n;
 #pragma unroll
                         for (int i = 0; i < 8; i++) {

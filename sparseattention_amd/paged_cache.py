@@ -26,6 +26,7 @@ import torch
 
 from . import _native
 from .mask_utils import MaskMetadata
+from .rotary import Rotary
 
 PAGE_SIZES = (32, 64, 128, 256)
 MOST_PAGES = 1 << 20
@@ -91,6 +92,19 @@ def paged_cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page
     what a block held before its first token of the sequence does not count.  Sequences of one call, or two entries of one, must not
     store into the same page (fork it first: :func:`paged_cache_fork`)."""
     _native.host().paged_append(cache, k, v, page_table, lens, counts)
+
+
+def paged_cache_append_rotated(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                               rotary: Rotary, counts: Optional[torch.Tensor] = None, *, positions: Optional[torch.Tensor] = None,
+                               parents: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                               eps: float = 1e-6) -> torch.Tensor:
+    """:func:`paged_cache_append` of keys that :func:`sparseattention_amd.rotate_heads` would give, and the queries that it would give: ``q``
+    [B,Hq,S,D], ``k``, ``v`` [B,H,S,D], D a multiple of 8.  Keys are rounded once, to what the cache holds; the queries that come back, for all rows up to
+    ``counts[b]`` whether their tokens were stored or not, to their type, with zeros in the rows behind.
+
+    Token ``s`` of sequence ``b`` has position ``lens[b] + s``; with ``parents`` (int32 [B,S], S <= 64: the tokens are a tree of drafts,
+    :func:`sparseattention_amd.sparse_attention_decode_tree`) ``lens[b]`` and its depth in the tree; or what ``positions`` says, as for rotate_heads."""
+    return _native.host().paged_append_rotated(cache, q, k, v, page_table, lens, rotary, counts, positions, parents, q_weight, k_weight, eps)
 
 
 def paged_cache_gather(cache: PagedCache, page_table: torch.Tensor, lens: torch.Tensor, length: Optional[int] = None,
