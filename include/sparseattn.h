@@ -650,6 +650,20 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
                                      const int64_t lse_strides[3], void *stream);
 
 /*
+ * The same for a tree of drafted tokens: the sequence's last n tokens (counts[b] of them, the rows behind are padding), 1 <= n <= 64, are a tree
+ * given by parents (device int32 [B,n], strides in elements): parents[b][i] in [0, i) is node i's parent, any other value says that it has none.
+ * Row i attends to all lens[b] - counts[b] keys in front of the tree, to itself and to its ancestors; with window > 0 to those of them less than
+ * `window` positions back, a node's position being lens[b] - counts[b] and its depth.  (A chain is parents[b][i] = i - 1.)
+ * Everything else as above, with sa_decode_tree_workspace_bytes.
+ */
+size_t sa_decode_tree_workspace_bytes(int B, int Hq, int H, int n, int D, int pages_per_sequence, int page_size);
+int sa_sparse_attention_decode_tree(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
+                                    const int64_t page_table_strides[2], const int32_t *lens, const int32_t *parents,
+                                    const int64_t parents_strides[2], const int32_t *counts, int pages_per_sequence, void *o,
+                                    const int64_t o_strides[4], int B, int Hq, int n, int window, int dtype, float sm_scale_log2,
+                                    void *workspace, size_t workspace_bytes, float *lse, const int64_t lse_strides[3], void *stream);
+
+/*
  * Merge of n attention results over disjoint key ranges of the same queries (what sharding the key axis over
  * devices, or over launches, ends with; the reference has no counterpart - it never hands out the row statistics):
  *   o = sum_i exp(lse_i - lse) o_i,   lse = log sum_i exp(lse_i)     (rows with every lse_i = -inf give 0 and -inf)

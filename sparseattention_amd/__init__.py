@@ -19,7 +19,7 @@ from .mask_utils import (MaskMetadata, MaskTerm, block_term, causal_term, comput
                          compute_mask_terms, materialize_mask_terms, select_block_sizes, select_tiling, Tiling,
                          with_list_stats)
 from .paged_cache import (PagedCache, empty_paged_cache, paged_cache_append, paged_cache_append_rotated, paged_cache_compact, paged_cache_copy,
-                          paged_cache_fork, paged_cache_free_pages, paged_cache_gather, sparse_attention_decode_paged)
+                          paged_cache_fork, paged_cache_free_pages, paged_cache_gather, sparse_attention_decode_paged, sparse_attention_decode_tree)
 from .rotary import Rotary, rotary_frequencies, rotate_heads, rotate_heads_backward, rotate_heads_trainable
 from .sparse_attn_kernel import (BackwardMetadata, compute_backward_metadata, compute_backward_metadata_terms,
                                  merge_attention_parts, sparse_attention,
@@ -33,4 +33,5 @@ __all__ = ["MaskMetadata", "compute_mask_kernel", "compute_mask_slow", "select_b
            "Tiling", "sparse_attention_tiled", "with_list_stats", "PagedCache", "empty_paged_cache", "paged_cache_append",
            "paged_cache_gather", "paged_cache_copy", "paged_cache_fork", "paged_cache_compact", "paged_cache_free_pages",
            "sparse_attention_decode_paged", "Rotary", "rotary_frequencies", "rotate_heads", "rotate_heads_backward",
-           "rotate_heads_trainable", "paged_cache_append_rotated"]
+           "rotate_heads_trainable", "paged_cache_append_rotated",
+           "sparse_attention_decode_tree"]

@@ -79,6 +79,8 @@ EXPORTS = (
     "sa_rotate_heads_bwd_workspace_bytes",
     "sa_rotate_heads_bwd",
     "sa_paged_cache_append_rotated",
+    "sa_decode_tree_workspace_bytes",
+    "sa_sparse_attention_decode_tree",
 )
 
 _lib = None
@@ -256,6 +258,13 @@ def load() -> ctypes.CDLL:
     lib.sa_paged_cache_append_rotated.restype = ctypes.c_int
     lib.sa_paged_cache_append_rotated.argtypes = (
         [cache] + [_vp, _i64p] * 4 + table + [_vp] + [_vp, _i64p] + [rotation] + [ctypes.c_int] * 5 + [_vp]
+    )
+    lib.sa_decode_tree_workspace_bytes.restype = ctypes.c_size_t
+    lib.sa_decode_tree_workspace_bytes.argtypes = [ctypes.c_int] * 7
+    lib.sa_sparse_attention_decode_tree.restype = ctypes.c_int
+    lib.sa_sparse_attention_decode_tree.argtypes = (
+        [_vp, _i64p, cache] + table + [_vp, _i64p] + [_vp, ctypes.c_int] + [_vp, _i64p] + [ctypes.c_int] * 5 + [ctypes.c_float]
+        + [_vp, ctypes.c_size_t] + [_vp, _i64p] + [_vp]
     )
     if lib.sa_abi_version() != SA_ABI_VERSION:
         raise RuntimeError(f"libsparseattn_hip ABI {lib.sa_abi_version()} != expected {SA_ABI_VERSION}")

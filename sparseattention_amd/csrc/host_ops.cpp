@@ -804,6 +804,42 @@ py::object decode_paged(const Tensor &q, py::object cache, const Tensor &table, 
     return as_object(r);
 }
 
+py::object decode_tree(const Tensor &q, py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &parents, const OptTensor &counts_in,
+                       std::optional<int64_t> window, bool return_lse) {
+    const Cache c = cache_of(cache);
+    Out r;
+    {
+        const py::gil_scoped_release unlocked;
+        const at::NoGradGuard no_grad;
+        const int64_t B = check_table(c, table), P = c.page(), H = c.H();
+        if (q.dim() != 4 || q.size(0) != B || q.size(3) != c.D || q.size(1) % H || q.size(1) == 0)
+            value_error("q must be [" + std::to_string(B) + ", a multiple of " + std::to_string(H) + ", n, " + std::to_string(c.D) + "] (got " + str(q.sizes()) + ")");
+        if (q.device() != c.k.device()) value_error("q is on " + q.device().str() + ", expected " + c.k.device().str() + " (the cache's device)");
+        const int dt = cache_dtype(q.scalar_type(), "q");
+        const int64_t Hq = q.size(1), n = q.size(2);
+        if (window && *window < 1) value_error("window must be positive (got " + std::to_string(*window) + ")");
+        const c10::DeviceGuard guard(q.device());
+        const Tensor lens = cache_ints(c, "lens", lens_in, B);
+        OptTensor counts;
+        if (counts_in) counts = cache_ints(c, "counts", *counts_in, B);
+        tree_parents(c.k, parents, B, n);
+        const Tensor qc = kernel_ready(pad_head_dim(q, c.cols()));
+        const Tensor o = at::empty_like(qc);
+        if (return_lse) r.lse = at::empty({B, Hq, n}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
+        if (B > 0 && n > 0) {
+            const int Bi = as_int(B, "B"), pages = as_int(table.size(1), "pages"), w = window ? (int)std::min<int64_t>(*window, 1 << 30) : 0;
+            const size_t bytes = sa_decode_tree_workspace_bytes(Bi, as_int(Hq, "Hq"), (int)H, (int)n, c.c.D, pages, (int)P);
+            Tensor ws;
+            if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+            check_rc(sa_sparse_attention_decode_tree(qc.data_ptr(), st(qc), &c.c, ptr<int32_t>(table), st(table), ptr<int32_t>(lens), ptr<int32_t>(parents), st(parents),
+                                                     ptr<int32_t>(counts), pages, o.data_ptr(), st(o), Bi, (int)Hq, (int)n, w, dt, (float)scale_log2(c.D),
+                                                     bytes ? ws.data_ptr() : nullptr, bytes, ptr<float>(r.lse), st(r.lse), stream_of(q)));
+        }
+        r.o = cut_head_dim(o, c.D);
+    }
+    return as_object(r);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------
 // Whether the kernels tile by the caller's own sizes (kernel_tiles of sparse_attn_kernel.py returns them unchanged).
 bool tiles_as_asked(int64_t Sq, int64_t Sk, int64_t D, int64_t BQ, int64_t BK, bool f32) {
@@ -1329,6 +1365,7 @@ PYBIND11_MODULE(_host, m) {
     m.def("forward_tiled", &forward_tiled);
     m.def("decode", &decode);
     m.def("decode_paged", &decode_paged);
+    m.def("decode_tree", &decode_tree);
     m.def("paged_append", &paged_append);
     m.def("paged_append_rotated", &paged_append_rotated);
     m.def("paged_gather", &paged_gather);

@@ -148,6 +148,9 @@ struct PagedDecodeParams {
     const int32_t *counts;  // valid query rows of each sequence, or null: Sq
     int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT tiles of 16 (all of them) or 32
     int window;             // or 0
+    // the rows are a tree (tree.h): each one's parent, or null
+    const int32_t *parents;
+    int64_t parents_stride[2];
     // tile lists, tile = page, all null: every key that causality and window leave
     const int32_t *full_ids, *full_lens, *part_ids, *part_lens;
     int64_t fis[3], fls[2], pis[3], pls[2];  // b, h (and entry) strides

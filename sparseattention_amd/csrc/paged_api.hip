@@ -246,14 +246,67 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
 
 static size_t units_bytes(int64_t units) { return (sizeof(sa::PagedUnits) + (size_t)units * 4 + 15) / 16 * 16; }
 
-size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
-    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > 32 || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
+static size_t decode_workspace_bytes(int most_rows, int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
+    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > most_rows || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
         (int64_t)Hq / H * Sq > kMostRows)
         return 0;
     const int R = Hq / H * Sq;
     const int64_t planes = (int64_t)B * H * ((R + 31) / 32);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units());
     return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8 + units_bytes((int64_t)B * H);
+}
+
+size_t sa_decode_paged_workspace_bytes(int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
+    return decode_workspace_bytes(32, B, Hq, H, Sq, D, pages_per_sequence, page_size);
+}
+size_t sa_decode_tree_workspace_bytes(int B, int Hq, int H, int n, int D, int pages_per_sequence, int page_size) {
+    return decode_workspace_bytes(kTreeNodes, B, Hq, H, n, D, pages_per_sequence, page_size);
+}
+
+// What the two attentions have in common: p has the cache, the table and who attends.
+static int decode(const char *who, sa::PagedDecodeParams &p, int most_rows, const void *q, const int64_t q_strides[4], void *o, const int64_t o_strides[4],
+                  const int32_t *counts, int B, int Hq, int Sq, int window, int dtype, float sm_scale_log2, void *workspace, size_t workspace_bytes, float *lse,
+                  const int64_t lse_strides[3], void *stream) {
+    SA_TRY(rows_of(who, "q", q, q_strides));
+    SA_TRY(rows_of(who, "o", o, o_strides));
+    SA_TRY(half_dtype(who, dtype));
+    if (Sq <= 0 || Sq > most_rows) return fail(SA_ERR_UNSUPPORTED, "%s: 1 .. %d query rows (got %d)", who, most_rows, Sq);
+    if (Hq <= 0 || Hq % p.c.H) return fail(SA_ERR_INVALID_ARGUMENT, "%s: Hq (%d) must be a multiple of the cache's H (%d)", who, Hq, p.c.H);
+    if (!(sm_scale_log2 > 0.f) || sm_scale_log2 > 3e38f) return fail(SA_ERR_INVALID_ARGUMENT, "%s: softmax scale must be positive and finite", who);
+    if (window < 0) return fail(SA_ERR_INVALID_ARGUMENT, "%s: window must not be negative (got %d)", who, window);
+    if (lse && !lse_strides) return fail(SA_ERR_INVALID_ARGUMENT, "%s: null lse strides", who);
+    p.q = static_cast<const uint16_t *>(q);
+    p.o = static_cast<uint16_t *>(o);
+    p.lse = lse;
+    for (int i = 0; i < 3; i++) {
+        p.qs[i] = q_strides[i];
+        p.os[i] = o_strides[i];
+        p.lses[i] = lse ? lse_strides[i] : 0;
+    }
+    p.counts = counts;
+    p.G = Hq / p.c.H;
+    p.Sq = Sq;
+    if ((int64_t)p.G * Sq > kMostRows) return fail(SA_ERR_UNSUPPORTED, "%s: more than %d rows per K/V head", who, kMostRows);
+    p.R = p.G * Sq;
+    p.RT = (p.R + 31) / 32;
+    p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
+    p.scale = sm_scale_log2;
+    const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)p.t.width << p.c.lper;
+    if (planes > (1 << 24) || planes * chunks > (1 << 30))
+        return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
+    const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
+                 need = units_at + units_bytes((int64_t)B * p.c.H);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
+    p.groups = plan.groups;
+    p.parts = plan.parts;
+    p.part_rows = plan.part_rows;
+    p.ws = static_cast<float *>(workspace);
+    p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + parts_bytes);
+    p.tag = sa::next_launch_tag() | 1;
+    if ((p.full_ids != nullptr ? (int64_t)B * p.c.H : B) > sa::kPagedFewUnits(p.full_ids != nullptr)) p.units = reinterpret_cast<sa::PagedUnits *>(static_cast<uint8_t *>(workspace) + units_at);
+    return launched(who, sa::launch_paged_decode(p, dtype, static_cast<hipStream_t>(stream)));
 }
 
 int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
@@ -267,14 +320,6 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
     sa::PagedDecodeParams p{};
     SA_TRY(pool_of(who, cache, p.c));
     SA_TRY(table_of(who, page_table, page_table_strides, lens, B, pages_per_sequence, cache->page_size, p.t));
-    SA_TRY(rows_of(who, "q", q, q_strides));
-    SA_TRY(rows_of(who, "o", o, o_strides));
-    SA_TRY(half_dtype(who, dtype));
-    if (Sq <= 0 || Sq > 32) return fail(SA_ERR_UNSUPPORTED, "%s: 1 .. 32 query rows (got %d)", who, Sq);
-    if (Hq <= 0 || Hq % p.c.H) return fail(SA_ERR_INVALID_ARGUMENT, "%s: Hq (%d) must be a multiple of the cache's H (%d)", who, Hq, p.c.H);
-    if (!(sm_scale_log2 > 0.f) || sm_scale_log2 > 3e38f) return fail(SA_ERR_INVALID_ARGUMENT, "%s: softmax scale must be positive and finite", who);
-    if (window < 0) return fail(SA_ERR_INVALID_ARGUMENT, "%s: window must not be negative (got %d)", who, window);
-    if (lse && !lse_strides) return fail(SA_ERR_INVALID_ARGUMENT, "%s: null lse strides", who);
     if (full_ids || full_lens || part_ids || part_lens || packed) {
         if (!full_ids || !full_lens || !part_ids || !part_lens || !packed || !full_ids_strides || !full_lens_strides || !part_ids_strides ||
             !part_lens_strides || !packed_strides)
@@ -300,38 +345,22 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
         p.pis[2] = part_ids_strides[3];
         p.nK = tiles;
     }
-    p.q = static_cast<const uint16_t *>(q);
-    p.o = static_cast<uint16_t *>(o);
-    p.lse = lse;
-    for (int i = 0; i < 3; i++) {
-        p.qs[i] = q_strides[i];
-        p.os[i] = o_strides[i];
-        p.lses[i] = lse ? lse_strides[i] : 0;
-    }
-    p.counts = counts;
-    p.G = Hq / p.c.H;
-    p.Sq = Sq;
-    if ((int64_t)p.G * Sq > kMostRows) return fail(SA_ERR_UNSUPPORTED, "%s: more than %d rows per K/V head", who, kMostRows);
-    p.R = p.G * Sq;
-    p.RT = (p.R + 31) / 32;
-    p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
-    p.scale = sm_scale_log2;
-    const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)pages_per_sequence << p.c.lper;
-    if (planes > (1 << 24) || planes * chunks > (1 << 30))
-        return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
-    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
-    const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
-                 need = units_at + units_bytes((int64_t)B * p.c.H);
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
-        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
-    p.groups = plan.groups;
-    p.parts = plan.parts;
-    p.part_rows = plan.part_rows;
-    p.ws = static_cast<float *>(workspace);
-    p.arrivals = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(workspace) + parts_bytes);
-    p.tag = sa::next_launch_tag() | 1;
-    if ((p.full_ids != nullptr ? (int64_t)B * p.c.H : B) > sa::kPagedFewUnits(p.full_ids != nullptr)) p.units = reinterpret_cast<sa::PagedUnits *>(static_cast<uint8_t *>(workspace) + units_at);
-    return launched(who, sa::launch_paged_decode(p, dtype, static_cast<hipStream_t>(stream)));
+    return decode(who, p, 32, q, q_strides, o, o_strides, counts, B, Hq, Sq, window, dtype, sm_scale_log2, workspace, workspace_bytes, lse, lse_strides, stream);
+}
+
+int sa_sparse_attention_decode_tree(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,
+                                    const int64_t page_table_strides[2], const int32_t *lens, const int32_t *parents, const int64_t parents_strides[2],
+                                    const int32_t *counts, int pages_per_sequence, void *o, const int64_t o_strides[4], int B, int Hq, int n, int window,
+                                    int dtype, float sm_scale_log2, void *workspace, size_t workspace_bytes, float *lse, const int64_t lse_strides[3],
+                                    void *stream) {
+    const char *who = "sa_sparse_attention_decode_tree";
+    sa::PagedDecodeParams p{};
+    SA_TRY(pool_of(who, cache, p.c));
+    SA_TRY(table_of(who, page_table, page_table_strides, lens, B, pages_per_sequence, cache->page_size, p.t));
+    if (!parents || !parents_strides) return fail(SA_ERR_INVALID_ARGUMENT, "%s: null parents", who);
+    p.parents = parents;
+    for (int i = 0; i < 2; i++) p.parents_stride[i] = parents_strides[i];
+    return decode(who, p, kTreeNodes, q, q_strides, o, o_strides, counts, B, Hq, n, window, dtype, sm_scale_log2, workspace, workspace_bytes, lse, lse_strides, stream);
 }
 
 }  // extern "C"

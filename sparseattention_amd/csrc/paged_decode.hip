@@ -19,6 +19,7 @@
 #include "fwd_common.h"
 #include "paged.h"
 #include "paged_pieces.h"
+#include "tree.h"
 
 namespace sa {
 
@@ -346,8 +347,11 @@ __global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDe
     }
 }
 
-template <int DT, int ND, int ROWS, bool FAR, bool LISTS>
+// What says which keys a row attends to: causality and window, lists, or a tree of the last tokens.
+enum Who { kCausal, kLists, kTree };
+template <int DT, int ND, int ROWS, bool FAR, int WHO>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
+    constexpr bool LISTS = WHO == kLists, TREE = WHO == kTree;
     using E = Elem<DT>;
     using X = Tile<DT, ND, ROWS, FAR>;
     constexpr int D = 32 * ND, PST = D + kPagedRowPad;
@@ -478,7 +482,23 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         const int row = ROWS * rt + lrow, g = by_rows(row), i = row - g * p.Sq;
         const bool live = row < p.R && i < cnt;
         // without lists it sees the keys from `lo` to `hi`
-        const int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
+        int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
+        // of a tree the keys in front of its nodes from `lo` on, and those of the nodes in `above`
+        uint64_t above = 0ull;
+        if constexpr (TREE) {
+            const int base = len - cnt;
+            if (p.window > 0 || 32 * (T0 + off + n) > base) {
+                const ArgPtr a = late();
+                const uint64_t nodes = tree_ancestors(a->parents + b * a->parents_stride[0], a->parents_stride[1], cnt, lane);
+                above = __shfl((unsigned long long)nodes, live ? i : 0);
+                if (p.window > 0) {
+                    const int depth = __popcll(above) - 1;
+                    lo = min(base, base + depth - p.window + 1);
+                    for (int far = depth + 1 - p.window; far > 0; far--) above &= above - 1;  // (ancestors' numbers are lower)
+                }
+            }
+            hi = base - 1;
+        }
 
         u32x4 qf[X::NQ];
         {
@@ -602,6 +622,14 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 if (c.slot >= 0) {
                     cut = true;
                     see &= c.bits;
+                }
+            } else if constexpr (TREE) {
+                if (key0 + 31 >= len - cnt || (p.window > 0 && key0 <= len - 1 - p.window)) {
+                    cut = true;
+                    const int in_front = hi + 1 - key0, from = lo - key0;  // bits from .. in_front - 1, and the nodes' behind
+                    const uint32_t nodes = in_front > 0 ? in_front > 31 ? 0u : (uint32_t)above << in_front : (uint32_t)(above >> (-in_front & 63));
+                    see &= nodes | (in_front >= 32 ? ~0u : in_front > 0 ? (1u << in_front) - 1u : 0u);
+                    see = from > 31 ? 0u : from > 0 ? see & ~((1u << from) - 1u) : see;
                 }
             } else {
                 if (key0 + 31 > len - cnt || (p.window > 0 && key0 <= len - 1 - p.window)) {
@@ -808,27 +836,28 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     }
 }
 
-template <int DT, int ND, int ROWS, bool FAR, bool LISTS>
+template <int DT, int ND, int ROWS, bool FAR, int WHO>
 hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
     constexpr int smem = kWaves * ROWS * (32 * ND + kPagedRowPad) * 4;
-    auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, LISTS>;
+    auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, WHO>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
     if (p.units != nullptr) {
-        hipLaunchKernelGGL(paged_units_kernel<LISTS>, dim3(1), dim3(kUnitThreads), 0, stream, p, p.groups);
+        hipLaunchKernelGGL(paged_units_kernel<WHO == kLists>, dim3(1), dim3(kUnitThreads), 0, stream, p, p.groups);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)p.groups), dim3(kWaves * 64), smem, stream, p);
     return hipGetLastError();
 }
 template <int DT, int ND, int ROWS, bool FAR>
-hipError_t launch_lists(const PagedDecodeParams &p, hipStream_t stream) {
-    return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, FAR, true>(p, stream) : launch_kind<DT, ND, ROWS, FAR, false>(p, stream);
+hipError_t launch_who(const PagedDecodeParams &p, hipStream_t stream) {
+    if (p.parents != nullptr) return launch_kind<DT, ND, ROWS, FAR, kTree>(p, stream);
+    return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, FAR, kLists>(p, stream) : launch_kind<DT, ND, ROWS, FAR, kCausal>(p, stream);
 }
 template <int DT, int ND>
 hipError_t launch_rows(const PagedDecodeParams &p, hipStream_t stream) {
-    if (p.R <= 16) return launch_lists<DT, ND, 16, true>(p, stream);
-    return p.RT == 1 ? launch_lists<DT, ND, 32, true>(p, stream) : launch_lists<DT, ND, 32, false>(p, stream);
+    if (p.R <= 16) return launch_who<DT, ND, 16, true>(p, stream);
+    return p.RT == 1 ? launch_who<DT, ND, 32, true>(p, stream) : launch_who<DT, ND, 32, false>(p, stream);
 }
 template <int DT>
 hipError_t launch_dim(const PagedDecodeParams &p, hipStream_t stream) {

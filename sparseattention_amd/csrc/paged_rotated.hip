@@ -6,6 +6,7 @@
 // a head, or rows of queries in turn.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.
 #include "paged_codes.h"
 #include "rotate.h"
+#include "tree.h"
 
 namespace sa {
 namespace {

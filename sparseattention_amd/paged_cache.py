@@ -162,3 +162,14 @@ def sparse_attention_decode_paged(q: torch.Tensor, cache: PagedCache, page_table
     Probabilities and values meet in q's type, sums are float32; with fp16 queries the values are those that
     ``paged_cache_gather(..., dtype=torch.float16)`` gives."""
     return _native.host().decode_paged(q, cache, page_table, lens, mask, mask_metadata, counts, window, return_lse)
+
+
+def sparse_attention_decode_tree(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, *,
+                                 counts: Optional[torch.Tensor] = None, window: Optional[int] = None, return_lse: bool = False):
+    """:func:`sparse_attention_decode_paged` for a tree of drafted tokens: the last n tokens of each sequence, ``q`` [B,Hq,n,D] (n <= 64) their
+    queries, ``lens`` counting them.  ``parents`` (int32 [B,n], any strides): ``parents[b, i]`` in ``[0, i)`` is node ``i``'s parent, any
+    other value says that it has none.  Row ``i`` attends to all keys in front of the tree, to itself and to its ancestors; with ``window`` to
+    those less than ``window`` positions back, where a node's position is the keys in front of the tree and its depth.
+
+    ``counts`` (int32 [B]): the tree has ``counts[b]`` nodes, the rows behind are padding and give 0 (``lse`` -inf)."""
+    return _native.host().decode_tree(q, cache, page_table, lens, parents, counts, window, return_lse)
