@@ -598,6 +598,17 @@ int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_
 int sa_paged_cache_copy(const sa_paged_cache *cache, const int32_t *src, const int32_t *dst, int n, void *stream);
 
 /*
+ * Keeps the accepted drafts of a tree: of the n <= 64 tokens that were stored behind the lens[b] (as sa_paged_cache_append has them: without the drafts) token
+ * lens[b] + path[b][i] becomes token lens[b] + i, i < accepted[b] (device int32 [B,n] with strides, and [B]).  All tokens are read before any is
+ * written.  A path entry outside [0, n), and a token whose old or new page does not exist, leaves its place as it is.  A block keeps its scale while it
+ * holds tokens in front of the drafts or keeps some of its own, or takes a larger one that tokens from other blocks need; what it keeps is then rounded
+ * again.  Tokens behind the last one kept are undefined.
+ */
+int sa_paged_cache_keep(const sa_paged_cache *cache, const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens,
+                        const int32_t *path, const int64_t path_strides[2], const int32_t *accepted, int B, int n, int pages_per_sequence,
+                        void *stream);
+
+/*
  * n new sequences that continue old ones: new_table[i] (int32 [n, pages_per_sequence], contiguous) is the row of parents[i] with -1
  * behind its last page, new_lens[i] its length.  Full pages are shared.  A last page that is not full is copied to page new_pages[i],
  * which takes its place in the row; where new_pages[i] is no page the child keeps the parent's.  A parent outside [0, B) gives an
@@ -662,6 +673,33 @@ int sa_sparse_attention_decode_tree(const void *q, const int64_t q_strides[4], c
                                     const int64_t parents_strides[2], const int32_t *counts, int pages_per_sequence, void *o,
                                     const int64_t o_strides[4], int B, int Hq, int n, int window, int dtype, float sm_scale_log2,
                                     void *workspace, size_t workspace_bytes, float *lse, const int64_t lse_strides[3], void *stream);
+
+/*
+ * Verification of drafted tokens against the target's probabilities.  Node 0 is the last token that the sequence has; node i's token was drafted behind
+ * that of parents[b][i] in [0, i) (device int32 [B,n], any other value: behind none), or with parents NULL behind node i - 1.  From node 0 on the children
+ * of the node at hand are tried in the order of their numbers, with p the target's probabilities there (row `node` of target_probs) and u the
+ * child's number in uniforms:
+ *   draft_probs NULL   accepted if u * rest < p(x), x its token; rest is 1 less the p of the siblings rejected before it, p(x) is 0 if x was one of
+ *                      them.  Tokens come out as the target would say them, however the drafts were made.
+ *   draft_probs        (chains) accepted if u * q(x) < p(x), q row node of draft_probs [B, n - 1 or more, V], from which x was drawn
+ * An accepted child is the next node.  Where no child is accepted the next token is the first v with cumsum(r)(v) > uniforms[b][0] * sum(r): r is p without the
+ * rejected tokens, or max(p - q, 0) after a rejection, p where none was rejected or that leaves nothing.
+ * All of it in 64 bits.  Rows are taken to add up to 1 in the tests.  Negative, infinite and NaN probabilities count as 0, numbers below 0 (and NaN) as 0.
+ * A node whose token is outside [0, V) is not there.
+ *   target_probs  [B,n,V], draft_probs: bf16, fp16 or float32, last dimension contiguous; V <= 2^21, n <= 64
+ *   tokens        [B,n] device int32, or int64 (tokens_64 != 0); node 0's is not looked at
+ *   uniforms      device float32 [B,n], in [0, 1)
+ *   counts        device int32 [B], nodes of each tree, or NULL: n.  Without nodes nothing is accepted and the next token is -1.
+ *   path          device int32 [B,n], contiguous: the accepted nodes, 0 first, -1 behind; accepted int32 [B]: how many
+ *   next_token    device [B], of the tokens' type: the token behind the last accepted one (-1: p has none)
+ * workspace: sa_verify_drafts_workspace_bytes(B, n, V) bytes, 8-byte aligned; holds nothing between calls.
+ */
+size_t sa_verify_drafts_workspace_bytes(int B, int n, int V);
+int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], const void *draft_probs, const int64_t draft_strides[3],
+                     const void *tokens, const int64_t tokens_strides[2], int tokens_64, const float *uniforms,
+                     const int64_t uniforms_strides[2], const int32_t *parents, const int64_t parents_strides[2], const int32_t *counts,
+                     int32_t *path, int32_t *accepted, void *next_token, int B, int n, int V, int dtype, void *workspace,
+                     size_t workspace_bytes, void *stream);
 
 /*
  * Merge of n attention results over disjoint key ranges of the same queries (what sharding the key axis over

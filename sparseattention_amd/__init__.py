@@ -15,11 +15,13 @@ Same Python surface as tomatillos/sparseattention for its one hot path:
 The device work is done by hand-written gfx950 HIP kernels in ``libsparseattn_hip.so``
 behind the C ABI of ``include/sparseattn.h``.
 """
+from .drafts import verify_drafts
 from .mask_utils import (MaskMetadata, MaskTerm, block_term, causal_term, compute_mask_kernel, compute_mask_slow,
                          compute_mask_terms, materialize_mask_terms, select_block_sizes, select_tiling, Tiling,
                          with_list_stats)
 from .paged_cache import (PagedCache, empty_paged_cache, paged_cache_append, paged_cache_append_rotated, paged_cache_compact, paged_cache_copy,
-                          paged_cache_fork, paged_cache_free_pages, paged_cache_gather, sparse_attention_decode_paged, sparse_attention_decode_tree)
+                          paged_cache_fork, paged_cache_free_pages, paged_cache_gather, paged_cache_keep, sparse_attention_decode_paged,
+                          sparse_attention_decode_tree)
 from .rotary import Rotary, rotary_frequencies, rotate_heads, rotate_heads_backward, rotate_heads_trainable
 from .sparse_attn_kernel import (BackwardMetadata, compute_backward_metadata, compute_backward_metadata_terms,
                                  merge_attention_parts, sparse_attention,
@@ -34,4 +36,4 @@ __all__ = ["MaskMetadata", "compute_mask_kernel", "compute_mask_slow", "select_b
            "paged_cache_gather", "paged_cache_copy", "paged_cache_fork", "paged_cache_compact", "paged_cache_free_pages",
            "sparse_attention_decode_paged", "Rotary", "rotary_frequencies", "rotate_heads", "rotate_heads_backward",
            "rotate_heads_trainable", "paged_cache_append_rotated",
-           "sparse_attention_decode_tree"]
+           "sparse_attention_decode_tree", "paged_cache_keep", "verify_drafts"]

@@ -81,6 +81,9 @@ EXPORTS = (
     "sa_paged_cache_append_rotated",
     "sa_decode_tree_workspace_bytes",
     "sa_sparse_attention_decode_tree",
+    "sa_paged_cache_keep",
+    "sa_verify_drafts_workspace_bytes",
+    "sa_verify_drafts",
 )
 
 _lib = None
@@ -265,6 +268,14 @@ def load() -> ctypes.CDLL:
     lib.sa_sparse_attention_decode_tree.argtypes = (
         [_vp, _i64p, cache] + table + [_vp, _i64p] + [_vp, ctypes.c_int] + [_vp, _i64p] + [ctypes.c_int] * 5 + [ctypes.c_float]
         + [_vp, ctypes.c_size_t] + [_vp, _i64p] + [_vp]
+    )
+    lib.sa_paged_cache_keep.restype = ctypes.c_int
+    lib.sa_paged_cache_keep.argtypes = [cache] + table + [_vp, _i64p, _vp] + [ctypes.c_int] * 3 + [_vp]
+    lib.sa_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
+    lib.sa_verify_drafts_workspace_bytes.argtypes = [ctypes.c_int] * 3
+    lib.sa_verify_drafts.restype = ctypes.c_int
+    lib.sa_verify_drafts.argtypes = (
+        [_vp, _i64p] * 3 + [ctypes.c_int] + [_vp, _i64p] * 2 + [_vp] * 4 + [ctypes.c_int] * 4 + [_vp, ctypes.c_size_t, _vp]
     )
     if lib.sa_abi_version() != SA_ABI_VERSION:
         raise RuntimeError(f"libsparseattn_hip ABI {lib.sa_abi_version()} != expected {SA_ABI_VERSION}")

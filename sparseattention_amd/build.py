@@ -29,7 +29,8 @@ UNITS = [("sparseattn_api.hip", "sparseattn_api.o", []), ("mask_classify.hip", "
          ("sparse_fwd_f32_mfma.hip", "sparse_fwd_f32_mfma.o", []), ("sparse_fwd_merge.hip", "sparse_fwd_merge.o", []),
          ("sparse_decode.hip", "sparse_decode.o", []), ("sparse_bwd.hip", "sparse_bwd.o", []),
          ("paged_api.hip", "paged_api.o", []), ("paged_cache.hip", "paged_cache.o", []), ("paged_decode.hip", "paged_decode.o", []),
-         ("rotate.hip", "rotate.o", []), ("rotate_api.hip", "rotate_api.o", []), ("paged_rotated.hip", "paged_rotated.o", [])]
+         ("rotate.hip", "rotate.o", []), ("rotate_api.hip", "rotate_api.o", []), ("paged_rotated.hip", "paged_rotated.o", []),
+         ("paged_keep.hip", "paged_keep.o", []), ("verify.hip", "verify.o", []), ("verify_api.hip", "verify_api.o", [])]
 UNITS += [("sparse_fwd_inst.hip", f"sparse_fwd_dt{dt}_pk{pk}_how{how}.o",
            [f"-DSA_FWD_DT={dt}", f"-DSA_FWD_PK={pk}", f"-DSA_FWD_HOW={how}"])
           for dt in (0, 1) for pk in (0, 1) for how in (0, 1, 2, 3, 4, 5) if pk or how != 3]

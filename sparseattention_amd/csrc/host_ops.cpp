@@ -674,6 +674,76 @@ void paged_copy(py::object cache, const Tensor &src_in, const Tensor &dst_in) {
     check_rc(sa_paged_cache_copy(&c.c, ptr<int32_t>(src), ptr<int32_t>(dst), as_int(n, "n"), stream_of(c.k)));
 }
 
+void paged_keep(py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &path, const Tensor &accepted_in) {
+    const Cache c = cache_of(cache);
+    const py::gil_scoped_release unlocked;
+    const int64_t B = check_table(c, table);
+    const c10::DeviceGuard guard(c.k.device());
+    const Tensor lens = cache_ints(c, "lens", lens_in, B), accepted = cache_ints(c, "accepted", accepted_in, B);
+    if (path.dim() != 2 || path.size(0) != B || path.scalar_type() != at::kInt || path.device() != c.k.device())
+        value_error("path: expected int32 (" + std::to_string(B) + ", n) on " + c.k.device().str() + ", got " + str(path));
+    if (path.size(1) > 64) value_error("trees of at most 64 nodes (got " + std::to_string(path.size(1)) + ")");
+    if (B == 0 || path.size(1) == 0) return;
+    check_rc(sa_paged_cache_keep(&c.c, ptr<int32_t>(table), st(table), ptr<int32_t>(lens), ptr<int32_t>(path), st(path), ptr<int32_t>(accepted), as_int(B, "B"),
+                                 (int)path.size(1), as_int(table.size(1), "pages"), stream_of(c.k)));
+}
+
+py::tuple verify_drafts(const Tensor &target_in, const Tensor &tokens, const Tensor &uniforms, const OptTensor &parents, const OptTensor &draft_in,
+                        const OptTensor &counts_in) {
+    Tensor path, accepted, next;
+    {
+        const py::gil_scoped_release unlocked;
+        if (target_in.dim() != 3) value_error("target_probs must be [B, n, V] (got " + str(target_in.sizes()) + ")");
+        const int64_t B = target_in.size(0), n = target_in.size(1), V = target_in.size(2);
+        const int dt = dtype_code(target_in.scalar_type());
+        if (dt < 0) type_error(std::string("target_probs must be bfloat16, float16 or float32 (got ") + c10::toString(target_in.scalar_type()) + ")");
+        if (!target_in.is_cuda()) throw std::runtime_error("verify_drafts needs tensors on a ROCm GPU; there is no CPU path");
+        const auto dev = target_in.device();
+        if (n < 1 || n > 64) value_error("trees of 1 to 64 nodes (got " + std::to_string(n) + ")");
+        if (V < 1 || V > (1 << 21)) value_error("1 to 2^21 tokens in the vocabulary (got " + std::to_string(V) + ")");
+        auto nodes = [&](const char *name, const Tensor &t, const char *what, bool type) {
+            if (t.dim() != 2 || t.size(0) != B || t.size(1) != n || !type || t.device() != dev)
+                value_error(std::string(name) + ": expected " + what + " (" + std::to_string(B) + ", " + std::to_string(n) + ") on " + dev.str() + ", got " + str(t));
+        };
+        nodes("tokens", tokens, "int32 or int64", tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong);
+        nodes("uniforms", uniforms, "float32", uniforms.scalar_type() == at::kFloat);
+        if (parents) nodes("parents", *parents, "int32", parents->scalar_type() == at::kInt);
+        const c10::DeviceGuard guard(dev);
+        auto rows = [](const Tensor &t) { return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous(); };
+        Tensor target = rows(target_in);
+        OptTensor draft;
+        if (draft_in) {
+            if (parents) value_error("draft_probs go with chains: tokens of a tree are verified without them");
+            if (draft_in->dim() != 3 || draft_in->size(0) != B || draft_in->size(1) < n - 1 || draft_in->size(2) != V || draft_in->device() != dev)
+                value_error("draft_probs: expected [" + std::to_string(B) + ", " + std::to_string(n - 1) + " or more, " + std::to_string(V) + "] on " + dev.str() + ", got " +
+                            str(*draft_in));
+            if (draft_in->scalar_type() != target.scalar_type()) type_error("target_probs and draft_probs must share a dtype");
+            if (n > 1) draft = rows(*draft_in);
+        }
+        OptTensor counts;
+        if (counts_in) {
+            if (counts_in->dim() != 1 || counts_in->size(0) != B || counts_in->scalar_type() != at::kInt || counts_in->device() != dev)
+                value_error("counts: expected int32 (" + std::to_string(B) + ",) on " + dev.str() + ", got " + str(*counts_in));
+            counts = counts_in->contiguous();
+        }
+        const auto ints = at::TensorOptions().dtype(at::kInt).device(dev);
+        path = at::empty({B, n}, ints);
+        accepted = at::empty({B}, ints);
+        next = at::empty({B}, tokens.options());
+        if (B > 0) {
+            const size_t bytes = sa_verify_drafts_workspace_bytes(as_int(B, "B"), (int)n, (int)V);
+            const Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+            const int64_t target_s[3] = {target.stride(0), target.stride(1), 1};
+            int64_t draft_s[3] = {0, 0, 1};
+            if (draft) draft_s[0] = draft->stride(0), draft_s[1] = draft->stride(1);
+            check_rc(sa_verify_drafts(target.data_ptr(), target_s, draft ? draft->data_ptr() : nullptr, draft_s, tokens.data_ptr(), st(tokens),
+                                      tokens.scalar_type() == at::kLong, ptr<float>(uniforms), st(uniforms), ptr<int32_t>(parents), st(parents), ptr<int32_t>(counts),
+                                      ptr<int32_t>(path), ptr<int32_t>(accepted), next.data_ptr(), (int)B, (int)n, (int)V, dt, ws.data_ptr(), bytes, stream_of(target)));
+        }
+    }
+    return py::make_tuple(path, accepted, next);
+}
+
 py::tuple paged_fork(py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &parents_in, const Tensor &new_pages_in) {
     const Cache c = cache_of(cache);
     Tensor new_table, new_lens;
@@ -1370,6 +1440,8 @@ PYBIND11_MODULE(_host, m) {
     m.def("paged_append_rotated", &paged_append_rotated);
     m.def("paged_gather", &paged_gather);
     m.def("paged_copy", &paged_copy);
+    m.def("paged_keep", &paged_keep);
+    m.def("verify_drafts", &verify_drafts);
     m.def("paged_fork", &paged_fork);
     m.def("paged_compact", &paged_compact);
     m.def("paged_free_pages", &paged_free_pages);

@@ -103,6 +103,16 @@ struct PagedCopyParams {
 };
 hipError_t launch_paged_copy(PagedCopyParams p, hipStream_t stream);
 
+struct PagedKeepParams {
+    PagedPool c;
+    PageTable t;             // lens: tokens in front of the drafts
+    const int32_t *path;     // [B, n] nodes
+    int64_t path_s[2];
+    const int32_t *accepted;  // [B] of them
+    int n;
+};
+hipError_t launch_paged_keep(const PagedKeepParams &p, hipStream_t stream);
+
 struct PagedForkParams {
     PagedPool c;
     PageTable t;

@@ -175,6 +175,22 @@ int sa_paged_cache_copy(const sa_paged_cache *cache, const int32_t *src, const i
     return launched(who, sa::launch_paged_copy(p, static_cast<hipStream_t>(stream)));
 }
 
+int sa_paged_cache_keep(const sa_paged_cache *cache, const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, const int32_t *path,
+                        const int64_t path_strides[2], const int32_t *accepted, int B, int n, int pages_per_sequence, void *stream) {
+    const char *who = "sa_paged_cache_keep";
+    sa::PagedKeepParams p{};
+    SA_TRY(pool_of(who, cache, p.c));
+    SA_TRY(table_of(who, page_table, page_table_strides, lens, B, pages_per_sequence, cache->page_size, p.t));
+    if (!path || !path_strides || !accepted) return fail(SA_ERR_INVALID_ARGUMENT, "%s: null path", who);
+    if (n <= 0 || n > kTreeNodes) return fail(SA_ERR_UNSUPPORTED, "%s: trees of 1 .. %d nodes (got %d)", who, kTreeNodes, n);
+    p.path = path;
+    for (int i = 0; i < 2; i++) p.path_s[i] = path_strides[i];
+    p.accepted = accepted;
+    p.n = n;
+    SA_TRY(grid_fits(who, (int64_t)2 * p.c.H * B));
+    return launched(who, sa::launch_paged_keep(p, static_cast<hipStream_t>(stream)));
+}
+
 int sa_paged_cache_fork(const sa_paged_cache *cache, const int32_t *page_table, const int64_t page_table_strides[2], const int32_t *lens, int B,
                         int pages_per_sequence, const int32_t *parents, const int32_t *new_pages, int n, int32_t *new_table, int32_t *new_lens,
                         void *stream) {

@@ -15,8 +15,16 @@ and a prompt's later chunk, which has more than 32 rows, reads its keys back:
 
 (sparse_attention has a K/V head per query head: with grouped heads the third line copies K and V for each of a group.)
 
+A step with drafted tokens (a tree of n, its root the last token the sequence has), of a model that norms and rotates its heads:
+
+    q = paged_cache_append_rotated(cache, q, k, v, page_table, lens, rotary, parents=parents)
+    o = sparse_attention_decode_tree(q, cache, page_table, lens + n, parents)            # ... the target's probabilities
+    path, accepted, token = verify_drafts(probabilities, tokens, uniforms, parents)
+    paged_cache_keep(cache, page_table, lens, path, accepted)                             # in every layer's cache
+    lens = lens + accepted
+
 All calls enqueue work on the current stream of the cache's device and read no tensor on the host, so they can be captured
-into a graph (tile lists that a caller wrote or changed are looked at on the host, once, by the first call that gets them).  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip and csrc/paged_decode.hip."""
+into a graph (tile lists that a caller wrote or changed are looked at on the host, once, by the first call that gets them).  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip, csrc/paged_rotated.hip, csrc/paged_keep.hip and csrc/paged_decode.hip."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -120,6 +128,17 @@ def paged_cache_copy(cache: PagedCache, src: torch.Tensor, dst: torch.Tensor) ->
     """Copies page ``src[i]`` to page ``dst[i]`` (int32 [n] on the cache's device).  Pairs with a number that is no page are left out; a
     destination named more than once takes the last one's page.  No page may be both a source and a destination."""
     _native.host().paged_copy(cache, src, dst)
+
+
+def paged_cache_keep(cache: PagedCache, page_table: torch.Tensor, lens: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
+    """Keeps the accepted drafts of a tree whose n <= 64 tokens were stored behind the ``lens[b]`` that sequence ``b`` holds: token ``lens[b] + path[b, i]``
+    becomes token ``lens[b] + i``, i < ``accepted[b]`` (``path`` int32 [B,n], ``accepted`` int32 [B]: what
+    :func:`sparseattention_amd.verify_drafts` gives); the sequence then holds ``lens[b] + accepted[b]``, what lies behind them is undefined.
+
+    Within a block of 32 tokens codes move as they are.  What comes from another block is rounded to the scale of the one it comes to, which grows, and what the
+    block keeps is rounded again, where that needs it; a block that keeps none of its own tokens takes the scale that the new ones need.  All are read before any is written.  A path
+    entry that is no node, and a token whose old or new page does not exist, leaves its place as it is."""
+    _native.host().paged_keep(cache, page_table, lens, path, accepted)
 
 
 def paged_cache_fork(cache: PagedCache, page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor,
