@@ -262,13 +262,16 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
 
 static size_t units_bytes(int64_t units) { return (sizeof(sa::PagedUnits) + (size_t)units * 4 + 15) / 16 * 16; }
 
+// Tiles of 32 rows that share a workgroup: of trees, whose rows are many, two or four where there are as many.
+static int decode_tiles(bool tree, int R) { return !tree || R <= 32 ? 1 : R <= 64 ? 2 : 4; }
+
 static size_t decode_workspace_bytes(int most_rows, int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > most_rows || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
         (int64_t)Hq / H * Sq > kMostRows)
         return 0;
-    const int R = Hq / H * Sq;
-    const int64_t planes = (int64_t)B * H * ((R + 31) / 32);
-    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units());
+    const int R = Hq / H * Sq, tiles = decode_tiles(most_rows == kTreeNodes, R), of_plane = 32 * tiles;
+    const int64_t planes = (int64_t)B * H * ((R + of_plane - 1) / of_plane);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units(), tiles);
     return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8 + units_bytes((int64_t)B * H);
 }
 
@@ -304,13 +307,14 @@ static int decode(const char *who, sa::PagedDecodeParams &p, int most_rows, cons
     p.Sq = Sq;
     if ((int64_t)p.G * Sq > kMostRows) return fail(SA_ERR_UNSUPPORTED, "%s: more than %d rows per K/V head", who, kMostRows);
     p.R = p.G * Sq;
-    p.RT = (p.R + 31) / 32;
+    p.tiles = decode_tiles(p.parents != nullptr, p.R);
+    p.RT = (p.R + 32 * p.tiles - 1) / (32 * p.tiles);
     p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
     p.scale = sm_scale_log2;
     const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)p.t.width << p.c.lper;
     if (planes > (1 << 24) || planes * chunks > (1 << 30))
         return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
-    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units());
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units(), p.tiles);
     const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
                  need = units_at + units_bytes((int64_t)B * p.c.H);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))

@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDe
     }
     over(sum, plus, sums[0], total);
     over(longest, most, sums[1], longest);
-    const PagedShare share = paged_share((unsigned)total * M, U * M, groups, (unsigned)longest, (unsigned)p.parts);
+    const PagedShare share = paged_share((unsigned)total * M, U * M, groups, (unsigned)longest, (unsigned)p.parts, kPagedWaves / p.tiles);
     sum = 0;
     for (int u = u0; u < u1; u++) sum += (int)paged_row_length(share, p.units->first[u]);
     unsigned at = (unsigned)over(sum, plus, sums[0], total);
@@ -349,15 +349,18 @@ __global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDe
 
 // What says which keys a row attends to: causality and window, lists, or a tree of the last tokens.
 enum Who { kCausal, kLists, kTree };
-template <int DT, int ND, int ROWS, bool FAR, int WHO>
+// TILES: of rows that a workgroup has, kWaves / TILES waves each, which take chunks in turn.  Several read the same K and V at about the same
+// time, from the caches: 8 trees of 64 nodes x 4 heads over 65536 keys, D = 64, fp16 RATES.
+template <int DT, int ND, int ROWS, bool FAR, int WHO, int TILES>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
     constexpr bool LISTS = WHO == kLists, TREE = WHO == kTree;
     using E = Elem<DT>;
     using X = Tile<DT, ND, ROWS, FAR>;
     constexpr int D = 32 * ND, PST = D + kPagedRowPad;
+    constexpr int TURNS = kWaves / TILES, PLANE = ROWS * TILES;  // waves that take turns, rows of a plane
     extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][ROWS][PST]
     const int tid = threadIdx.x, lane = tid & 63, lrow = lane & (ROWS - 1), lgrp = lane / ROWS;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), turn = wave / TILES, tile = wave % TILES;
     const int lP = p.c.lper + 5, sub_mask = (1 << p.c.lper) - 1;
     // What is read from the argument block where it is used: hoisted out of the loop over the segments, the strides of everything had
     // the inner loop's scalars spilled.
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 longest = max(longest, mine[k]);
             }
         longest = __builtin_amdgcn_readlane(scan(longest, [](int a, int x) { return max(a, x); }), 63);
-        share = paged_share((unsigned)sum * M, U * M, gridDim.x, (unsigned)longest, (unsigned)p.parts);
+        share = paged_share((unsigned)sum * M, U * M, gridDim.x, (unsigned)longest, (unsigned)p.parts, TURNS);
         if (share.cuts) {
             sum = 0;
 #pragma unroll
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         const bool keys = unit.T > 0;
         if (x < x1 && x == base) unit = of_lane(unit_of<LISTS>(p, u), 0);  // (the next segment's)
         // this lane's row: query i of query head g
-        const int row = ROWS * rt + lrow, g = by_rows(row), i = row - g * p.Sq;
+        const int row = PLANE * rt + ROWS * tile + lrow, g = by_rows(row), i = row - g * p.Sq;
         const bool live = row < p.R && i < cnt;
         // without lists it sees the keys from `lo` to `hi`
         int hi = len - cnt + i, lo = p.window > 0 ? hi - p.window + 1 : 0;
@@ -513,8 +516,8 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         X out_rows;
         out_rows.clear();
 
-        // This wave's chunks are off + wave + 4 j, j < nw.  Lane j of a round of 64 of them finds where chunk j lies.
-        const int nw = (n - wave + kWaves - 1) / kWaves;
+        // This wave's chunks are off + turn + TURNS j, j < nw.  Lane j of a round of 64 of them finds where chunk j lies.
+        const int nw = TILES > 1 && PLANE * rt + ROWS * tile >= p.R ? 0 : (n - turn + TURNS - 1) / TURNS;
         struct Places {
             int block, tile, slot;  // block of the pool or -1; with lists the tile, and the slot of a PARTIAL one or -1
             float ks, vs;
@@ -524,7 +527,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             int block = -1, at_tile = 0, slot = -1;
             float ks = 0.f, vs = 0.f;
             const int j = j0 + lane;
-            const int t = T0 + off + wave + kWaves * j;
+            const int t = T0 + off + turn + TURNS * j;
             if (j < nw && keys) {
                 int tile = t >> p.c.lper;
                 if constexpr (LISTS) {
@@ -556,7 +559,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             uint32_t bits;
         };
         auto chunk = [&](const Places &at, int j) __attribute__((always_inline)) {
-            const int in = min(j, nw - 1) & 63, t = T0 + off + wave + kWaves * min(j, nw - 1);
+            const int in = min(j, nw - 1) & 63, t = T0 + off + turn + TURNS * min(j, nw - 1);
             const int block = __builtin_amdgcn_readlane(at.block, in);
             Chunk c{j < nw ? block : -1, t << 5, -1, 0u};
             if constexpr (LISTS) {
@@ -588,7 +591,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
                 request_v(under_way[i], ops[i]);
             });
         auto step = [&](int j, Chunk &c, typename X::Operands &x) __attribute__((always_inline)) {
-            if (done + 4u * j >= lower_at) {
+            if (done + (unsigned)TURNS * j >= lower_at) {
                 lower_at += share.share / 4;
                 quarter++;
                 if (quarter == 1) __builtin_amdgcn_s_setprio(2);
@@ -707,7 +710,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         __syncthreads();
         constexpr int LPR = D / 4;  // lanes per row
         const ArgPtr a = late();
-        const int rows = min(a->R - ROWS * rt, ROWS);
+        const int rows = min(a->R - PLANE * rt, PLANE);
         struct Sum {
             float M = kNegInf, L = 0.f;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -732,7 +735,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
             s.M = M;
         };
         auto finish = [&](int r, int d0, const Sum &s) __attribute__((always_inline)) {
-            const int at = ROWS * rt + r, gg = by_rows(at), ii = at - gg * p.Sq, head = h * a->G + gg;
+            const int at = PLANE * rt + r, gg = by_rows(at), ii = at - gg * p.Sq, head = h * a->G + gg;
             const bool none = ii >= cnt || s.L == 0.f;  // (a row of padding may have met a NaN)
             const float inv = 1.f / s.L;
             const f32x4 y = none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{s.x.x * inv, s.x.y * inv, s.x.z * inv, s.x.w * inv};
@@ -748,12 +751,12 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         const HandOver out(ws + (int64_t)(2 * me + (off == 0 ? 1 : 0)) * part_bytes, whole ? 0u : part_bytes);
         for (int it = tid; it < rows * LPR; it += kWaves * 64) {
             const int r = it / LPR, d0 = 4 * (it - r * LPR);
-            f32x4 v[kWaves];
-            f32x2 ml[kWaves];
+            f32x4 v[TURNS];
+            f32x2 ml[TURNS];
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                v[w] = *(const f32x4 *)(part + (w * ROWS + r) * PST + d0);
-                ml[w] = *(const f32x2 *)(part + (w * ROWS + r) * PST + D);
+            for (int w = 0; w < TURNS; w++) {
+                v[w] = *(const f32x4 *)(part + (w * PLANE + r) * PST + d0);
+                ml[w] = *(const f32x2 *)(part + (w * PLANE + r) * PST + D);
             }
             Sum s;
             add_to(s, v, ml);
@@ -836,10 +839,10 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
     }
 }
 
-template <int DT, int ND, int ROWS, bool FAR, int WHO>
+template <int DT, int ND, int ROWS, bool FAR, int WHO, int TILES = 1>
 hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
     constexpr int smem = kWaves * ROWS * (32 * ND + kPagedRowPad) * 4;
-    auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, WHO>;
+    auto kern = paged_decode_kernel<DT, ND, ROWS, FAR, WHO, TILES>;
     static unsigned long long attr_done = 0;
     if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
     if (p.units != nullptr) {
@@ -851,11 +854,14 @@ hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
 }
 template <int DT, int ND, int ROWS, bool FAR>
 hipError_t launch_who(const PagedDecodeParams &p, hipStream_t stream) {
-    if (p.parents != nullptr) return launch_kind<DT, ND, ROWS, FAR, kTree>(p, stream);
+    if constexpr (FAR)
+        if (p.parents != nullptr) return launch_kind<DT, ND, ROWS, FAR, kTree>(p, stream);
     return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, FAR, kLists>(p, stream) : launch_kind<DT, ND, ROWS, FAR, kCausal>(p, stream);
 }
 template <int DT, int ND>
 hipError_t launch_rows(const PagedDecodeParams &p, hipStream_t stream) {
+    if (p.tiles == 2) return launch_kind<DT, ND, 32, false, kTree, 2>(p, stream);
+    if (p.tiles == 4) return launch_kind<DT, ND, 32, false, kTree, 4>(p, stream);
     if (p.R <= 16) return launch_who<DT, ND, 16, true>(p, stream);
     return p.RT == 1 ? launch_who<DT, ND, 32, true>(p, stream) : launch_who<DT, ND, 32, false>(p, stream);
 }

@@ -39,15 +39,17 @@ constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ?
 struct PagedDecodePlan {
     int groups, parts, part_rows;
 };
-inline PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus) {
+// tiles: of 32 rows that a workgroup has, kPagedWaves / tiles waves each.
+inline PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus, int tiles = 1) {
     PagedDecodePlan r;
+    const int waves = kPagedWaves / tiles;
     const int64_t even = (int64_t)cus * (D == 64 ? 2 : 1) / planes;
     r.parts = (int)(even < 16 ? 16 : even < kPagedMostParts - 2 ? even : kPagedMostParts - 2);
     const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
-    const int64_t fine = (chunks + kPagedWaves - 1) / kPagedWaves;  // parts of a plane of a chunk a wave
+    const int64_t fine = (chunks + waves - 1) / waves;  // parts of a plane of a chunk a wave
     const int64_t most = planes * ((fine < r.parts ? fine : r.parts) + 1);
     r.groups = ((int)(most < resident ? most : resident) + 7) / 8 * 8;
-    r.part_rows = R < 32 ? R : 32;
+    r.part_rows = R < 32 * tiles ? R : 32 * tiles;
     return r;
 }
 
@@ -57,12 +59,12 @@ inline PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t c
 // planes of 63 chunks 12.1 -> 9.1, 104 planes of one chunk 14 -> 11; at 3 parts (256 planes of 700 ... 1024) it would be 290 -> 319.
 // A plane has no more parts than `parts`, and no more than balance the chunks that a wave has one after the other (1.15 us each) with the
 // sum over the parts: sqrt(2 T) of T chunks, but 16 at least.
-// total: chunks of all planes (less than 2^31); longest: of a plane.  No division more than it takes: each costs as much as a step of the scan.
+// total: chunks of all planes (less than 2^31); longest: of a plane; waves: of a workgroup that take chunks in turn.  No division more than it takes: each costs as much as a step of the scan.
 struct PagedShare {
     bool cuts;
     unsigned share;
 };
-SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned groups, unsigned longest, unsigned parts) {
+SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned groups, unsigned longest, unsigned parts, unsigned waves = kPagedWaves) {
 #ifdef __HIP_DEVICE_COMPILE__
     const unsigned balanced = (unsigned)__builtin_amdgcn_sqrtf(2.f * (float)longest);
 #else
@@ -71,11 +73,11 @@ SA_PIECES_FN PagedShare paged_share(unsigned total, unsigned planes, unsigned gr
     const unsigned most = balanced < 16u ? 16u : balanced;
     parts = parts < most ? parts : most;
     PagedShare r;
-    r.cuts = planes < groups && (8 * planes <= groups || total <= 2 * kPagedWaves * (groups - planes));
+    r.cuts = planes < groups && (8 * planes <= groups || total <= 2 * waves * (groups - planes));
     const unsigned among = r.cuts ? groups - planes : groups;  // (a part of each plane may be short)
     if (!r.cuts) total += planes * kPagedComing;  // (the host: at most 2^24 planes)
     r.share = (total + among - 1) / among;
-    if (r.cuts && r.share < (unsigned)kPagedWaves) r.share = kPagedWaves;
+    if (r.cuts && r.share < waves) r.share = waves;
     if ((uint64_t)longest > (uint64_t)r.share * parts) r.share = (longest + parts - 1) / parts;
     return r;
 }
