@@ -156,8 +156,8 @@ struct PagedDecodeParams {
     float *lse;  // or null
     int64_t qs[3], os[3], lses[3];  // b, h, row strides in elements
     const int32_t *counts;  // valid query rows of each sequence, or null: Sq
-    int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT planes of a tile of 16 (all of them) or of `tiles` tiles of 32
-    int tiles;              // that share a workgroup: 1, of trees up to 4
+    int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT planes
+    int plane_rows, tiles;  // of a plane: 16, or `tiles` tiles of 32 that share a workgroup (more than one of trees only)
     int window;             // or 0
     // the rows are a tree (tree.h): each one's parent, or null
     const int32_t *parents;

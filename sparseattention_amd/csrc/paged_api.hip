@@ -262,16 +262,31 @@ int sa_paged_cache_free_pages(const int32_t *page_table, const int64_t page_tabl
 
 static size_t units_bytes(int64_t units) { return (sizeof(sa::PagedUnits) + (size_t)units * 4 + 15) / 16 * 16; }
 
-// Tiles of 32 rows that share a workgroup: of trees, whose rows are many, two or four where there are as many.
-static int decode_tiles(bool tree, int R) { return !tree || R <= 32 ? 1 : R <= 64 ? 2 : 4; }
+// Rows of a plane.  Trees have many: where there is little work planes are small, as one workgroup adds a plane's parts up, row by row; where there is much
+// several tiles of rows read K and V together.  us with planes of 16 | 32 | 64 | 128 rows, D = 128, bf16, of R rows of H K/V heads, C chunks in all:
+//   R  32, H   8: C  504  12.4 | 18.9; 8000  26.8 | 37.1;    H 512: C 32256  76 | 59
+//   R 128, H   8: C  504  18.6 | 21.6 | 26.7 | 42.9;         H 64: C 4032  30 | 34 | 33 | 45
+//          H 256: C 16128  116 | 67 | 63 | 71; 32000  240 | 127 | 99 | 114; 65536  488 | 249 | 204 | 199; 160000  1338 | 674 | 455 | 434
+//          H  16: C 32768  271 | 97 | 108 | 160 (few planes, of many parts)
+//   R  64, H 256: C 32000  140 | 64 | 66; 65536  290 | 133 | 126; 262144  1224 | 532 | 400
+static int decode_plane_rows(bool tree, int64_t heads, int R, int64_t chunks) {
+    if (R <= 16) return 16;
+    if (!tree) return 32;
+    const int64_t work = heads * chunks;  // (of the tables: the sequences may be shorter)
+    if (work * ((R + 15) / 16) <= 24 << 10) return 16;
+    if (R <= 32 || heads < 64 || work * ((R + 63) / 64) <= 40 << 10) return 32;
+    return R <= 64 || work < 64 << 10 ? 64 : 128;
+}
 
 static size_t decode_workspace_bytes(int most_rows, int B, int Hq, int H, int Sq, int D, int pages_per_sequence, int page_size) {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || Sq <= 0 || Sq > most_rows || (D != 64 && D != 128 && D != 256) || pages_per_sequence <= 0 || page_size < 32 ||
         (int64_t)Hq / H * Sq > kMostRows)
         return 0;
-    const int R = Hq / H * Sq, tiles = decode_tiles(most_rows == kTreeNodes, R), of_plane = 32 * tiles;
-    const int64_t planes = (int64_t)B * H * ((R + of_plane - 1) / of_plane);
-    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, (int64_t)pages_per_sequence * (page_size / 32), compute_units(), tiles);
+    const int R = Hq / H * Sq;
+    const int64_t heads = (int64_t)B * H, chunks = (int64_t)pages_per_sequence * (page_size / 32);
+    const int plane_rows = decode_plane_rows(most_rows == kTreeNodes, heads, R, chunks);
+    const int64_t planes = heads * ((R + plane_rows - 1) / plane_rows);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, R, D, chunks, compute_units(), plane_rows);
     return sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, D) + (size_t)(planes + plan.groups) * 8 + units_bytes((int64_t)B * H);
 }
 
@@ -307,14 +322,16 @@ static int decode(const char *who, sa::PagedDecodeParams &p, int most_rows, cons
     p.Sq = Sq;
     if ((int64_t)p.G * Sq > kMostRows) return fail(SA_ERR_UNSUPPORTED, "%s: more than %d rows per K/V head", who, kMostRows);
     p.R = p.G * Sq;
-    p.tiles = decode_tiles(p.parents != nullptr, p.R);
-    p.RT = (p.R + 32 * p.tiles - 1) / (32 * p.tiles);
+    const int64_t heads = (int64_t)B * p.c.H, chunks = (int64_t)p.t.width << p.c.lper;
+    p.plane_rows = decode_plane_rows(p.parents != nullptr, heads, p.R, chunks);
+    p.tiles = p.plane_rows < 64 ? 1 : p.plane_rows / 32;
+    p.RT = (p.R + p.plane_rows - 1) / p.plane_rows;
     p.window = window < (1 << 30) ? window : 0;  // (no table is that long)
     p.scale = sm_scale_log2;
-    const int64_t planes = (int64_t)B * p.c.H * p.RT, chunks = (int64_t)p.t.width << p.c.lper;
+    const int64_t planes = heads * p.RT;
     if (planes > (1 << 24) || planes * chunks > (1 << 30))
         return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
-    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units(), p.tiles);
+    const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units(), p.plane_rows);
     const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
                  need = units_at + units_bytes((int64_t)B * p.c.H);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))

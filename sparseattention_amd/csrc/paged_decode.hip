@@ -349,10 +349,11 @@ __global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDe
 
 // What says which keys a row attends to: causality and window, lists, or a tree of the last tokens.
 enum Who { kCausal, kLists, kTree };
-// TILES: of rows that a workgroup has, kWaves / TILES waves each, which take chunks in turn.  Several read the same K and V at about the same
-// time, from the caches: 8 trees of 64 nodes x 4 heads over 65536 keys, D = 64, fp16 RATES.
+// TILES: of rows that a workgroup has, kWaves / TILES waves each, which take chunks in turn.  Several read the same K and V at about the same time, from the
+// caches (8 trees of 64 nodes, 8 x 4 heads, over up to 65536 keys, D = 64, fp16: 514 us with one, 406 with four, 593 TFLOP/s); what is left then is vector work,
+// 130 instructions for the 32 x 32 scores of a chunk, 16 of them exponentials.
 template <int DT, int ND, int ROWS, bool FAR, int WHO, int TILES>
-__global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_decode_kernel(const PagedDecodeParams p) {
+__global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS, TILES)) void paged_decode_kernel(const PagedDecodeParams p) {
     constexpr bool LISTS = WHO == kLists, TREE = WHO == kTree;
     using E = Elem<DT>;
     using X = Tile<DT, ND, ROWS, FAR>;
@@ -552,8 +553,9 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS)) void paged_
         };
         // What is requested next takes the registers of what has just gone into a product: K of a later chunk is on its way during the
         // softmax and the second product, V behind it.  At D = 64 two chunks are under way, as their bytes are half as many; with
-        // more registers for more there would be fewer waves, which hide as much.
-        constexpr int PRE = ND == 2 ? 2 : 1;
+        // more registers for more there would be fewer waves, which hide as much.  Tiles that share K and V find them in the caches, and have a third
+        // wave per SIMD instead (419 -> 406 us).
+        constexpr int PRE = ND == 2 && TILES == 1 ? 2 : 1;
         struct Chunk {
             int block, key0, slot;
             uint32_t bits;
@@ -854,15 +856,14 @@ hipError_t launch_kind(const PagedDecodeParams &p, hipStream_t stream) {
 }
 template <int DT, int ND, int ROWS, bool FAR>
 hipError_t launch_who(const PagedDecodeParams &p, hipStream_t stream) {
-    if constexpr (FAR)
-        if (p.parents != nullptr) return launch_kind<DT, ND, ROWS, FAR, kTree>(p, stream);
+    if (p.parents != nullptr) return launch_kind<DT, ND, ROWS, FAR, kTree>(p, stream);
     return p.full_ids != nullptr ? launch_kind<DT, ND, ROWS, FAR, kLists>(p, stream) : launch_kind<DT, ND, ROWS, FAR, kCausal>(p, stream);
 }
 template <int DT, int ND>
 hipError_t launch_rows(const PagedDecodeParams &p, hipStream_t stream) {
     if (p.tiles == 2) return launch_kind<DT, ND, 32, false, kTree, 2>(p, stream);
     if (p.tiles == 4) return launch_kind<DT, ND, 32, false, kTree, 4>(p, stream);
-    if (p.R <= 16) return launch_who<DT, ND, 16, true>(p, stream);
+    if (p.plane_rows == 16) return p.RT == 1 ? launch_who<DT, ND, 16, true>(p, stream) : launch_kind<DT, ND, 16, false, kTree>(p, stream);
     return p.RT == 1 ? launch_who<DT, ND, 32, true>(p, stream) : launch_who<DT, ND, 32, false>(p, stream);
 }
 template <int DT>

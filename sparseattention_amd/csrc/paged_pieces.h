@@ -28,7 +28,7 @@ constexpr unsigned kPagedComing = 8;
 // 16384 164 | 122.
 constexpr int kPagedFewUnits(bool lists) { return lists ? 64 : 256; }
 // Workgroups that a compute unit holds (a wave of each per SIMD), by D / 32 and the rows of a tile.
-constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
+constexpr int paged_occupancy(int nd, int rows, int tiles = 1) { return nd == 2 ? (rows == 16 || tiles > 1 ? 3 : 2) : nd == 4 ? (rows == 16 ? 3 : 2) : 1; }
 
 // A launch: its workgroups (a multiple of 8), the most parts a plane is meant to have, rows of a part.
 // As many workgroups as the device holds at once: with more, the pieces of a workgroup that starts late do not make up for its start
@@ -39,17 +39,18 @@ constexpr int paged_occupancy(int nd, int rows) { return nd == 2 ? (rows == 16 ?
 struct PagedDecodePlan {
     int groups, parts, part_rows;
 };
-// tiles: of 32 rows that a workgroup has, kPagedWaves / tiles waves each.
-inline PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus, int tiles = 1) {
+// plane_rows: 16, or tiles of 32 that a workgroup has, kPagedWaves / tiles waves each (0: one tile).
+inline PagedDecodePlan paged_decode_plan(int64_t planes, int R, int D, int64_t chunks, int cus, int plane_rows = 0) {
     PagedDecodePlan r;
-    const int waves = kPagedWaves / tiles;
+    if (plane_rows == 0) plane_rows = R <= 16 ? 16 : 32;
+    const int tiles = plane_rows < 64 ? 1 : plane_rows / 32, waves = kPagedWaves / tiles;
     const int64_t even = (int64_t)cus * (D == 64 ? 2 : 1) / planes;
     r.parts = (int)(even < 16 ? 16 : even < kPagedMostParts - 2 ? even : kPagedMostParts - 2);
-    const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, R <= 16 ? 16 : 32);
+    const int64_t resident = (int64_t)cus * paged_occupancy(D / 32, plane_rows == 16 ? 16 : 32, tiles);
     const int64_t fine = (chunks + waves - 1) / waves;  // parts of a plane of a chunk a wave
     const int64_t most = planes * ((fine < r.parts ? fine : r.parts) + 1);
     r.groups = ((int)(most < resident ? most : resident) + 7) / 8 * 8;
-    r.part_rows = R < 32 * tiles ? R : 32 * tiles;
+    r.part_rows = R < plane_rows ? R : plane_rows;
     return r;
 }
 
