@@ -81,10 +81,12 @@ struct PagedRotatedParams {
     const int32_t *parents;               // or null: a chain
     int64_t parents_stride[2];
     int Hq, S, blocks;
-    int splits, steps;  // workgroups that share a block; steps of an item of queries
+    // Set by the plan: workgroups for keys and for values; key heads of a workgroup; waves that share a group of query tokens and heads of each.
+    int key_groups, value_groups, key_heads, splits, heads;
 };
-int paged_rotated_splits(int B, int blocks, int H, int Hq, int S);
-hipError_t launch_paged_rotated(const PagedRotatedParams &p, int dtype, hipStream_t stream);
+// The launch's workgroups, -1: more than it can have.
+int64_t paged_rotated_plan(PagedRotatedParams &p);
+hipError_t launch_paged_rotated(const PagedRotatedParams &p, int64_t groups, int dtype, hipStream_t stream);
 
 struct PagedGatherParams {
     PagedPool c;

@@ -138,10 +138,9 @@ int sa_paged_cache_append_rotated(const sa_paged_cache *cache, const void *q, co
     p.Hq = Hq;
     p.S = S;
     p.blocks = (S + 62) / 32;
-    p.steps = S == 1 ? 1 : 8;
-    p.splits = sa::paged_rotated_splits(B, p.blocks, p.c.H, Hq, S);
-    SA_TRY(grid_fits(who, (int64_t)p.splits * p.blocks * B));
-    return launched(who, sa::launch_paged_rotated(p, dtype, static_cast<hipStream_t>(stream)));
+    const int64_t groups = sa::paged_rotated_plan(p);
+    if (groups < 0) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens or workgroups", who);
+    return launched(who, sa::launch_paged_rotated(p, groups, dtype, static_cast<hipStream_t>(stream)));
 }
 
 int sa_paged_cache_gather(const sa_paged_cache *cache, void *k, const int64_t k_strides[4], void *v, const int64_t v_strides[4],

@@ -2,8 +2,11 @@
 // counterpart in the reference.  The formula of a row is rotate.h's, a block's and its scale's paged_cache.hip's; keys go from float32 to codes in
 // one rounding, queries to their own type.
 //
-// A workgroup has the tokens of one block of a sequence, 32 or fewer: it makes their angles once in LDS, and its waves take keys of a head, values of
-// a head, or rows of queries in turn.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.
+// One launch, whose workgroups have one of three things to do: keys of a block of a sequence, 32 tokens or fewer, a wave a head at a time, with the angles made once in LDS;
+// values of blocks, a wave each, as paged_append_kernel stores them; or queries, a wave 64 / LPR tokens with their angles in registers, as
+// rotate_kernel has them.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.
+#include <algorithm>
+
 #include "paged_codes.h"
 #include "rotate.h"
 #include "tree.h"
@@ -12,35 +15,87 @@ namespace sa {
 namespace {
 
 constexpr int kRotatedThreads = 64 * kCacheWaves;
-// The words of LDS: angles [32][4 ND] of 4 cosines and 4 sines, then 16 rows or a block's codes for each wave.
-template <int ND>
-constexpr int angle_bytes = 32 * 4 * ND * 32;
-template <int ND>
-constexpr int wave_bytes = ND * 1024 > 16 * row_bytes<ND> ? ND * 1024 : 16 * row_bytes<ND>;
 
 template <int DT, int ND, bool INTER>
-__global__ __launch_bounds__(kRotatedThreads, 2) void paged_rotated_kernel(const PagedRotatedParams p) {
+__global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotated_kernel(const PagedRotatedParams p) {
     using X = Run4<DT>;
     constexpr int LPR = 4 * ND, T = 64 / LPR, U = 4;  // lanes of a row, rows of a step, steps under way
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    f32x4 *const angles = (f32x4 *)smem;  // of row r, four pairs l: [(r * LPR + l) * 2], cosines and sines
+    constexpr int kRows = 16 * row_bytes<ND>, kCodes = ND * 1024, kWave = kCodes > kRows ? kCodes : kRows;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kCacheWaves * kWave];
+    __shared__ f32x4 angles[32 * LPR * 2];  // of row r, four pairs l: [(r * LPR + l) * 2], cosines and sines
+    __shared__ int depth[64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane % LPR, r0 = lane / LPR;
-    uint8_t *const mine = smem + angle_bytes<ND> + wave * wave_bytes<ND>;
+    uint8_t *const mine = smem + wave * kWave;
+    const float share = 1.f / (float)p.c.cols;
+    const auto count_of = [&](int b) { return p.counts != nullptr ? min(max(p.counts[b], 0), p.S) : p.S; };
 
+    if (blockIdx.x >= (unsigned)p.key_groups + (unsigned)p.value_groups) {
+        // ---- queries: a wave has T tokens and some of their heads ----
+        const unsigned id = (blockIdx.x - p.key_groups - p.value_groups) * kCacheWaves + wave;
+        const int group = (int)(id / (unsigned)p.splits), h0 = (int)(id - (unsigned)group * p.splits) * p.heads, h1 = min(h0 + p.heads, p.Hq);
+        if (h0 >= h1) return;
+        const Columns c = columns_of(l, p.c.cols, p.r.R, INTER);
+        int b, s;
+        if (p.parents != nullptr) {  // (a wave has one sequence's, whose tree it looks through)
+            const int each = (p.S + T - 1) / T;
+            b = group / each;
+            s = (group - b * each) * T + r0;
+        } else {
+            const int64_t token = (int64_t)group * T + r0;
+            b = (int)(min(token, (int64_t)p.t.B * p.S) / p.S);
+            s = (int)(token - (int64_t)b * p.S);
+        }
+        if (__builtin_amdgcn_ballot_w64(b < p.t.B && s < p.S) == 0ull) return;
+        const bool live = c.live && b < p.t.B && s < p.S;
+        b = min(b, p.t.B - 1);
+        const int n = count_of(b);
+        const bool zero = s >= n;
+        double at = (double)max(p.t.lens[b], 0) + s;
+        if (p.parents != nullptr) {
+            const int above = __popcll(tree_ancestors(p.parents + b * p.parents_stride[0], p.parents_stride[1], n, lane)) - 1;
+            at += __shfl(above, s & 63) - s;
+        }
+        Turns t;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            t.c[i] = 1.f, t.s[i] = 0.f;
+            if (live && c.rot && !zero) {
+                if (p.r.positions != nullptr) at = position_at(p.r, axis_of(p.r, 4 * l + i), b, s);
+                turn(at, p.r.frequencies[4 * l + i], t.c[i], t.s[i]);
+            }
+        }
+        float w[2][4];
+        weights_of(p.r.q_weight, p.r.weight_dtype, c, w);
+        rotate_rows<DT, LPR, INTER>(p.q + b * p.qs[0] + s * p.qs[2], p.qo + b * p.qos[0] + s * p.qos[2], p.qs[1], p.qos[1], h0, h1, c, live, zero, t, p.r.q_weight, w, share,
+                                    p.r.eps);
+        return;
+    }
+    if (blockIdx.x >= (unsigned)p.key_groups) {
+        // ---- values: a wave a block of a head ----
+        unsigned item = (blockIdx.x - p.key_groups) * kCacheWaves + wave;
+        const int h = (int)(item % (unsigned)p.c.H);
+        item /= (unsigned)p.c.H;
+        const int nb = (int)(item % (unsigned)p.blocks), b = (int)(item / (unsigned)p.blocks);
+        if (b >= p.t.B) return;
+        const int len = max(p.t.lens[b], 0), first = 32 * nb - (len & 31);  // (row r of the block is token first + r of the call)
+        const int held = max(-first, 0), z = min(count_of(b) - first, 32), blk = (len >> 5) + nb;
+        if (held >= z) return;
+        const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
+        append_block<DT, ND>(p.c, p.v + b * p.vs[0] + h * p.vs[1] + (int64_t)first * p.vs[2], p.vs[2], true, page, h, blk & ((1 << p.c.lper) - 1), held, held, z, mine);
+        return;
+    }
+    // ---- keys: of some heads of a block ----
     unsigned item = blockIdx.x;
-    const int split = (int)(item % (unsigned)p.splits);
-    item /= (unsigned)p.splits;
+    const unsigned parts = ((unsigned)p.c.H + p.key_heads - 1) / p.key_heads;
+    const int part = (int)(item % parts);
+    item /= parts;
     const int nb = (int)(item % (unsigned)p.blocks), b = (int)(item / (unsigned)p.blocks);
-    const int len = max(p.t.lens[b], 0);
-    const int n = p.counts != nullptr ? min(max(p.counts[b], 0), p.S) : p.S;
-    // row r of the block is token 32 nb + r - len % 32 of the call; rows a .. zs - 1 are the call's, a .. z - 1 new tokens, 0 .. held - 1 there already
-    const int first = 32 * nb - (len & 31);
-    const int held = max(-first, 0), a = held, z = min(n - first, 32), zs = min(p.S - first, 32);
-    if (a >= zs) return;
+    const int len = max(p.t.lens[b], 0), first = 32 * nb - (len & 31), n = count_of(b);
+    const int held = max(-first, 0), a = held, z = min(n - first, 32), blk = (len >> 5) + nb, sub = blk & ((1 << p.c.lper) - 1);
+    if (a >= z) return;
+    const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
+    if (page < 0) return;
     const Columns c = columns_of(l, p.c.cols, p.r.R, INTER);
-
-    // ---- angles of rows a .. z - 1 ----
-    int *const depth = (int *)(smem + angle_bytes<ND>);
     if (p.parents != nullptr) {  // (at most 64 tokens)
         if (wave == 0) depth[lane] = __popcll(tree_ancestors(p.parents + b * p.parents_stride[0], p.parents_stride[1], n, lane)) - 1;
         __syncthreads();
@@ -57,70 +112,10 @@ __global__ __launch_bounds__(kRotatedThreads, 2) void paged_rotated_kernel(const
         to[4] = si;
     }
     __syncthreads();
-    auto turns_of = [&](int r) {
-        Turns t;
-        const f32x4 co = angles[(r * LPR + l) * 2], si = angles[(r * LPR + l) * 2 + 1];
-#pragma unroll
-        for (int i = 0; i < 4; i++) t.c[i] = co[i], t.s[i] = si[i];
-        return t;
-    };
-    const float share = 1.f / (float)p.c.cols;
-    auto row_done = [&](float (&f)[2][4], const float (&w)[2][4], bool norm, int r) __attribute__((always_inline)) {
-        if (norm) norm_row<LPR>(f, w, share, p.r.eps);
-        if (c.rot) rotate<INTER, false>(f, turns_of(r));
-    };
-
-    // ---- keys and values of a head each, then queries by QR rows ----
-    const int blk = (len >> 5) + nb, sub = blk & ((1 << p.c.lper) - 1);
-    const int page = a < z ? page_at(p.t, b, blk >> p.c.lper, p.c.pages) : -1;
-    const int kv = page >= 0 ? 2 * p.c.H : 0, rows = (zs - a) * p.Hq, per = T * p.steps;
-    const int items = kv + (rows + per - 1) / per;
-    float wq[2][4], wk[2][4];
-    weights_of(p.r.q_weight, p.r.weight_dtype, c, wq);
-    weights_of(p.r.k_weight, p.r.weight_dtype, c, wk);
-    for (int it = split * kCacheWaves + wave; it < items; it += p.splits * kCacheWaves) {
-        if (it >= kv) {
-            const int from = (it - kv) * per, to = min(from + per, rows);
-            const unsigned each = (unsigned)(zs - a);
-#pragma unroll 1
-            for (int at = from; at < to; at += T * U) {
-                typename X::T in[U][2] = {};
-                int r[U], h[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int row = min(at + u * T + r0, to - 1);
-                    h[u] = (int)((unsigned)row / each);
-                    r[u] = a + row - h[u] * (int)each;
-                    const uint16_t *const x = p.q + b * p.qs[0] + h[u] * p.qs[1] + (int64_t)(first + r[u]) * p.qs[2];
-                    if (c.live && at + u * T + r0 < to && r[u] < z) {
-                        in[u][0] = *(const typename X::T *)(x + c.at[0]);
-                        in[u][1] = *(const typename X::T *)(x + c.at[1]);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (at + u * T >= to) break;
-                    const bool live = r[u] < z;  // (rows of padding are 0)
-                    float f[2][4];
-                    X::floats(in[u][0], f[0]);
-                    X::floats(in[u][1], f[1]);
-                    row_done(f, wq, p.r.q_weight != nullptr, live ? r[u] : a);
-                    if (c.live && at + u * T + r0 < to) {
-                        uint16_t *const y = p.qo + b * p.qos[0] + h[u] * p.qos[1] + (int64_t)(first + r[u]) * p.qos[2];
-                        const typename X::T none = {0u, 0u};
-                        *(typename X::T *)(y + c.at[0]) = live ? X::rounded(f[0]) : none;
-                        *(typename X::T *)(y + c.at[1]) = live ? X::rounded(f[1]) : none;
-                    }
-                }
-            }
-            continue;
-        }
-        const int h = it >> 1;
-        if (it & 1) {
-            append_block<DT, ND>(p.c, p.v + b * p.vs[0] + h * p.vs[1] + (int64_t)first * p.vs[2], p.vs[2], true, page, h, sub, held, a, z, mine);
-            in_order();
-            continue;
-        }
+    float w[2][4];
+    weights_of(p.r.k_weight, p.r.weight_dtype, c, w);
+    const int h_end = min((part + 1) * p.key_heads, p.c.H);
+    for (int h = part * p.key_heads + wave; h < h_end; h += kCacheWaves) {
         // Rows come in groups of U steps and are made twice, for the largest finite magnitude and for the codes; where there is more than one
         // group they are read again from the caches.  (A block's rows kept in float32 were 128 registers at D = 256.)
         const uint16_t *const x = p.k + b * p.ks[0] + h * p.ks[1] + (int64_t)first * p.ks[2];
@@ -139,13 +134,20 @@ __global__ __launch_bounds__(kRotatedThreads, 2) void paged_rotated_kernel(const
             }
         };
         auto row = [&](int r, int u, float (&y)[2][4]) __attribute__((always_inline)) {
-            const bool live = r >= a && r < z;
+            const bool live = c.live && r >= a && r < z;
             X::floats(in[u][0], y[0]);
             X::floats(in[u][1], y[1]);
-            row_done(y, wk, p.r.k_weight != nullptr, live ? r : a);
+            if (p.r.k_weight != nullptr) norm_row<LPR>(y, w, share, p.r.eps);
+            if (c.rot) {
+                const f32x4 co = angles[((live ? r : a) * LPR + l) * 2], si = angles[((live ? r : a) * LPR + l) * 2 + 1];
+                Turns t;
+#pragma unroll
+                for (int i = 0; i < 4; i++) t.c[i] = co[i], t.s[i] = si[i];
+                rotate<INTER, false>(y, t);
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (!live || !c.live) y[j >> 2][j & 3] = 0.f;
+                if (!live) y[j >> 2][j & 3] = 0.f;
         };
         uint32_t m = 0u, all = 0u;
         load(g0);
@@ -211,35 +213,39 @@ __global__ __launch_bounds__(kRotatedThreads, 2) void paged_rotated_kernel(const
     }
 }
 
-template <int DT, int ND, bool INTER>
-hipError_t launch(const PagedRotatedParams &p, hipStream_t stream) {
-    constexpr int smem = angle_bytes<ND> + kCacheWaves * wave_bytes<ND>;
-    auto kern = paged_rotated_kernel<DT, ND, INTER>;
-    static unsigned long long attr_done = 0;
-    if (const hipError_t e = allow_dynamic_smem(kern, smem, attr_done); e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(p.splits * p.blocks * p.t.B)), dim3(kRotatedThreads), smem, stream, p);
-    return hipGetLastError();
-}
 template <int DT, bool INTER>
-hipError_t launch_dim(const PagedRotatedParams &p, hipStream_t stream) {
-    if (p.c.D == 64) return launch<DT, 2, INTER>(p, stream);
-    if (p.c.D == 128) return launch<DT, 4, INTER>(p, stream);
-    if (p.c.D == 256) return launch<DT, 8, INTER>(p, stream);
-    return hipErrorInvalidValue;
+hipError_t launch_dim(const PagedRotatedParams &p, int64_t groups, hipStream_t stream) {
+    const dim3 grid((unsigned)groups), block(kRotatedThreads);
+    if (p.c.D == 64) hipLaunchKernelGGL((paged_rotated_kernel<DT, 2, INTER>), grid, block, 0, stream, p);
+    else if (p.c.D == 128) hipLaunchKernelGGL((paged_rotated_kernel<DT, 4, INTER>), grid, block, 0, stream, p);
+    else if (p.c.D == 256) hipLaunchKernelGGL((paged_rotated_kernel<DT, 8, INTER>), grid, block, 0, stream, p);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
 }
 
 }  // namespace
 
-// Workgroups that share a block's heads: as many as give each compute unit three workgroups, with an item for every wave.
-int paged_rotated_splits(int B, int blocks, int H, int Hq, int S) {
-    const int64_t tiles = (int64_t)B * blocks, want = (768 + tiles - 1) / tiles;
-    const int64_t items = 2ll * H + (S == 1 ? (Hq + 3) / 4 : Hq), most = (items + kCacheWaves - 1) / kCacheWaves;
-    return (int)(want < most ? want : most);
+// Keys: a wave has one head of a block, or two where there are workgroups enough, as the angles are made for each workgroup.  Queries: heads are dealt out to as many waves
+// as fill the device, four at least to one.
+int64_t paged_rotated_plan(PagedRotatedParams &p) {
+    const int T = p.c.D == 64 ? 8 : p.c.D == 128 ? 4 : 2;
+    const int64_t tiles = (int64_t)p.t.B * p.blocks;
+    p.key_heads = tiles >= 512 ? 2 * kCacheWaves : kCacheWaves;
+    const int64_t keys = tiles * ((p.c.H + p.key_heads - 1) / p.key_heads), values = (tiles * p.c.H + kCacheWaves - 1) / kCacheWaves;
+    const int64_t groups = p.parents != nullptr ? (int64_t)p.t.B * ((p.S + T - 1) / T) : ((int64_t)p.t.B * p.S + T - 1) / T;
+    const int64_t want = (4096 + groups - 1) / groups, most = (p.Hq + 3) / 4;
+    p.splits = (int)std::min(want, most);
+    p.heads = (p.Hq + p.splits - 1) / p.splits;
+    const int64_t queries = (groups * p.splits + kCacheWaves - 1) / kCacheWaves, all = keys + values + queries;
+    if (all > 0x7fffffff || (int64_t)p.t.B * p.S > 0x7fffffff) return -1;
+    p.key_groups = (int)keys;
+    p.value_groups = (int)values;
+    return all;
 }
 
-hipError_t launch_paged_rotated(const PagedRotatedParams &p, int dtype, hipStream_t stream) {
-    if (dtype == 0) return p.r.interleaved ? launch_dim<0, true>(p, stream) : launch_dim<0, false>(p, stream);
-    if (dtype == 1) return p.r.interleaved ? launch_dim<1, true>(p, stream) : launch_dim<1, false>(p, stream);
+hipError_t launch_paged_rotated(const PagedRotatedParams &p, int64_t groups, int dtype, hipStream_t stream) {
+    if (dtype == 0) return p.r.interleaved ? launch_dim<0, true>(p, groups, stream) : launch_dim<0, false>(p, groups, stream);
+    if (dtype == 1) return p.r.interleaved ? launch_dim<1, true>(p, groups, stream) : launch_dim<1, false>(p, groups, stream);
     return hipErrorInvalidValue;
 }
 

@@ -150,5 +150,37 @@ __device__ __forceinline__ double position_at(const Rotation &r, int axis, int64
 }
 __device__ __forceinline__ int axis_of(const Rotation &r, int j) { return r.axes != nullptr ? min(max(r.axes[j], 0), r.num_axes - 1) : 0; }
 
+// Heads a .. z - 1 of the tokens at x (and y, where they go): of each `heads` elements apart the lane's columns, normed if there is a weight, and turned.  live: the lane
+// has columns of a token; its rows are read, or are 0 where `zero`.
+template <int DT, int LPR, bool INTER>
+__device__ __forceinline__ void rotate_rows(const RowElem<DT> *x, RowElem<DT> *y, int64_t x_head, int64_t y_head, int a, int z, const Columns &c, bool live, bool zero,
+                                            const Turns &t, const void *weight, const float (&w)[2][4], float share, float eps) {
+    using X = Run4<DT>;
+    constexpr int U = 4;  // heads under way
+    for (int h = a; h < z; h += U) {
+        typename X::T in[U][2] = {};
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (h + u < z && live && !zero) {
+                in[u][0] = *(const typename X::T *)(x + (h + u) * x_head + c.at[0]);
+                in[u][1] = *(const typename X::T *)(x + (h + u) * x_head + c.at[1]);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (h + u >= z) break;
+            float f[2][4];
+            X::floats(in[u][0], f[0]);
+            X::floats(in[u][1], f[1]);
+            if (weight != nullptr) norm_row<LPR>(f, w, share, eps);
+            if (c.rot) rotate<INTER, false>(f, t);
+            if (live) {
+                const typename X::T none = {};
+                *(typename X::T *)(y + (h + u) * y_head + c.at[0]) = zero ? none : X::rounded(f[0]);
+                *(typename X::T *)(y + (h + u) * y_head + c.at[1]) = zero ? none : X::rounded(f[1]);
+            }
+        }
+    }
+}
+
 }  // namespace
 }  // namespace sa

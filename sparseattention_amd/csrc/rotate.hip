@@ -42,7 +42,6 @@ struct WaveRows {
 template <int DT, int LPR, bool INTER>
 __global__ __launch_bounds__(64 * kRotateWaves) void rotate_kernel(const RotateParams p) {
     using E = RowElem<DT>;
-    using X = Run4<DT>;
     const int id = blockIdx.x * kRotateWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = id / p.splits, h0 = (id - group * p.splits) * p.heads, h1 = min(h0 + p.heads, p.q.H + p.k.H);
     if (h0 >= h1 || (int64_t)group * WaveRows<DT, LPR>::T >= (int64_t)p.B * p.S) return;
@@ -52,31 +51,8 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_kernel(const RotateP
     weights_of(p.r.k_weight, p.r.weight_dtype, w.c, wk);
     const float share = 1.f / (float)p.D;
     auto rows = [&](const RotateRows &r, const void *weight, const float (&ww)[2][4], int a, int z) __attribute__((always_inline)) {
-        const E *const x = (const E *)r.x + w.b * r.xs[0] + w.s * r.xs[2];
-        E *const y = (E *)r.y + w.b * r.ys[0] + w.s * r.ys[2];
-        constexpr int U = 4;  // heads under way
-        for (int h = a; h < z; h += U) {
-            typename X::T in[U][2] = {};
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (h + u < z && w.live) {
-                    in[u][0] = *(const typename X::T *)(x + (h + u) * r.xs[1] + w.c.at[0]);
-                    in[u][1] = *(const typename X::T *)(x + (h + u) * r.xs[1] + w.c.at[1]);
-                }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (h + u >= z) break;
-                float f[2][4];
-                X::floats(in[u][0], f[0]);
-                X::floats(in[u][1], f[1]);
-                if (weight != nullptr) norm_row<LPR>(f, ww, share, p.r.eps);
-                if (w.c.rot) rotate<INTER, false>(f, w.t);
-                if (w.live) {
-                    *(typename X::T *)(y + (h + u) * r.ys[1] + w.c.at[0]) = X::rounded(f[0]);
-                    *(typename X::T *)(y + (h + u) * r.ys[1] + w.c.at[1]) = X::rounded(f[1]);
-                }
-            }
-        }
+        rotate_rows<DT, LPR, INTER>((const E *)r.x + w.b * r.xs[0] + w.s * r.xs[2], (E *)r.y + w.b * r.ys[0] + w.s * r.ys[2], r.xs[1], r.ys[1], a, z, w.c, w.live, false, w.t, weight,
+                                    ww, share, p.r.eps);
     };
     if (h0 < p.q.H) rows(p.q, p.r.q_weight, wq, h0, min(h1, p.q.H));
     if (h1 > p.q.H) rows(p.k, p.r.k_weight, wk, max(h0 - p.q.H, 0), h1 - p.q.H);
