@@ -66,8 +66,8 @@ __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotate
         }
         float w[2][4];
         weights_of(p.r.q_weight, p.r.weight_dtype, c, w);
-        rotate_rows<DT, LPR, INTER>(p.q + b * p.qs[0] + s * p.qs[2], p.qo + b * p.qos[0] + s * p.qos[2], p.qs[1], p.qos[1], h0, h1, c, live, zero, t, p.r.q_weight, w, share,
-                                    p.r.eps);
+        rotate_rows<DT, LPR, INTER, false>(p.q + b * p.qs[0] + s * p.qs[2], p.qo + b * p.qos[0] + s * p.qos[2], p.qs[1], p.qos[1], h0, h1, c, live, zero, t, p.r.q_weight, w, share,
+                                           p.r.eps);
         return;
     }
     if (blockIdx.x >= (unsigned)p.key_groups) {
@@ -128,9 +128,8 @@ __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotate
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int r = (g * U + u) * T + r0;
-                const bool there = c.live && r >= a && r < z;
-#pragma unroll
-                for (int k = 0; k < 2; k++) in[u][k] = there ? *(const typename X::T *)(x + r * p.ks[2] + c.at[k]) : typename X::T{0u, 0u};
+                in[u][0] = in[u][1] = typename X::T{0u, 0u};
+                if (c.live && r >= a && r < z) load_runs<DT, INTER>(x + r * p.ks[2], c, in[u]);
             }
         };
         auto row = [&](int r, int u, float (&y)[2][4]) __attribute__((always_inline)) {

@@ -71,6 +71,35 @@ __device__ __forceinline__ Columns columns_of(int l, int D, int R, bool interlea
     return c;
 }
 
+// A lane's two runs from and to memory: where they lie behind one another, 16 bits wide, in one piece.
+template <int DT, bool INTER>
+__device__ __forceinline__ void load_runs(const RowElem<DT> *x, const Columns &c, typename Run4<DT>::T (&in)[2]) {
+    if constexpr (INTER && DT != 2) {
+        const u32x4 w = *(const u32x4 *)(x + c.at[0]);
+        in[0] = u32x2{w.x, w.y};
+        in[1] = u32x2{w.z, w.w};
+    } else {
+        in[0] = *(const typename Run4<DT>::T *)(x + c.at[0]);
+        in[1] = *(const typename Run4<DT>::T *)(x + c.at[1]);
+    }
+}
+// FAR: past the caches (a number of the kernel: of a choice at run time the compiler makes one store through them).
+template <int DT, bool INTER, bool FAR>
+__device__ __forceinline__ void store_runs(RowElem<DT> *y, const Columns &c, const typename Run4<DT>::T &a, const typename Run4<DT>::T &b) {
+    typedef typename Run4<DT>::T T;
+    if constexpr (INTER && DT != 2) {
+        const u32x4 w = {a.x, a.y, b.x, b.y};
+        if constexpr (FAR) __builtin_nontemporal_store(w, (u32x4 *)(y + c.at[0]));
+        else *(u32x4 *)(y + c.at[0]) = w;
+    } else if constexpr (FAR) {
+        __builtin_nontemporal_store(a, (T *)(y + c.at[0]));
+        __builtin_nontemporal_store(b, (T *)(y + c.at[1]));
+    } else {
+        *(T *)(y + c.at[0]) = a;
+        *(T *)(y + c.at[1]) = b;
+    }
+}
+
 // The sum over the LPR lanes of a row, in all of them.
 template <int LPR>
 __device__ __forceinline__ float row_total(float x) {
@@ -152,7 +181,7 @@ __device__ __forceinline__ int axis_of(const Rotation &r, int j) { return r.axes
 
 // Heads a .. z - 1 of the tokens at x (and y, where they go): of each `heads` elements apart the lane's columns, normed if there is a weight, and turned.  live: the lane
 // has columns of a token; its rows are read, or are 0 where `zero`.
-template <int DT, int LPR, bool INTER>
+template <int DT, int LPR, bool INTER, bool FAR>
 __device__ __forceinline__ void rotate_rows(const RowElem<DT> *x, RowElem<DT> *y, int64_t x_head, int64_t y_head, int a, int z, const Columns &c, bool live, bool zero,
                                             const Turns &t, const void *weight, const float (&w)[2][4], float share, float eps) {
     using X = Run4<DT>;
@@ -161,10 +190,7 @@ __device__ __forceinline__ void rotate_rows(const RowElem<DT> *x, RowElem<DT> *y
         typename X::T in[U][2] = {};
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (h + u < z && live && !zero) {
-                in[u][0] = *(const typename X::T *)(x + (h + u) * x_head + c.at[0]);
-                in[u][1] = *(const typename X::T *)(x + (h + u) * x_head + c.at[1]);
-            }
+            if (h + u < z && live && !zero) load_runs<DT, INTER>(x + (h + u) * x_head, c, in[u]);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (h + u >= z) break;
@@ -175,8 +201,7 @@ __device__ __forceinline__ void rotate_rows(const RowElem<DT> *x, RowElem<DT> *y
             if (c.rot) rotate<INTER, false>(f, t);
             if (live) {
                 const typename X::T none = {};
-                *(typename X::T *)(y + (h + u) * y_head + c.at[0]) = zero ? none : X::rounded(f[0]);
-                *(typename X::T *)(y + (h + u) * y_head + c.at[1]) = zero ? none : X::rounded(f[1]);
+                store_runs<DT, INTER, FAR>(y + (h + u) * y_head, c, zero ? none : X::rounded(f[0]), zero ? none : X::rounded(f[1]));
             }
         }
     }

@@ -39,7 +39,7 @@ struct WaveRows {
     }
 };
 
-template <int DT, int LPR, bool INTER>
+template <int DT, int LPR, bool INTER, bool FAR>
 __global__ __launch_bounds__(64 * kRotateWaves) void rotate_kernel(const RotateParams p) {
     using E = RowElem<DT>;
     const int id = blockIdx.x * kRotateWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -51,14 +51,14 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_kernel(const RotateP
     weights_of(p.r.k_weight, p.r.weight_dtype, w.c, wk);
     const float share = 1.f / (float)p.D;
     auto rows = [&](const RotateRows &r, const void *weight, const float (&ww)[2][4], int a, int z) __attribute__((always_inline)) {
-        rotate_rows<DT, LPR, INTER>((const E *)r.x + w.b * r.xs[0] + w.s * r.xs[2], (E *)r.y + w.b * r.ys[0] + w.s * r.ys[2], r.xs[1], r.ys[1], a, z, w.c, w.live, false, w.t, weight,
+        rotate_rows<DT, LPR, INTER, FAR>((const E *)r.x + w.b * r.xs[0] + w.s * r.xs[2], (E *)r.y + w.b * r.ys[0] + w.s * r.ys[2], r.xs[1], r.ys[1], a, z, w.c, w.live, false, w.t, weight,
                                     ww, share, p.r.eps);
     };
     if (h0 < p.q.H) rows(p.q, p.r.q_weight, wq, h0, min(h1, p.q.H));
     if (h1 > p.q.H) rows(p.k, p.r.k_weight, wk, max(h0 - p.q.H, 0), h1 - p.q.H);
 }
 
-template <int DT, int LPR, bool INTER>
+template <int DT, int LPR, bool INTER, bool FAR>
 __global__ __launch_bounds__(64 * kRotateWaves) void rotate_backward_kernel(const RotateParams p) {
     using E = RowElem<DT>;
     using X = Run4<DT>;
@@ -86,11 +86,8 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_backward_kernel(cons
 #pragma unroll
                 for (int u = 0; u < U; u++)
                     if (h + u < z && w.live) {
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            up[u][k] = *(const typename X::T *)(dy + (h + u) * r.dys[1] + c.at[k]);
-                            if (weight != nullptr) in[u][k] = *(const typename X::T *)(x + (h + u) * r.xs[1] + c.at[k]);
-                        }
+                        load_runs<DT, INTER>(dy + (h + u) * r.dys[1], c, up[u]);
+                        if (weight != nullptr) load_runs<DT, INTER>(x + (h + u) * r.xs[1], c, in[u]);
                     }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
@@ -115,10 +112,7 @@ __global__ __launch_bounds__(64 * kRotateWaves) void rotate_backward_kernel(cons
                             g[i >> 2][i & 3] = n * (ww[i >> 2][i & 3] * gi - xi * m);
                         }
                     }
-                    if (w.live) {
-                        *(typename X::T *)(dx + (h + u) * r.ys[1] + c.at[0]) = X::rounded(g[0]);
-                        *(typename X::T *)(dx + (h + u) * r.ys[1] + c.at[1]) = X::rounded(g[1]);
-                    }
+                    if (w.live) store_runs<DT, INTER, FAR>(dx + (h + u) * r.ys[1], c, X::rounded(g[0]), X::rounded(g[1]));
                 }
             }
         };
@@ -173,6 +167,10 @@ __global__ __launch_bounds__(kWeightThreads) void rotate_weights_kernel(const Ro
     else ((__bf16 *)out)[col] = (__bf16)(float)x;
 }
 
+// Outputs of that many bytes go past the caches, which would not hold them for who reads them next (336 MB read and 168 MB written by the backward, 168 and 168 by the
+// forward: 188 us through them, 165 past them).
+constexpr int64_t kRotateFar = 128ll << 20;
+
 // Heads are dealt out to as many waves as fill the device, four at least to one, as the angles of its tokens are made once for all of them.
 void share_heads(RotateParams &p) {
     const int T = p.D <= 64 ? 8 : p.D <= 128 ? 4 : 2, heads = p.q.H + p.k.H;
@@ -183,8 +181,11 @@ void share_heads(RotateParams &p) {
 }
 
 template <class F>
-hipError_t with_rows(int dtype, int D, bool interleaved, F &&f) {
-    auto pairs = [&](auto dt, auto lpr) { return interleaved ? f(dt, lpr, std::true_type{}) : f(dt, lpr, std::false_type{}); };
+hipError_t with_rows(const RotateParams &p, int dtype, F &&f) {
+    const int D = p.D;
+    const bool far = (int64_t)p.B * p.S * (p.q.H + p.k.H) * D * (dtype == 2 ? 4 : 2) >= kRotateFar;
+    auto stores = [&](auto dt, auto lpr, auto inter) { return far ? f(dt, lpr, inter, std::true_type{}) : f(dt, lpr, inter, std::false_type{}); };
+    auto pairs = [&](auto dt, auto lpr) { return p.r.interleaved ? stores(dt, lpr, std::true_type{}) : stores(dt, lpr, std::false_type{}); };
     auto lanes = [&](auto dt) {
         if (D <= 64) return pairs(dt, std::integral_constant<int, 8>{});
         if (D <= 128) return pairs(dt, std::integral_constant<int, 16>{});
@@ -199,10 +200,10 @@ hipError_t with_rows(int dtype, int D, bool interleaved, F &&f) {
 
 hipError_t launch_rotate(RotateParams p, int dtype, hipStream_t stream) {
     share_heads(p);
-    return with_rows(dtype, p.D, p.r.interleaved, [&](auto dt, auto lpr, auto inter) {
+    return with_rows(p, dtype, [&](auto dt, auto lpr, auto inter, auto past) {
         constexpr int T = 64 / decltype(lpr)::value;
         const int64_t waves = ((int64_t)p.B * p.S + T - 1) / T * p.splits;
-        hipLaunchKernelGGL((rotate_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value>), dim3((unsigned)((waves + kRotateWaves - 1) / kRotateWaves)), dim3(64 * kRotateWaves), 0, stream, p);
+        hipLaunchKernelGGL((rotate_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value, decltype(past)::value>), dim3((unsigned)((waves + kRotateWaves - 1) / kRotateWaves)), dim3(64 * kRotateWaves), 0, stream, p);
         return hipGetLastError();
     });
 }
@@ -219,8 +220,8 @@ int rotate_backward_groups(int B, int S, int heads, int D) {
 hipError_t launch_rotate_backward(RotateParams p, int dtype, hipStream_t stream) {
     share_heads(p);
     p.groups = rotate_backward_groups(p.B, p.S, p.q.H + p.k.H, p.D);
-    const hipError_t e = with_rows(dtype, p.D, p.r.interleaved, [&](auto dt, auto lpr, auto inter) {
-        hipLaunchKernelGGL((rotate_backward_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value>), dim3((unsigned)p.groups), dim3(64 * kRotateWaves), 0, stream, p);
+    const hipError_t e = with_rows(p, dtype, [&](auto dt, auto lpr, auto inter, auto past) {
+        hipLaunchKernelGGL((rotate_backward_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value, decltype(past)::value>), dim3((unsigned)p.groups), dim3(64 * kRotateWaves), 0, stream, p);
         return hipGetLastError();
     });
     if (e != hipSuccess || p.parts == nullptr) return e;

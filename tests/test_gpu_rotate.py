@@ -277,3 +277,21 @@ def test_repeatable(gpu):
     first = sa.rotate_heads_backward(q, k, q, k, at, r, qw, kw)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(sa.rotate_heads_backward(q, k, q, k, at, r, qw, kw), first))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_large_outputs(gpu, interleaved):
+    """Outputs that go past the caches are, to the bit, those of parts of them that do not."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    B, S, H, D = 4, 2049, 64, 128
+    q = torch.randn(B, S, H + 8, D, generator=g, device="cuda").bfloat16().transpose(1, 2)
+    q, k = q[:, :H], q[:, H:]
+    qw, kw = weights(g, D, torch.bfloat16)
+    r, at = sa.rotary_frequencies(D, interleaved=interleaved), torch.arange(S, device="cuda")
+    ups = [torch.randn(x.shape, generator=g, device="cuda").bfloat16() for x in (q, k)]
+    whole = (*sa.rotate_heads(q, k, at, r, qw, kw), *sa.rotate_heads_backward(*ups, q, k, at, r, qw, kw)[:2])
+    parts = [(*sa.rotate_heads(q[b:b + 1], k[b:b + 1], at, r, qw, kw), *sa.rotate_heads_backward(ups[0][b:b + 1], ups[1][b:b + 1], q[b:b + 1], k[b:b + 1], at, r, qw, kw)[:2])
+             for b in range(B)]
+    assert (q.numel() + k.numel()) * 2 >= 128 << 20 > (q.numel() + k.numel()) // 2
+    for a, b in zip(whole, zip(*parts)):
+        assert torch.equal(a, torch.cat(b))
