@@ -2,9 +2,9 @@
 // counterpart in the reference.  The formula of a row is rotate.h's, a block's and its scale's paged_cache.hip's; keys go from float32 to codes in
 // one rounding, queries to their own type.
 //
-// One launch, whose workgroups have one of three things to do: keys of a block of a sequence, 32 tokens or fewer, a wave a head at a time, with the angles made once in LDS;
-// values of blocks, a wave each, as paged_append_kernel stores them; or queries, a wave 64 / LPR tokens with their angles in registers, as
-// rotate_kernel has them.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.
+// One launch, whose workgroups have one of three things to do: keys of a block of a sequence, 32 tokens or fewer, 8 a wave, head by head with the angles in registers; values of
+// blocks, a wave each, as paged_append_kernel stores them; or queries, a wave 64 / LPR tokens with their angles in registers, as rotate_kernel has
+// them.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.
 #include <algorithm>
 
 #include "paged_codes.h"
@@ -19,13 +19,11 @@ constexpr int kRotatedThreads = 64 * kCacheWaves;
 template <int DT, int ND, bool INTER>
 __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotated_kernel(const PagedRotatedParams p) {
     using X = Run4<DT>;
-    constexpr int LPR = 4 * ND, T = 64 / LPR, U = 4;  // lanes of a row, rows of a step, steps under way
-    constexpr int kRows = 16 * row_bytes<ND>, kCodes = ND * 1024, kWave = kCodes > kRows ? kCodes : kRows;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[kCacheWaves * kWave];
-    __shared__ f32x4 angles[32 * LPR * 2];  // of row r, four pairs l: [(r * LPR + l) * 2], cosines and sines
-    __shared__ int depth[64];
+    constexpr int LPR = 4 * ND, T = 64 / LPR;  // lanes of a row, rows of a step
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kCacheWaves * 16 * row_bytes<ND>];  // (values: 16 rows of each wave; keys: a block)
+    __shared__ u32x2 sizes[kCacheWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane % LPR, r0 = lane / LPR;
-    uint8_t *const mine = smem + wave * kWave;
+    uint8_t *const mine = smem + wave * 16 * row_bytes<ND>;
     const float share = 1.f / (float)p.c.cols;
     const auto count_of = [&](int b) { return p.counts != nullptr ? min(max(p.counts[b], 0), p.S) : p.S; };
 
@@ -84,7 +82,8 @@ __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotate
         append_block<DT, ND>(p.c, p.v + b * p.vs[0] + h * p.vs[1] + (int64_t)first * p.vs[2], p.vs[2], true, page, h, blk & ((1 << p.c.lper) - 1), held, held, z, mine);
         return;
     }
-    // ---- keys: of some heads of a block ----
+    // ---- keys: some heads of a block, whose rows lie in the registers of four waves, 8 each, from their loads to their codes ----
+    constexpr int STEPS = 8 / T;
     unsigned item = blockIdx.x;
     const unsigned parts = ((unsigned)p.c.H + p.key_heads - 1) / p.key_heads;
     const int part = (int)(item % parts);
@@ -96,111 +95,104 @@ __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotate
     const int page = page_at(p.t, b, blk >> p.c.lper, p.c.pages);
     if (page < 0) return;
     const Columns c = columns_of(l, p.c.cols, p.r.R, INTER);
-    if (p.parents != nullptr) {  // (at most 64 tokens)
-        if (wave == 0) depth[lane] = __popcll(tree_ancestors(p.parents + b * p.parents_stride[0], p.parents_stride[1], n, lane)) - 1;
-        __syncthreads();
+    const int h0 = part * p.key_heads, h_end = min(h0 + p.key_heads, p.c.H), row0 = 8 * wave + r0;  // the lane's rows are row0 + T i
+    const uint16_t *x = p.k + b * p.ks[0] + h0 * p.ks[1] + (int64_t)(first + row0) * p.ks[2];
+    auto is_new = [&](int i) { return row0 + T * i >= a && row0 + T * i < z; };
+    typename X::T in[STEPS][2];
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            in[i][0] = in[i][1] = typename X::T{0u, 0u};
+            if (c.live && is_new(i)) load_runs<DT, INTER>(x + (T * i) * p.ks[2], c, in[i]);
+        }
+    };
+    load();
+    int64_t at = block_at(p.c, page, h0, sub);
+    int e_old = held > 0 ? exp_of_scale(p.c.k_scales[at]) : kScaleExpMin;
+    uint64_t above = 0ull;
+    if (p.parents != nullptr) above = tree_ancestors(p.parents + b * p.parents_stride[0], p.parents_stride[1], n, lane);
+    Turns t[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const int token = first + row0 + T * i;
+        double position = (double)len + token;
+        if (p.parents != nullptr) position = (double)len + __popcll(__shfl((unsigned long long)above, token & 63)) - 1;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            t[i].c[j] = 1.f, t[i].s[j] = 0.f;
+            if (c.rot && is_new(i)) {
+                if (p.r.positions != nullptr) position = position_at(p.r, axis_of(p.r, 4 * l + j), b, token);
+                turn(position, p.r.frequencies[4 * l + j], t[i].c[j], t[i].s[j]);
+            }
+        }
     }
-    for (int i = threadIdx.x; i < (z - a) * (p.r.R / 2); i += kRotatedThreads) {
-        const int r = a + i / (p.r.R / 2), j = i - (r - a) * (p.r.R / 2), token = first + r;
-        double at;
-        if (p.r.positions != nullptr) at = position_at(p.r, axis_of(p.r, j), b, token);
-        else at = (double)len + (p.parents != nullptr ? depth[token] : token);
-        float co, si;
-        turn(at, p.r.frequencies[j], co, si);
-        float *const to = (float *)(angles + (r * LPR + (j >> 2)) * 2) + (j & 3);
-        to[0] = co;
-        to[4] = si;
-    }
-    __syncthreads();
     float w[2][4];
     weights_of(p.r.k_weight, p.r.weight_dtype, c, w);
-    const int h_end = min((part + 1) * p.key_heads, p.c.H);
-    for (int h = part * p.key_heads + wave; h < h_end; h += kCacheWaves) {
-        // Rows come in groups of U steps and are made twice, for the largest finite magnitude and for the codes; where there is more than one
-        // group they are read again from the caches.  (A block's rows kept in float32 were 128 registers at D = 256.)
-        const uint16_t *const x = p.k + b * p.ks[0] + h * p.ks[1] + (int64_t)first * p.ks[2];
-        const int64_t at = block_at(p.c, page, h, sub);
+#pragma unroll 1
+    for (int h = h0; h < h_end; h++) {
+        float y[STEPS][2][4];
+        uint32_t m = 0u, all = 0u;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            X::floats(in[i][0], y[i][0]);
+            X::floats(in[i][1], y[i][1]);
+            if (p.r.k_weight != nullptr) norm_row<LPR>(y[i], w, share, p.r.eps);
+            if (c.rot) rotate<INTER, false>(y[i], t[i]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float &f = y[i][j >> 2][j & 3];
+                if (!c.live || !is_new(i)) f = 0.f;
+                const uint32_t size = __float_as_uint(f) & 0x7fffffffu;
+                all = max(all, size);
+                m = max(m, size < 0x7f800000u ? size : 0u);
+            }
+        }
         uint8_t *const out = p.c.k + at * (ND * 1024);
         float *const scale = p.c.k_scales + at;
-        const int g0 = a / (T * U), g1 = (z - 1) / (T * U);
-        typename X::T in[U][2];
-        auto load = [&](int g) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int r = (g * U + u) * T + r0;
-                in[u][0] = in[u][1] = typename X::T{0u, 0u};
-                if (c.live && r >= a && r < z) load_runs<DT, INTER>(x + r * p.ks[2], c, in[u]);
-            }
-        };
-        auto row = [&](int r, int u, float (&y)[2][4]) __attribute__((always_inline)) {
-            const bool live = c.live && r >= a && r < z;
-            X::floats(in[u][0], y[0]);
-            X::floats(in[u][1], y[1]);
-            if (p.r.k_weight != nullptr) norm_row<LPR>(y, w, share, p.r.eps);
-            if (c.rot) {
-                const f32x4 co = angles[((live ? r : a) * LPR + l) * 2], si = angles[((live ? r : a) * LPR + l) * 2 + 1];
-                Turns t;
-#pragma unroll
-                for (int i = 0; i < 4; i++) t.c[i] = co[i], t.s[i] = si[i];
-                rotate<INTER, false>(y, t);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (!live) y[j >> 2][j & 3] = 0.f;
-        };
-        uint32_t m = 0u, all = 0u;
-        load(g0);
-        const int e_old = held > 0 ? exp_of_scale(*scale) : kScaleExpMin;
-#pragma unroll 1
-        for (int g = g0;; load(++g)) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float y[2][4];
-                row((g * U + u) * T + r0, u, y);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint32_t size = __float_as_uint(y[j >> 2][j & 3]) & 0x7fffffffu;
-                    all = max(all, size);
-                    m = max(m, size < 0x7f800000u ? size : 0u);
-                }
-            }
-            if (g == g1) break;
+        const int e_was = e_old;
+        if (h + 1 < h_end) {  // (the next head's rows and scale, on their way meanwhile)
+            x += p.ks[1];
+            load();
+            at += (int64_t)1 << p.c.lper;
+            if (held > 0) e_old = exp_of_scale(p.c.k_scales[at]);
         }
         m = wave_max(m);
         all = wave_max(all);
-        const int e = max(e_old, scale_exp(__uint_as_float(m)));
+        if (lane == 0) sizes[wave] = u32x2{m, all};
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kCacheWaves; i++) {
+            const u32x2 other = sizes[i];
+            m = max(m, other.x);
+            all = max(all, other.y);
+        }
+        const int e = max(e_was, scale_exp(__uint_as_float(m)));
         const float inv = exp2i(-e);
         const bool plain = all < 0x7f800000u && e < kScaleExpMax;
-        const bool grows = held > 0 && e > e_old;
-        const float f = exp2i(max(e_old - e, -126));
-        if (lane == 0 && (grows || held == 0)) *scale = exp2i(e);
+        const bool grows = held > 0 && e > e_was;
+        const float f = exp2i(max(e_was - e, -126));
+        if (threadIdx.x == 0 && (grows || held == 0)) *scale = exp2i(e);
         // codes into LDS, four columns of a row a word, where the block has them
-#pragma unroll 1
-        for (int g = g1; g >= g0; g--) {
-            if (g != g1) load(g);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int r = (g * U + u) * T + r0;
-                float y[2][4];
-                row(r, u, y);
+        for (int i = 0; i < STEPS; i++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const float(&v)[4] = y[k];
-                    const int col = c.at[k];
-                    *(uint32_t *)(mine + 1024 * (col >> 5) + 16 * (32 * ((col >> 4) & 1) + r) + (col & 15)) =
-                        plain ? codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv)
-                              : codes4(scaled(v[0], inv), scaled(v[1], inv), scaled(v[2], inv), scaled(v[3], inv));
-                }
+            for (int k = 0; k < 2; k++) {
+                const float(&v)[4] = y[i][k];
+                const int col = c.at[k];
+                *(uint32_t *)(smem + 1024 * (col >> 5) + 16 * (32 * ((col >> 4) & 1) + row0 + T * i) + (col & 15)) =
+                    plain ? codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv)
+                          : codes4(scaled(v[0], inv), scaled(v[1], inv), scaled(v[2], inv), scaled(v[3], inv));
             }
-        }
-        in_order();
+        __syncthreads();
         const int key = lane & 31;
         const bool fresh = key >= a && key < z, old = grows && key < held;
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            u32x4 *const to = (u32x4 *)(out + 1024 * d + 16 * lane);
+        for (int d = 0; d < ND; d += kCacheWaves) {
+            if (ND < kCacheWaves && wave >= ND) break;
+            const int piece = 1024 * (d + wave) + 16 * lane;
+            u32x4 *const to = (u32x4 *)(out + piece);
             if (fresh) {
-                *to = *(const u32x4 *)(mine + 1024 * d + 16 * lane);
+                *to = *(const u32x4 *)(smem + piece);
             } else if (old) {
                 u32x4 u = *to;
 #pragma unroll
@@ -208,7 +200,7 @@ __global__ __launch_bounds__(kRotatedThreads, ND == 8 ? 2 : 4) void paged_rotate
                 *to = u;
             }
         }
-        in_order();
+        __syncthreads();
     }
 }
 
@@ -224,12 +216,12 @@ hipError_t launch_dim(const PagedRotatedParams &p, int64_t groups, hipStream_t s
 
 }  // namespace
 
-// Keys: a wave has one head of a block, or two where there are workgroups enough, as the angles are made for each workgroup.  Queries: heads are dealt out to as many waves
-// as fill the device, four at least to one.
+// Keys: the angles are made for each workgroup, which has as many heads of its block as leave about 1024 workgroups.  Queries: heads are dealt out to as many waves as fill the
+// device, four at least to one.
 int64_t paged_rotated_plan(PagedRotatedParams &p) {
     const int T = p.c.D == 64 ? 8 : p.c.D == 128 ? 4 : 2;
     const int64_t tiles = (int64_t)p.t.B * p.blocks;
-    p.key_heads = tiles >= 512 ? 2 * kCacheWaves : kCacheWaves;
+    p.key_heads = (int)std::min<int64_t>(p.c.H, std::max<int64_t>(1, tiles * p.c.H / 1024));
     const int64_t keys = tiles * ((p.c.H + p.key_heads - 1) / p.key_heads), values = (tiles * p.c.H + kCacheWaves - 1) / kCacheWaves;
     const int64_t groups = p.parents != nullptr ? (int64_t)p.t.B * ((p.S + T - 1) / T) : ((int64_t)p.t.B * p.S + T - 1) / T;
     const int64_t want = (4096 + groups - 1) / groups, most = (p.Hq + 3) / 4;
