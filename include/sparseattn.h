@@ -692,7 +692,7 @@ int sa_sparse_attention_decode_tree(const void *q, const int64_t q_strides[4], c
  *   counts        device int32 [B], nodes of each tree, or NULL: n.  Without nodes nothing is accepted and the next token is -1.
  *   path          device int32 [B,n], contiguous: the accepted nodes, 0 first, -1 behind; accepted int32 [B]: how many
  *   next_token    device [B], of the tokens' type: the token behind the last accepted one (-1: p has none)
- * workspace: sa_verify_drafts_workspace_bytes(B, n, V) bytes, 8-byte aligned; holds nothing between calls.
+ * workspace: sa_verify_drafts_workspace_bytes(B, n, V) bytes, 16-byte aligned; holds nothing between calls.
  */
 size_t sa_verify_drafts_workspace_bytes(int B, int n, int V);
 int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], const void *draft_probs, const int64_t draft_strides[3],

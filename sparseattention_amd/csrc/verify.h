@@ -22,7 +22,7 @@ struct VerifyParams {
     int32_t *path, *accepted;  // [B, n], [B]
     void *next;                // [B], of the tokens' type
     int parts, each;           // workgroups of a row, and its values for each
-    double *sums;              // [B, parts]
+    double *sums;              // [B, parts, 4]
     uint64_t *arrivals;        // [B, parts] words (all_arrived)
     uint64_t tag;
 };

@@ -18,7 +18,9 @@
 namespace sa {
 namespace {
 
-constexpr int kVerifyThreads = 256;
+constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64;
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 constexpr int kVerifyStep = 4 * kVerifyThreads;
 
 // A probability; what is none counts as 0.
@@ -139,12 +141,23 @@ __device__ __forceinline__ Walk walk(const VerifyParams &p, int b, int lane, boo
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyParams p) {
     __shared__ uint32_t without[kVerifyMostEach / 32];  // the rejected tokens of a part, a bit each
-    __shared__ double sums[kVerifyThreads / 64];
-    __shared__ int shared[4];
+    __shared__ f64x4 quarters;
+    __shared__ double ends[kVerifyWaves];
+    __shared__ uint64_t rejected_by;
+    __shared__ float u0_by;
+    __shared__ int node_by, last_by, first_by, end_by;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = (int)(blockIdx.x / (unsigned)p.parts), part = (int)(blockIdx.x - (unsigned)b * p.parts);
-    const Walk w = walk<DT>(p, b, lane, part == 0 && wave == 0);
-    if (w.node < 0) {
+    int64_t token_of_lane = -1;  // (of the first wave)
+    if (wave == 0) {
+        const Walk w = walk<DT>(p, b, lane, part == 0);
+        token_of_lane = w.token;
+        if (lane == 0) node_by = w.node, rejected_by = w.rejected, u0_by = w.u0;
+    }
+    __syncthreads();
+    const int node = __builtin_amdgcn_readfirstlane(node_by);
+    const uint64_t rejected = rejected_by;
+    if (node < 0) {
         if (part == 0 && tid == 0) {
             if (p.tokens_64) ((int64_t *)p.next)[b] = -1;
             else ((int32_t *)p.next)[b] = -1;
@@ -152,22 +165,22 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyPara
         return;
     }
     const int64_t size = DT == 2 ? 4 : 2;
-    const void *const row = (const uint8_t *)p.target + size * (b * p.target_s[0] + w.node * p.target_s[1]);
-    const void *const drawn = p.draft != nullptr && w.rejected != 0ull ? (const uint8_t *)p.draft + size * (b * p.draft_s[0] + w.node * p.draft_s[1]) : nullptr;
-    const bool some_without = p.draft == nullptr && w.rejected != 0ull;
+    const void *const row = (const uint8_t *)p.target + size * (b * p.target_s[0] + node * p.target_s[1]);
+    const void *const drawn = p.draft != nullptr && rejected != 0ull ? (const uint8_t *)p.draft + size * (b * p.draft_s[0] + node * p.draft_s[1]) : nullptr;
+    const bool some_without = p.draft == nullptr && rejected != 0ull;
+    const int quarter = p.each / kVerifyWaves;
 
     bool plain = false;  // r = p, where nothing is left of it otherwise
     auto mark = [&](int from) {  // the rejected tokens of [from, from + each)
+        if (!some_without) return;
         __syncthreads();
-        if (some_without) {
-            for (int i = tid; i < (p.each + 31) / 32; i += kVerifyThreads) without[i] = 0u;
-            __syncthreads();
-            if (wave == 0 && (w.rejected >> lane & 1) != 0 && w.token >= from && w.token < (int64_t)from + p.each) {
-                const int at = (int)(w.token - from);
-                atomicOr(&without[at >> 5], 1u << (at & 31));
-            }
-            __syncthreads();
+        for (int i = tid; i < (p.each + 31) / 32; i += kVerifyThreads) without[i] = 0u;
+        __syncthreads();
+        if (wave == 0 && (rejected >> lane & 1) != 0 && token_of_lane >= from && token_of_lane < (int64_t)from + p.each) {
+            const int at = (int)(token_of_lane - from);
+            atomicOr(&without[at >> 5], 1u << (at & 31));
         }
+        __syncthreads();
     };
     // r of values v .. v + 3, v a multiple of 4 behind `from`
     auto four_of = [&](int from, int v, double (&r)[4]) __attribute__((always_inline)) {
@@ -182,116 +195,130 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyPara
             r[i] = d > 0.0 && (out >> i & 1u) == 0u ? d : 0.0;
         }
     };
-    auto total = [&](double x) {  // over the workgroup, in all threads
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) x += __shfl_xor(x, step);
-        __syncthreads();
-        if (lane == 0) sums[wave] = x;
-        __syncthreads();
-        double all = 0.0;
-#pragma unroll
-        for (int i = 0; i < kVerifyThreads / 64; i++) all += sums[i];
-        return all;
-    };
-    auto part_sum = [&](int from) {
-        mark(from);
-        const int to = min(from + p.each, p.V);
+    auto quarter_sum = [&](int from) {  // this wave's of the part that begins there, in all its lanes
+        const int v0 = from + wave * quarter, v1 = min(v0 + quarter, p.V);
         double x = 0.0;
 #pragma unroll 4
-        for (int v = from + 4 * tid; v < to; v += kVerifyStep) {
+        for (int v = v0 + 4 * lane; v < v1; v += 4 * 64) {
             double r[4];
             four_of(from, v, r);
             x += (r[0] + r[1]) + (r[2] + r[3]);
         }
-        return total(x);
+#pragma unroll
+        for (int step = 1; step < 64; step *= 2) x += __shfl_xor(x, step);
+        return x;
     };
 
-    const double mine = part_sum(part * p.each);
-    double *const all_sums = p.sums + (int64_t)b * p.parts;
+    mark(part * p.each);
+    const double mine = quarter_sum(part * p.each);
+    f64x4 held = {0.0, 0.0, 0.0, 0.0};  // part `lane`'s quarters
     if (p.parts > 1) {
-        const HandOver out(all_sums, 8u * (uint32_t)p.parts);
-        if (tid == 0) out.put(8u * (uint32_t)part, __builtin_bit_cast(f32x2, mine));
+        f64x4 *const all_sums = (f64x4 *)p.sums + (int64_t)b * p.parts;
+        const HandOver io(all_sums, 32u * (uint32_t)p.parts);
+        if (lane == 0) io.put(32u * (uint32_t)part + 8u * (uint32_t)wave, __builtin_bit_cast(f32x2, mine));
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (wave == 0) {
             const bool last = all_arrived(p.arrivals + (int64_t)b * p.parts, p.tag, part, p.parts);
-            if (lane == 0) shared[0] = last;
+            if (lane == 0) last_by = last;
         }
         __syncthreads();
-        if (shared[0] == 0) return;
+        if (last_by == 0) return;
+        if (lane < p.parts) {
+            const f32x4 lo = io.get4(32u * (uint32_t)lane), hi = io.get4(32u * (uint32_t)lane + 16u);
+            const f64x2 x = __builtin_bit_cast(f64x2, lo), y = __builtin_bit_cast(f64x2, hi);
+            held = f64x4{x.x, x.y, y.x, y.y};
+        }
+    } else {
+        if (lane == 0) ((double *)&quarters)[wave] = mine;
+        __syncthreads();
+        if (lane == 0) held = quarters;
     }
-    // ---- the last workgroup: the part that the token is in, then the token ----
-    double held = 0.0;  // part `lane`'s sum
-    {
-        const HandOver in(all_sums, 8u * (uint32_t)p.parts);
-        if (lane < p.parts) held = p.parts > 1 ? __builtin_bit_cast(double, in.get2(8u * (uint32_t)lane)) : mine;
-    }
-    double upto = sum_upto(held, lane);
+    // ---- the last workgroup: the part and the quarter of it that the token is in, then the token ----
+    auto whole_of = [](const f64x4 &q) { return ((q.x + q.y) + q.z) + q.w; };
+    double upto = sum_upto(whole_of(held), lane);
     if (!(of_lane(upto, 63) > 0.0) && (drawn != nullptr || some_without)) {  // (the rejected tokens were all that the target would say)
         plain = true;
         for (int i = 0; i < p.parts; i++) {
-            const double x = part_sum(i * p.each);
-            if (lane == i) held = x;
+            const double x = quarter_sum(i * p.each);
+            __syncthreads();
+            if (lane == 0) ((double *)&quarters)[wave] = x;
+            __syncthreads();
+            if (lane == i) held = quarters;
         }
-        upto = sum_upto(held, lane);
+        upto = sum_upto(whole_of(held), lane);
     }
     const double whole = of_lane(upto, 63);
     int token = -1;
     if (whole > 0.0) {
-        const double want = (double)w.u0 * whole;
-        uint64_t beyond = __builtin_amdgcn_ballot_w64(upto > want);
-        const uint64_t some = __builtin_amdgcn_ballot_w64(held > 0.0);
+        const double want = (double)u0_by * whole;
+        const uint64_t beyond = __builtin_amdgcn_ballot_w64(upto > want), some = __builtin_amdgcn_ballot_w64(whole_of(held) > 0.0);
         const int at = beyond != 0ull ? __ffsll((unsigned long long)beyond) - 1 : 63 - __clzll((long long)some);
-        const double before = at > 0 ? of_lane(upto, at - 1) : 0.0;
-        const int from = at * p.each, to = min(from + p.each, p.V);
+        double before = at > 0 ? of_lane(upto, at - 1) : 0.0;
+        int k = -1;  // the quarter: the first whose end is beyond, or the last that is not empty
+        {
+            double c = before, start = before;
+#pragma unroll
+            for (int i = 0; i < kVerifyWaves; i++) {
+                const double x = of_lane(held[i], at);
+                if (x > 0.0 && (k < 0 || !(c > want))) {
+                    k = i;
+                    start = c;
+                    c += x;
+                }
+            }
+            before = start;
+        }
+        const int from = at * p.each;
         mark(from);
-        // each thread a run of the part
-        const int run = (p.each / kVerifyThreads + 3) / 4 * 4, v0 = from + tid * run, v1 = min(v0 + run, to);
+        const int q0 = from + k * quarter, q1 = min(q0 + quarter, p.V);
+        // each thread a run of it
+        const int run = max((quarter + kVerifyThreads - 1) / kVerifyThreads, 4), v0 = q0 + tid * run, v1 = min(v0 + run, q1);
         double x = 0.0;
-        int last = -1;  // the last value of the run that is not 0
-#pragma unroll 4
+        bool any = false;
         for (int v = v0; v < v1; v += 4) {
             double r[4];
             four_of(from, v, r);
             x += (r[0] + r[1]) + (r[2] + r[3]);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (r[i] > 0.0) last = v + i;
+            any = any || r[0] > 0.0 || r[1] > 0.0 || r[2] > 0.0 || r[3] > 0.0;
         }
         double end = sum_upto(x, lane);
-        __syncthreads();
-        if (lane == 63) sums[wave] = end;
-        if (tid < 2) shared[1 + tid] = tid == 0 ? 0x7fffffff : -1;
+        if (lane == 63) ends[wave] = end;
+        if (tid == 0) first_by = 0x7fffffff, end_by = -1;
         __syncthreads();
         double base = before;
-        for (int i = 0; i < wave; i++) base += sums[i];
+        for (int i = 0; i < wave; i++) base += ends[i];
         end += base;
-        double start = __shfl_up(end, 1);
-        if (lane == 0) start = base;
-        if (end > want && last >= 0) atomicMin(&shared[1], tid);
-        if (last >= 0) atomicMax(&shared[2], last);
-        __syncthreads();
-        if (shared[1] == tid) {
-            int found = last;
-            double c = start;
-            for (int v = v0; v < v1; v += 4) {
-                double r[4];
-                four_of(from, v, r);
-                bool done = false;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    c += r[i];
-                    if (!done && r[i] > 0.0 && c > want) {
-                        found = v + i;
-                        done = true;
-                    }
-                }
-                if (done) break;
-            }
-            shared[3] = found;
+        if (any) {
+            if (end > want) atomicMin(&first_by, tid);
+            atomicMax(&end_by, tid);
         }
         __syncthreads();
-        token = shared[1] != 0x7fffffff ? shared[3] : shared[2];  // (beyond the last sum by a rounding: the last token)
+        const int found = first_by != 0x7fffffff ? first_by : end_by;  // (beyond the last sum by a rounding: the last run that is not empty)
+        if (found == tid) ends[0] = end - x;  // (where it begins)
+        __syncthreads();
+        if (wave == 0) {
+            // the run's values, 64 a time
+            double c = ends[0];
+            const int r0 = q0 + found * run, r1 = min(r0 + run, q1);
+            for (int v = r0; v < r1; v += 64) {
+                double r = 0.0;
+                if (v + lane < r1) {
+                    double q[4];
+                    const int v4 = v + (lane & ~3);
+                    four_of(from, v4, q);
+                    r = lane & 2 ? lane & 1 ? q[3] : q[2] : lane & 1 ? q[1] : q[0];
+                }
+                const double sum = c + sum_upto(r, lane);
+                const uint64_t over = __builtin_amdgcn_ballot_w64(r > 0.0 && sum > want), there = __builtin_amdgcn_ballot_w64(r > 0.0);
+                if (there != 0ull) token = v + 63 - __clzll((long long)there);  // (the last so far)
+                if (over != 0ull) {
+                    token = v + __ffsll((unsigned long long)over) - 1;
+                    break;
+                }
+                c = of_lane(sum, 63);
+            }
+        }
     }
     if (tid == 0) {
         if (p.tokens_64) ((int64_t *)p.next)[b] = token;

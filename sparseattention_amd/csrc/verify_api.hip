@@ -10,6 +10,7 @@ namespace {
 
 using sa::fail;
 
+constexpr size_t kWordBytes = 5 * 8;  // four sums and an arrival of each workgroup
 constexpr int kNodes = 64, kMostTokens = sa::kVerifyMostParts * sa::kVerifyMostEach;
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -26,7 +27,7 @@ int64_t words(int B, int V) {
 
 extern "C" {
 
-size_t sa_verify_drafts_workspace_bytes(int B, int n, int V) { return fits(B, n, V) ? (size_t)words(B, V) * 16 : 0; }
+size_t sa_verify_drafts_workspace_bytes(int B, int n, int V) { return fits(B, n, V) ? (size_t)words(B, V) * kWordBytes : 0; }
 
 int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], const void *draft_probs, const int64_t draft_strides[3], const void *tokens,
                      const int64_t tokens_strides[2], int tokens_64, const float *uniforms, const int64_t uniforms_strides[2], const int32_t *parents,
@@ -69,11 +70,11 @@ int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], 
     sa::verify_plan(p);
     const int64_t count = (int64_t)B * p.parts;
     if (count > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 workgroups", who);
-    const size_t need = (size_t)count * 16;
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 8))
-        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 8-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
+    const size_t need = (size_t)count * kWordBytes;
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+        return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);
     p.sums = static_cast<double *>(workspace);
-    p.arrivals = reinterpret_cast<uint64_t *>(p.sums + count);
+    p.arrivals = reinterpret_cast<uint64_t *>(p.sums + 4 * count);
     p.tag = sa::next_launch_tag() | 1;
     const hipError_t e = sa::launch_verify(p, dtype, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? SA_OK : fail(SA_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
