@@ -12,6 +12,7 @@ namespace sa {
 namespace {
 
 constexpr int kKeepBlocks = 3, kKeepThreads = 256;
+constexpr uint32_t kNoChange = 128;  // (changes are brought to -126 .. 127)
 
 // Where K and V have four codes of a word of a block: word w holds columns of one row (K) or rows of one column (V).
 __device__ __forceinline__ int k_row(int w) { return w >> 2 & 31; }
@@ -23,8 +24,9 @@ template <int ND>
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKeepParams p) {
     constexpr int W = ND * 256;  // words of a block
     __shared__ __attribute__((aligned(16))) uint32_t codes[kKeepBlocks][W];
-    __shared__ int source[32 * kKeepBlocks], goes[32 * kKeepBlocks];  // of a row: where it comes from; to which other blocks, a bit each
-    __shared__ float factor[32 * kKeepBlocks];
+    // of a row: where it comes from, and above that what its exponent changes by, + kNoChange; to which other blocks it goes, a bit each in a byte
+    __shared__ __attribute__((aligned(16))) uint32_t source[32 * kKeepBlocks];
+    __shared__ uint32_t goes[8 * kKeepBlocks], shared[2];
     __shared__ unsigned largest[kKeepBlocks][kKeepBlocks];  // code of those that block [to] takes from block [from]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool values = blockIdx.x & 1u;
@@ -52,7 +54,8 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
         if (at[k] >= 0)
             for (int i = tid; i < W / 4; i += kKeepThreads) ((u32x4 *)codes[k])[i] = ((const u32x4 *)(base + at[k] * (4 * W)))[i];
     }
-    for (int r = tid; r < 32 * kKeepBlocks; r += kKeepThreads) source[r] = r, goes[r] = 0;
+    if (tid < 32 * kKeepBlocks) source[tid] = (uint32_t)tid;
+    if (tid < 8 * kKeepBlocks) goes[tid] = 0u;
     if (tid < kKeepBlocks * kKeepBlocks) largest[tid / kKeepBlocks][tid % kKeepBlocks] = 0u;
     __syncthreads();
     uint32_t written = 0u, own = off > 0 ? 1u : 0u;  // blocks with a row from another place; those whose scale counts
@@ -63,8 +66,8 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
         for (int k = 0; k < kKeepBlocks; k++)
             if (((s >> 5) == k || (to >> 5) == k) && at[k] < 0) there = false;
         if (there) {
-            source[to] = s;
-            if ((s >> 5) != (to >> 5)) atomicOr(&goes[s], 1 << (to >> 5));
+            source[to] = (uint32_t)s;
+            if ((s >> 5) != (to >> 5)) atomicOr(&goes[s >> 2], 1u << (8 * (s & 3) + (to >> 5)));
         }
 #pragma unroll
         for (int k = 0; k < kKeepBlocks; k++) {
@@ -72,25 +75,31 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
             // (a token that is not moved stays as it is)
             if (__builtin_amdgcn_ballot_w64(lane < n && (to >> 5) == k && (!there || (s >> 5) == k)) != 0ull) own |= 1u << k;
         }
-        if (lane == 0) factor[0] = __uint_as_float(written), factor[1] = __uint_as_float(own);
+        // (and blocks from which a row goes to another)
+#pragma unroll
+        for (int k = 0; k < kKeepBlocks; k++)
+            if (__builtin_amdgcn_ballot_w64(there && (s >> 5) == k && (to >> 5) != k) != 0ull) own |= 0x100u << k;
+        if (lane == 0) shared[0] = written, shared[1] = own;
     }
     __syncthreads();
-    written = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(factor[0]));
-    own = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(factor[1]));
+    written = (uint32_t)__builtin_amdgcn_readfirstlane((int)shared[0]);
+    own = (uint32_t)__builtin_amdgcn_readfirstlane((int)shared[1]);
     if (written == 0u) return;
 
     // ---- the largest code that each block takes from each other ----
 #pragma unroll
     for (int k = 0; k < kKeepBlocks; k++) {
-        if (k >= blocks || at[k] < 0) continue;
+        if ((own >> (8 + k) & 1u) == 0u) continue;
         uint32_t most[kKeepBlocks] = {};
         for (int w = tid; w < W; w += kKeepThreads) {
-            const uint32_t word = codes[k][w];
             const int row = 32 * k + (values ? v_row(w) : k_row(w));
+            uint32_t four = goes[row >> 2];
+            if (!values) four = (four >> (8 * (row & 3)) & 0xffu) * 0x01010101u;
+            if (four == 0u) continue;
+            const uint32_t word = codes[k][w];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int to = goes[row + (values ? i : 0)];
-                const uint32_t size = word >> (8 * i) & 0x7fu;
+                const uint32_t to = four >> (8 * i), size = word >> (8 * i) & 0x7fu;
 #pragma unroll
                 for (int j = 0; j < kKeepBlocks; j++)
                     if (j != k && (to >> j & 1) != 0 && size != 0x7fu) most[j] = max(most[j], size);
@@ -115,32 +124,45 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
         }
     }
     if (tid < 32 * kKeepBlocks) {
-        const int to = tid >> 5, k = source[tid] >> 5;
+        const int to = tid >> 5, k = (int)source[tid] >> 5;
         int diff = 0;  // (rows behind the last kept one stay as they are)
 #pragma unroll
         for (int i = 0; i < kKeepBlocks; i++)
 #pragma unroll
             for (int j = 0; j < kKeepBlocks; j++)
                 if (i == k && j == to && tid < off + n) diff = e[i] - e_new[j];
-        factor[tid] = exp2i(min(max(diff, -126), 127));
+        source[tid] |= (kNoChange + (uint32_t)min(max(diff, -126), 127)) << 8;
     }
     __syncthreads();
+    // Words that keep their bytes are not written: those of rows in front of the drafts, as long as the scale stays.
 #pragma unroll
     for (int j = 0; j < kKeepBlocks; j++) {
         if ((written >> j & 1u) == 0u) continue;
         uint32_t *const out = (uint32_t *)(base + at[j] * (4 * W));
         for (int w = tid; w < W; w += kKeepThreads) {
             const int row = 32 * j + (values ? v_row(w) : k_row(w));
-            uint32_t word = 0u;
-            float f[4];
+            u32x4 s;
+            if (values) s = *(const u32x4 *)&source[row];
+            else s.x = s.y = s.z = s.w = source[row];
+            bool same = true, exact = true;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int to = row + (values ? i : 0), s = source[to];
-                f[i] = factor[to];
-                if (values) word |= (uint32_t)((const uint8_t *)codes[s >> 5])[v_byte(w, s & 31)] << (8 * i);
-                else if (i == 0) word = codes[s >> 5][(w & ~0x7c) | (s & 31) << 2];
+                same = same && s[i] == (kNoChange << 8 | (uint32_t)(row + (values ? i : 0)));
+                exact = exact && s[i] >> 8 == kNoChange;
             }
-            if (f[0] != 1.f || f[1] != 1.f || f[2] != 1.f || f[3] != 1.f) {
+            if (same) continue;
+            uint32_t word;
+            if (values) {
+                word = 0u;
+#pragma unroll
+                for (int i = 0; i < 4; i++) word |= (uint32_t)((const uint8_t *)codes[s[i] >> 5 & 7u])[v_byte(w, s[i] & 31)] << (8 * i);
+            } else {
+                word = codes[s.x >> 5 & 7u][(w & ~0x7c) | (s.x & 31) << 2];
+            }
+            if (!exact) {
+                float f[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[i] = exp2i((int)(s[i] >> 8) - (int)kNoChange);
                 const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
                 word = codes4(lo.x * f[0], lo.y * f[1], hi.x * f[2], hi.y * f[3]);
             }
