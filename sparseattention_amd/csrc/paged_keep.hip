@@ -75,10 +75,12 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
             // (a token that is not moved stays as it is)
             if (__builtin_amdgcn_ballot_w64(lane < n && (to >> 5) == k && (!there || (s >> 5) == k)) != 0ull) own |= 1u << k;
         }
-        // (and blocks from which a row goes to another)
+        // (and from which block a row goes to which other)
 #pragma unroll
         for (int k = 0; k < kKeepBlocks; k++)
-            if (__builtin_amdgcn_ballot_w64(there && (s >> 5) == k && (to >> 5) != k) != 0ull) own |= 0x100u << k;
+#pragma unroll
+            for (int j = 0; j < kKeepBlocks; j++)
+                if (j != k && __builtin_amdgcn_ballot_w64(there && (s >> 5) == k && (to >> 5) == j) != 0ull) own |= 0x100u << (kKeepBlocks * k + j);
         if (lane == 0) shared[0] = written, shared[1] = own;
     }
     __syncthreads();
@@ -86,10 +88,14 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(const PagedKee
     own = (uint32_t)__builtin_amdgcn_readfirstlane((int)shared[1]);
     if (written == 0u) return;
 
-    // ---- the largest code that each block takes from each other ----
+    // ---- the largest code that each block takes from each other, where that block's scale is not the larger one anyway ----
 #pragma unroll
     for (int k = 0; k < kKeepBlocks; k++) {
-        if ((own >> (8 + k) & 1u) == 0u) continue;
+        bool looked_at = false;
+#pragma unroll
+        for (int j = 0; j < kKeepBlocks; j++)
+            looked_at = looked_at || ((own >> (8 + kKeepBlocks * k + j) & 1u) != 0u && ((own >> j & 1u) == 0u || e[k] > e[j]));
+        if (!looked_at) continue;
         uint32_t most[kKeepBlocks] = {};
         for (int w = tid; w < W; w += kKeepThreads) {
             const int row = 32 * k + (values ? v_row(w) : k_row(w));
