@@ -13,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
@@ -1417,8 +1418,21 @@ struct RotateFunction : public torch::autograd::Function<RotateFunction> {
         return {g.dq, g.dk, g.dqw.value_or(Tensor()), g.dkw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+// Under capture, leaves that another living graph already accumulates into on another stream: the backward would wait for that stream, which a capture
+// cannot, and the error ends the process.
+void leaves_fit_capture(const Tensor &ref, std::initializer_list<const Tensor *> inputs) {
+    if (!ref.is_cuda() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(ref.device().index());
+    for (const Tensor *t : inputs) {
+        if (t == nullptr || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (node && node->stream() && *node->stream() != now)
+            throw std::runtime_error("rotate_heads_trainable under capture: a graph made before, on another stream, still holds these leaves; let go of its outputs first");
+    }
+}
 py::tuple rotate_heads_trainable(const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw, const OptTensor &kw, double eps) {
     const Rotary r = rotary_of(rotary);
+    leaves_fit_capture(q, {&q, &k, qw ? &*qw : nullptr, kw ? &*kw : nullptr});
     const auto out = RotateFunction::apply(q, k, qw, kw, positions, r.frequencies, r.axes, r.interleaved, eps);
     return py::make_tuple(out[0], out[1]);
 }

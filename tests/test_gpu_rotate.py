@@ -295,3 +295,36 @@ def test_large_outputs(gpu, interleaved):
     assert (q.numel() + k.numel()) * 2 >= 128 << 20 > (q.numel() + k.numel()) // 2
     for a, b in zip(whole, zip(*parts)):
         assert torch.equal(a, torch.cat(b))
+
+
+def test_backward_captured_and_replayed(gpu):
+    """A training step's forward and gradients in a graph; where an eager graph of the same leaves lives, the capture is refused and the process goes on."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    q, k = rows(g, 2, 4, 50, 128, torch.bfloat16), rows(g, 2, 2, 50, 128, torch.bfloat16)
+    leaves = [x.requires_grad_() for x in (q, k, *weights(g, 128, torch.bfloat16))]
+    r, at = sa.rotary_frequencies(128), torch.arange(50, device="cuda")
+    ups = [torch.randn(x.shape, generator=g, device="cuda").to(x.dtype) for x in (q, k)]
+
+    def step():
+        y = sa.rotate_heads_trainable(leaves[0], leaves[1], at, r, leaves[2], leaves[3])
+        return [x.detach() for x in y] + list(torch.autograd.grad(y, leaves, ups))
+
+    step()
+    torch.cuda.synchronize()
+    alive = sa.rotate_heads_trainable(leaves[0], leaves[1], at, r, leaves[2], leaves[3])
+    torch.autograd.grad(alive, leaves, ups, retain_graph=True)
+    with pytest.raises(RuntimeError, match="still holds these leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            q.normal_()
+            leaves[2].uniform_(0.5, 1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), i
