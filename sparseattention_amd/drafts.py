@@ -1,6 +1,15 @@
 """Verification of drafted tokens against the target's probabilities.
 
-The reference decodes nothing; a step with drafts over the paged cache is in paged_cache.py.  Kernel: csrc/verify.hip."""
+The reference decodes nothing.  A step with drafted tokens over a paged cache (paged_cache.py), a tree of n whose root is the last token that the sequence
+has, of a model that norms and rotates its heads:
+
+    q = paged_cache_append_rotated(cache, q, k, v, page_table, lens, rotary, parents=parents)
+    o = sparse_attention_decode_tree(q, cache, page_table, lens + n, parents)
+    path, accepted, token = verify_drafts(probabilities(o), tokens, uniforms, parents)
+    paged_cache_keep(cache, page_table, lens, path, accepted)
+    lens = lens + accepted
+
+(first, second and fourth line in each layer with its own cache), after which ``token`` is the root of the next tree.  Kernel: csrc/verify.hip."""
 from __future__ import annotations
 
 from typing import Optional

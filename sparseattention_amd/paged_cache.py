@@ -15,16 +15,11 @@ and a prompt's later chunk, which has more than 32 rows, reads its keys back:
 
 (sparse_attention has a K/V head per query head: with grouped heads the third line copies K and V for each of a group.)
 
-A step with drafted tokens (a tree of n, its root the last token the sequence has), of a model that norms and rotates its heads:
-
-    q = paged_cache_append_rotated(cache, q, k, v, page_table, lens, rotary, parents=parents)
-    o = sparse_attention_decode_tree(q, cache, page_table, lens + n, parents)            # ... the target's probabilities
-    path, accepted, token = verify_drafts(probabilities, tokens, uniforms, parents)
-    paged_cache_keep(cache, page_table, lens, path, accepted)                             # in every layer's cache
-    lens = lens + accepted
+(A step with drafted tokens: drafts.py.)
 
 All calls enqueue work on the current stream of the cache's device and read no tensor on the host, so they can be captured
-into a graph (tile lists that a caller wrote or changed are looked at on the host, once, by the first call that gets them).  The steps of a call are native (csrc/host_ops.cpp), the kernels csrc/paged_cache.hip, csrc/paged_rotated.hip, csrc/paged_keep.hip and csrc/paged_decode.hip."""
+into a graph (tile lists that a caller wrote or changed are looked at on the host, once, by the first call that gets them).  The steps of a call are native (csrc/host_ops.cpp), the
+kernels csrc/paged_cache.hip, csrc/paged_rotated.hip, csrc/paged_keep.hip and csrc/paged_decode.hip."""
 from __future__ import annotations
 
 from dataclasses import dataclass

@@ -1,11 +1,13 @@
 """The operators as they are used together: steps with drafted tokens over a paged cache, and a training step's rotation and attention."""
 import math
+import textwrap
 
 import pytest
 import torch
 
 import rotary_reference as ref
 import sparseattention_amd as sa
+from sparseattention_amd import drafts
 from test_gpu_paged_decode import check as check_attention
 from test_gpu_paged_keep import check as check_keep
 from test_gpu_paged_rotated import check as check_append
@@ -113,6 +115,26 @@ def test_a_step_captured_and_replayed(gpu):
         assert torch.equal(lens[0], lens[1])
         for a, b in zip(held_rows(caches[0], table, lens[0].tolist()), held_rows(caches[1], table, lens[1].tolist())):
             assert torch.equal(a, b), i
+
+
+def test_the_documented_step(gpu):
+    """The calls that the module's documentation shows, run as they stand there."""
+    block = [line for line in drafts.__doc__.splitlines() if line.startswith("    ")]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache = sa.empty_paged_cache(8, 2, 64, page_size=32)
+    table, lens, n = ints(*range(8)).view(2, 4), ints(33, 60), 5
+    q, k, v = (torch.randn(2, h, n, 64, generator=g, device="cuda").bfloat16() for h in (4, 2, 2))
+    parents, tokens = tree("deep", 2, n, 4).cuda(), torch.randint(20, (2, n), generator=g, device="cuda")
+    names = dict(vars(sa), cache=cache, page_table=table, lens=lens, n=n, q=q, k=k, v=v, parents=parents, tokens=tokens, rotary=sa.rotary_frequencies(64),
+                 uniforms=torch.zeros(2, n, device="cuda"), probabilities=lambda o: torch.full((2, n, 20), 0.05, device="cuda"))
+    exec(textwrap.dedent("\n".join(block)), names)
+    # (numbers of 0 accept every draft that has a chance: the first child each time, down to a leaf)
+    for b, row in enumerate(parents.tolist()):
+        path = [0]
+        while path[-1] in row[path[-1] + 1:]:
+            path.append(row.index(path[-1], path[-1] + 1))
+        assert names["path"][b].tolist() == path + [-1] * (n - len(path)) and int(names["lens"][b] - lens[b]) == len(path)
+    assert names["token"].tolist() == [0, 0] and names["o"].shape == q.shape
 
 
 def test_training_step(gpu):
