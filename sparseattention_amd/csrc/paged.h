@@ -159,11 +159,7 @@ struct PagedDecodeParams {
     int64_t qs[3], os[3], lses[3];  // b, h, row strides in elements
     const int32_t *counts;  // valid query rows of each sequence, or null: Sq
     int G, Sq, R, RT;       // query heads of a K/V head; rows of one: R = G * Sq in RT planes
-    int plane_rows, tiles;  // of a plane: 16, or `tiles` tiles of 32 that share a workgroup (more than one of trees only)
     int window;             // or 0
-    // the rows are a tree (tree.h): each one's parent, or null
-    const int32_t *parents;
-    int64_t parents_stride[2];
     // tile lists, tile = page, all null: every key that causality and window leave
     const int32_t *full_ids, *full_lens, *part_ids, *part_lens;
     int64_t fis[3], fls[2], pis[3], pls[2];  // b, h (and entry) strides
@@ -180,6 +176,11 @@ struct PagedDecodeParams {
     uint64_t *arrivals;
     uint64_t tag;
     PagedUnits *units;  // or null: every workgroup finds them itself
+    // (what only some kernels read, behind what all do)
+    int plane_rows, tiles;  // of a plane: 16, or `tiles` tiles of 32 that share a workgroup (more than one of trees only)
+    // the rows are a tree (tree.h): each one's parent, or null
+    const int32_t *parents;
+    int64_t parents_stride[2];
 };
 // Bytes of ws.
 size_t paged_decode_parts_bytes(int groups, int part_rows, int D);
