@@ -12,4 +12,7 @@ int fail(int code, const char *fmt, ...);
 // process left behind holds none of them.
 uint64_t next_launch_tag();
 
+// Workgroups of 256 that a launch can have (its threads have 32 bits).
+constexpr int64_t kMostGroups256 = (1 << 24) - 1;
+
 }  // namespace sa

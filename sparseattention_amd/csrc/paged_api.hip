@@ -139,7 +139,7 @@ int sa_paged_cache_append_rotated(const sa_paged_cache *cache, const void *q, co
     p.S = S;
     p.blocks = (S + 62) / 32;
     const int64_t groups = sa::paged_rotated_plan(p);
-    if (groups < 0) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens or workgroups", who);
+    if (groups < 0 || groups > sa::kMostGroups256) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens or 2^24 - 1 workgroups", who);
     return launched(who, sa::launch_paged_rotated(p, groups, dtype, static_cast<hipStream_t>(stream)));
 }
 
@@ -186,7 +186,7 @@ int sa_paged_cache_keep(const sa_paged_cache *cache, const int32_t *page_table, 
     for (int i = 0; i < 2; i++) p.path_s[i] = path_strides[i];
     p.accepted = accepted;
     p.n = n;
-    SA_TRY(grid_fits(who, (int64_t)2 * p.c.H * B));
+    if ((int64_t)2 * p.c.H * B > sa::kMostGroups256) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^23 sequences' heads", who);
     return launched(who, sa::launch_paged_keep(p, static_cast<hipStream_t>(stream)));
 }
 

@@ -198,24 +198,23 @@ hipError_t with_rows(const RotateParams &p, int dtype, F &&f) {
 
 }  // namespace
 
-hipError_t launch_rotate(RotateParams p, int dtype, hipStream_t stream) {
-    share_heads(p);
-    return with_rows(p, dtype, [&](auto dt, auto lpr, auto inter, auto past) {
-        constexpr int T = 64 / decltype(lpr)::value;
-        const int64_t waves = ((int64_t)p.B * p.S + T - 1) / T * p.splits;
-        hipLaunchKernelGGL((rotate_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value, decltype(past)::value>), dim3((unsigned)((waves + kRotateWaves - 1) / kRotateWaves)), dim3(64 * kRotateWaves), 0, stream, p);
-        return hipGetLastError();
-    });
-}
-
-int rotate_backward_groups(int B, int S, int heads, int D) {
+int64_t rotate_groups(int B, int S, int heads, int D) {
     RotateParams p{};
     p.B = B, p.S = S, p.D = D, p.q.H = heads;
     share_heads(p);
     const int T = D <= 64 ? 8 : D <= 128 ? 4 : 2;
-    const int64_t waves = ((int64_t)B * S + T - 1) / T * p.splits;
-    return (int)std::min<int64_t>((waves + kRotateWaves - 1) / kRotateWaves, kBackwardGroups);
+    return (((int64_t)B * S + T - 1) / T * p.splits + kRotateWaves - 1) / kRotateWaves;
 }
+
+hipError_t launch_rotate(RotateParams p, int dtype, hipStream_t stream) {
+    share_heads(p);
+    return with_rows(p, dtype, [&](auto dt, auto lpr, auto inter, auto past) {
+        hipLaunchKernelGGL((rotate_kernel<decltype(dt)::value, decltype(lpr)::value, decltype(inter)::value, decltype(past)::value>), dim3((unsigned)rotate_groups(p.B, p.S, p.q.H + p.k.H, p.D)), dim3(64 * kRotateWaves), 0, stream, p);
+        return hipGetLastError();
+    });
+}
+
+int rotate_backward_groups(int B, int S, int heads, int D) { return (int)std::min<int64_t>(rotate_groups(B, S, heads, D), kBackwardGroups); }
 
 hipError_t launch_rotate_backward(RotateParams p, int dtype, hipStream_t stream) {
     share_heads(p);

@@ -54,6 +54,7 @@ int sa_rotate_heads(const void *q, const int64_t q_strides[4], const void *k, co
     p.q.x = q, p.q.y = q_out, p.q.H = Hq;
     p.k.x = k, p.k.y = k_out, p.k.H = H;
     p.B = B, p.S = S, p.D = D;
+    if (sa::rotate_groups(B, S, Hq + H, D) > sa::kMostGroups256) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^24 - 1 workgroups", who);
     return launched(who, sa::launch_rotate(p, dtype, static_cast<hipStream_t>(stream)));
 }
 

@@ -33,6 +33,8 @@ struct RotateParams {
     float *parts;       // backward: [workgroups][2][D], a workgroup's sums for the weights
     int groups;         // its workgroups
 };
+// Workgroups of the forward, of 256.
+int64_t rotate_groups(int B, int S, int heads, int D);
 hipError_t launch_rotate(RotateParams p, int dtype, hipStream_t stream);
 // Workgroups of the backward.
 int rotate_backward_groups(int B, int S, int heads, int D);

@@ -69,7 +69,7 @@ int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], 
     p.V = V;
     sa::verify_plan(p);
     const int64_t count = (int64_t)B * p.parts;
-    if (count > 0x7fffffff) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 workgroups", who);
+    if (count > sa::kMostGroups256) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^24 - 1 workgroups", who);
     const size_t need = (size_t)count * kWordBytes;
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return fail(SA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, 16-byte aligned (got %zu)", who, need, workspace ? workspace_bytes : (size_t)0);

@@ -1,4 +1,5 @@
 """The operators as they are used together: steps with drafted tokens over a paged cache, and a training step's rotation and attention."""
+import concurrent.futures
 import math
 import textwrap
 
@@ -135,6 +136,59 @@ def test_the_documented_step(gpu):
             path.append(row.index(path[-1], path[-1] + 1))
         assert names["path"][b].tolist() == path + [-1] * (n - len(path)) and int(names["lens"][b] - lens[b]) == len(path)
     assert names["token"].tolist() == [0, 0] and names["o"].shape == q.shape
+
+
+def test_far_into_a_large_pool(gpu):
+    """Pages whose codes lie beyond 2^32 bytes of the pool: the step there is, to the bit, the step in a small one."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    H, D, P, n = 8, 128, 64, 9
+    pages = (5 << 30) // (H * P * D)  # 5 GiB of K, as much of V
+    large, small = sa.empty_paged_cache(pages, H, D, page_size=P), sa.empty_paged_cache(6, H, D, page_size=P)
+    far = ints(pages - 1, pages - 5, 3, pages - 2, 0, pages - 7).view(2, 3)
+    near, lens = ints(5, 1, 3, 4, 0, 2).view(2, 3), ints(120, 58)
+    x = [torch.randn(2, H, 130, D, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    qkv = torch.randn(2, 4 * H, n, D, generator=g, device="cuda").bfloat16()
+    parents, rotary = tree("deep", 2, n, 6).cuda(), sa.rotary_frequencies(D)
+    path, accepted = ints(0, 2, 5, 7, *[-1] * 5)[None].expand(2, n), ints(4, 3)
+    outs = []
+    for cache, table in ((large, far), (small, near)):
+        sa.paged_cache_append(cache, *x, table, torch.zeros_like(lens), counts=lens)
+        q = sa.paged_cache_append_rotated(cache, qkv[:, :2 * H], qkv[:, 2 * H:3 * H], qkv[:, 3 * H:], table, lens, rotary, parents=parents)
+        o = sa.sparse_attention_decode_tree(q, cache, table, lens + n, parents)
+        sa.paged_cache_keep(cache, table, lens, path, accepted)
+        outs.append([q, o, *sa.paged_cache_gather(cache, table, lens + accepted)])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_calls_side_by_side(gpu):
+    """Threads with a stream each, all operators in all of them."""
+    def work(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            cache = sa.empty_paged_cache(12, 2, 64, page_size=32)
+            table, lens, n = ints(*range(12)).view(3, 4), ints(33, 60, 5), 7
+            q, k, v = (torch.randn(3, h, n, 64, generator=g, device="cuda").bfloat16() for h in (4, 2, 2))
+            parents, rotary = tree("deep", 3, n, seed).cuda(), sa.rotary_frequencies(64)
+            p = torch.softmax(3.0 * torch.randn(3, n, 9000, generator=g, device="cuda"), -1)
+            tokens, u = torch.argmax(p, -1).gather(1, parents.long().clamp(min=0)), torch.rand(3, n, generator=g, device="cuda")
+            w = torch.ones(64, device="cuda")
+            results = []
+            for _ in range(20):
+                y = sa.paged_cache_append_rotated(cache, q, k, v, table, lens, rotary, parents=parents, q_weight=w)
+                o = sa.sparse_attention_decode_tree(y, cache, table, lens + n, parents)
+                path, accepted, token = sa.verify_drafts(p, tokens, u, parents)
+                sa.paged_cache_keep(cache, table, lens, path, accepted)
+                grads = sa.rotate_heads_backward(q, k, q, k, lens[:, None].expand(3, n).contiguous(), rotary, w, w)
+                results.append([y, o, path, accepted, token, *grads])
+            torch.cuda.current_stream().synchronize()
+            for r in results[2:]:  # (the first keeping may make scales grow, which stay)
+                assert all(torch.equal(a, b) for a, b in zip(r, results[1]))
+            return [t.cpu() for t in results[1]]
+
+    alone = [work(s) for s in range(4)]
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for a, b in zip(alone, pool.map(work, range(4))):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_training_step(gpu):

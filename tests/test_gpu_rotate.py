@@ -328,3 +328,38 @@ def test_backward_captured_and_replayed(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), i
+
+
+def test_broadcast_inputs(gpu):
+    """Rows, weights and gradients that are one tensor expanded: their own gradients are the sums over what they were expanded to."""
+    g = torch.Generator(device="cuda").manual_seed(18)
+    q, k = rows(g, 1, 4, 9, 64, torch.float32).requires_grad_(), rows(g, 2, 1, 9, 64, torch.float32).requires_grad_()
+    w = (1.0 + 0.3 * torch.randn((), generator=g, device="cuda")).requires_grad_()
+    r, at = sa.rotary_frequencies(64), torch.arange(9, device="cuda")[None]
+    ups = [torch.randn(1, 1, 9, 64, generator=g, device="cuda").expand(2, 4, 9, 64), torch.randn(2, 3, 1, 64, generator=g, device="cuda").expand(2, 3, 9, 64)]
+    wide = q.expand(2, 4, 9, 64), k.expand(2, 3, 9, 64), w.expand(64), w.expand(64)
+    y = sa.rotate_heads_trainable(wide[0], wide[1], at, r, wide[2], wide[3])
+    got = torch.autograd.grad(y, [q, k, w], ups)
+    full = [x.detach().contiguous() for x in wide]
+    for a, b in zip(y, sa.rotate_heads(full[0], full[1], at, r, full[2], full[3])):
+        assert torch.equal(a, b)
+    dq, dk, dqw, dkw = sa.rotate_heads_backward(*(u.contiguous() for u in ups), full[0], full[1], at, r, full[2], full[3])
+    assert torch.equal(got[0], dq.sum(0, keepdim=True)) and torch.equal(got[1], dk.sum(1, keepdim=True))
+    assert torch.allclose(got[2], dqw.sum() + dkw.sum(), rtol=2.0 ** -18, atol=0.0)  # (128 numbers added up in float32, in some order)
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """Sequences, tokens and heads further apart than 2^32 bytes, in and out."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    store = torch.zeros((5 << 29) + (1 << 20), dtype=torch.bfloat16, device="cuda")  # 5 GiB
+    far = 5 << 28
+    r, at = sa.rotary_frequencies(64), torch.arange(2, device="cuda")
+    for strides in ((far, 1024, 64, 1), (4096, 1024, far, 1), (256, far, 64, 1)):
+        q = store.as_strided((2, 2, 2, 64), strides)
+        q.copy_(rows(g, 2, 2, 2, 64, torch.bfloat16))
+        w = torch.ones(64, device="cuda")
+        want = sa.rotate_heads(q.contiguous(), q.contiguous(), at, r, w, w)
+        assert all(torch.equal(a, b) for a, b in zip(sa.rotate_heads(q, q, at, r, w, w), want))
+        up = rows(g, 2, 2, 2, 64, torch.bfloat16)
+        want = sa.rotate_heads_backward(up, up, q.contiguous(), q.contiguous(), at, r, w, w)
+        assert all(torch.equal(a, b) for a, b in zip(sa.rotate_heads_backward(up, up, q, q, at, r, w, w), want))

@@ -267,6 +267,22 @@ def test_on_two_streams(gpu):
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
 
 
+def test_offsets_beyond_32_bits(gpu):
+    """Rows further apart than 2^32 bytes, target and draft."""
+    store = torch.zeros((3 << 29) + 200000, device="cuda")  # 6 GiB
+    for strides in ((3 << 29, 50000, 1), (50000, 3 << 28, 1)):
+        for drawn in (False, True):
+            p, tokens, u, parents, q = make(14, 2, 3, 40000, torch.float32, drawn)
+            a = store.as_strided((2, 3, 40000) if strides[1] < strides[0] else (1, 3, 40000), strides)
+            a.copy_(p[:len(a)])
+            got = sa.verify_drafts(a, tokens[:len(a)], u[:len(a)], None if drawn else parents[:len(a)], q[:len(a)] if drawn else None)
+            assert all(torch.equal(x, y[:len(a)]) for x, y in zip(got, sa.verify_drafts(p, tokens, u, parents, q)))
+            if drawn:
+                a.copy_(q[:len(a)])
+                got = sa.verify_drafts(p[:len(a)], tokens[:len(a)], u[:len(a)], None, a)
+                assert all(torch.equal(x, y[:len(a)]) for x, y in zip(got, sa.verify_drafts(p, tokens, u, parents, q)))
+
+
 def test_refusals(gpu):
     p, tokens, u, parents, _ = make(13, 2, 4, 30, torch.float32, False)
     for bad in (dict(tokens=tokens[:, :3]), dict(tokens=tokens.float()), dict(uniforms=u.double()), dict(uniforms=u[:1]), dict(parents=parents.long()), dict(tokens=tokens.cpu()),

@@ -39,6 +39,10 @@ def test_rotations(call):
     assert call(B=1 << 16, S=1 << 16) == UNSUPPORTED and call(H=(1 << 20) + 1) == UNSUPPORTED
 
 
+def test_more_than_a_launch_has():
+    assert forward(B=1 << 15, S=1 << 15) == UNSUPPORTED
+
+
 def test_rows_and_weights():
     assert forward(q=None) == BAD and forward(k=None) == BAD and forward(out=None) == BAD and forward(q=FAKE + 8) == UNSUPPORTED
     assert forward(qs=_native.strides((1024, 128, 124, 1))) == UNSUPPORTED and forward(qs=_native.strides((1024, 128, 128, 2))) == UNSUPPORTED

@@ -40,6 +40,7 @@ def test_keep():
     for name in ("c", "table", "lens", "path", "ps", "accepted"):
         assert keep(**{name: None}) == BAD, name
     assert keep(B=0) == BAD and keep(pages=0) == BAD and keep(n=0) == UNSUPPORTED and keep(n=65) == UNSUPPORTED
+    assert keep(B=1 << 22) == UNSUPPORTED  # (more workgroups than a launch has)
     assert keep(c=ctypes.byref(_native.PagedCacheStruct(FAKE, FAKE, FAKE, FAKE, 8, 2, 48, 128, 128))) == UNSUPPORTED
 
 
