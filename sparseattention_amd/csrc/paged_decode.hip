@@ -350,8 +350,9 @@ __global__ __launch_bounds__(kUnitThreads) void paged_units_kernel(const PagedDe
 // What says which keys a row attends to: causality and window, lists, or a tree of the last tokens.
 enum Who { kCausal, kLists, kTree };
 // TILES: of rows that a workgroup has, kWaves / TILES waves each, which take chunks in turn.  Several read the same K and V at about the same time, from the
-// caches (8 trees of 64 nodes, 8 x 4 heads, over up to 65536 keys, D = 64, fp16: 514 us with one, 406 with four, 593 TFLOP/s); what is left then is vector work,
-// 130 instructions for the 32 x 32 scores of a chunk, 16 of them exponentials.
+// caches (8 trees of 64 nodes, 8 x 4 heads, over up to 65536 keys, D = 64, fp16: 514 us with one, 369 with four, 653 TFLOP/s).  What is left then (us of these trees and of
+// 25-node ones of 32 sequences up to 8192 keys, D = 128, found by leaving each out in a copy): codes to 16 bits 72 and 9, exponentials 40 and 7, parts of planes 2 and 16.
+// Not kept: blocks fetched into LDS once for all tiles, four ahead (both as fast as from the caches), products of K in two sums (2 to 8 % slower).
 template <int DT, int ND, int ROWS, bool FAR, int WHO, int TILES>
 __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS, TILES)) void paged_decode_kernel(const PagedDecodeParams p) {
     constexpr bool LISTS = WHO == kLists, TREE = WHO == kTree;
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS, TILES)) void
         // What is requested next takes the registers of what has just gone into a product: K of a later chunk is on its way during the
         // softmax and the second product, V behind it.  At D = 64 two chunks are under way, as their bytes are half as many; with
         // more registers for more there would be fewer waves, which hide as much.  Tiles that share K and V find them in the caches, and have a third
-        // wave per SIMD instead (419 -> 406 us).
+        // wave per SIMD instead (419 -> 406 us when this was tried).
         constexpr int PRE = ND == 2 && TILES == 1 ? 2 : 1;
         struct Chunk {
             int block, key0, slot;
@@ -574,15 +575,24 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS, TILES)) void
         };
         // Of no block, and behind the last chunk, nothing is requested: 64 ragged sequences 102.2 -> 98.3 us, 16 in a window 18.2 -> 17.4
         // against that chunk again.  With lists the branch costs more than the pool's first block over and over, which the caches
-        // hold: 31.6 | 30.8 us.
+        // hold: 31.6 | 30.8 us.  Where tiles share a workgroup it does, too: of requests that may not have been made none can be counted, so that K was waited for
+        // with V behind it.
+        constexpr bool ALWAYS = LISTS || TILES > 1;
         auto request_k = [&](const Chunk &c, typename X::Operands &x) {
-            if (LISTS || c.block >= 0) X::load_k(x, p.c.k + (int64_t)max(c.block, 0) * (1024 * ND), lane);
+            if (ALWAYS || c.block >= 0) X::load_k(x, p.c.k + (int64_t)max(c.block, 0) * (1024 * ND), lane);
         };
         auto request_v = [&](const Chunk &c, typename X::Operands &x) {
-            if (LISTS || c.block >= 0) X::load_v(x, p.c.v + (int64_t)max(c.block, 0) * (1024 * ND), lane);
+            if (ALWAYS || c.block >= 0) X::load_v(x, p.c.v + (int64_t)max(c.block, 0) * (1024 * ND), lane);
         };
         // (of the round of 64 chunks that is requested: their places; of the round behind it, on their way; of the round at hand: scales)
+        // (There: scales that may still be on their way where the loop begins are waited for at every step, and with them all that has been requested since.  With this and the
+        // requests that are always made 25-node trees of 32 sequences up to 8192, D = 128: 137 -> 124 us; 64 nodes, 8 up to 65536, D = 64: 410 -> 369.)
+        auto there = [](Places &at) __attribute__((always_inline)) {
+            if constexpr (TILES > 1) asm volatile("" : "+v"(at.ks), "+v"(at.vs));
+        };
         Places here = places(0), next = places(64);
+        there(here);
+        there(next);
         float ks_at = 0.f, vs_at = 0.f;
         typename X::Operands ops[PRE] = {};  // (codes of 0 where nothing is requested)
         Chunk under_way[PRE];
@@ -610,6 +620,7 @@ __global__ __launch_bounds__(kWaves * 64, paged_occupancy(ND, ROWS, TILES)) void
             if ((jn & 63) == 0 && jn < nw) {
                 here = next;
                 next = places(jn + 64);  // (none behind the last chunk)
+                there(next);
             }
             const Chunk nc = chunk(here, jn);
             const int key0 = c.key0;
