@@ -7,6 +7,9 @@ Same Python surface as tomatillos/sparseattention for its one hot path:
   decode kernels as future work, ``README.md:65``)
 * :func:`sparse_attention_decode_paged`: the same over a K/V cache in pages of 8-bit numbers (:class:`PagedCache`), with the
   operators that store, read back, copy, fork, compact and free its pages
+* :func:`rotate_heads`, :func:`rotate_heads_trainable`: norms of queries and keys and their rotation by position in front of attention
+* :func:`paged_cache_append_rotated`, :func:`sparse_attention_decode_tree`, :func:`verify_drafts`, :func:`paged_cache_keep`: a step
+  with trees of drafted tokens over the paged cache (drafts.py)
 * :func:`compute_mask_kernel`, :func:`compute_mask_slow`, :class:`MaskMetadata`
   (reference: ``sparseattention/mask_utils.py:85``, ``:14``, ``:6``)
 * :func:`compute_mask_terms`: the same metadata for masks given by a formula (:class:`MaskTerm`), without the

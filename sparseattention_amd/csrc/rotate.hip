@@ -4,7 +4,11 @@
 // Backward, with g = the upstream gradient turned back, per row:
 //     dx = r w g - x r^3 mean(x w g),   dw = sum over rows of g x r       (without a norm dx = g, and x is not read)
 // Everything between the loads and the one rounding at the end is float32.  Bound by memory: every row is read and written once, q and k
-// in one launch.
+// in one launch.  A wave has 64 / LPR tokens and some of their heads, so that the angles, which take as long as four rows, are made once for these.
+//
+// Measured: 4 x 4096 tokens, 32 + 8 heads, D = 128, bf16, norms: forward 63 us, 5.3 TB/s read and written, backward 86, 5.9, and 5 for the sums of the weights
+// (a copy of 1 GiB: 5.1); 2 x 1031 tokens of three axes, 16 + 16 heads, D = 80, fp16: 8.6 us a call, a launch, the angles and 21 MB.
+// Not kept: rows requested before the angles (no gain); reads past the caches, too (8.6 -> 9.8 us).
 #include <algorithm>
 
 #include "rotate.h"
