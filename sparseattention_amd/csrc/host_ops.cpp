@@ -449,7 +449,13 @@ RotationIn rotation_in(const Tensor &ref, const Rotary &rotary, const OptTensor 
     return r;
 }
 
+// A trace would not hold the call, and hold its outputs as they were allocated.
+void not_traced(const char *what) {
+    if (torch::jit::tracer::isTracing()) throw std::runtime_error(std::string(what) + " cannot be recorded by torch.jit.trace");
+}
+
 void check_heads(const Tensor &q, const Tensor &k, const char *what) {
+    not_traced(what);
     if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(3) != k.size(3) || q.size(1) < 1 || k.size(1) < 1)
         value_error(std::string(what) + " takes q [B,Hq,S,D] and k [B,H,S,D] (got " + str(q.sizes()) + ", " + str(k.sizes()) + ")");
     if (dtype_code(q.scalar_type()) < 0) type_error(std::string("q and k must be bfloat16, float16 or float32 (got ") + c10::toString(q.scalar_type()) + ")");
@@ -612,6 +618,7 @@ const Tensor &tree_parents(const Tensor &ref, const Tensor &t, int64_t B, int64_
 
 Tensor paged_append_rotated(py::object cache, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &lens_in, py::object rotary,
                             const OptTensor &counts_in, const OptTensor &positions, const OptTensor &parents, const OptTensor &qw, const OptTensor &kw, double eps) {
+    not_traced("paged_cache_append_rotated");
     const Cache c = cache_of(cache);
     const Rotary rot = rotary_of(rotary);
     const py::gil_scoped_release unlocked;
@@ -676,6 +683,7 @@ void paged_copy(py::object cache, const Tensor &src_in, const Tensor &dst_in) {
 }
 
 void paged_keep(py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &path, const Tensor &accepted_in) {
+    not_traced("paged_cache_keep");
     const Cache c = cache_of(cache);
     const py::gil_scoped_release unlocked;
     const int64_t B = check_table(c, table);
@@ -694,6 +702,7 @@ py::tuple verify_drafts(const Tensor &target_in, const Tensor &tokens, const Ten
     Tensor path, accepted, next;
     {
         const py::gil_scoped_release unlocked;
+        not_traced("verify_drafts");
         if (target_in.dim() != 3) value_error("target_probs must be [B, n, V] (got " + str(target_in.sizes()) + ")");
         const int64_t B = target_in.size(0), n = target_in.size(1), V = target_in.size(2);
         const int dt = dtype_code(target_in.scalar_type());
@@ -877,6 +886,7 @@ py::object decode_paged(const Tensor &q, py::object cache, const Tensor &table, 
 
 py::object decode_tree(const Tensor &q, py::object cache, const Tensor &table, const Tensor &lens_in, const Tensor &parents, const OptTensor &counts_in,
                        std::optional<int64_t> window, bool return_lse) {
+    not_traced("sparse_attention_decode_tree");
     const Cache c = cache_of(cache);
     Out r;
     {
@@ -1432,6 +1442,7 @@ void leaves_fit_capture(const Tensor &ref, std::initializer_list<const Tensor *>
 }
 py::tuple rotate_heads_trainable(const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw, const OptTensor &kw, double eps) {
     const Rotary r = rotary_of(rotary);
+    not_traced("rotate_heads_trainable");
     leaves_fit_capture(q, {&q, &k, qw ? &*qw : nullptr, kw ? &*kw : nullptr});
     const auto out = RotateFunction::apply(q, k, qw, kw, positions, r.frequencies, r.axes, r.interleaved, eps);
     return py::make_tuple(out[0], out[1]);

@@ -111,6 +111,16 @@ def test_sizes(gpu, B, H, G, D, n, length):
 
 
 @gpu_test
+@pytest.mark.parametrize("n,G,pages,window", [(20, 2, 76, None), (40, 2, 112, None), (40, 2, 112, 30)])
+def test_many_short_sequences_of_wide_tables(gpu, n, G, pages, window):
+    """More sequences than a wave has lanes for, with planes of 64 and of 128 rows, as the tables have room for much more than the sequences hold."""
+    lens = [n + 7 * b % 90 for b in range(300)]
+    cache, table = make(300, 1, 64, 64, lens, torch.bfloat16, 21, gpu)
+    table = torch.cat([table, torch.full((300, pages - table.shape[1]), -1, dtype=torch.int32, device=gpu)], 1)
+    run(cache, table, lens, queries(300, G, n, 64, torch.bfloat16, 22, gpu), tree("deep", 300, n, 23), window=window)
+
+
+@gpu_test
 def test_a_chain_is_causal(gpu):
     """Up to 16 rows of a K/V head, to the bit what sparse_attention_decode_paged gives, windows and padding among them."""
     lens, counts = [40, 999, 32], [5, 0, 9]

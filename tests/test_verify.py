@@ -56,3 +56,20 @@ def test_python_refuses_without_a_gpu():
     table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="GPU"):
         sa.paged_cache_keep(cache, table, lens, table, lens)
+
+
+def test_not_recorded_by_a_trace():
+    """torch.jit.trace would keep the outputs as they were allocated, without the call."""
+    p, x, u = torch.zeros(2, 3, 10), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    cache = sa.PagedCache(torch.zeros(4, 2, 2, 2048, dtype=torch.uint8), torch.zeros(4, 2, 2, 2048, dtype=torch.uint8), torch.zeros(4, 2, 2), torch.zeros(4, 2, 2), 64)
+    table, lens, r = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), sa.rotary_frequencies(64, device="cpu")
+    q, k, at = torch.zeros(1, 2, 2, 64), torch.zeros(1, 2, 2, 64), torch.arange(2)
+    for name, call in (("rotate_heads ", lambda q: sa.rotate_heads(q, k, at, r)), ("rotate_heads_trainable", lambda q: sa.rotate_heads_trainable(q, k, at, r)),
+                       ("rotate_heads_backward", lambda q: sa.rotate_heads_backward(q, k, q, k, at, r)),
+                       ("paged_cache_append_rotated", lambda q: sa.paged_cache_append_rotated(cache, q, k, k, table, lens, r)),
+                       ("sparse_attention_decode_tree", lambda q: sa.sparse_attention_decode_tree(q, cache, table, lens, table)),
+                       ("paged_cache_keep", lambda q: sa.paged_cache_keep(cache, table, lens, table, lens) or q)):
+        with pytest.raises(RuntimeError, match=name + ".*cannot be recorded" if name[-1] != " " else "rotate_heads cannot be recorded"):
+            torch.jit.trace(call, (q,))
+    with pytest.raises(RuntimeError, match="verify_drafts cannot be recorded"):
+        torch.jit.trace(lambda p: sa.verify_drafts(p, x, u), (p,))
