@@ -3,10 +3,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-namespace sa {
+#include "verify_plan.h"
 
-constexpr int kVerifyMostParts = 64;      // of a row, which one wave adds up
-constexpr int kVerifyMostEach = 1 << 15;  // values of a part, which have a bit in LDS each
+namespace sa {
 
 struct VerifyParams {
     const void *target, *draft;  // [B, n, V]; draft or null
@@ -21,13 +20,11 @@ struct VerifyParams {
     int B, n, V, tokens_64;
     int32_t *path, *accepted;  // [B, n], [B]
     void *next;                // [B], of the tokens' type
-    int parts, each;           // workgroups of a row, and its values for each
+    int parts, each;           // workgroups of a row, and its values for each (verify_plan.h)
     double *sums;              // [B, parts, 4]
     uint64_t *arrivals;        // [B, parts] words (all_arrived)
     uint64_t tag;
 };
-// Sets parts and each.
-void verify_plan(VerifyParams &p);
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t stream);
 
 }  // namespace sa

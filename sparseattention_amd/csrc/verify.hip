@@ -12,8 +12,6 @@
 //
 // Measured (float32): 64 trees of 32 nodes, V = 131072: 21.6 us, of which the row's 33.5 MB take 6.6 at the rate of a copy; the rest is the chain walk, sum, hand-over,
 // search, which alone takes 12.8 us for 8 chains of 6 nodes, V = 32000.  (Parts of 512 workgroups in all 24 us, of 2048 26; eight rows of four under way 33.)
-#include <algorithm>
-
 #include "fwd_common.h"
 #include "tree.h"
 #include "verify.h"
@@ -21,10 +19,8 @@
 namespace sa {
 namespace {
 
-constexpr int kVerifyThreads = 256, kVerifyWaves = kVerifyThreads / 64;
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-constexpr int kVerifyStep = 4 * kVerifyThreads;
 
 // A probability; what is none counts as 0.
 __device__ __forceinline__ double chance(float x) { return x > 0.f && x < __builtin_inff() ? (double)x : 0.0; }
@@ -276,7 +272,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyPara
         mark(from);
         const int q0 = from + k * quarter, q1 = min(q0 + quarter, p.V);
         // each thread a run of it
-        const int run = max((quarter + kVerifyThreads - 1) / kVerifyThreads, 4), v0 = q0 + tid * run, v1 = min(v0 + run, q1);
+        const int run = verify_run(quarter), v0 = q0 + tid * run, v1 = min(v0 + run, q1);
         double x = 0.0;
         bool any = false;
         for (int v = v0; v < v1; v += 4) {
@@ -330,14 +326,6 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyPara
 }
 
 }  // namespace
-
-// Parts of 2048 values at least (and no more than have a bit in LDS), as many as make 1024 workgroups of all rows.
-void verify_plan(VerifyParams &p) {
-    const int64_t want = std::min<int64_t>(kVerifyMostParts, (1024 + p.B - 1) / p.B), least = 2048;
-    const int64_t each = std::min<int64_t>(std::max((p.V + want - 1) / want, least), kVerifyMostEach);
-    p.each = (int)((each + kVerifyStep - 1) / kVerifyStep * kVerifyStep);
-    p.parts = (p.V + p.each - 1) / p.each;
-}
 
 hipError_t launch_verify(const VerifyParams &p, int dtype, hipStream_t stream) {
     const dim3 grid((unsigned)(p.B * p.parts));

@@ -15,13 +15,7 @@ constexpr int kNodes = 64, kMostTokens = sa::kVerifyMostParts * sa::kVerifyMostE
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 bool fits(int B, int n, int V) { return B > 0 && n > 0 && n <= kNodes && V > 0 && V <= kMostTokens; }
-int64_t words(int B, int V) {
-    sa::VerifyParams p{};
-    p.B = B;
-    p.V = V;
-    sa::verify_plan(p);
-    return (int64_t)B * p.parts;
-}
+int64_t words(int B, int V) { return (int64_t)B * sa::verify_plan(B, V).parts; }
 
 }  // namespace
 
@@ -67,7 +61,9 @@ int sa_verify_drafts(const void *target_probs, const int64_t target_strides[3], 
     p.B = B;
     p.n = n;
     p.V = V;
-    sa::verify_plan(p);
+    const sa::VerifyPlan plan = sa::verify_plan(B, V);
+    p.parts = plan.parts;
+    p.each = plan.each;
     const int64_t count = (int64_t)B * p.parts;
     if (count > sa::kMostGroups256) return fail(SA_ERR_UNSUPPORTED, "%s: more than 2^24 - 1 workgroups", who);
     const size_t need = (size_t)count * kWordBytes;
