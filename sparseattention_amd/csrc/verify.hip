@@ -251,7 +251,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(const VerifyPara
     int token = -1;
     if (whole > 0.0) {
         const double want = (double)u0_by * whole;
-        const uint64_t beyond = __builtin_amdgcn_ballot_w64(upto > want), some = __builtin_amdgcn_ballot_w64(whole_of(held) > 0.0);
+        // (of an empty part the running sum may be beyond what it is in front of it by a rounding)
+        const bool any_there = whole_of(held) > 0.0;
+        const uint64_t some = __builtin_amdgcn_ballot_w64(any_there), beyond = __builtin_amdgcn_ballot_w64(any_there && upto > want);
         const int at = beyond != 0ull ? __ffsll((unsigned long long)beyond) - 1 : 63 - __clzll((long long)some);
         double before = at > 0 ? of_lane(upto, at - 1) : 0.0;
         int k = -1;  // the quarter: the first whose end is beyond, or the last that is not empty
