@@ -21,6 +21,8 @@
 #include <memory>
 #include <optional>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "sparseattn.h"
 
@@ -1408,6 +1410,27 @@ py::object trainable(const Tensor &q, const Tensor &k, const Tensor &v, const Op
     return py::cast(AttentionFunction::apply(q, k, v, mask, *r, bmd));
 }
 
+// In a backward under capture, before anything of it is captured: gradients that go on, near or far, to a node of the default stream, such as a leaf into which a graph made
+// on it before, and still alive, accumulates.  The engine would have that stream wait for the captured one, which it cannot, and the error ends the process.  (Any
+// other stream joins the capture.)
+void gradients_fit_capture() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto start = torch::autograd::get_current_node();
+    std::vector<torch::autograd::Node *> ahead{start.get()};
+    std::unordered_set<const torch::autograd::Node *> seen;
+    while (!ahead.empty() && ahead.back() != nullptr) {
+        torch::autograd::Node *const node = ahead.back();
+        ahead.pop_back();
+        for (size_t i = 0; i < node->num_outputs(); i++) {
+            torch::autograd::Node *const next = node->next_edge(i).function.get();
+            if (next == nullptr || !node->task_should_compute_output(i) || !seen.insert(next).second) continue;
+            if (const auto stream = next->stream(); stream && stream->id() == 0)
+                throw std::runtime_error("rotate_heads_trainable under capture: a graph made before, on the default stream, still holds these leaves; let go of its outputs first");
+            ahead.push_back(next);
+        }
+    }
+}
+
 struct RotateFunction : public torch::autograd::Function<RotateFunction> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const OptTensor &qw, const OptTensor &kw,
                                                   const Tensor &positions, const Tensor &frequencies, const OptTensor &axes, bool interleaved, double eps) {
@@ -1422,28 +1445,16 @@ struct RotateFunction : public torch::autograd::Function<RotateFunction> {
         auto opt = [](const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; };
         const auto g = with_python_errors([&] {
             if (at::GradMode::is_enabled()) throw std::runtime_error("rotate_heads_trainable has no second derivative (create_graph)");
+            gradients_fit_capture();
             return rotate_backward_impl(grads[0], grads[1], s[0], s[1], s[4], {s[5], opt(s[6]), ctx->saved_data["interleaved"].toBool()}, opt(s[2]), opt(s[3]),
                                         ctx->saved_data["eps"].toDouble());
         });
         return {g.dq, g.dk, g.dqw.value_or(Tensor()), g.dkw.value_or(Tensor()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-// Under capture, leaves that another living graph already accumulates into on another stream: the backward would wait for that stream, which a capture
-// cannot, and the error ends the process.
-void leaves_fit_capture(const Tensor &ref, std::initializer_list<const Tensor *> inputs) {
-    if (!ref.is_cuda() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(ref.device().index());
-    for (const Tensor *t : inputs) {
-        if (t == nullptr || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (node && node->stream() && *node->stream() != now)
-            throw std::runtime_error("rotate_heads_trainable under capture: a graph made before, on another stream, still holds these leaves; let go of its outputs first");
-    }
-}
 py::tuple rotate_heads_trainable(const Tensor &q, const Tensor &k, const Tensor &positions, py::object rotary, const OptTensor &qw, const OptTensor &kw, double eps) {
     const Rotary r = rotary_of(rotary);
     not_traced("rotate_heads_trainable");
-    leaves_fit_capture(q, {&q, &k, qw ? &*qw : nullptr, kw ? &*kw : nullptr});
     const auto out = RotateFunction::apply(q, k, qw, kw, positions, r.frequencies, r.axes, r.interleaved, eps);
     return py::make_tuple(out[0], out[1]);
 }
