@@ -329,7 +329,8 @@ static int decode(const char *who, sa::PagedDecodeParams &p, int most_rows, cons
     p.scale = sm_scale_log2;
     const int64_t planes = heads * p.RT;
     if (planes > (1 << 24) || planes * chunks > (1 << 30))
-        return fail(SA_ERR_UNSUPPORTED, "%s: more planes of 32 rows or keys than a launch has", who);
+        return fail(SA_ERR_UNSUPPORTED, "%s: %lld planes of %d rows and %lld chunks of 32 keys each; a launch has at most 2^24 planes and 2^30 chunks of all of them", who, (long long)planes,
+                    p.plane_rows, (long long)chunks);
     const sa::PagedDecodePlan plan = sa::paged_decode_plan(planes, p.R, p.c.D, chunks, compute_units(), p.plane_rows);
     const size_t parts_bytes = sa::paged_decode_parts_bytes(plan.groups, plan.part_rows, p.c.D), units_at = parts_bytes + (size_t)(planes + plan.groups) * 8,
                  need = units_at + units_bytes((int64_t)B * p.c.H);
