@@ -550,7 +550,7 @@ int sa_rotate_heads_bwd(const void *dq_out, const int64_t dq_out_strides[4], con
  *   page_table         device int32 [B, pages_per_sequence], strides in elements; token t of sequence b lies in page page_table[b][t / page_size].
  *                      An entry that is no page (outside [0, num_pages)) is as if nothing were there: nothing is stored, read as zeros,
  *                      attended to.
- *   lens               device int32 [B]: tokens that each sequence holds; below 0 counts as 0.
+ *   lens               device int32 [B]: tokens that each sequence holds; below 0 counts as 0, where they are read beyond the table as the table's tokens.
  * Pages may be shared by sequences that read them.  Two sequences of one call, or two entries of one, that store into the same block leave it
  * undefined.
  */
@@ -665,7 +665,8 @@ int sa_sparse_attention_decode_paged(const void *q, const int64_t q_strides[4], 
  * given by parents (device int32 [B,n], strides in elements): parents[b][i] in [0, i) is node i's parent, any other value says that it has none.
  * Row i attends to all lens[b] - counts[b] keys in front of the tree, to itself and to its ancestors; with window > 0 to those of them less than
  * `window` positions back, a node's position being lens[b] - counts[b] and its depth.  (A chain is parents[b][i] = i - 1.)
- * Everything else as above, with sa_decode_tree_workspace_bytes.
+ * Everything else as above, with sa_decode_tree_workspace_bytes.  How rows are dealt out goes by pages_per_sequence: give the pages in use, not all that
+ * a sequence may ever need.
  */
 size_t sa_decode_tree_workspace_bytes(int B, int Hq, int H, int n, int D, int pages_per_sequence, int page_size);
 int sa_sparse_attention_decode_tree(const void *q, const int64_t q_strides[4], const sa_paged_cache *cache, const int32_t *page_table,

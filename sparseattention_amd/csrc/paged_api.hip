@@ -268,6 +268,10 @@ static size_t units_bytes(int64_t units) { return (sizeof(sa::PagedUnits) + (siz
 //          H 256: C 16128  116 | 67 | 63 | 71; 32000  240 | 127 | 99 | 114; 65536  488 | 249 | 204 | 199; 160000  1338 | 674 | 455 | 434
 //          H  16: C 32768  271 | 97 | 108 | 160 (few planes, of many parts)
 //   R  64, H 256: C 32000  140 | 64 | 66; 65536  290 | 133 | 126; 262144  1224 | 532 | 400
+// At the other head dims the same numbers are used, not always to their best:
+//   D  64, R  32, H   8: C  504  10 | 13;   R 128, H 64: C 4032  24 | 23 | 26 | 46;    H 256: C 16128   80 |  41 |  48 |  53; 32000  157 |  68 |  75 |  74; 64000   301 | 125 | 124 | 125
+//   D 256, R  32, H   8: C  504  19 | 30;   R 128, H 64: C 4032  61 | 39 | 65 | 84;    H 256: C 16128  308 | 176 | 125 | 124; 32000  713 | 377 | 253 | 218; 64000  1382 | 707 | 462 | 413
+// C goes by the tables' width: 64 heads, R 128, C 4032, D 128 take 31 us with tables of 63 chunks, 46 with such of 4096.
 static int decode_plane_rows(bool tree, int64_t heads, int R, int64_t chunks) {
     if (R <= 16) return 16;
     if (!tree) return 32;

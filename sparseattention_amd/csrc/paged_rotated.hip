@@ -7,8 +7,8 @@
 // them.  Bound by memory where there are many tokens, by the chain length, table, scale, block where there are few.  (With the read-back, the prompts below took 93 us by
 // workgroups that had all three of a block, 75 by these, and 70 since a block's keys stay in the registers of four waves instead of 72.)
 //
-// Measured (32 + 8 heads, D = 128, bf16, norms, where nothing else is said): 1 token of 64 sequences 7.8 us; 4096 tokens of one 24 us, 3.8 TB/s read and written;
-// 16 prompts of up to 2047, 12 heads, D = 64, fp16, interleaved, no norms 45 us, 4.0 TB/s (a copy of 1 GiB: 5.1).
+// Measured (32 + 8 heads, D = 128, bf16, norms, where nothing else is said): 1 token of 64 sequences 7.8 us; 4096 tokens of one 24 us, 3.8 TB/s read and written (1.2 less
+// with no angles made); 16 prompts of up to 2047, 12 heads, D = 64, fp16, interleaved, no norms 45 us, 4.0 TB/s (0.8 less; a copy of 1 GiB: 5.1).
 #include <algorithm>
 
 #include "paged_codes.h"

@@ -7,7 +7,8 @@
 // in one launch.  A wave has 64 / LPR tokens and some of their heads, so that the angles, which take as long as four rows, are made once for these.
 //
 // Measured: 4 x 4096 tokens, 32 + 8 heads, D = 128, bf16, norms: forward 63 us, 5.3 TB/s read and written, backward 86, 5.9, and 5 for the sums of the weights
-// (a copy of 1 GiB: 5.1); 2 x 1031 tokens of three axes, 16 + 16 heads, D = 80, fp16: 8.6 us a call, a launch, the angles and 21 MB.
+// (a copy of 1 GiB: 5.1); 2 x 1031 tokens of three axes, 16 + 16 heads, D = 80, fp16: 8.6 us a call, a launch and 21 MB (as
+// long with no angles made); 2 x 4096 tokens, float32, norms: forward 55 us, 6.1 TB/s, with the backward 145, 5.8.
 // Not kept: rows requested before the angles (no gain); reads past the caches, too (8.6 -> 9.8 us).
 #include <algorithm>
 
@@ -171,8 +172,13 @@ __global__ __launch_bounds__(kWeightThreads) void rotate_weights_kernel(const Ro
     else ((__bf16 *)out)[col] = (__bf16)(float)x;
 }
 
-// Outputs of that many bytes go past the caches, which would not hold them for who reads them next (336 MB read and 168 MB written by the backward, 168 and 168 by the
-// forward: 188 us through them, 165 past them).
+// Outputs of that many bytes go past the caches, for training's sake: what a forward writes there drives out what the backward reads.  us through the caches | past them, 32 + 8 heads,
+// D = 128, bf16, norms, inputs that change from call to call, by MiB of outputs (float32 at D = 64 likewise):
+//   forward and backward   80 95 | -;        128 159 | 144;   160 188 | 165;   320 350 | 330
+//   backward               64 47.5 | 47.5;   96 66 | 63;      128 93 | 81;     192 136 | 133;   256 176 | 172;   512 336 | 331
+//   forward                64 29 | 31;       96 39 | 45;      128 51 | 58;     192 86 | 84;     256 114 | 112;   512 216 | 210
+//   and its outputs read   64 52 | 59;       96 71 | 80;      128 97 | 108;    192 151 | 160;   256 202 | 212;   512 398 | 401
+// (A forward alone would do better with a border of its own, at about 192 MiB, or none where its outputs are read next.)
 constexpr int64_t kRotateFar = 128ll << 20;
 
 // Heads are dealt out to as many waves as fill the device, four at least to one, as the angles of its tokens are made once for all of them.

@@ -10,7 +10,7 @@
 // which part the token is in and goes through that again.  Probabilities are at most 32 bits wide and all that is done with them has 64: a row of 10^5
 // has sums off by 2^-37 of it, in float32 by more than most of its values.  Bound by memory: p (and q) of one row a sequence.
 //
-// Measured (float32): 64 trees of 32 nodes, V = 131072: 21.6 us, of which the row's 33.5 MB take 6.6 at the rate of a copy; the rest is the chain walk, sum, hand-over,
+// Measured (float32): 64 trees of 32 nodes, V = 131072: 21.6 us (V = 151936 24.1), of which the row's 33.5 MB take 6.6 at the rate of a copy; the rest is the chain walk, sum, hand-over,
 // search, which alone takes 12.8 us for 8 chains of 6 nodes, V = 32000.  (Parts of 512 workgroups in all 24 us, of 2048 26; eight rows of four under way 33.)
 #include "fwd_common.h"
 #include "tree.h"

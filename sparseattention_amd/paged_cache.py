@@ -185,5 +185,9 @@ def sparse_attention_decode_tree(q: torch.Tensor, cache: PagedCache, page_table:
     other value says that it has none.  Row ``i`` attends to all keys in front of the tree, to itself and to its ancestors; with ``window`` to
     those less than ``window`` positions back, where a node's position is the keys in front of the tree and its depth.
 
-    ``counts`` (int32 [B]): the tree has ``counts[b]`` nodes, the rows behind are padding and give 0 (``lse`` -inf)."""
+    ``counts`` (int32 [B]): the tree has ``counts[b]`` nodes, the rows behind are padding and give 0 (``lse`` -inf).  A length beyond the table counts as the
+    table's tokens, so drafts that found no room in it have to be left out of ``counts`` and ``lens``.
+
+    As there, weights are rounded to q's type before they meet the values, sums are float32: next to a float32 attention the error of a long batch grows by about a third.  How rows are dealt out goes by
+    the table's width, as lengths are not read on the host: pass the columns in use (``page_table[:, :pages]``), not all that a sequence may ever need."""
     return _native.host().decode_tree(q, cache, page_table, lens, parents, counts, window, return_lse)

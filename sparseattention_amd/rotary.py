@@ -53,7 +53,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rota
 
     ``positions``: int32 or int64, [S] or [B,S] (or [1,S]); [axes,B,S] with ``rotary.axes``, whose entries are taken as the nearest axis there is.
     Angles are exact to 2^-24 of a turn up to positions of 2^31; all else is float32, rounded once.  (Squares of values beyond 1e18 do not fit
-    float32.)  Weights are of q's type or float32, both the same."""
+    float32, nor, where ``eps`` is below 1e-37, those of rows below 1e-18.)  Weights are of q's type or float32, both the same."""
     return _native.host().rotate_heads(q, k, positions, rotary, q_weight, k_weight, eps)
 
 
@@ -66,5 +66,8 @@ def rotate_heads_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
 
 def rotate_heads_trainable(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, q_weight: Optional[torch.Tensor] = None,
                            k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6):
-    """:func:`rotate_heads` for autograd: gradients for q, k and the weights (once; second derivatives are refused)."""
+    """:func:`rotate_heads` for autograd: gradients for q, k and the weights (once; second derivatives are refused).
+
+    A backward under graph capture is refused where gradients it is asked for go on to something of the default stream, which cannot join a capture: leaves that a graph made
+    there before holds as long as its outputs live, or inputs made there."""
     return _native.host().rotate_heads_trainable(q, k, positions, rotary, q_weight, k_weight, eps)
